@@ -17,7 +17,8 @@ The cache (n sequences, h kv heads, L rows, D dims; groups of 32 dims share a st
   k_meta  fp16  [n, h, L, D/32, 2]        step, low
   v_codes uint8 [n, h, L/8, D/4, 16]      row t, element d in byte 2 (t % 8) + (d % 4) / 2, even d in the low 4 bits
   v_meta  fp16  [n, h, L/8, D/32, 2, 8]   the steps of 8 rows, then their lows
-Code c stands for fp16(low + step c); low = fp16(min), step = fp16((max - min) / 15), c = the nearest code.
+Code c stands for fp16(low + step c); low = fp16(min), step = (max - min) / 15 in fp16 rounded towards zero (so that
+no finite value reads back as an infinity), c = the nearest code, ties to even.
 """
 
 import random
@@ -195,11 +196,17 @@ def prepare(case, seed):
 # ---- the plain form ---------------------------------------------------------------------------
 
 
+def _half_down(x):
+    """x >= 0 in fp16, rounded towards zero."""
+    near = x.half()
+    return torch.where(near.to(x.dtype) > x, (near.view(torch.int16) - 1).view(torch.float16), near)
+
+
 def _quantise(x):
     """(step, low) fp16 [..., D/32] and codes uint8 [..., D] of rows x [..., D]."""
     g = x.float().unflatten(-1, (-1, GROUP))
     high, low = g.amax(-1), g.amin(-1)
-    step, low = ((high - low) * (1 / 15)).half(), low.half()
+    step, low = _half_down((high - low) * (1 / 15)), low.half()
     divisor = torch.where(step > 0, step, 1.0).float()  # a group of one value: code 0
     codes = ((g - low.float().unsqueeze(-1)) / divisor.unsqueeze(-1)).round_().clamp_(0, 15)
     return step, low, codes.to(torch.uint8).flatten(-2)
@@ -366,7 +373,9 @@ def _held64(x):
     """The values that the cache holds for rows x [..., D]."""
     g = x.double().reshape(*x.shape[:-1], -1, GROUP)
     low = g.min(-1, keepdim=True).values
-    step = ((g.max(-1, keepdim=True).values - low) / 15).to(torch.float16).double()
+    wide = (g.max(-1, keepdim=True).values - low) / 15
+    last = torch.exp2((torch.frexp(wide).exponent - 1).clamp(min=-14).double() - 10)  # fp16's last place
+    step = torch.floor(wide / last) * last
     low = low.to(torch.float16).double()
     code = torch.round((g - low) / torch.where(step == 0, torch.ones_like(step), step)).clamp(0, 15)
     code = torch.where(step == 0, torch.zeros_like(code), code)

@@ -17,6 +17,7 @@ LIB_PATH = Path(os.environ.get('FW_LIBRARY') or Path(__file__).resolve().parent 
 FW_OK, FW_EINVAL, FW_EHIP = 0, -1, -2
 NOALLOC_ATTN_SLOTS = 2048  # FW_NOALLOC_ATTN_SLOTS
 ACT_NONE, ACT_GELU = 0, 1
+F16, BF16 = 0, 1  # FW_F16, FW_BF16
 EPI_BIAS, EPI_BIAS_GELU, EPI_BIAS_RESID, EPI_BIAS_RESID_CLAMP, EPI_BIAS_GELU_POS, EPI_SCALE_Q = range(6)
 
 P = c_void_p
@@ -59,6 +60,16 @@ SIGNATURES = {
     'fw_encoder_pack_vt': (c_int, [P, P, c_int, c_int, P]),
     'fw_encoder_attention': (c_int, [P, P, P, c_int, c_int, P]),
     'fw_cross_kv': (c_int, [P, c_int, P, P, P, c_int, c_int, P]),
+    'fw_prompt_attention': (c_int, [P, c_int64, c_int64, P, c_int64, c_int64, P, c_int64, c_int64, P, c_int64, c_int64,
+                                    P, P, c_int, c_int64, c_int64, c_int, c_int, c_int, c_int, c_float, c_int, P]),
+    'fw_kv_q4_append': (c_int, [P, c_int64, c_int64, P, c_int64, c_int64, c_int64, P, P, P, P, P, P, c_int, c_int, c_int,
+                                c_int, c_int, P]),
+    'fw_kv_q4_read': (c_int, [P, P, P, P, c_int, c_int, c_int, c_int, P, P, c_int64, P, c_int64, c_int64, P, c_int64,
+                              c_int64, c_int, P]),
+    'fw_decode_attention_q4': (c_int, [P, c_int64, c_int64, P, P, P, P, P, P, c_int64, c_int64, P, c_int64, c_int64, P,
+                                       c_int64, c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_float, P, c_int64,
+                                       P]),
+    'fw_decode_attention_q4_ws_floats': (c_int64, [c_int, c_int, c_int, c_int, c_int]),
     'fw_synth_normal_f16': (c_int, [P, c_int64, c_int64, c_uint64, c_uint64, c_float, c_float, P]),
     'fw_synth_normal_f16_host': (c_int, [P, c_int64, c_int64, c_uint64, c_uint64, c_float, c_float]),
     'fw_decoder_step_workspace_bytes': (ctypes.c_size_t, [c_int]),

@@ -15,6 +15,7 @@ compiler's per-kernel register, LDS and spill report, like the reference's ``mai
 import argparse
 import ctypes
 import sys
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -84,6 +85,72 @@ def _check_rows(t, name, cols):
 def _check(t, name, dtype, what):
     _require(isinstance(t, torch.Tensor) and t.is_cuda and t.is_contiguous() and t.dtype == dtype,
              f'{name} must be contiguous CUDA {what}')
+
+
+# The prompt attention and the 4-bit cache take fp16 or bf16 rows of any strides that keep 16-byte pieces whole.
+_DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+
+
+def _current_device():
+    """The current device's index; before torch's first GPU call None, which no tensor is on."""
+    return _device() if torch.cuda.is_initialized() and _device is not None else None
+
+
+def _heads_view(t, name, dtype, dev, heads, dim):
+    """Checks a [rows, heads, dim] CUDA view of `dtype` with unit element stride and strides in multiples of 8 (heads
+    None: any count); returns its row and head strides (0 where there is one row or head)."""
+    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.dim() == 3 and t.get_device() == dev):
+        (rows, h, d), (sr, sh, sd) = t.shape, t.stride()
+        if d == dim and sd == 1 and (heads is None or h == heads):
+            sr, sh = sr if rows > 1 else 0, sh if h > 1 else 0
+            if (sr | sh) & 7 == 0 and t.data_ptr() & 15 == 0:
+                return sr, sh
+    raise RuntimeError(f'{name} must be a [rows, {"heads" if heads is None else heads}, {dim}] {dtype} view on the '
+                       'current device with unit element stride, other strides in multiples of 8 and 16-byte aligned data')
+
+
+def _out_view(t, name, dtype, dev, heads, dim):
+    """_heads_view of a tensor that is written: its rows must not overlap each other."""
+    sr, sh = _heads_view(t, name, dtype, dev, heads, dim)
+    rows, h, _ = t.shape
+    if rows > 1 and h > 1:
+        apart = min(sr, sh) >= dim and (sr >= (h - 1) * sh + dim or sh >= (rows - 1) * sr + dim)
+    else:
+        apart = (rows <= 1 or sr >= dim) and (h <= 1 or sh >= dim)
+    _require(apart, f'the rows of {name} must not overlap')
+    return sr, sh
+
+
+def _index(t, name, n, dev):
+    if not (isinstance(t, torch.Tensor) and t.dtype is _I64 and t.get_device() == dev and t.dim() == 1
+            and (n is None or t.size(0) == n) and t.is_contiguous()):
+        raise RuntimeError(f'{name} must be contiguous int64 [{"n + 1" if n is None else n}] on the current device')
+
+
+class KvQ4Cache(NamedTuple):
+    """A key/value cache held in 4 bits (layout: fw_kv_q4_append in include/flash_whisper.h)."""
+    k_codes: torch.Tensor  # uint8 [n_seq, kv_heads, max_len, head_dim / 2]
+    k_meta: torch.Tensor   # fp16 [n_seq, kv_heads, max_len, head_dim / 32, 2]
+    v_codes: torch.Tensor  # uint8 [n_seq, kv_heads, max_len / 8, head_dim / 4, 16]
+    v_meta: torch.Tensor   # fp16 [n_seq, kv_heads, max_len / 8, head_dim / 32, 2, 8]
+
+
+def _cache_sizes(cache, dev):
+    """Checks the four arrays of a cache; returns n_seq, kv_heads, max_len, head_dim."""
+    k_codes, k_meta, v_codes, v_meta = cache
+    for t, dtype, name in ((k_codes, torch.uint8, 'k_codes'), (k_meta, _F16, 'k_meta'), (v_codes, torch.uint8, 'v_codes'),
+                           (v_meta, _F16, 'v_meta')):
+        if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev and t.is_contiguous()):
+            raise RuntimeError(f'{name} must be contiguous {dtype} on the current device')
+    if k_codes.dim() != 4:
+        raise RuntimeError('k_codes must be [n_seq, kv_heads, max_len, head_dim / 2]')
+    n, heads, max_len, half = k_codes.shape
+    if max_len % 32 or half not in (32, 64):
+        raise RuntimeError('max_len must be a multiple of 32 and head_dim 64 or 128')
+    if (k_meta.shape != (n, heads, max_len, half // 16, 2) or v_codes.shape != (n, heads, max_len // 8, half // 2, 16)
+            or v_meta.shape != (n, heads, max_len // 8, half // 16, 2, 8)):
+        raise RuntimeError('the arrays of the cache do not belong together')
+    return n, heads, max_len, 2 * half
 
 
 class HostTokens:
@@ -322,6 +389,105 @@ class WhisperExt:
             self._call('fw_attn_out_gemv', *args, _stream())
         else:
             self._call('fw_attn_out_gemv_batch', *args, nv, _stream())
+
+    # ---- many sequences: prompts and the 4-bit cache ------------------------------------------
+    def prompt_attention(self, q, k, v, out, cu_q, cu_k, scale, causal=True):
+        """Attention over the prompts of several sequences (fw_prompt_attention). q, out [rows, heads, head_dim] and k,
+        v [rows, kv_heads, head_dim], fp16 or bf16, head_dim 64 or 128, any row and head strides in multiples of 8;
+        sequence s has the rows cu_q[s] .. cu_q[s + 1] - 1 of q and cu_k[s] .. cu_k[s + 1] - 1 of k and v (int64, on
+        the device). causal: a query sees the keys up to its own place counted from the end of both. A query that sees
+        no key gets zeros; rows of out behind the last sequence are left as they are."""
+        dev = _current_device()
+        dtype = getattr(q, 'dtype', None)
+        if dtype not in _DTYPES or q.dim() != 3 or q.size(2) not in (64, 128):
+            raise RuntimeError('q must be fp16 or bf16 [rows, heads, 64 or 128]')
+        dim = q.size(2)
+        q_row, q_head = _heads_view(q, 'q', dtype, dev, None, dim)
+        k_row, k_head = _heads_view(k, 'k', dtype, dev, None, dim)
+        v_row, v_head = _heads_view(v, 'v', dtype, dev, k.size(1), dim)
+        o_row, o_head = _out_view(out, 'out', dtype, dev, q.size(1), dim)
+        if out.size(0) != q.size(0) or v.size(0) != k.size(0):
+            raise RuntimeError('out must have the rows of q, and v those of k')
+        _index(cu_q, 'cu_q', None, dev)
+        _index(cu_k, 'cu_k', cu_q.size(0), dev)
+        self._call('fw_prompt_attention', q.data_ptr(), q_row, q_head, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row,
+                   v_head, out.data_ptr(), o_row, o_head, cu_q.data_ptr(), cu_k.data_ptr(), cu_q.size(0) - 1, q.size(0),
+                   k.size(0), q.size(1), k.size(1), dim, _DTYPES[dtype], float(scale), bool(causal), _stream())
+
+    def kv_q4_cache(self, n_seq, kv_heads, max_len, head_dim, device='cuda'):
+        """An empty KvQ4Cache; max_len is rounded up to a multiple of 32 rows."""
+        _require(n_seq > 0 and kv_heads > 0 and max_len > 0 and head_dim in (64, 128),
+                 'n_seq, kv_heads and max_len must be positive and head_dim 64 or 128')
+        rows = -(-max_len // 32) * 32
+        new = lambda dtype, *shape: torch.zeros(n_seq, kv_heads, *shape, dtype=dtype, device=device)
+        return KvQ4Cache(new(torch.uint8, rows, head_dim // 2), new(_F16, rows, head_dim // 32, 2),
+                         new(torch.uint8, rows // 8, head_dim // 4, 16), new(_F16, rows // 8, head_dim // 32, 2, 8))
+
+    def _packed(self, k, v, cu, pos, cache, view):
+        """The checks and the arguments that kv_q4_append and kv_q4_read share: rows, cache, places."""
+        dev = _current_device()
+        n, heads, max_len, dim = _cache_sizes(cache, dev)
+        dtype = getattr(k, 'dtype', None)
+        if dtype not in _DTYPES:
+            raise RuntimeError('k and v must be fp16 or bf16')
+        k_strides, v_strides = view(k, 'k', dtype, dev, heads, dim), view(v, 'v', dtype, dev, heads, dim)
+        rows = (k.data_ptr(), *k_strides, v.data_ptr(), *v_strides)
+        if k.size(0) != v.size(0):
+            raise RuntimeError('k and v must have the same rows')
+        _index(cu, 'cu', n + 1, dev)
+        _index(pos, 'pos', n, dev)
+        return rows, tuple(t.data_ptr() for t in cache), (n, heads, max_len, dim), (cu.data_ptr(), pos.data_ptr()), dtype
+
+    def kv_q4_append(self, k, v, cu, pos, cache):
+        """Writes the packed rows cu[s] .. cu[s + 1] - 1 of k and v ([rows, kv_heads, head_dim], fp16 or bf16) into rows
+        pos[s] .. of sequence s of the 4-bit cache (fw_kv_q4_append). Rows that fall outside it are dropped."""
+        rows, arrays, sizes, places, dtype = self._packed(k, v, cu, pos, cache, _heads_view)
+        self._call('fw_kv_q4_append', *rows, k.size(0), *places, *arrays, *sizes, _DTYPES[dtype], _stream())
+
+    def kv_q4_read(self, cache, cu, pos, k, v):
+        """The values that the cache holds for its rows pos[s] .. into rows cu[s] .. cu[s + 1] - 1 of k and v
+        (fw_kv_q4_read): the counterpart of kv_q4_append, for a prompt that goes on where an earlier one ended."""
+        rows, arrays, sizes, places, dtype = self._packed(k, v, cu, pos, cache, _out_view)
+        self._call('fw_kv_q4_read', *arrays, *sizes, *places, k.size(0), *rows, _DTYPES[dtype], _stream())
+
+    def decode_attention_q4_workspace(self, n_seq, heads, cache):
+        """Workspace of decode_attention_q4 for n_seq sequences and `heads` query heads over `cache` (one per stream)."""
+        _, kv_heads, max_len, half = cache[0].shape
+        n = self.lib.fw_decode_attention_q4_ws_floats(int(n_seq), int(heads), kv_heads, max_len, 2 * half)
+        _require(n > 0, 'decode_attention_q4: heads must be a multiple of the cache\'s heads')
+        return torch.empty(n, dtype=torch.float32, device=cache[0].device)
+
+    def decode_attention_q4(self, q, cache, lens, out, ws, scale, k_new=None, v_new=None):
+        """One query a sequence, q and out [n_seq, heads, head_dim], over the first lens[s] rows of the 4-bit cache; with
+        k_new and v_new ([n_seq, kv_heads, head_dim]) their row is written to row lens[s] first and attended to as well
+        (fw_decode_attention_q4). lens is int64 on the device and is not advanced; a negative one marks an idle
+        sequence, which gets zeros and whose cache stays as it is."""
+        dev = _current_device()
+        n, kv_heads, max_len, dim = _cache_sizes(cache, dev)
+        dtype = getattr(q, 'dtype', None)
+        if dtype not in _DTYPES:
+            raise RuntimeError('q must be fp16 or bf16')
+        q_row, q_head = _heads_view(q, 'q', dtype, dev, None, dim)
+        heads = q.size(1)
+        o_row, o_head = _out_view(out, 'out', dtype, dev, heads, dim)
+        if q.size(0) != n or out.size(0) != n:
+            raise RuntimeError('q and out must have a row for each sequence of the cache')
+        _index(lens, 'lens', n, dev)
+        if not (isinstance(ws, torch.Tensor) and ws.dtype is _F32 and ws.get_device() == dev and ws.is_contiguous()):
+            raise RuntimeError('workspace must be contiguous fp32 on the current device')
+        fresh = (None, 0, 0, None, 0, 0)
+        if k_new is not None or v_new is not None:
+            if k_new is None or v_new is None:
+                raise RuntimeError('k_new and v_new must be given together')
+            k_strides = _heads_view(k_new, 'k_new', dtype, dev, kv_heads, dim)
+            v_strides = _heads_view(v_new, 'v_new', dtype, dev, kv_heads, dim)
+            fresh = (k_new.data_ptr(), *k_strides, v_new.data_ptr(), *v_strides)
+            if k_new.size(0) != n or v_new.size(0) != n:
+                raise RuntimeError('k_new and v_new must have a row for each sequence of the cache')
+        k_codes, k_meta, v_codes, v_meta = cache
+        self._call('fw_decode_attention_q4', q.data_ptr(), q_row, q_head, k_codes.data_ptr(), k_meta.data_ptr(),
+                   v_codes.data_ptr(), v_meta.data_ptr(), lens.data_ptr(), out.data_ptr(), o_row, o_head, *fresh, n, heads,
+                   kv_heads, max_len, dim, _DTYPES[dtype], float(scale), ws.data_ptr(), ws.numel(), _stream())
 
     # ---- the decoder layers of one token in one launch --------------------------------------
     def decoder_step_supported(self, n_layers, vocab, max_pos, enc_len, prompt=False):

@@ -39,6 +39,10 @@ extern "C" {
 #define FW_EPI_BIAS_GELU_POS 4 /* out = fp16(fp16(gelu(fp16(acc + b))) + res)           */
 #define FW_EPI_SCALE_Q 5       /* columns < q_cols: fp16(fp16(acc + b) * 0.125); k/v as BIAS */
 
+/* Element types of the prompt attention and the 4-bit cache. */
+#define FW_F16 0
+#define FW_BF16 1
+
 const char* fw_last_error(void);
 int fw_version(void);
 
@@ -418,6 +422,62 @@ int fw_encoder_attention(const void* qkv, const void* vt, void* out, int seq, in
  * bias fp16[layers * 2 * 1280]; cross_kv fp16[layers, 2, heads, t, 64]. */
 int fw_cross_kv(const void* enc, int t, const void* w, const void* bias, void* cross_kv, int layers, int heads,
                 hipStream_t stream);
+
+/* ---- many sequences: prompts and a key/value cache held in 4 bits (no reference counterpart: the
+ *      reference serves one clip, its prompt a token at a time over an fp16 cache) -------------- */
+
+/* Attention over whole prompts. q, out [q_rows, heads, head_dim] and k, v [k_rows, kv_heads, head_dim] of one
+ * type (FW_F16 or FW_BF16), each with its row and head strides in elements (multiples of 8; pointers 16-byte
+ * aligned). Sequence s has the query rows cu_q[s] .. cu_q[s + 1] - 1 and the key rows cu_k[s] .. cu_k[s + 1] - 1
+ * (int64, device, n_seq + 1 entries, ascending; entries outside the rows are clamped to them). Query head h reads
+ * key/value head h / (heads / kv_heads), heads a multiple of kv_heads; head_dim 64 or 128.
+ * out[i] <- sum_j softmax_j(scale q[i] . k[j]) v[j] over the keys j of i's sequence; causal: the last query sees every
+ * key, each one before it a key less (j <= i + n_keys - n_queries, both counted within the sequence). A query that
+ * sees no key gets zeros. What a query does not see does not reach its output, whatever it holds (infinities and NaN
+ * too). Rows of out behind the last sequence are left as they are. Scores, softmax and sums are fp32; the weights
+ * are rounded to the type for the product with v. out overlaps no input. */
+int fw_prompt_attention(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
+                        const void* v, int64_t v_row, int64_t v_head, void* out, int64_t o_row, int64_t o_head,
+                        const int64_t* cu_q, const int64_t* cu_k, int n_seq, int64_t q_rows, int64_t k_rows, int heads,
+                        int kv_heads, int head_dim, int dtype, float scale, int causal, hipStream_t stream);
+
+/* The 4-bit cache of n_seq sequences, kv_heads heads and max_len rows (a multiple of 32) of head_dim (64 or 128)
+ * elements: 5 bits a value. 32 elements of a row share a step and a low value (fp16), and a code c of 0 .. 15 stands
+ * for fp16(low + step c). All four arrays are dense and 16-byte aligned:
+ *   k_codes u8   [n_seq][kv_heads][max_len][head_dim / 2]          element d in byte d / 2, even d in the low bits
+ *   k_meta  fp16 [n_seq][kv_heads][max_len][head_dim / 32][2]      step, low
+ *   v_codes u8   [n_seq][kv_heads][max_len / 8][head_dim / 4][16]  row t, element d in byte 2 (t % 8) + (d % 4) / 2
+ *   v_meta  fp16 [n_seq][kv_heads][max_len / 8][head_dim / 32][2][8]  the steps of 8 rows, then their lows
+ *
+ * fw_kv_q4_append writes the packed rows cu[s] .. cu[s + 1] - 1 of k and v ([rows, kv_heads, head_dim], strides as in
+ * fw_prompt_attention) into the cache rows pos[s] .. of sequence s (cu, pos int64, device); rows that fall outside
+ * [0, max_len) are dropped, every other row of the cache is left as it is. Per group: low = fp16(min), step =
+ * (max - min) / 15 in fp16 rounded towards zero, c = the code nearest to (x - low) / step, ties to even. A group
+ * holding a NaN or an infinity reads back as NaN; bf16 values beyond fp16's range read back as non-finite ones. */
+int fw_kv_q4_append(const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head,
+                    int64_t rows, const int64_t* cu, const int64_t* pos, void* k_codes, void* k_meta, void* v_codes,
+                    void* v_meta, int n_seq, int kv_heads, int max_len, int head_dim, int dtype, hipStream_t stream);
+
+/* The values that the cache holds for its rows pos[s] .. into the packed rows cu[s] .. cu[s + 1] - 1 of k and v, as
+ * fw_kv_q4_append takes them (zeros for rows outside the cache); bf16 ones are rounded once more. */
+int fw_kv_q4_read(const void* k_codes, const void* k_meta, const void* v_codes, const void* v_meta, int n_seq,
+                  int kv_heads, int max_len, int head_dim, const int64_t* cu, const int64_t* pos, int64_t rows, void* k,
+                  int64_t k_row, int64_t k_head, void* v, int64_t v_row, int64_t v_head, int dtype, hipStream_t stream);
+
+/* Attention of one query a sequence over the 4-bit cache: q, out [n_seq, heads, head_dim] with strides, heads grouped as
+ * in fw_prompt_attention. Without k_new and v_new sequence s attends to its first lens[s] rows (int64, device; at
+ * most max_len). With them ([n_seq, kv_heads, head_dim]; both or neither) their row is written to cache row lens[s]
+ * first, as fw_kv_q4_append would, and lens[s] + 1 rows are attended to; at lens[s] >= max_len the last row is
+ * overwritten. A sequence without rows, and an idle one (lens[s] < 0: nothing is written to its cache), gets zeros.
+ * lens is not advanced. ws: fw_decode_attention_q4_ws_floats floats, 16-byte aligned, uninitialised; calls that may
+ * overlap need one each. */
+int fw_decode_attention_q4(const void* q, int64_t q_row, int64_t q_head, void* k_codes, void* k_meta, void* v_codes,
+                           void* v_meta, const int64_t* lens, void* out, int64_t o_row, int64_t o_head,
+                           const void* k_new, int64_t k_row, int64_t k_head, const void* v_new, int64_t v_row,
+                           int64_t v_head, int n_seq, int heads, int kv_heads, int max_len, int head_dim, int dtype,
+                           float scale, float* ws, int64_t ws_floats, hipStream_t stream);
+/* Floats of its workspace (0 for sizes it refuses). */
+int64_t fw_decode_attention_q4_ws_floats(int n_seq, int heads, int kv_heads, int max_len, int head_dim);
 
 /* ---- seeded synthetic weights (the random-init N(mean, std) fp16 generator) -------------- */
 

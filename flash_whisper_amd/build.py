@@ -40,6 +40,7 @@ PER_FILE_FLAGS = {
     # MFMA results in VGPRs: the attention softmax reads every score and rescales O in place
     'attention_enc.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form', *PRELOAD],
     'decode.hip': PRELOAD,
+    'kv_q4.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form', *PRELOAD],
     'encoder.hip': PRELOAD,
     'logmel.hip': PRELOAD,
 }

@@ -214,8 +214,20 @@ __global__ void __launch_bounds__(256) kv_q4_read_kernel(Q4Rows out, const int64
 }
 
 // ------------------------------------------------------------------------------------------
-// Single-token attention: block = (sequence, query head), 4 waves; a wave takes a key at a time, lanes hold
-// D / 64 dims each. The fresh row of the head is written first by the block itself.
+// Single-token attention. An item is a sequence, a key/value head and up to 16 of the query heads that read it;
+// S^T = K Q^T and O^T = V^T P^T are MFMAs of 16 keys or head dims by 16 query heads, so grouped heads share
+// every row that is read and dequantised. A wave takes 32 keys at a time, four waves a unit of 128 keys.
+//  - The scores' rows are assigned to keys so that lane group g = lane / 16 ends with the scores of keys
+//    8 g .. 8 g + 7 for query head lane % 16: row i of the first 16 is key 8 (i / 4) + i % 4, of the second 4
+//    more. These are the keys of one 16-byte unit of V, which the lane loads as the PV operand's source, so
+//    neither scores nor values cross lanes.
+//  - Codes become fp16 by or-ing them into 1024's mantissa (1024 + c), subtracting 1024, and one packed fma with
+//    step and low, which rounds once as the cache's definition does. Q's dims are permuted to the order in
+//    which masking a dword's nibbles yields pairs (0 4, 1 5, 2 6, 3 7).
+//  - The running maximum only moves when a score passes it by 2^kSlack (log2 units); weights stay within fp16.
+// Work is shared out on the device, since only it knows the lengths: all units of all items in a row, each block
+// an equal run of them. A block that covers an item finishes it; the others leave (m, l, O) in the workspace
+// for the combine launch.
 // ------------------------------------------------------------------------------------------
 struct Q4Attn {
   const void* q;
@@ -226,7 +238,17 @@ struct Q4Attn {
   Q4Cache c;
   int heads;  // query heads
   float scale;
+  float* ws;  // ws_acc [2 blocks][16][D], then ws_ml [2 blocks][16][2]
+  int blocks;  // of the split launch
 };
+
+constexpr int kUnitKeys = 128;  // keys of a unit: a 32-key tile for each of 4 waves
+constexpr int kTileKeys = 32;
+constexpr int kCols = 16;       // query heads of an item
+constexpr int kDirectKeys = 512;    // longest cache of a block an item
+constexpr int kSplitBlocks = 1024;  // of the shared-out form: 4 a CU
+constexpr float kSlack = 8.f;
+constexpr float kLog2e = 1.4426950408889634f;
 
 // Row `row` of a head from its fresh values: waves 0 and 1 write K and V, lane = dims {lane, lane + 64}.
 template <class T, int D>
@@ -271,56 +293,444 @@ __device__ __forceinline__ int q4_keys(const Q4Attn& a, int seq, int& fresh_row)
   return fresh_row + 1;
 }
 
+// A tile's data as loaded: K codes and meta of the lane's two keys, V codes and meta of its 8 keys.
+template <int D>
+struct Q4Tile {
+  uint32_t k[2][D / 32];
+  h2v km[2];
+  u32x4 v[D / 64];
+  h8v vs[D / 64], vl[D / 64];
+};
+
+// Where a lane's data of the item's first tile lie; a tile later is kTileKeys rows on.
+struct Q4Base {
+  const uint8_t *k, *v;
+  const _Float16 *km, *vm;
+};
+
+template <int D>
+__device__ __forceinline__ Q4Base q4_base(const Q4Cache& c, int64_t hr, int lane) {
+  const int i = lane & 15, g = lane >> 4;
+  const int64_t row = hr + 8 * (i >> 2) + (i & 3), block = hr / 8 + g;
+  return Q4Base{c.k_codes + row * (D / 2) + g * (D / 8), c.v_codes + (block * (D / 4) + i) * 16,
+                c.k_meta + (row * (D / 32) + g * (D / 32) / 4) * 2, c.v_meta + (block * (D / 32) + i / 8) * 16};
+}
+
+template <int D>
+__device__ __forceinline__ void q4_load(const Q4Base& b, int tile, Q4Tile<D>& t) {
+  const int64_t row = static_cast<int64_t>(tile) * kTileKeys;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const uint8_t* k = b.k + (row + 4 * s) * (D / 2);
+    if constexpr (D == 128) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(k);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) t.k[s][j] = x[j];
+    } else {
+      const uint2 x = *reinterpret_cast<const uint2*>(k);
+      t.k[s][0] = x.x;
+      t.k[s][1] = x.y;
+    }
+    t.km[s] = *reinterpret_cast<const h2v*>(b.km + (row + 4 * s) * (D / 32) * 2);
+  }
+#pragma unroll
+  for (int h = 0; h < D / 64; ++h) {
+    t.v[h] = *reinterpret_cast<const u32x4*>(b.v + (row / 8 * (D / 4) + 16 * h) * 16);
+    const h8v* m = reinterpret_cast<const h8v*>(b.vm + (row / 8 * (D / 32) + 2 * h) * 16);
+    t.vs[h] = m[0];
+    t.vl[h] = m[1];
+  }
+}
+
+// Nibble j of both halves of u as fp16, then low + step c.
+__device__ __forceinline__ h2v q4_pair(uint32_t u, int j, h2v step, h2v low) {
+  const uint32_t bits = ((u >> (4 * j)) & 0x000F000Fu) | 0x64006400u;
+  const h2v c = __builtin_bit_cast(h2v, bits) - static_cast<_Float16>(1024.f);
+  return __builtin_elementwise_fma(c, step, low);
+}
+
+template <int D>
+struct Q4State {
+  f4v o[D / 64][4];  // O^T: [64-dim half][dim % 4], lane (h, g), register r: dim 16 g + 4 r + dim % 4
+  float m, l;        // l: this lane's keys only
+};
+
+template <int D, bool kTail>
+__device__ __forceinline__ void q4_tile(const Q4Tile<D>& t, const h8v (&q)[D / 32], float factor, int left, int lane,
+                                        Q4State<D>& st) {
+  const int g = lane >> 4;
+  f4v s[2];
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt) {
+    s[kt] = f4v{0.f, 0.f, 0.f, 0.f};
+    const h2v step = h2v{t.km[kt][0], t.km[kt][0]}, low = h2v{t.km[kt][1], t.km[kt][1]};
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+      h8v k;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const h2v x = q4_pair(t.k[kt][j], e, step, low);
+        k[2 * e] = x[0];
+        k[2 * e + 1] = x[1];
+      }
+      s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[j], s[kt], 0, 0, 0);
+    }
+  }
+  float top = -INFINITY;
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if constexpr (kTail) {
+        if (8 * g + 4 * kt + r >= left) s[kt][r] = -INFINITY;
+      }
+      top = fmaxf(top, s[kt][r]);
+    }
+  top = xor_max<32>(xor_max<16>(top)) * factor;
+  if (__builtin_amdgcn_ballot_w64(top > st.m + kSlack)) {
+    const float m_new = fmaxf(st.m, top), corr = __builtin_amdgcn_exp2f(st.m - m_new);
+    st.l *= corr;
+#pragma unroll
+    for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) st.o[h][j] *= corr;
+    st.m = m_new;
+  }
+  h8v p;
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+    for (int r = 0; r < 4; r += 2) {
+      h2v x;
+      x[0] = f2h(__builtin_amdgcn_exp2f(fmaf(s[kt][r], factor, -st.m)));
+      x[1] = f2h(__builtin_amdgcn_exp2f(fmaf(s[kt][r + 1], factor, -st.m)));
+      st.l = __builtin_amdgcn_fdot2(x, h2v{static_cast<_Float16>(1.f), static_cast<_Float16>(1.f)}, st.l, false);
+      p[4 * kt + r] = x[0];
+      p[4 * kt + r + 1] = x[1];
+    }
+#pragma unroll
+  for (int h = 0; h < D / 64; ++h) {
+    h8v vs = t.vs[h], vl = t.vl[h];
+    if constexpr (kTail) {  // whatever the rows past the end hold, their values count as zeros
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (8 * g + e >= left) vs[e] = vl[e] = static_cast<_Float16>(0.f);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      h8v v;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const h2v x = q4_pair(t.v[h][w], j, h2v{vs[2 * w], vs[2 * w + 1]}, h2v{vl[2 * w], vl[2 * w + 1]});
+        v[2 * w] = x[0];
+        v[2 * w + 1] = x[1];
+      }
+      st.o[h][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p, st.o[h][j], 0, 0, 0);
+    }
+  }
+}
+
+// The item's queries as the products' operand, lane (h, g): dims D / 4 g + 8 j .. in the order of q4_pair's
+// pairs, and the factor from raw scores to log2 units. A bf16 query is scaled by a power of two to fit fp16 (its
+// elements 2^-24 of the largest and less lose bits); the factor undoes it. A negative scale negates the query,
+// a zero one becomes so small that scores vanish.
 template <class T, int D>
-__global__ void __launch_bounds__(256) decode_attention_q4_kernel(Q4Attn a) {
-  constexpr int kPer = D / 64;
-  __shared__ float sm[4], sl[4], sacc[4][D];
-  const int seq = blockIdx.y, head = blockIdx.x, kvh = head / (a.heads / a.c.heads);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__device__ __forceinline__ float q4_queries(const Q4Attn& a, int seq, int head, bool live, int lane, h8v (&q)[D / 32]) {
+  const int g = lane >> 4;
+  float f[D / 32][8], big = 0.f;
+  const T* src = static_cast<const T*>(a.q) + seq * a.q_row + head * a.q_head + D / 4 * g;
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) {
+    typename Vec8<T>::type x = {};
+    if (live) x = *reinterpret_cast<const typename Vec8<T>::type*>(src + 8 * j);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      f[j][e] = a.scale < 0.f ? -static_cast<float>(x[e]) : static_cast<float>(x[e]);
+      big = fmaxf(big, __builtin_fabsf(f[j][e]));
+    }
+  }
+  float factor = fmaxf(__builtin_fabsf(a.scale) * kLog2e, 1e-30f);
+  if constexpr (!__is_same(T, _Float16)) {
+    big = xor_max<32>(xor_max<16>(big));
+    const int ex = big < INFINITY ? __builtin_amdgcn_frexp_expf(big) : 0;
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[j][e] = __builtin_amdgcn_ldexpf(f[j][e], -ex);
+    factor = __builtin_amdgcn_ldexpf(factor, ex);
+  }
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      q[j][2 * e] = f2h(f[j][e]);
+      q[j][2 * e + 1] = f2h(f[j][e + 4]);
+    }
+  return factor;
+}
+
+// Tiles first, first + step, ... below `end` of an item whose keys end in tile keys / 32, the next one's data
+// requested while a tile is worked on.
+template <int D>
+__device__ __forceinline__ void q4_tiles(const Q4Base& b, int first, int step, int end, int keys, const h8v (&q)[D / 32],
+                                         float factor, int lane, Q4State<D>& st) {
+#pragma unroll
+  for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) st.o[h][j] = f4v{0.f, 0.f, 0.f, 0.f};
+  st.m = -INFINITY;
+  st.l = 0.f;
+  const int tiles = min(end, (keys + kTileKeys - 1) / kTileKeys);
+  if (first >= tiles) return;
+  Q4Tile<D> now, next;
+  q4_load<D>(b, first, now);
+  int t = first;
+  for (; t + step < tiles; t += step) {
+    q4_load<D>(b, t + step, next);
+    q4_tile<D, false>(now, q, factor, 0, lane, st);  // only the last tile may be partial
+    now = next;
+  }
+  const int left = keys - t * kTileKeys;
+  if (left >= kTileKeys) q4_tile<D, false>(now, q, factor, 0, lane, st);
+  else q4_tile<D, true>(now, q, factor, left, lane, st);
+}
+
+// Where the waves' results of an item meet; `cols` query heads of it.
+template <int D>
+struct Q4Merge {
+  static constexpr int kPitch = D + 4;  // 16 lanes' rows on different banks
+  float *acc, *m, *l;                   // [waves][cols][kPitch], [waves][16], [waves][16]
+  __device__ Q4Merge(float* lds, int waves, int cols) : acc(lds + 2 * waves * kCols), m(lds), l(lds + waves * kCols) {}
+  static constexpr int bytes(int waves, int cols) { return 4 * waves * (2 * kCols + cols * kPitch); }
+};
+
+template <int D>
+__device__ __forceinline__ void q4_hand_in(const Q4Merge<D>& x, const Q4State<D>& st, int wave, int cols, int lane) {
+  const int h = lane & 15, g = lane >> 4;
+  const float l = xor_add<32>(xor_add<16>(st.l));
+  if (h >= cols) return;
+  if (g == 0) {
+    x.m[wave * kCols + h] = st.m;
+    x.l[wave * kCols + h] = l;
+  }
+  float* to = x.acc + (wave * cols + h) * Q4Merge<D>::kPitch + 16 * g;
+#pragma unroll
+  for (int half = 0; half < D / 64; ++half)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      *reinterpret_cast<f4v*>(to + 64 * half + 4 * r) =
+          f4v{st.o[half][0][r], st.o[half][1][r], st.o[half][2][r], st.o[half][3][r]};
+}
+
+// The sum over the waves for query head h and dim d: (m, l, o) with o, l relative to exp2(m).
+template <int D>
+__device__ __forceinline__ float q4_sum(const Q4Merge<D>& x, int waves, int cols, int h, int d, float& m, float& l) {
+  m = -INFINITY;
+  for (int w = 0; w < waves; ++w) m = fmaxf(m, x.m[w * kCols + h]);
+  float o = 0.f;
+  l = 0.f;
+  for (int w = 0; w < waves; ++w) {
+    const float mw = x.m[w * kCols + h], e = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - m);
+    l = fmaf(e, x.l[w * kCols + h], l);
+    o = fmaf(e, x.acc[(w * cols + h) * Q4Merge<D>::kPitch + d], o);
+  }
+  return o;
+}
+
+// An item's place: query heads [head, head + cols) of key/value head kvh.
+struct Q4Item {
+  int kvh, head, cols;
+};
+__device__ __forceinline__ Q4Item q4_item(const Q4Attn& a, int item) {
+  const int group = a.heads / a.c.heads, parts = (group + kCols - 1) / kCols;
+  const int kvh = item / parts, first = item % parts * kCols;
+  return Q4Item{kvh, kvh * group + first, min(kCols, group - first)};
+}
+
+template <class T>
+__device__ __forceinline__ void q4_store(const Q4Attn& a, int seq, int head, int d, float o, float l) {
+  static_cast<T*>(a.out)[seq * a.o_row + head * a.o_head + d] = static_cast<T>(l > 0.f ? o / l : 0.f);
+}
+
+// A block an item, for caches so short that no item is worth sharing out.
+template <class T, int D>
+__global__ void __launch_bounds__(512) q4_direct_kernel(Q4Attn a) {
+  extern __shared__ float lds[];
+  const int seq = blockIdx.y, waves = blockDim.x / 64;
+  const Q4Item it = q4_item(a, blockIdx.x);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int fresh;
   const int keys = q4_keys(a, seq, fresh);
   if (fresh >= 0) {
-    q4_write_row<T, D>(a, seq, kvh, fresh, wave, lane);
+    q4_write_row<T, D>(a, seq, it.kvh, fresh, wave, lane);
     __syncthreads();
   }
-  const int64_t hr = (static_cast<int64_t>(seq) * a.c.heads + kvh) * a.c.max_len;
-  float q[kPer], acc[kPer] = {}, m = -INFINITY, l = 0.f;
-  const T* qp = static_cast<const T*>(a.q) + seq * a.q_row + head * a.q_head;
-  for (int i = 0; i < kPer; ++i) q[i] = static_cast<float>(qp[lane + 64 * i]) * a.scale;
-  for (int t = wave; t < keys; t += 4) {
-    float s = 0.f, v[kPer];
-    for (int i = 0; i < kPer; ++i) {
-      const int d = lane + 64 * i, sh = 4 * (d & 1);
-      const _Float16* km = a.c.k_meta + ((hr + t) * (D / 32) + d / 32) * 2;
-      const float kc = static_cast<float>((a.c.k_codes[(hr + t) * (D / 2) + d / 2] >> sh) & 15);
-      s += q[i] * h2f(__builtin_fmaf16(static_cast<_Float16>(kc), km[0], km[1]));
-      const int64_t block = hr / 8 + t / 8;
-      const _Float16* vm = a.c.v_meta + (block * (D / 32) + d / 32) * 16 + (t & 7);
-      const float vc = static_cast<float>((a.c.v_codes[(block * (D / 4) + d / 4) * 16 + 2 * (t & 7) + (d & 3) / 2] >> sh) & 15);
-      v[i] = h2f(__builtin_fmaf16(static_cast<_Float16>(vc), vm[0], vm[8]));
-    }
-    s = group_sum<64>(s);
-    const float m_new = fmaxf(m, s), corr = __expf(m - m_new), p = __expf(s - m_new);
-    l = l * corr + p;
-    for (int i = 0; i < kPer; ++i) acc[i] = acc[i] * corr + p * v[i];
-    m = m_new;
-  }
-  if (lane == 0) {
-    sm[wave] = m;
-    sl[wave] = l;
-  }
-  for (int i = 0; i < kPer; ++i) sacc[wave][lane + 64 * i] = acc[i];
+  h8v q[D / 32];
+  const bool live = (lane & 15) < it.cols;
+  const float factor = q4_queries<T, D>(a, seq, it.head + (lane & 15), live, lane, q);
+  const Q4Base base = q4_base<D>(a.c, (static_cast<int64_t>(seq) * a.c.heads + it.kvh) * a.c.max_len, lane);
+  Q4State<D> st;
+  q4_tiles<D>(base, wave, waves, a.c.max_len / kTileKeys, keys, q, factor, lane, st);
+  const Q4Merge<D> x(lds, waves, it.cols);
+  q4_hand_in<D>(x, st, wave, it.cols, lane);
   __syncthreads();
-  if (threadIdx.x >= D) return;
-  float top = -INFINITY, num = 0.f, den = 0.f;
-  for (int w = 0; w < 4; ++w) top = fmaxf(top, sm[w]);
-  for (int w = 0; w < 4; ++w) {
-    if (sl[w] == 0.f) continue;
-    const float e = __expf(sm[w] - top);
-    num += e * sacc[w][threadIdx.x];
-    den += e * sl[w];
+  for (int i = threadIdx.x; i < it.cols * D; i += blockDim.x) {
+    float m, l;
+    const float o = q4_sum<D>(x, waves, it.cols, i / D, i % D, m, l);
+    q4_store<T>(a, seq, it.head + i / D, i % D, o, l);
   }
-  static_cast<T*>(a.out)[seq * a.o_row + head * a.o_head + threadIdx.x] = static_cast<T>(den > 0.f ? num / den : 0.f);
+}
+
+// Units before sequence `seq` (of one item of each) and in all, found by whole waves.
+__device__ __forceinline__ int q4_units(const Q4Attn& a, int seq) {
+  int fresh;
+  return (q4_keys(a, seq, fresh) + kUnitKeys - 1) / kUnitKeys;
+}
+__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive sum over the wave
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const int x = __shfl_up(v, o);
+    if (lane >= o) v += x;
+  }
+  return v;
+}
+// Blocks that have work: each at least a unit, so that every block of an item's range leaves its part.
+__device__ __forceinline__ int q4_blocks(const Q4Attn& a, int64_t all) {
+  return static_cast<int>(min(all, static_cast<int64_t>(a.blocks)));
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(256) q4_split_kernel(Q4Attn a) {
+  extern __shared__ float lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = a.heads / a.c.heads, items = a.c.heads * ((group + kCols - 1) / kCols);
+  int total = 0;
+  for (int s0 = 0; s0 < a.c.n_seq; s0 += 64) {
+    const int u = s0 + lane < a.c.n_seq ? q4_units(a, s0 + lane) : 0;
+    total += __builtin_amdgcn_readlane(wave_scan(u, lane), 63);
+  }
+  const int64_t all = static_cast<int64_t>(total) * items;
+  const int blocks = q4_blocks(a, all);
+  if (static_cast<int>(blockIdx.x) >= blocks) return;
+  const int begin = static_cast<int>(all * blockIdx.x / blocks), end = static_cast<int>(all * (blockIdx.x + 1) / blocks);
+  // the sequence of the first unit
+  int seq = 0, before = 0, units = 0;
+  for (int s0 = 0, sum = 0; s0 < a.c.n_seq; s0 += 64) {
+    const int u = s0 + lane < a.c.n_seq ? q4_units(a, s0 + lane) : 0;
+    const int incl = wave_scan(u, lane) + sum;
+    const uint64_t past = __builtin_amdgcn_ballot_w64(static_cast<int64_t>(incl) * items > begin);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      seq = s0 + at;
+      units = __builtin_amdgcn_readlane(u, at);
+      before = __builtin_amdgcn_readlane(incl, at) - units;
+      break;
+    }
+    sum = __builtin_amdgcn_readlane(incl, 63);
+  }
+  for (int u = begin; u < end;) {
+    const int local = u - before * items, item = local / units, from = local % units;
+    const int to = min(units, from + end - u);  // this block's units of the item
+    const Q4Item it = q4_item(a, item);
+    int fresh;
+    const int keys = q4_keys(a, seq, fresh);
+    if (fresh >= 0 && to == units) {
+      q4_write_row<T, D>(a, seq, it.kvh, fresh, wave, lane);
+      __syncthreads();
+    }
+    h8v q[D / 32];
+    const float factor = q4_queries<T, D>(a, seq, it.head + (lane & 15), (lane & 15) < it.cols, lane, q);
+    const Q4Base base = q4_base<D>(a.c, (static_cast<int64_t>(seq) * a.c.heads + it.kvh) * a.c.max_len, lane);
+    Q4State<D> st;
+    q4_tiles<D>(base, from * (kUnitKeys / kTileKeys) + wave, 4, to * (kUnitKeys / kTileKeys), keys, q, factor, lane, st);
+    const Q4Merge<D> x(lds, 4, it.cols);
+    q4_hand_in<D>(x, st, wave, it.cols, lane);
+    __syncthreads();
+    const bool whole = from == 0 && to == units;
+    const int slot = 2 * blockIdx.x + (u == begin ? 0 : 1);
+    float* acc = a.ws + static_cast<int64_t>(slot) * kCols * D;
+    float* ml = a.ws + (static_cast<int64_t>(2 * a.blocks) * D + 2 * slot) * kCols;
+    for (int i = threadIdx.x; i < it.cols * D; i += 256) {
+      float m, l;
+      const int h = i / D, d = i % D;
+      const float o = q4_sum<D>(x, 4, it.cols, h, d, m, l);
+      if (whole) {
+        q4_store<T>(a, seq, it.head + h, d, o, l);
+      } else {
+        acc[i] = o;
+        if (d == 0) {
+          ml[2 * h] = m;
+          ml[2 * h + 1] = l;
+        }
+      }
+    }
+    u += to - from;
+    if (u < end) {
+      __syncthreads();  // the merge buffer is free again
+      if (u == (before + units) * items) {  // on to the next sequence that has units
+        before += units;
+        do units = q4_units(a, ++seq);
+        while (units == 0);
+      }
+    }
+  }
+}
+
+// Block = (query head, sequence): the parts of an item that several blocks worked on, or the zeros of a sequence
+// without keys.
+template <class T, int D>
+__global__ void __launch_bounds__(256) q4_combine_kernel(Q4Attn a) {
+  constexpr int kLanes = 256 / D;
+  __shared__ float weight[1024], red[4], part[kLanes][D];
+  const int seq = blockIdx.y, head = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int group = a.heads / a.c.heads, parts = (group + kCols - 1) / kCols, items = a.c.heads * parts;
+  const int in_group = head % group, item = head / group * parts + in_group / kCols, h = in_group % kCols;
+  int total = 0, before = 0;
+  for (int s0 = 0; s0 < a.c.n_seq; s0 += 64) {
+    const int u = s0 + lane < a.c.n_seq ? q4_units(a, s0 + lane) : 0;
+    total += __builtin_amdgcn_readlane(wave_scan(u, lane), 63);
+    before += __builtin_amdgcn_readlane(wave_scan(s0 + lane < seq ? u : 0, lane), 63);
+  }
+  const int units = q4_units(a, seq);
+  if (units == 0) {
+    if (tid < D) q4_store<T>(a, seq, head, tid, 0.f, 0.f);
+    return;
+  }
+  // block b has the units all b / blocks ..: the blocks of the item's first and last unit
+  const int64_t all = static_cast<int64_t>(total) * items, u0 = static_cast<int64_t>(before) * items + static_cast<int64_t>(item) * units;
+  const int blocks = q4_blocks(a, all);
+  const int b0 = static_cast<int>(((u0 + 1) * blocks - 1) / all), b1 = static_cast<int>(((u0 + units) * blocks - 1) / all);
+  if (b0 == b1) return;  // that block finished it
+  const float* ml = a.ws + static_cast<int64_t>(2 * a.blocks) * D * kCols;
+  const auto slot = [&](int b) {  // an item that begins before the block does is the block's first
+    return 2 * b + (all * b / blocks >= u0 ? 0 : 1);
+  };
+  const int n = b1 - b0 + 1;
+  float m = -INFINITY;
+  for (int i = tid; i < n; i += 256) {
+    weight[i] = ml[(static_cast<int64_t>(slot(b0 + i)) * kCols + h) * 2];
+    m = fmaxf(m, weight[i]);
+  }
+  m = group_max<64>(m);
+  if (lane == 0) red[tid / 64] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  float l = 0.f;
+  for (int i = tid; i < n; i += 256) {
+    weight[i] = __builtin_amdgcn_exp2f(weight[i] - m);
+    l = fmaf(weight[i], ml[(static_cast<int64_t>(slot(b0 + i)) * kCols + h) * 2 + 1], l);
+  }
+  __syncthreads();
+  l = block_sum_once<256>(l, red);
+  const int d = tid % D, from = tid / D;
+  float o = 0.f;
+  for (int i = from; i < n; i += kLanes)
+    o = fmaf(weight[i], a.ws[(static_cast<int64_t>(slot(b0 + i)) * kCols + h) * D + d], o);
+  part[from][d] = o;
+  __syncthreads();
+  if (tid >= D) return;
+  for (int i = 1; i < kLanes; ++i) o += part[i][d];
+  q4_store<T>(a, seq, head, d, o, l);
 }
 
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
@@ -340,12 +750,12 @@ int check_cache(const char* what, const Q4Cache& c, int dim) {
 bool rows_ok(const void* p, int64_t row, int64_t head) { return aligned(p, 16) && row % 8 == 0 && head % 8 == 0; }
 
 // kernel<T, D> for a dtype and a head size.
-#define Q4_LAUNCH(kernel, dtype, dim, grid, block, stream, ...)                                           \
+#define Q4_LAUNCH(kernel, dtype, dim, grid, block, lds, stream, ...)                                      \
   do {                                                                                                    \
-    if ((dtype) == FW_F16 && (dim) == 64) hipLaunchKernelGGL((kernel<_Float16, 64>), grid, block, 0, stream, __VA_ARGS__); \
-    else if ((dtype) == FW_F16) hipLaunchKernelGGL((kernel<_Float16, 128>), grid, block, 0, stream, __VA_ARGS__);          \
-    else if ((dim) == 64) hipLaunchKernelGGL((kernel<__bf16, 64>), grid, block, 0, stream, __VA_ARGS__);  \
-    else hipLaunchKernelGGL((kernel<__bf16, 128>), grid, block, 0, stream, __VA_ARGS__);                  \
+    if ((dtype) == FW_F16 && (dim) == 64) hipLaunchKernelGGL((kernel<_Float16, 64>), grid, block, lds, stream, __VA_ARGS__); \
+    else if ((dtype) == FW_F16) hipLaunchKernelGGL((kernel<_Float16, 128>), grid, block, lds, stream, __VA_ARGS__);          \
+    else if ((dim) == 64) hipLaunchKernelGGL((kernel<__bf16, 64>), grid, block, lds, stream, __VA_ARGS__);  \
+    else hipLaunchKernelGGL((kernel<__bf16, 128>), grid, block, lds, stream, __VA_ARGS__);                  \
   } while (0)
 
 int check_packed(const char* what, const Q4Rows& r, const int64_t* cu, const int64_t* pos, int64_t rows, const Q4Cache& c,
@@ -377,7 +787,7 @@ extern "C" int fw_kv_q4_append(const void* k, int64_t k_row, int64_t k_head, con
   if (const int rc = check_packed("kv_q4_append", r, cu, pos, rows, c, head_dim, dtype)) return rc;
   if (rows == 0) return FW_OK;
   const int64_t slots = rows / 8 + 2 * static_cast<int64_t>(n_seq), units = slots * kv_heads * (head_dim / 64);
-  Q4_LAUNCH(kv_q4_append_kernel, dtype, head_dim, dim3(static_cast<unsigned>((units + 3) / 4)), dim3(256), stream, r, cu,
+  Q4_LAUNCH(kv_q4_append_kernel, dtype, head_dim, dim3(static_cast<unsigned>((units + 3) / 4)), dim3(256), 0, stream, r, cu,
             pos, rows, slots, c);
   return fw_check_launch("kv_q4_append");
 }
@@ -393,7 +803,7 @@ extern "C" int fw_kv_q4_read(const void* k_codes, const void* k_meta, const void
   if (const int rc = check_packed("kv_q4_read", r, cu, pos, rows, c, head_dim, dtype)) return rc;
   if (rows == 0) return FW_OK;
   const int64_t slots = rows / 8 + 2 * static_cast<int64_t>(n_seq), units = slots * kv_heads * (head_dim / 64);
-  Q4_LAUNCH(kv_q4_read_kernel, dtype, head_dim, dim3(static_cast<unsigned>((units + 3) / 4)), dim3(256), stream, r, cu,
+  Q4_LAUNCH(kv_q4_read_kernel, dtype, head_dim, dim3(static_cast<unsigned>((units + 3) / 4)), dim3(256), 0, stream, r, cu,
             pos, rows, slots, c);
   return fw_check_launch("kv_q4_read");
 }
@@ -402,7 +812,7 @@ extern "C" int64_t fw_decode_attention_q4_ws_floats(int n_seq, int heads, int kv
   if (n_seq <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_len <= 0 || max_len % 32 ||
       (head_dim != 64 && head_dim != 128))
     return 0;
-  return 4;
+  return static_cast<int64_t>(2 * kSplitBlocks) * kCols * (head_dim + 2);
 }
 
 extern "C" int fw_decode_attention_q4(const void* q, int64_t q_row, int64_t q_head, void* k_codes, void* k_meta,
@@ -423,7 +833,22 @@ extern "C" int fw_decode_attention_q4(const void* q, int64_t q_row, int64_t q_he
   const int64_t need = fw_decode_attention_q4_ws_floats(n_seq, heads, kv_heads, max_len, head_dim);
   if (!ws || ws_floats < need || !aligned(ws, 16))
     return fw_fail(FW_EINVAL, "decode_attention_q4: workspace needs %lld floats, 16-byte aligned", static_cast<long long>(need));
-  const Q4Attn a{q, out, q_row, q_head, o_row, o_head, Q4Rows{k_new, v_new, k_row, k_head, v_row, v_head}, lens, c, heads, scale};
-  Q4_LAUNCH(decode_attention_q4_kernel, dtype, head_dim, dim3(heads, n_seq), dim3(256), stream, a);
-  return fw_check_launch("decode_attention_q4");
+  const int cols = min(kCols, heads / kv_heads), items = kv_heads * ((heads / kv_heads + kCols - 1) / kCols);
+  if (n_seq > 65535 || static_cast<int64_t>(n_seq) * items * ((max_len + kUnitKeys - 1) / kUnitKeys) > 0x7FFFFFFF)
+    return fw_fail(FW_EINVAL, "decode_attention_q4: too many sequences");
+  Q4Attn a{q, out, q_row, q_head, o_row, o_head, Q4Rows{k_new, v_new, k_row, k_head, v_row, v_head}, lens, c, heads, scale, ws, 0};
+  const auto lds = [&](int waves) {
+    return head_dim == 64 ? Q4Merge<64>::bytes(waves, cols) : Q4Merge<128>::bytes(waves, cols);
+  };
+  if (max_len <= kDirectKeys) {
+    // 8 waves, 4 where the merge of so many heads would pass 64 KB
+    const int waves = min(max_len / kTileKeys, lds(8) <= 65536 ? 8 : 4);
+    Q4_LAUNCH(q4_direct_kernel, dtype, head_dim, dim3(items, n_seq), dim3(64 * waves), lds(waves), stream, a);
+    return fw_check_launch("decode_attention_q4");
+  }
+  a.blocks = kSplitBlocks;
+  Q4_LAUNCH(q4_split_kernel, dtype, head_dim, dim3(kSplitBlocks), dim3(256), lds(4), stream, a);
+  if (const int rc = fw_check_launch("decode_attention_q4")) return rc;
+  Q4_LAUNCH(q4_combine_kernel, dtype, head_dim, dim3(heads, n_seq), dim3(256), 0, stream, a);
+  return fw_check_launch("decode_attention_q4 combine");
 }

@@ -245,41 +245,16 @@ struct Q4Attn {
 constexpr int kUnitKeys = 128;  // keys of a unit: a 32-key tile for each of 4 waves
 constexpr int kTileKeys = 32;
 constexpr int kCols = 16;       // query heads of an item
-constexpr int kDirectKeys = 512;    // longest cache of a block an item
-constexpr int kSplitBlocks = 1024;  // of the shared-out form: 4 a CU
+#ifndef Q4_DK
+#define Q4_DK 512
+#endif
+constexpr int kDirectKeys = Q4_DK;    // longest cache of a block an item
+#ifndef Q4_B
+#define Q4_B 1024
+#endif
+constexpr int kSplitBlocks = Q4_B;  // of the shared-out form: 4 a CU
 constexpr float kSlack = 8.f;
 constexpr float kLog2e = 1.4426950408889634f;
-
-// Row `row` of a head from its fresh values: waves 0 and 1 write K and V, lane = dims {lane, lane + 64}.
-template <class T, int D>
-__device__ __forceinline__ void q4_write_row(const Q4Attn& a, int seq, int kvh, int row, int wave, int lane) {
-  if (wave > 1) return;
-  const Q4Cache& c = a.c;
-  const int64_t hr = (static_cast<int64_t>(seq) * c.heads + kvh) * c.max_len;
-  const T* src = wave == 0 ? static_cast<const T*>(a.fresh.k) + seq * a.fresh.k_row + kvh * a.fresh.k_head
-                           : static_cast<const T*>(a.fresh.v) + seq * a.fresh.v_row + kvh * a.fresh.v_head;
-#pragma unroll
-  for (int h = 0; h < D / 64; ++h) {
-    const int d = 64 * h + 8 * (lane & 7);  // every 8 lanes do the same; the first 8 store
-    _Float16 step, low;
-    const uint32_t codes = q4_pack8<T>(*reinterpret_cast<const typename Vec8<T>::type*>(src + d), step, low);
-    if (lane >= 8) continue;
-    if (wave == 0) {
-      *reinterpret_cast<uint32_t*>(c.k_codes + (hr + row) * (D / 2) + d / 2) = codes;
-      if ((lane & 3) == 0) *reinterpret_cast<h2v*>(c.k_meta + ((hr + row) * (D / 32) + d / 32) * 2) = h2v{step, low};
-    } else {
-      const int64_t block = hr / 8 + row / 8;
-      uint8_t* vu = c.v_codes + (block * (D / 4) + d / 4) * 16 + 2 * (row & 7);
-      *reinterpret_cast<u16*>(vu) = static_cast<u16>(codes);
-      *reinterpret_cast<u16*>(vu + 16) = static_cast<u16>(codes >> 16);
-      if ((lane & 3) == 0) {
-        _Float16* vm = c.v_meta + (block * (D / 32) + d / 32) * 16 + (row & 7);
-        vm[0] = step;
-        vm[8] = low;
-      }
-    }
-  }
-}
 
 // Cached keys of a sequence, and the row that a fresh token goes to (-1: none). A negative length is an idle
 // sequence; a full cache has its last row overwritten, as the position of the batch-1 decoder stays at its
@@ -339,6 +314,66 @@ __device__ __forceinline__ void q4_load(const Q4Base& b, int tile, Q4Tile<D>& t)
     const h8v* m = reinterpret_cast<const h8v*>(b.vm + (row / 8 * (D / 32) + 2 * h) * 16);
     t.vs[h] = m[0];
     t.vl[h] = m[1];
+  }
+}
+
+// The fresh row of a head, quantised by the wave that has its tile: lanes 0 .. D / 8 - 1 take 8 dims of K each, lanes
+// 32 .. 32 + D / 8 - 1 of V. They write it to the cache, and the lanes that hold its place in the tile take it over
+// from them: nobody waits for the store, or reads it back.
+template <class T, int D>
+__device__ __forceinline__ void q4_fresh(const Q4Attn& a, int seq, int kvh, int64_t hr, int row, int lane, Q4Tile<D>& t) {
+  const Q4Cache& c = a.c;
+  const int d = 8 * (lane & (D / 8 - 1)), i = lane & 15, g = lane >> 4;
+  const T* src = lane < 32 ? static_cast<const T*>(a.fresh.k) + seq * a.fresh.k_row + kvh * a.fresh.k_head
+                           : static_cast<const T*>(a.fresh.v) + seq * a.fresh.v_row + kvh * a.fresh.v_head;
+  _Float16 step, low;
+  const uint32_t codes = q4_pack8<T>(*reinterpret_cast<const typename Vec8<T>::type*>(src + d), step, low);
+  const h2v meta{step, low};
+  if ((lane & 31) < D / 8) {
+    if (lane < 32) {
+      *reinterpret_cast<uint32_t*>(c.k_codes + (hr + row) * (D / 2) + d / 2) = codes;
+      if ((lane & 3) == 0) *reinterpret_cast<h2v*>(c.k_meta + ((hr + row) * (D / 32) + d / 32) * 2) = meta;
+    } else {
+      const int64_t block = hr / 8 + row / 8;
+      uint8_t* vu = c.v_codes + (block * (D / 4) + d / 4) * 16 + 2 * (row & 7);
+      *reinterpret_cast<u16*>(vu) = static_cast<u16>(codes);
+      *reinterpret_cast<u16*>(vu + 16) = static_cast<u16>(codes >> 16);
+      if ((lane & 3) == 0) {
+        _Float16* vm = c.v_meta + (block * (D / 32) + d / 32) * 16 + (row & 7);
+        vm[0] = step;
+        vm[8] = low;
+      }
+    }
+  }
+  const int at = row & (kTileKeys - 1), in_group = at & 7;  // of lane group at / 8; of its 8 keys
+  const int word = __builtin_bit_cast(int, meta);
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {  // K: lane i holds key 8 (i / 4) + 4 s + i % 4
+    const bool mine = 8 * (i >> 2) + 4 * s + (i & 3) == at;
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+      const uint32_t x = __shfl(static_cast<int>(codes), D / 32 * g + j);
+      t.k[s][j] = mine ? x : t.k[s][j];
+    }
+    const int m = __shfl(word, 4 * (g * (D / 32) / 4));
+    if (mine) t.km[s] = __builtin_bit_cast(h2v, m);
+  }
+#pragma unroll
+  for (int h = 0; h < D / 64; ++h) {  // V: lane group g holds keys 8 g .., lane i dims 4 i .. of each half
+    const uint32_t x = static_cast<uint32_t>(__shfl(static_cast<int>(codes), 32 + 8 * h + i / 2)) >> (16 * (i & 1));
+    const h2v m = __builtin_bit_cast(h2v, __shfl(word, 32 + 8 * h + 4 * (i / 8)));
+    const bool mine = g == at / 8;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (mine && in_group == 2 * w) t.v[h][w] = (t.v[h][w] & 0xFFFF0000u) | (x & 0xFFFFu);
+      if (mine && in_group == 2 * w + 1) t.v[h][w] = (t.v[h][w] & 0xFFFFu) | x << 16;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (mine && in_group == e) {
+        t.vs[h][e] = m[0];
+        t.vl[h][e] = m[1];
+      }
   }
 }
 
@@ -469,30 +504,31 @@ __device__ __forceinline__ float q4_queries(const Q4Attn& a, int seq, int head, 
   return factor;
 }
 
-// Tiles first, first + step, ... below `end` of an item whose keys end in tile keys / 32, the next one's data
-// requested while a tile is worked on.
-template <int D>
-__device__ __forceinline__ void q4_tiles(const Q4Base& b, int first, int step, int end, int keys, const h8v (&q)[D / 32],
-                                         float factor, int lane, Q4State<D>& st) {
+// Tiles first, first + step, ... below `end` of an item with `keys` keys; fresh: the row that is written now, or -1.
+template <class T, int D>
+__device__ __forceinline__ void q4_tiles(const Q4Attn& a, int seq, int kvh, int first, int step, int end, int keys, int fresh,
+                                         const h8v (&q)[D / 32], float factor, int lane, Q4State<D>& st) {
 #pragma unroll
   for (int h = 0; h < D / 64; ++h)
 #pragma unroll
     for (int j = 0; j < 4; ++j) st.o[h][j] = f4v{0.f, 0.f, 0.f, 0.f};
   st.m = -INFINITY;
   st.l = 0.f;
-  const int tiles = min(end, (keys + kTileKeys - 1) / kTileKeys);
-  if (first >= tiles) return;
-  Q4Tile<D> now, next;
-  q4_load<D>(b, first, now);
+  const int64_t hr = (static_cast<int64_t>(seq) * a.c.heads + kvh) * a.c.max_len;
+  const Q4Base b = q4_base<D>(a.c, hr, lane);
+  const int full = min(end, keys / kTileKeys - (fresh >= 0 && keys % kTileKeys == 0));  // tiles without the fresh row or an end
   int t = first;
-  for (; t + step < tiles; t += step) {
-    q4_load<D>(b, t + step, next);
-    q4_tile<D, false>(now, q, factor, 0, lane, st);  // only the last tile may be partial
-    now = next;
+  for (; t < full; t += step) {
+    Q4Tile<D> x;
+    q4_load<D>(b, t, x);
+    q4_tile<D, false>(x, q, factor, 0, lane, st);
   }
-  const int left = keys - t * kTileKeys;
-  if (left >= kTileKeys) q4_tile<D, false>(now, q, factor, 0, lane, st);
-  else q4_tile<D, true>(now, q, factor, left, lane, st);
+  if (t < end && t * kTileKeys < keys) {
+    Q4Tile<D> x;
+    q4_load<D>(b, t, x);
+    if (fresh >= 0) q4_fresh<T, D>(a, seq, kvh, hr, fresh, lane, x);
+    q4_tile<D, true>(x, q, factor, keys - t * kTileKeys, lane, st);
+  }
 }
 
 // Where the waves' results of an item meet; `cols` query heads of it.
@@ -561,16 +597,11 @@ __global__ void __launch_bounds__(512) q4_direct_kernel(Q4Attn a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int fresh;
   const int keys = q4_keys(a, seq, fresh);
-  if (fresh >= 0) {
-    q4_write_row<T, D>(a, seq, it.kvh, fresh, wave, lane);
-    __syncthreads();
-  }
   h8v q[D / 32];
   const bool live = (lane & 15) < it.cols;
   const float factor = q4_queries<T, D>(a, seq, it.head + (lane & 15), live, lane, q);
-  const Q4Base base = q4_base<D>(a.c, (static_cast<int64_t>(seq) * a.c.heads + it.kvh) * a.c.max_len, lane);
   Q4State<D> st;
-  q4_tiles<D>(base, wave, waves, a.c.max_len / kTileKeys, keys, q, factor, lane, st);
+  q4_tiles<T, D>(a, seq, it.kvh, wave, waves, a.c.max_len / kTileKeys, keys, fresh, q, factor, lane, st);
   const Q4Merge<D> x(lds, waves, it.cols);
   q4_hand_in<D>(x, st, wave, it.cols, lane);
   __syncthreads();
@@ -581,11 +612,16 @@ __global__ void __launch_bounds__(512) q4_direct_kernel(Q4Attn a) {
   }
 }
 
-// Units before sequence `seq` (of one item of each) and in all, found by whole waves.
+// Units of one item of a sequence, and what it costs in units: an item that is begun costs kItemCost more.
+#ifndef Q4_COST
+#define Q4_COST 1
+#endif
+constexpr int kItemCost = Q4_COST;
 __device__ __forceinline__ int q4_units(const Q4Attn& a, int seq) {
   int fresh;
   return (q4_keys(a, seq, fresh) + kUnitKeys - 1) / kUnitKeys;
 }
+__device__ __forceinline__ int q4_cost(int units) { return units > 0 ? units + kItemCost : 0; }
 __device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive sum over the wave
 #pragma unroll
   for (int o = 1; o < 64; o *= 2) {
@@ -600,49 +636,52 @@ __device__ __forceinline__ int q4_blocks(const Q4Attn& a, int64_t all) {
 }
 
 template <class T, int D>
-__global__ void __launch_bounds__(256) q4_split_kernel(Q4Attn a) {
+__global__ void __launch_bounds__(256, 4) q4_split_kernel(Q4Attn a) {
   extern __shared__ float lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int group = a.heads / a.c.heads, items = a.c.heads * ((group + kCols - 1) / kCols);
   int total = 0;
   for (int s0 = 0; s0 < a.c.n_seq; s0 += 64) {
-    const int u = s0 + lane < a.c.n_seq ? q4_units(a, s0 + lane) : 0;
+    const int u = s0 + lane < a.c.n_seq ? q4_cost(q4_units(a, s0 + lane)) : 0;
     total += __builtin_amdgcn_readlane(wave_scan(u, lane), 63);
   }
   const int64_t all = static_cast<int64_t>(total) * items;
   const int blocks = q4_blocks(a, all);
   if (static_cast<int>(blockIdx.x) >= blocks) return;
   const int begin = static_cast<int>(all * blockIdx.x / blocks), end = static_cast<int>(all * (blockIdx.x + 1) / blocks);
-  // the sequence of the first unit
-  int seq = 0, before = 0, units = 0;
+  // the sequence of the first place
+  int seq = 0, before = 0, cost = 0;
   for (int s0 = 0, sum = 0; s0 < a.c.n_seq; s0 += 64) {
-    const int u = s0 + lane < a.c.n_seq ? q4_units(a, s0 + lane) : 0;
+    const int u = s0 + lane < a.c.n_seq ? q4_cost(q4_units(a, s0 + lane)) : 0;
     const int incl = wave_scan(u, lane) + sum;
     const uint64_t past = __builtin_amdgcn_ballot_w64(static_cast<int64_t>(incl) * items > begin);
     if (past) {
       const int at = __builtin_ctzll(past);
       seq = s0 + at;
-      units = __builtin_amdgcn_readlane(u, at);
-      before = __builtin_amdgcn_readlane(incl, at) - units;
+      cost = __builtin_amdgcn_readlane(u, at);
+      before = __builtin_amdgcn_readlane(incl, at) - cost;
       break;
     }
     sum = __builtin_amdgcn_readlane(incl, 63);
   }
   for (int u = begin; u < end;) {
-    const int local = u - before * items, item = local / units, from = local % units;
-    const int to = min(units, from + end - u);  // this block's units of the item
+    // Lane-dependent values are made anew for each item: kept across items they take some 50 registers
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & 63;
+    // the item's place: its kItemCost first places are its beginning, the others its units
+    const int local = u - before * items, item = local / cost, place = local % cost, units = cost - kItemCost;
+    const int from = max(place - kItemCost, 0), to = min(units, place + end - u - kItemCost);  // this block's units of it
+    const int next = u + cost - place;
+    if (to <= from) break;  // the run ends in the item's beginning
     const Q4Item it = q4_item(a, item);
     int fresh;
     const int keys = q4_keys(a, seq, fresh);
-    if (fresh >= 0 && to == units) {
-      q4_write_row<T, D>(a, seq, it.kvh, fresh, wave, lane);
-      __syncthreads();
-    }
     h8v q[D / 32];
     const float factor = q4_queries<T, D>(a, seq, it.head + (lane & 15), (lane & 15) < it.cols, lane, q);
-    const Q4Base base = q4_base<D>(a.c, (static_cast<int64_t>(seq) * a.c.heads + it.kvh) * a.c.max_len, lane);
     Q4State<D> st;
-    q4_tiles<D>(base, from * (kUnitKeys / kTileKeys) + wave, 4, to * (kUnitKeys / kTileKeys), keys, q, factor, lane, st);
+    q4_tiles<T, D>(a, seq, it.kvh, from * (kUnitKeys / kTileKeys) + wave, 4, to * (kUnitKeys / kTileKeys), keys, fresh, q, factor,
+                   lane, st);
     const Q4Merge<D> x(lds, 4, it.cols);
     q4_hand_in<D>(x, st, wave, it.cols, lane);
     __syncthreads();
@@ -650,7 +689,7 @@ __global__ void __launch_bounds__(256) q4_split_kernel(Q4Attn a) {
     const int slot = 2 * blockIdx.x + (u == begin ? 0 : 1);
     float* acc = a.ws + static_cast<int64_t>(slot) * kCols * D;
     float* ml = a.ws + (static_cast<int64_t>(2 * a.blocks) * D + 2 * slot) * kCols;
-    for (int i = threadIdx.x; i < it.cols * D; i += 256) {
+    for (int i = tid; i < it.cols * D; i += 256) {
       float m, l;
       const int h = i / D, d = i % D;
       const float o = q4_sum<D>(x, 4, it.cols, h, d, m, l);
@@ -664,30 +703,31 @@ __global__ void __launch_bounds__(256) q4_split_kernel(Q4Attn a) {
         }
       }
     }
-    u += to - from;
+    u = next;
     if (u < end) {
       __syncthreads();  // the merge buffer is free again
-      if (u == (before + units) * items) {  // on to the next sequence that has units
-        before += units;
-        do units = q4_units(a, ++seq);
-        while (units == 0);
+      if (u == (before + cost) * items) {  // on to the next sequence that has units
+        before += cost;
+        do cost = q4_cost(q4_units(a, ++seq));
+        while (cost == 0);
       }
     }
   }
 }
 
+constexpr int kCombine = 512;
 // Block = (query head, sequence): the parts of an item that several blocks worked on, or the zeros of a sequence
 // without keys.
 template <class T, int D>
-__global__ void __launch_bounds__(256) q4_combine_kernel(Q4Attn a) {
-  constexpr int kLanes = 256 / D;
-  __shared__ float weight[1024], red[4], part[kLanes][D];
+__global__ void __launch_bounds__(kCombine) q4_combine_kernel(Q4Attn a) {
+  constexpr int kLanes = kCombine / D;
+  __shared__ float weight[kSplitBlocks], red[kCombine / 64], part[kLanes][D];
   const int seq = blockIdx.y, head = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const int group = a.heads / a.c.heads, parts = (group + kCols - 1) / kCols, items = a.c.heads * parts;
   const int in_group = head % group, item = head / group * parts + in_group / kCols, h = in_group % kCols;
   int total = 0, before = 0;
   for (int s0 = 0; s0 < a.c.n_seq; s0 += 64) {
-    const int u = s0 + lane < a.c.n_seq ? q4_units(a, s0 + lane) : 0;
+    const int u = s0 + lane < a.c.n_seq ? q4_cost(q4_units(a, s0 + lane)) : 0;
     total += __builtin_amdgcn_readlane(wave_scan(u, lane), 63);
     before += __builtin_amdgcn_readlane(wave_scan(s0 + lane < seq ? u : 0, lane), 63);
   }
@@ -696,40 +736,52 @@ __global__ void __launch_bounds__(256) q4_combine_kernel(Q4Attn a) {
     if (tid < D) q4_store<T>(a, seq, head, tid, 0.f, 0.f);
     return;
   }
-  // block b has the units all b / blocks ..: the blocks of the item's first and last unit
-  const int64_t all = static_cast<int64_t>(total) * items, u0 = static_cast<int64_t>(before) * items + static_cast<int64_t>(item) * units;
+  // block b has the places all b / blocks ..: the blocks of the item's first and last unit
+  const int64_t all = static_cast<int64_t>(total) * items;
+  const int64_t u0 = static_cast<int64_t>(before) * items + static_cast<int64_t>(item) * q4_cost(units);
   const int blocks = q4_blocks(a, all);
-  const int b0 = static_cast<int>(((u0 + 1) * blocks - 1) / all), b1 = static_cast<int>(((u0 + units) * blocks - 1) / all);
+  const int b0 = static_cast<int>(((u0 + kItemCost + 1) * blocks - 1) / all);
+  const int b1 = static_cast<int>(((u0 + kItemCost + units) * blocks - 1) / all);
   if (b0 == b1) return;  // that block finished it
   const float* ml = a.ws + static_cast<int64_t>(2 * a.blocks) * D * kCols;
-  const auto slot = [&](int b) {  // an item that begins before the block does is the block's first
-    return 2 * b + (all * b / blocks >= u0 ? 0 : 1);
-  };
+  // the item is the first one of every block but b0, and of that one if it begins there
+  const int64_t first = 2 * static_cast<int64_t>(b0) + (all * b0 / blocks < u0);
+  const auto slot = [&](int i) { return i == 0 ? first : 2 * static_cast<int64_t>(b0 + i); };
   const int n = b1 - b0 + 1;
   float m = -INFINITY;
-  for (int i = tid; i < n; i += 256) {
-    weight[i] = ml[(static_cast<int64_t>(slot(b0 + i)) * kCols + h) * 2];
+  for (int i = tid; i < n; i += kCombine) {
+    weight[i] = ml[(slot(i) * kCols + h) * 2];
     m = fmaxf(m, weight[i]);
   }
   m = group_max<64>(m);
   if (lane == 0) red[tid / 64] = m;
   __syncthreads();
-  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+#pragma unroll
+  for (int i = 0; i < kCombine / 64; ++i) m = fmaxf(m, red[i]);
   float l = 0.f;
-  for (int i = tid; i < n; i += 256) {
+  for (int i = tid; i < n; i += kCombine) {
     weight[i] = __builtin_amdgcn_exp2f(weight[i] - m);
-    l = fmaf(weight[i], ml[(static_cast<int64_t>(slot(b0 + i)) * kCols + h) * 2 + 1], l);
+    l = fmaf(weight[i], ml[(slot(i) * kCols + h) * 2 + 1], l);
   }
   __syncthreads();
-  l = block_sum_once<256>(l, red);
+  l = block_sum_once<kCombine>(l, red);
   const int d = tid % D, from = tid / D;
+  const float* acc = a.ws + h * D + d;
   float o = 0.f;
-  for (int i = from; i < n; i += kLanes)
-    o = fmaf(weight[i], a.ws[(static_cast<int64_t>(slot(b0 + i)) * kCols + h) * D + d], o);
+  int i = from;
+  for (; i + 7 * kLanes < n; i += 8 * kLanes) {  // 8 loads in flight
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = acc[slot(i + j * kLanes) * kCols * D];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o = fmaf(weight[i + j * kLanes], x[j], o);
+  }
+  for (; i < n; i += kLanes) o = fmaf(weight[i], acc[slot(i) * kCols * D], o);
   part[from][d] = o;
   __syncthreads();
   if (tid >= D) return;
-  for (int i = 1; i < kLanes; ++i) o += part[i][d];
+#pragma unroll
+  for (int j = 1; j < kLanes; ++j) o += part[j][d];
   q4_store<T>(a, seq, head, d, o, l);
 }
 
@@ -834,7 +886,7 @@ extern "C" int fw_decode_attention_q4(const void* q, int64_t q_row, int64_t q_he
   if (!ws || ws_floats < need || !aligned(ws, 16))
     return fw_fail(FW_EINVAL, "decode_attention_q4: workspace needs %lld floats, 16-byte aligned", static_cast<long long>(need));
   const int cols = min(kCols, heads / kv_heads), items = kv_heads * ((heads / kv_heads + kCols - 1) / kCols);
-  if (n_seq > 65535 || static_cast<int64_t>(n_seq) * items * ((max_len + kUnitKeys - 1) / kUnitKeys) > 0x7FFFFFFF)
+  if (n_seq > 65535 || static_cast<int64_t>(n_seq) * items * ((max_len + kUnitKeys - 1) / kUnitKeys + kItemCost) > 0x7FFFFFFF)
     return fw_fail(FW_EINVAL, "decode_attention_q4: too many sequences");
   Q4Attn a{q, out, q_row, q_head, o_row, o_head, Q4Rows{k_new, v_new, k_row, k_head, v_row, v_head}, lens, c, heads, scale, ws, 0};
   const auto lds = [&](int waves) {
@@ -849,6 +901,6 @@ extern "C" int fw_decode_attention_q4(const void* q, int64_t q_row, int64_t q_he
   a.blocks = kSplitBlocks;
   Q4_LAUNCH(q4_split_kernel, dtype, head_dim, dim3(kSplitBlocks), dim3(256), lds(4), stream, a);
   if (const int rc = fw_check_launch("decode_attention_q4")) return rc;
-  Q4_LAUNCH(q4_combine_kernel, dtype, head_dim, dim3(heads, n_seq), dim3(256), 0, stream, a);
+  Q4_LAUNCH(q4_combine_kernel, dtype, head_dim, dim3(heads, n_seq), dim3(kCombine), 0, stream, a);
   return fw_check_launch("decode_attention_q4 combine");
 }

@@ -225,9 +225,9 @@ __global__ void __launch_bounds__(256) kv_q4_read_kernel(Q4Rows out, const int64
 //    step and low, which rounds once as the cache's definition does. Q's dims are permuted to the order in
 //    which masking a dword's nibbles yields pairs (0 4, 1 5, 2 6, 3 7).
 //  - The running maximum only moves when a score passes it by 2^kSlack (log2 units); weights stay within fp16.
-// Work is shared out on the device, since only it knows the lengths: all units of all items in a row, each block
-// an equal run of them. A block that covers an item finishes it; the others leave (m, l, O) in the workspace
-// for the combine launch.
+// A block takes a chunk of an item's keys; an item of one chunk is finished by its block, the chunks of a longer one
+// leave (m, l, O) in the workspace for the combine launch. Only the device knows the lengths: blocks without keys
+// end at once.
 // ------------------------------------------------------------------------------------------
 struct Q4Attn {
   const void* q;
@@ -238,21 +238,12 @@ struct Q4Attn {
   Q4Cache c;
   int heads;  // query heads
   float scale;
-  float* ws;  // ws_acc [2 blocks][16][D], then ws_ml [2 blocks][16][2]
-  int blocks;  // of the split launch
+  int chunk, chunks;  // keys of a chunk (a multiple of kTileKeys), chunks of a full cache
+  float* ws;          // O [n_seq][items][chunks][cols][D], then (m, l) [n_seq][items][chunks][cols][2]
 };
 
-constexpr int kUnitKeys = 128;  // keys of a unit: a 32-key tile for each of 4 waves
 constexpr int kTileKeys = 32;
-constexpr int kCols = 16;       // query heads of an item
-#ifndef Q4_DK
-#define Q4_DK 512
-#endif
-constexpr int kDirectKeys = Q4_DK;    // longest cache of a block an item
-#ifndef Q4_B
-#define Q4_B 1024
-#endif
-constexpr int kSplitBlocks = Q4_B;  // of the shared-out form: 4 a CU
+constexpr int kCols = 16;  // query heads of an item
 constexpr float kSlack = 8.f;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -292,7 +283,7 @@ __device__ __forceinline__ Q4Base q4_base(const Q4Cache& c, int64_t hr, int lane
 }
 
 template <int D>
-__device__ __forceinline__ void q4_load(const Q4Base& b, int tile, Q4Tile<D>& t) {
+__device__ __forceinline__ void q4_load_k(const Q4Base& b, int tile, Q4Tile<D>& t) {
   const int64_t row = static_cast<int64_t>(tile) * kTileKeys;
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
@@ -308,6 +299,10 @@ __device__ __forceinline__ void q4_load(const Q4Base& b, int tile, Q4Tile<D>& t)
     }
     t.km[s] = *reinterpret_cast<const h2v*>(b.km + (row + 4 * s) * (D / 32) * 2);
   }
+}
+template <int D>
+__device__ __forceinline__ void q4_load_v(const Q4Base& b, int tile, Q4Tile<D>& t) {
+  const int64_t row = static_cast<int64_t>(tile) * kTileKeys;
 #pragma unroll
   for (int h = 0; h < D / 64; ++h) {
     t.v[h] = *reinterpret_cast<const u32x4*>(b.v + (row / 8 * (D / 4) + 16 * h) * 16);
@@ -321,13 +316,18 @@ __device__ __forceinline__ void q4_load(const Q4Base& b, int tile, Q4Tile<D>& t)
 // 32 .. 32 + D / 8 - 1 of V. They write it to the cache, and the lanes that hold its place in the tile take it over
 // from them: nobody waits for the store, or reads it back.
 template <class T, int D>
-__device__ __forceinline__ void q4_fresh(const Q4Attn& a, int seq, int kvh, int64_t hr, int row, int lane, Q4Tile<D>& t) {
-  const Q4Cache& c = a.c;
-  const int d = 8 * (lane & (D / 8 - 1)), i = lane & 15, g = lane >> 4;
+__device__ __forceinline__ typename Vec8<T>::type q4_fresh_values(const Q4Attn& a, int seq, int kvh, int lane) {
   const T* src = lane < 32 ? static_cast<const T*>(a.fresh.k) + seq * a.fresh.k_row + kvh * a.fresh.k_head
                            : static_cast<const T*>(a.fresh.v) + seq * a.fresh.v_row + kvh * a.fresh.v_head;
+  return *reinterpret_cast<const typename Vec8<T>::type*>(src + 8 * (lane & (D / 8 - 1)));
+}
+template <class T, int D>
+__device__ __forceinline__ void q4_fresh(const Q4Attn& a, const typename Vec8<T>::type& values, int64_t hr, int row, int lane,
+                                         Q4Tile<D>& t) {
+  const Q4Cache& c = a.c;
+  const int d = 8 * (lane & (D / 8 - 1)), i = lane & 15, g = lane >> 4;
   _Float16 step, low;
-  const uint32_t codes = q4_pack8<T>(*reinterpret_cast<const typename Vec8<T>::type*>(src + d), step, low);
+  const uint32_t codes = q4_pack8<T>(values, step, low);
   const h2v meta{step, low};
   if ((lane & 31) < D / 8) {
     if (lane < 32) {
@@ -377,10 +377,18 @@ __device__ __forceinline__ void q4_fresh(const Q4Attn& a, int seq, int kvh, int6
   }
 }
 
-// Nibble j of both halves of u as fp16, then low + step c.
-__device__ __forceinline__ h2v q4_pair(uint32_t u, int j, h2v step, h2v low) {
-  const uint32_t bits = ((u >> (4 * j)) & 0x000F000Fu) | 0x64006400u;
-  const h2v c = __builtin_bit_cast(h2v, bits) - static_cast<_Float16>(1024.f);
+// The 4-bit fields at bits 0 (j = 0) or 4 (j = 1) of both halves of u as fp16, then low + step c. Or-ed into the
+// mantissa of 1024 a field at bit 0 counts ones, into that of 64 one at bit 4 does: subtracting that leaves c, and
+// only the upper byte of a half needs a shift. Mask and exponent are hidden from constant folding, which keeps the
+// mask in a scalar register and the exponent in a vector one: v_and_or_b32 takes them so, and no two literals.
+// (The instruction itself cannot stand in an asm: the compiler then leaves out the waits that a write to
+// registers of an unfinished MFMA needs.)
+template <int J>
+__device__ __forceinline__ h2v q4_pair(uint32_t u, h2v step, h2v low) {
+  uint32_t mask = J ? 0x00F000F0u : 0x000F000Fu, one = J ? 0x54005400u : 0x64006400u;
+  asm("" : "+s"(mask));
+  asm("" : "+v"(one));
+  const h2v c = __builtin_bit_cast(h2v, (u & mask) | one) - static_cast<_Float16>(J ? 64.f : 1024.f);
   return __builtin_elementwise_fma(c, step, low);
 }
 
@@ -390,11 +398,9 @@ struct Q4State {
   float m, l;        // l: this lane's keys only
 };
 
-template <int D, bool kTail>
-__device__ __forceinline__ void q4_tile(const Q4Tile<D>& t, const h8v (&q)[D / 32], float factor, int left, int lane,
-                                        Q4State<D>& st) {
-  const int g = lane >> 4;
-  f4v s[2];
+// Scores of a tile's keys.
+template <int D>
+__device__ __forceinline__ void q4_scores(const Q4Tile<D>& t, const h8v (&q)[D / 32], f4v (&s)[2]) {
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt) {
     s[kt] = f4v{0.f, 0.f, 0.f, 0.f};
@@ -402,24 +408,33 @@ __device__ __forceinline__ void q4_tile(const Q4Tile<D>& t, const h8v (&q)[D / 3
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) {
       h8v k;
+      const uint32_t u = t.k[kt][j];
+      const h2v x[4] = {q4_pair<0>(u, step, low), q4_pair<1>(u, step, low), q4_pair<0>(u >> 8, step, low), q4_pair<1>(u >> 8, step, low)};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const h2v x = q4_pair(t.k[kt][j], e, step, low);
-        k[2 * e] = x[0];
-        k[2 * e + 1] = x[1];
+        k[2 * e] = x[e][0];
+        k[2 * e + 1] = x[e][1];
       }
       s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[j], s[kt], 0, 0, 0);
     }
   }
+}
+
+// Their weights and the sum over the values; kTail: only the first `left` keys of the tile count.
+template <int D, bool kTail>
+__device__ __forceinline__ void q4_values(const Q4Tile<D>& t, f4v (&s)[2], float factor, int left, int lane, Q4State<D>& st) {
+  const int g = lane >> 4;
   float top = -INFINITY;
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
+    for (int r = 0; r < 4; r += 2) {
       if constexpr (kTail) {
         if (8 * g + 4 * kt + r >= left) s[kt][r] = -INFINITY;
+        if (8 * g + 4 * kt + r + 1 >= left) s[kt][r + 1] = -INFINITY;
       }
-      top = fmaxf(top, s[kt][r]);
+      // (a NaN score stays one: its row is NaN anyway; fmaxf would quiet every operand first)
+      top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, s[kt][r]), s[kt][r + 1]);
     }
   top = xor_max<32>(xor_max<16>(top)) * factor;
   if (__builtin_amdgcn_ballot_w64(top > st.m + kSlack)) {
@@ -451,17 +466,20 @@ __device__ __forceinline__ void q4_tile(const Q4Tile<D>& t, const h8v (&q)[D / 3
       for (int e = 0; e < 8; ++e)
         if (8 * g + e >= left) vs[e] = vl[e] = static_cast<_Float16>(0.f);
     }
+    h8v v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      h8v v;
+    for (int w = 0; w < 4; ++w) {
+      const h2v step{vs[2 * w], vs[2 * w + 1]}, low{vl[2 * w], vl[2 * w + 1]};
+      const uint32_t u = t.v[h][w];
+      const h2v x[4] = {q4_pair<0>(u, step, low), q4_pair<1>(u, step, low), q4_pair<0>(u >> 8, step, low), q4_pair<1>(u >> 8, step, low)};
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const h2v x = q4_pair(t.v[h][w], j, h2v{vs[2 * w], vs[2 * w + 1]}, h2v{vl[2 * w], vl[2 * w + 1]});
-        v[2 * w] = x[0];
-        v[2 * w + 1] = x[1];
+      for (int j = 0; j < 4; ++j) {
+        v[j][2 * w] = x[j][0];
+        v[j][2 * w + 1] = x[j][1];
       }
-      st.o[h][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p, st.o[h][j], 0, 0, 0);
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) st.o[h][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[j], p, st.o[h][j], 0, 0, 0);
   }
 }
 
@@ -470,17 +488,26 @@ __device__ __forceinline__ void q4_tile(const Q4Tile<D>& t, const h8v (&q)[D / 3
 // elements 2^-24 of the largest and less lose bits); the factor undoes it. A negative scale negates the query,
 // a zero one becomes so small that scores vanish.
 template <class T, int D>
-__device__ __forceinline__ float q4_queries(const Q4Attn& a, int seq, int head, bool live, int lane, h8v (&q)[D / 32]) {
-  const int g = lane >> 4;
+struct Q4Query {
+  typename Vec8<T>::type x[D / 32];
+};
+template <class T, int D>
+__device__ __forceinline__ Q4Query<T, D> q4_load_query(const Q4Attn& a, int seq, int head, bool live, int lane) {
+  Q4Query<T, D> r = {};
+  const T* src = static_cast<const T*>(a.q) + seq * a.q_row + head * a.q_head + D / 4 * (lane >> 4);
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j)
+    if (live) r.x[j] = *reinterpret_cast<const typename Vec8<T>::type*>(src + 8 * j);
+  return r;
+}
+template <class T, int D>
+__device__ __forceinline__ float q4_queries(const Q4Attn& a, const Q4Query<T, D>& in, h8v (&q)[D / 32]) {
   float f[D / 32][8], big = 0.f;
-  const T* src = static_cast<const T*>(a.q) + seq * a.q_row + head * a.q_head + D / 4 * g;
 #pragma unroll
   for (int j = 0; j < D / 32; ++j) {
-    typename Vec8<T>::type x = {};
-    if (live) x = *reinterpret_cast<const typename Vec8<T>::type*>(src + 8 * j);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      f[j][e] = a.scale < 0.f ? -static_cast<float>(x[e]) : static_cast<float>(x[e]);
+      f[j][e] = a.scale < 0.f ? -static_cast<float>(in.x[j][e]) : static_cast<float>(in.x[j][e]);
       big = fmaxf(big, __builtin_fabsf(f[j][e]));
     }
   }
@@ -505,30 +532,37 @@ __device__ __forceinline__ float q4_queries(const Q4Attn& a, int seq, int head, 
 }
 
 // Tiles first, first + step, ... below `end` of an item with `keys` keys; fresh: the row that is written now, or -1.
+// Each half of a tile's registers is loaded again as soon as it is used up: K's while weights and values are worked
+// on, V's while the next tile's scores are.
 template <class T, int D>
-__device__ __forceinline__ void q4_tiles(const Q4Attn& a, int seq, int kvh, int first, int step, int end, int keys, int fresh,
-                                         const h8v (&q)[D / 32], float factor, int lane, Q4State<D>& st) {
+__device__ __forceinline__ void q4_tiles(const Q4Attn& a, int64_t hr, int first, int step, int end, int keys, int fresh,
+                                         const typename Vec8<T>::type& fresh_values, const h8v (&q)[D / 32], float factor,
+                                         int lane, Q4State<D>& st) {
 #pragma unroll
   for (int h = 0; h < D / 64; ++h)
 #pragma unroll
     for (int j = 0; j < 4; ++j) st.o[h][j] = f4v{0.f, 0.f, 0.f, 0.f};
   st.m = -INFINITY;
   st.l = 0.f;
-  const int64_t hr = (static_cast<int64_t>(seq) * a.c.heads + kvh) * a.c.max_len;
+  const int all = (keys + kTileKeys - 1) / kTileKeys, tiles = min(end, all);
+  if (first >= tiles) return;
   const Q4Base b = q4_base<D>(a.c, hr, lane);
-  const int full = min(end, keys / kTileKeys - (fresh >= 0 && keys % kTileKeys == 0));  // tiles without the fresh row or an end
+  Q4Tile<D> x;
+  f4v s[2];
+  q4_load_k<D>(b, first, x);
+  q4_load_v<D>(b, first, x);
   int t = first;
-  for (; t < full; t += step) {
-    Q4Tile<D> x;
-    q4_load<D>(b, t, x);
-    q4_tile<D, false>(x, q, factor, 0, lane, st);
+  for (; t + step < tiles; t += step) {
+    q4_scores<D>(x, q, s);
+    q4_load_k<D>(b, t + step, x);
+    q4_values<D, false>(x, s, factor, 0, lane, st);
+    q4_load_v<D>(b, t + step, x);
   }
-  if (t < end && t * kTileKeys < keys) {
-    Q4Tile<D> x;
-    q4_load<D>(b, t, x);
-    if (fresh >= 0) q4_fresh<T, D>(a, seq, kvh, hr, fresh, lane, x);
-    q4_tile<D, true>(x, q, factor, keys - t * kTileKeys, lane, st);
-  }
+  const int left = keys - t * kTileKeys;
+  if (fresh >= 0 && t == all - 1) q4_fresh<T, D>(a, fresh_values, hr, fresh, lane, x);
+  q4_scores<D>(x, q, s);
+  if (left >= kTileKeys) q4_values<D, false>(x, s, factor, 0, lane, st);
+  else q4_values<D, true>(x, s, factor, left, lane, st);
 }
 
 // Where the waves' results of an item meet; `cols` query heads of it.
@@ -577,6 +611,7 @@ __device__ __forceinline__ float q4_sum(const Q4Merge<D>& x, int waves, int cols
 struct Q4Item {
   int kvh, head, cols;
 };
+__device__ __forceinline__ int q4_cols(const Q4Attn& a) { return min(kCols, a.heads / a.c.heads); }  // of the largest item
 __device__ __forceinline__ Q4Item q4_item(const Q4Attn& a, int item) {
   const int group = a.heads / a.c.heads, parts = (group + kCols - 1) / kCols;
   const int kvh = item / parts, first = item % parts * kCols;
@@ -588,169 +623,78 @@ __device__ __forceinline__ void q4_store(const Q4Attn& a, int seq, int head, int
   static_cast<T*>(a.out)[seq * a.o_row + head * a.o_head + d] = static_cast<T>(l > 0.f ? o / l : 0.f);
 }
 
-// A block an item, for caches so short that no item is worth sharing out.
+// The first arguments, which arrive in scalar registers, are what the way to the first tile needs; the rest of `a`
+// is read from memory meanwhile.
 template <class T, int D>
-__global__ void __launch_bounds__(512) q4_direct_kernel(Q4Attn a) {
+__global__ void __launch_bounds__(512, 4) q4_attention_kernel(const int64_t* lens, uint8_t* k_codes, _Float16* k_meta,
+                                                              uint8_t* v_codes, _Float16* v_meta, int max_len, int kv_heads,
+                                                              int heads, int chunk, Q4Attn a) {
   extern __shared__ float lds[];
-  const int seq = blockIdx.y, waves = blockDim.x / 64;
+  a.lens = lens;
+  a.c.k_codes = k_codes;
+  a.c.k_meta = k_meta;
+  a.c.v_codes = v_codes;
+  a.c.v_meta = v_meta;
+  a.c.max_len = max_len;
+  a.c.heads = kv_heads;
+  a.heads = heads;
+  a.chunk = chunk;
+  const int seq = blockIdx.y, waves = blockDim.x / 64, begin = static_cast<int>(gridDim.z - 1 - blockIdx.z) * a.chunk;
   const Q4Item it = q4_item(a, blockIdx.x);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int fresh;
+  if (begin > 0 && begin >= q4_keys(a, seq, fresh)) return;
+  // requested before the length is known
+  const Q4Query<T, D> query = q4_load_query<T, D>(a, seq, it.head + (lane & 15), (lane & 15) < it.cols, lane);
+  typename Vec8<T>::type fresh_values = {};
+  if (a.fresh.k) fresh_values = q4_fresh_values<T, D>(a, seq, it.kvh, lane);
   const int keys = q4_keys(a, seq, fresh);
   h8v q[D / 32];
-  const bool live = (lane & 15) < it.cols;
-  const float factor = q4_queries<T, D>(a, seq, it.head + (lane & 15), live, lane, q);
+  const float factor = q4_queries<T, D>(a, query, q);
   Q4State<D> st;
-  q4_tiles<T, D>(a, seq, it.kvh, wave, waves, a.c.max_len / kTileKeys, keys, fresh, q, factor, lane, st);
+  q4_tiles<T, D>(a, (static_cast<int64_t>(seq) * a.c.heads + it.kvh) * a.c.max_len, begin / kTileKeys + wave, waves,
+                 (begin + a.chunk) / kTileKeys, keys, fresh, fresh_values, q, factor, lane, st);
   const Q4Merge<D> x(lds, waves, it.cols);
   q4_hand_in<D>(x, st, wave, it.cols, lane);
   __syncthreads();
+  const bool whole = keys <= a.chunk;
+  const int64_t slot = (static_cast<int64_t>(seq) * gridDim.x + blockIdx.x) * a.chunks + begin / a.chunk;
+  const int cols = q4_cols(a);
+  float* ml = a.ws + static_cast<int64_t>(gridDim.x) * gridDim.y * a.chunks * cols * D + slot * cols * 2;
   for (int i = threadIdx.x; i < it.cols * D; i += blockDim.x) {
     float m, l;
-    const float o = q4_sum<D>(x, waves, it.cols, i / D, i % D, m, l);
-    q4_store<T>(a, seq, it.head + i / D, i % D, o, l);
-  }
-}
-
-// Units of one item of a sequence, and what it costs in units: an item that is begun costs kItemCost more.
-#ifndef Q4_COST
-#define Q4_COST 1
-#endif
-constexpr int kItemCost = Q4_COST;
-__device__ __forceinline__ int q4_units(const Q4Attn& a, int seq) {
-  int fresh;
-  return (q4_keys(a, seq, fresh) + kUnitKeys - 1) / kUnitKeys;
-}
-__device__ __forceinline__ int q4_cost(int units) { return units > 0 ? units + kItemCost : 0; }
-__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive sum over the wave
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const int x = __shfl_up(v, o);
-    if (lane >= o) v += x;
-  }
-  return v;
-}
-// Blocks that have work: each at least a unit, so that every block of an item's range leaves its part.
-__device__ __forceinline__ int q4_blocks(const Q4Attn& a, int64_t all) {
-  return static_cast<int>(min(all, static_cast<int64_t>(a.blocks)));
-}
-
-template <class T, int D>
-__global__ void __launch_bounds__(256, 4) q4_split_kernel(Q4Attn a) {
-  extern __shared__ float lds[];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int group = a.heads / a.c.heads, items = a.c.heads * ((group + kCols - 1) / kCols);
-  int total = 0;
-  for (int s0 = 0; s0 < a.c.n_seq; s0 += 64) {
-    const int u = s0 + lane < a.c.n_seq ? q4_cost(q4_units(a, s0 + lane)) : 0;
-    total += __builtin_amdgcn_readlane(wave_scan(u, lane), 63);
-  }
-  const int64_t all = static_cast<int64_t>(total) * items;
-  const int blocks = q4_blocks(a, all);
-  if (static_cast<int>(blockIdx.x) >= blocks) return;
-  const int begin = static_cast<int>(all * blockIdx.x / blocks), end = static_cast<int>(all * (blockIdx.x + 1) / blocks);
-  // the sequence of the first place
-  int seq = 0, before = 0, cost = 0;
-  for (int s0 = 0, sum = 0; s0 < a.c.n_seq; s0 += 64) {
-    const int u = s0 + lane < a.c.n_seq ? q4_cost(q4_units(a, s0 + lane)) : 0;
-    const int incl = wave_scan(u, lane) + sum;
-    const uint64_t past = __builtin_amdgcn_ballot_w64(static_cast<int64_t>(incl) * items > begin);
-    if (past) {
-      const int at = __builtin_ctzll(past);
-      seq = s0 + at;
-      cost = __builtin_amdgcn_readlane(u, at);
-      before = __builtin_amdgcn_readlane(incl, at) - cost;
-      break;
-    }
-    sum = __builtin_amdgcn_readlane(incl, 63);
-  }
-  for (int u = begin; u < end;) {
-    // Lane-dependent values are made anew for each item: kept across items they take some 50 registers
-    int tid = threadIdx.x;
-    asm volatile("" : "+v"(tid));
-    const int lane = tid & 63;
-    // the item's place: its kItemCost first places are its beginning, the others its units
-    const int local = u - before * items, item = local / cost, place = local % cost, units = cost - kItemCost;
-    const int from = max(place - kItemCost, 0), to = min(units, place + end - u - kItemCost);  // this block's units of it
-    const int next = u + cost - place;
-    if (to <= from) break;  // the run ends in the item's beginning
-    const Q4Item it = q4_item(a, item);
-    int fresh;
-    const int keys = q4_keys(a, seq, fresh);
-    h8v q[D / 32];
-    const float factor = q4_queries<T, D>(a, seq, it.head + (lane & 15), (lane & 15) < it.cols, lane, q);
-    Q4State<D> st;
-    q4_tiles<T, D>(a, seq, it.kvh, from * (kUnitKeys / kTileKeys) + wave, 4, to * (kUnitKeys / kTileKeys), keys, fresh, q, factor,
-                   lane, st);
-    const Q4Merge<D> x(lds, 4, it.cols);
-    q4_hand_in<D>(x, st, wave, it.cols, lane);
-    __syncthreads();
-    const bool whole = from == 0 && to == units;
-    const int slot = 2 * blockIdx.x + (u == begin ? 0 : 1);
-    float* acc = a.ws + static_cast<int64_t>(slot) * kCols * D;
-    float* ml = a.ws + (static_cast<int64_t>(2 * a.blocks) * D + 2 * slot) * kCols;
-    for (int i = tid; i < it.cols * D; i += 256) {
-      float m, l;
-      const int h = i / D, d = i % D;
-      const float o = q4_sum<D>(x, 4, it.cols, h, d, m, l);
-      if (whole) {
-        q4_store<T>(a, seq, it.head + h, d, o, l);
-      } else {
-        acc[i] = o;
-        if (d == 0) {
-          ml[2 * h] = m;
-          ml[2 * h + 1] = l;
-        }
-      }
-    }
-    u = next;
-    if (u < end) {
-      __syncthreads();  // the merge buffer is free again
-      if (u == (before + cost) * items) {  // on to the next sequence that has units
-        before += cost;
-        do cost = q4_cost(q4_units(a, ++seq));
-        while (cost == 0);
+    const int h = i / D, d = i % D;
+    const float o = q4_sum<D>(x, waves, it.cols, h, d, m, l);
+    if (whole) {
+      q4_store<T>(a, seq, it.head + h, d, o, l);
+    } else {
+      a.ws[slot * cols * D + i] = o;
+      if (d == 0) {
+        ml[2 * h] = m;
+        ml[2 * h + 1] = l;
       }
     }
   }
 }
 
-constexpr int kCombine = 512;
-// Block = (query head, sequence): the parts of an item that several blocks worked on, or the zeros of a sequence
-// without keys.
+// Block = (query head, sequence): joins the chunks of an item that has several.
+constexpr int kCombine = 256;
 template <class T, int D>
 __global__ void __launch_bounds__(kCombine) q4_combine_kernel(Q4Attn a) {
   constexpr int kLanes = kCombine / D;
-  __shared__ float weight[kSplitBlocks], red[kCombine / 64], part[kLanes][D];
+  __shared__ float red[kCombine / 64], part[kLanes][D];
+  extern __shared__ float weight[];  // [chunks]
   const int seq = blockIdx.y, head = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
-  const int group = a.heads / a.c.heads, parts = (group + kCols - 1) / kCols, items = a.c.heads * parts;
+  int fresh;
+  const int keys = q4_keys(a, seq, fresh), n = (keys + a.chunk - 1) / a.chunk;
+  if (n <= 1) return;  // its block finished it
+  const int group = a.heads / a.c.heads, parts = (group + kCols - 1) / kCols, items = a.c.heads * parts, cols = q4_cols(a);
   const int in_group = head % group, item = head / group * parts + in_group / kCols, h = in_group % kCols;
-  int total = 0, before = 0;
-  for (int s0 = 0; s0 < a.c.n_seq; s0 += 64) {
-    const int u = s0 + lane < a.c.n_seq ? q4_cost(q4_units(a, s0 + lane)) : 0;
-    total += __builtin_amdgcn_readlane(wave_scan(u, lane), 63);
-    before += __builtin_amdgcn_readlane(wave_scan(s0 + lane < seq ? u : 0, lane), 63);
-  }
-  const int units = q4_units(a, seq);
-  if (units == 0) {
-    if (tid < D) q4_store<T>(a, seq, head, tid, 0.f, 0.f);
-    return;
-  }
-  // block b has the places all b / blocks ..: the blocks of the item's first and last unit
-  const int64_t all = static_cast<int64_t>(total) * items;
-  const int64_t u0 = static_cast<int64_t>(before) * items + static_cast<int64_t>(item) * q4_cost(units);
-  const int blocks = q4_blocks(a, all);
-  const int b0 = static_cast<int>(((u0 + kItemCost + 1) * blocks - 1) / all);
-  const int b1 = static_cast<int>(((u0 + kItemCost + units) * blocks - 1) / all);
-  if (b0 == b1) return;  // that block finished it
-  const float* ml = a.ws + static_cast<int64_t>(2 * a.blocks) * D * kCols;
-  // the item is the first one of every block but b0, and of that one if it begins there
-  const int64_t first = 2 * static_cast<int64_t>(b0) + (all * b0 / blocks < u0);
-  const auto slot = [&](int i) { return i == 0 ? first : 2 * static_cast<int64_t>(b0 + i); };
-  const int n = b1 - b0 + 1;
+  const int64_t first = (static_cast<int64_t>(seq) * items + item) * a.chunks;
+  const float* ml = a.ws + static_cast<int64_t>(items) * a.c.n_seq * a.chunks * cols * D + (first * cols + h) * 2;
   float m = -INFINITY;
   for (int i = tid; i < n; i += kCombine) {
-    weight[i] = ml[(slot(i) * kCols + h) * 2];
+    weight[i] = ml[i * cols * 2];
     m = fmaxf(m, weight[i]);
   }
   m = group_max<64>(m);
@@ -761,28 +705,61 @@ __global__ void __launch_bounds__(kCombine) q4_combine_kernel(Q4Attn a) {
   float l = 0.f;
   for (int i = tid; i < n; i += kCombine) {
     weight[i] = __builtin_amdgcn_exp2f(weight[i] - m);
-    l = fmaf(weight[i], ml[(slot(i) * kCols + h) * 2 + 1], l);
+    l = fmaf(weight[i], ml[i * cols * 2 + 1], l);
   }
   __syncthreads();
   l = block_sum_once<kCombine>(l, red);
-  const int d = tid % D, from = tid / D;
-  const float* acc = a.ws + h * D + d;
+  const int d = tid % D, from = tid / D, step = cols * D;
+  const float* acc = a.ws + (first * cols + h) * D + d;
   float o = 0.f;
   int i = from;
   for (; i + 7 * kLanes < n; i += 8 * kLanes) {  // 8 loads in flight
     float x[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = acc[slot(i + j * kLanes) * kCols * D];
+    for (int j = 0; j < 8; ++j) x[j] = acc[static_cast<int64_t>(i + j * kLanes) * step];
 #pragma unroll
     for (int j = 0; j < 8; ++j) o = fmaf(weight[i + j * kLanes], x[j], o);
   }
-  for (; i < n; i += kLanes) o = fmaf(weight[i], acc[slot(i) * kCols * D], o);
+  for (; i < n; i += kLanes) o = fmaf(weight[i], acc[static_cast<int64_t>(i) * step], o);
   part[from][d] = o;
   __syncthreads();
   if (tid >= D) return;
 #pragma unroll
   for (int j = 1; j < kLanes; ++j) o += part[j][d];
   q4_store<T>(a, seq, head, d, o, l);
+}
+
+// How a call is shared out, by sizes alone (the lengths are on the device). A cache of up to kOneChunk rows is one
+// chunk: a second launch to join chunks costs more than it gains there (16 sequences x 20 heads of 64 over 1500 keys
+// 14.4 us in one chunk, 19.2 shared out further). Longer ones are cut so that full lengths give about kWantBlocks
+// blocks, two a CU (131000 keys x 8 heads of 128: 42.7 us, with twice the blocks 48.4), into chunks of at most 256
+// keys a wave, which bounds how long a few long sequences among short ones keep their CUs (64 ragged sequences of
+// up to 8000 keys x 8 heads: 42 us, with 512 keys a wave 61), and of at least 1 / kMostBlocks of everything, which
+// bounds the workspace. Blocks have 8 waves where items are few and 4 where they fill the CUs anyway (those 64
+// sequences: 33.5 us against 39.5; 64 x 20 heads of 64 over 700 keys 15.0 against 17.2, but 16 x 20 over 1500 keys as
+// two chunks of 4 waves 14.8 against 12.2), or where the merge of 16 heads of 128 would pass 64 KB of LDS.
+struct Q4Plan {
+  int items, cols, waves, chunk, chunks;
+  int64_t parts() const { return static_cast<int64_t>(items) * chunks; }  // of a sequence
+};
+constexpr int kOneChunk = 2048, kWaveKeys = 256, kWantBlocks = 512, kMostBlocks = 8192, kManyItems = 512;
+
+Q4Plan q4_plan(int n_seq, int heads, int kv_heads, int max_len, int dim) {
+  Q4Plan p;
+  const int group = heads / kv_heads;
+  p.items = kv_heads * ((group + kCols - 1) / kCols);
+  p.cols = min(kCols, group);
+  const int lds8 = dim == 64 ? Q4Merge<64>::bytes(8, p.cols) : Q4Merge<128>::bytes(8, p.cols);
+  const bool many = static_cast<int64_t>(n_seq) * p.items >= kManyItems;
+  p.waves = min(max_len / kTileKeys, many || lds8 > 65536 ? 4 : 8);
+  p.chunk = max_len;
+  if (max_len > kOneChunk) {
+    const int64_t keys = static_cast<int64_t>(n_seq) * p.items * max_len, unit = kTileKeys * p.waves;
+    const int64_t want = max(min(keys / kWantBlocks, static_cast<int64_t>(kWaveKeys * p.waves)), keys / kMostBlocks);
+    p.chunk = static_cast<int>(min((want + unit) / unit * unit, static_cast<int64_t>(max_len)));
+  }
+  p.chunks = (max_len + p.chunk - 1) / p.chunk;
+  return p;
 }
 
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
@@ -864,7 +841,8 @@ extern "C" int64_t fw_decode_attention_q4_ws_floats(int n_seq, int heads, int kv
   if (n_seq <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_len <= 0 || max_len % 32 ||
       (head_dim != 64 && head_dim != 128))
     return 0;
-  return static_cast<int64_t>(2 * kSplitBlocks) * kCols * (head_dim + 2);
+  const Q4Plan p = q4_plan(n_seq, heads, kv_heads, max_len, head_dim);
+  return p.chunks == 1 ? 4 : (n_seq * p.parts() * p.cols * (head_dim + 2) + 3) / 4 * 4;
 }
 
 extern "C" int fw_decode_attention_q4(const void* q, int64_t q_row, int64_t q_head, void* k_codes, void* k_meta,
@@ -885,22 +863,15 @@ extern "C" int fw_decode_attention_q4(const void* q, int64_t q_row, int64_t q_he
   const int64_t need = fw_decode_attention_q4_ws_floats(n_seq, heads, kv_heads, max_len, head_dim);
   if (!ws || ws_floats < need || !aligned(ws, 16))
     return fw_fail(FW_EINVAL, "decode_attention_q4: workspace needs %lld floats, 16-byte aligned", static_cast<long long>(need));
-  const int cols = min(kCols, heads / kv_heads), items = kv_heads * ((heads / kv_heads + kCols - 1) / kCols);
-  if (n_seq > 65535 || static_cast<int64_t>(n_seq) * items * ((max_len + kUnitKeys - 1) / kUnitKeys + kItemCost) > 0x7FFFFFFF)
-    return fw_fail(FW_EINVAL, "decode_attention_q4: too many sequences");
-  Q4Attn a{q, out, q_row, q_head, o_row, o_head, Q4Rows{k_new, v_new, k_row, k_head, v_row, v_head}, lens, c, heads, scale, ws, 0};
-  const auto lds = [&](int waves) {
-    return head_dim == 64 ? Q4Merge<64>::bytes(waves, cols) : Q4Merge<128>::bytes(waves, cols);
-  };
-  if (max_len <= kDirectKeys) {
-    // 8 waves, 4 where the merge of so many heads would pass 64 KB
-    const int waves = min(max_len / kTileKeys, lds(8) <= 65536 ? 8 : 4);
-    Q4_LAUNCH(q4_direct_kernel, dtype, head_dim, dim3(items, n_seq), dim3(64 * waves), lds(waves), stream, a);
-    return fw_check_launch("decode_attention_q4");
-  }
-  a.blocks = kSplitBlocks;
-  Q4_LAUNCH(q4_split_kernel, dtype, head_dim, dim3(kSplitBlocks), dim3(256), lds(4), stream, a);
+  const Q4Plan p = q4_plan(n_seq, heads, kv_heads, max_len, head_dim);
+  if (n_seq > 65535) return fw_fail(FW_EINVAL, "decode_attention_q4: too many sequences");
+  const Q4Attn a{q, out, q_row, q_head, o_row, o_head, Q4Rows{k_new, v_new, k_row, k_head, v_row, v_head}, lens, c, heads, scale,
+                 p.chunk, p.chunks, ws};
+  const int lds = head_dim == 64 ? Q4Merge<64>::bytes(p.waves, p.cols) : Q4Merge<128>::bytes(p.waves, p.cols);
+  Q4_LAUNCH(q4_attention_kernel, dtype, head_dim, dim3(p.items, n_seq, p.chunks), dim3(64 * p.waves), lds, stream, lens,
+            c.k_codes, c.k_meta, c.v_codes, c.v_meta, max_len, kv_heads, heads, p.chunk, a);
   if (const int rc = fw_check_launch("decode_attention_q4")) return rc;
-  Q4_LAUNCH(q4_combine_kernel, dtype, head_dim, dim3(heads, n_seq), dim3(kCombine), 0, stream, a);
+  if (p.chunks == 1) return FW_OK;
+  Q4_LAUNCH(q4_combine_kernel, dtype, head_dim, dim3(heads, n_seq), dim3(kCombine), 4 * p.chunks, stream, a);
   return fw_check_launch("decode_attention_q4 combine");
 }

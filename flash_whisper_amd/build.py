@@ -39,6 +39,7 @@ PER_FILE_FLAGS = {
     'synth.hip': ['-ffp-contract=off'],
     # MFMA results in VGPRs: the attention softmax reads every score and rescales O in place
     'attention_enc.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form', *PRELOAD],
+    'attention_prompt.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form', *PRELOAD],
     'decode.hip': PRELOAD,
     'kv_q4.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form', *PRELOAD],
     'encoder.hip': PRELOAD,

@@ -1,9 +1,44 @@
 // Attention over whole prompts for gfx950: sequences of different lengths packed one after another, query
 // heads grouped over key/value heads, causal from the end of the keys or not.
-#include "fw_common.h"
+// Built with MFMA results in VGPRs (-mllvm -amdgpu-mfma-vgpr-form), as the encoder attention and for its reason.
+#include <type_traits>
+
+#include "lds_pipe.h"
 
 namespace fw {
 namespace {
+
+typedef __bf16 b8v __attribute__((ext_vector_type(8)));
+typedef __bf16 b2v __attribute__((ext_vector_type(2)));
+typedef short s4v __attribute__((ext_vector_type(4)));
+
+template <class T>
+struct Types;
+template <>
+struct Types<_Float16> {
+  typedef h8v v8;
+  typedef h2v v2;
+  static constexpr uint32_t kExp = 0x7C007C00u, kExpOne = 0x04000400u;  // a pair's exponent fields, and their last bits
+};
+template <>
+struct Types<__bf16> {
+  typedef b8v v8;
+  typedef b2v v2;
+  static constexpr uint32_t kExp = 0x7F807F80u, kExpOne = 0x00800080u;
+};
+
+__device__ __forceinline__ f16v mfma32(const h8v& a, const h8v& b, const f16v& c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f16v mfma32(const b8v& a, const b8v& b, const f16v& c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ float add_pair(h2v x, float s) {
+  return __builtin_amdgcn_fdot2(x, h2v{static_cast<_Float16>(1.f), static_cast<_Float16>(1.f)}, s, false);
+}
+__device__ __forceinline__ float add_pair(b2v x, float s) {
+  return __builtin_amdgcn_fdot2_f32_bf16(x, b2v{static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)}, s, false);
+}
 
 struct PromptArgs {
   const void *q, *k, *v;
@@ -15,41 +50,390 @@ struct PromptArgs {
   float scale;
 };
 
-// One wave a query and head: a key at a time, D / 64 dims a lane.
-template <class T, int D, bool CAUSAL>
-__global__ void __launch_bounds__(256) prompt_attention_kernel(PromptArgs a) {
-  constexpr int kPer = D / 64;
-  const int lane = threadIdx.x & 63;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6), row = unit / a.heads;
-  const int head = static_cast<int>(unit % a.heads), kvh = head / (a.heads / a.kv_heads);
-  if (row >= a.q_rows) return;
-  int seq = -1;
-  for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
-    const uint64_t at = __builtin_amdgcn_ballot_w64(s0 + lane < a.n_seq && a.cu_q[min(s0 + lane, a.n_seq)] <= row);
-    seq += __popcll(at);
-    if (at != ~uint64_t{0}) break;
+// ------------------------------------------------------------------------------------------
+// A row of a block is a query and one of the heads that share a key/value head: row i of a sequence is query
+// i / group and head i % group, so grouped heads share every key that is staged, and a few queries fill a tile.
+// Block = QG waves of 32 rows x KP key parts (TK-key tiles t with t % KP == part); the parts' (m, l, O) are
+// merged through LDS at the end. Per tile a wave computes S^T = K Q^T (keys x rows), so that a lane holds scores of
+// one row and maximum and sum need one cross-lane step, and feeds P^T from the S^T layout as the B operand of
+// O^T = V^T P^T: a lane of half lg = lane / 32 holds keys 4 lg .. 4 lg + 3 and 8 more of every 16.
+//  - K and V tiles arrive row-major by direct-to-LDS copies in a ring of ST stages, their 16-byte chunks swizzled:
+//    K so that 16 rows' same chunk lies in 16 different bank groups, V so that 4 rows' 64 bytes do.
+//  - V^T operands are read with the transposing LDS read: 16 lanes name 4 keys x 16 dims, 8 bytes each, and lane i
+//    gets dim i of the 4 keys. Two reads give the 8 keys the lane holds in P^T.
+//  - The running maximum only moves when a score passes it by 2^kSlack; weights stay within fp16.
+//  - Masked tiles (the causal diagonal, the last one of a sequence): a masked score is replaced before the maximum,
+//    whatever it is. A masked weight of 0 does not undo an infinity or NaN in V, so the block looks for them in
+//    the tile, puts zeros there, and keeps for each dim the first key with either infinity and with a NaN: a row sees
+//    the keys up to its limit, so at the end it gets those whose first key it sees.
+// ------------------------------------------------------------------------------------------
+constexpr float kSlack = 8.f;
+constexpr float kLog2e = 1.4426950408889634f;
+#ifndef PA_AHEAD
+#define PA_AHEAD 2
+#endif
+constexpr int kAhead = PA_AHEAD;
+
+template <int D>
+__device__ __forceinline__ int k_slot(int row, int chunk) {
+  return D == 64 ? chunk ^ ((row >> 1) & 7) : chunk ^ (row & 15);
+}
+template <int D>
+__device__ __forceinline__ int v_slot(int row, int chunk) {
+  return D == 64 ? chunk ^ (((row >> 1) & 1) << 2) : chunk ^ ((row & 3) << 2);
+}
+
+// Where a block works: sequence rows [row0, row0 + ROWS) of `rows`, queries from packed row q0, keys from k0.
+struct Job {
+  int seq, row0, rows, nq, nk;
+  int64_t q0, k0;
+};
+
+__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive sum over the wave
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const int x = __shfl_up(v, o);
+    if (lane >= o) v += x;
   }
-  if (seq < 0) return;
-  const int64_t q0 = max(a.cu_q[seq], int64_t{0}), q1 = min(a.cu_q[seq + 1], a.q_rows);
-  if (row >= q1) return;
-  const int64_t k0 = min(max(a.cu_k[seq], int64_t{0}), a.k_rows), k1 = min(max(a.cu_k[seq + 1], k0), a.k_rows);
-  const int64_t keys = CAUSAL ? min(max(row - q0 + 1 + (k1 - k0) - (q1 - q0), int64_t{0}), k1 - k0) : k1 - k0;
-  float q[kPer], acc[kPer] = {}, m = -INFINITY, l = 0.f;
-  const T* qp = static_cast<const T*>(a.q) + row * a.q_row + head * a.q_head;
-  for (int i = 0; i < kPer; ++i) q[i] = static_cast<float>(qp[lane + 64 * i]) * a.scale;
-  for (int64_t t = k0; t < k0 + keys; ++t) {
-    const T* kp = static_cast<const T*>(a.k) + t * a.k_row + kvh * a.k_head;
-    const T* vp = static_cast<const T*>(a.v) + t * a.v_row + kvh * a.v_head;
-    float s = 0.f;
-    for (int i = 0; i < kPer; ++i) s += q[i] * static_cast<float>(kp[lane + 64 * i]);
-    s = group_sum<64>(s);
-    const float m_new = fmaxf(m, s), corr = __expf(m - m_new), p = __expf(s - m_new);
-    l = l * corr + p;
-    for (int i = 0; i < kPer; ++i) acc[i] = acc[i] * corr + p * static_cast<float>(vp[lane + 64 * i]);
-    m = m_new;
+  return v;
+}
+
+// Query rows of sequence s, its starts clamped to the rows there are.
+__device__ __forceinline__ int seq_rows(const int64_t* cu, int64_t rows, int s, int64_t& begin) {
+  begin = min(max(cu[s], int64_t{0}), rows);
+  return static_cast<int>(min(max(cu[s + 1], begin), rows) - begin);
+}
+
+// Block `index` of the blocks that all sequences take; from the last one if `reverse`. False: there are fewer.
+template <int ROWS>
+__device__ __forceinline__ bool find_job(const PromptArgs& a, int index, bool reverse, Job& job) {
+  const int lane = threadIdx.x & 63, group = a.heads / a.kv_heads;
+  const auto blocks = [&](int s, int64_t& begin, int& nq) {
+    nq = s < a.n_seq ? seq_rows(a.cu_q, a.q_rows, s, begin) : 0;
+    return (nq * group + ROWS - 1) / ROWS;
+  };
+  if (reverse) {
+    int total = 0;
+    for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
+      int64_t begin;
+      int nq;
+      total += __builtin_amdgcn_readlane(wave_scan(blocks(s0 + lane, begin, nq), lane), 63);
+    }
+    index = total - 1 - index;
+    if (index < 0) return false;
   }
-  T* op = static_cast<T*>(a.out) + row * a.o_row + head * a.o_head;
-  for (int i = 0; i < kPer; ++i) op[lane + 64 * i] = static_cast<T>(keys > 0 ? acc[i] / l : 0.f);
+  for (int s0 = 0, sum = 0; s0 < a.n_seq; s0 += 64) {
+    int64_t begin = 0;
+    int nq;
+    const int n = blocks(s0 + lane, begin, nq), incl = wave_scan(n, lane) + sum;
+    const uint64_t past = __builtin_amdgcn_ballot_w64(incl > index);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      job.seq = s0 + at;
+      job.row0 = (index - (__builtin_amdgcn_readlane(incl, at) - __builtin_amdgcn_readlane(n, at))) * ROWS;
+      job.nq = __builtin_amdgcn_readlane(nq, at);
+      job.rows = job.nq * group;
+      int64_t q0, k0;
+      seq_rows(a.cu_q, a.q_rows, job.seq, q0);
+      job.nk = seq_rows(a.cu_k, a.k_rows, job.seq, k0);
+      job.q0 = q0;
+      job.k0 = k0;
+      return true;
+    }
+    sum = __builtin_amdgcn_readlane(incl, 63);
+  }
+  return false;
+}
+
+template <int D>
+struct State {
+  f16v o[D / 32];  // O^T blocks of 32 dims; lane (row, lg), register r: dim 8 (r / 4) + 4 lg + r % 4
+  float m, l;
+};
+
+// V^T operand of dims 32 db .. and the 16 keys from row `key` of a staged V tile.
+template <class T, int D>
+__device__ __forceinline__ typename Types<T>::v8 read_vt(uint32_t v, int key, int db, int lane) {
+  const int i = lane & 15, row = key + 4 * (lane >> 5) + (i >> 2), chunk = 4 * db + 2 * ((lane >> 4) & 1) + ((i >> 1) & 1);
+  typedef __attribute__((address_space(3))) s4v lds_s4;
+  typedef short s8v __attribute__((ext_vector_type(8)));
+  const auto at = [&](int r) {
+    return reinterpret_cast<lds_s4*>(static_cast<uintptr_t>(v + r * (2 * D) + v_slot<D>(r, chunk) * 16 + (i & 1) * 8));
+  };
+  const s4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(row)), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(row + 8));
+  return __builtin_bit_cast(typename Types<T>::v8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// The first keys with a value that is no number, by dim: infinities, negative ones, NaNs.
+constexpr int kNoKey = 0x7FFFFFFF;
+template <int D>
+struct OddValues {
+  int first[3][D];
+  int any;
+};
+
+// Looks through 16 bytes of a staged V tile: 8 dims from d of key `key`.
+template <class T, int D>
+__device__ __forceinline__ void set_aside(uint32_t at, int key, int d, OddValues<D>& odd) {
+  typedef __attribute__((address_space(3))) u32x4 lds_u4;
+  u32x4 x = *reinterpret_cast<lds_u4*>(static_cast<uintptr_t>(at));
+  uint32_t found = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) found |= (x[e] & Types<T>::kExp) + Types<T>::kExpOne;
+  if ((found & 0x80008000u) == 0) return;
+  typename Types<T>::v8 y = __builtin_bit_cast(typename Types<T>::v8, x);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float f = static_cast<float>(y[e]);
+    if (__builtin_fabsf(f) < INFINITY) continue;
+    atomicMin(&odd.first[f != f ? 2 : f > 0.f ? 0 : 1][d + e], key);
+    y[e] = static_cast<T>(0.f);
+  }
+  *reinterpret_cast<lds_u4*>(static_cast<uintptr_t>(at)) = __builtin_bit_cast(u32x4, y);
+  odd.any = 1;
+}
+
+// A wave's tile: K at LDS address k, V at v; keys kv0 .., of which the lane's row sees those up to `limit`; masked:
+// some row does not see all of them.
+template <class T, int D, int TK>
+__device__ __forceinline__ void tile(uint32_t k, uint32_t v, const typename Types<T>::v8 (&q)[D / 16], float factor, int kv0,
+                                     int limit, bool masked, int lane, State<D>& st) {
+  typedef typename Types<T>::v8 v8;
+  typedef typename Types<T>::v2 v2;
+  const int lr = lane & 31, lg = lane >> 5;
+  typedef __attribute__((address_space(3))) v8 lds_v8;
+  constexpr int NB = TK / 32, NJ = D / 16, NP = TK / 16, ND = D / 32;
+  f16v s[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
+  // Operands are read kAhead steps before the products that take them; the scheduling barriers keep it at that,
+  // since all of a tile's operands at once do not fit the registers.
+  v8 kf[kAhead + 1][NB];
+  const auto read_k = [&](int j) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const int row = 32 * b + lr;
+      kf[j % (kAhead + 1)][b] = *reinterpret_cast<lds_v8*>(static_cast<uintptr_t>(k + row * (2 * D) + k_slot<D>(row, 2 * j + lg) * 16));
+    }
+  };
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) read_k(j);
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    if (j + kAhead < NJ) read_k(j + kAhead);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) s[b] = mfma32(kf[j % (kAhead + 1)][b], q[j], s[b]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  v8 vf[2][ND];  // V^T operands: the first step's wait behind the softmax
+  const auto read_v = [&](int j) {
+#pragma unroll
+    for (int db = 0; db < ND; ++db) vf[j % 2][db] = read_vt<T, D>(v, 16 * j, db, lane);
+  };
+  read_v(0);
+  if (masked) {  // wave-uniform
+    const int rel = limit - kv0 - 4 * lg;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (32 * b + 8 * (r >> 2) + (r & 3) > rel) s[b][r] = -INFINITY;
+  }
+  float top = -INFINITY;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
+  top = xor_max<32>(top) * factor;
+  if (__builtin_amdgcn_ballot_w64(top > st.m + kSlack)) {  // wave-uniform
+    const float m_new = fmaxf(st.m, top);
+    const float corr = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m - m_new);
+    st.l *= corr;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) st.o[db][r] *= corr;
+    st.m = m_new;
+  }
+  const float m = st.m == -INFINITY ? 0.f : st.m;  // a row that has seen no key yet: its weights are 0
+  float sum = 0.f;
+  v8 p[TK / 16];
+#pragma unroll
+  for (int b = 0; b < TK / 32; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; r += 2) {
+      v2 x;
+      x[0] = static_cast<T>(__builtin_amdgcn_exp2f(fmaf(s[b][r], factor, -m)));
+      x[1] = static_cast<T>(__builtin_amdgcn_exp2f(fmaf(s[b][r + 1], factor, -m)));
+      sum = add_pair(x, sum);
+      p[2 * b + (r >> 3)][r & 7] = x[0];
+      p[2 * b + (r >> 3)][(r & 7) + 1] = x[1];
+    }
+  st.l += xor_add<32>(sum);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int j = 0; j < NP; ++j) {
+    if (j + 1 < NP) read_v(j + 1);
+#pragma unroll
+    for (int db = 0; db < ND; ++db) st.o[db] = mfma32(vf[j % 2][db], p[j], st.o[db]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+template <class T, int D, int QG, int KP, int TK, int ST, bool CAUSAL>
+__global__ void __launch_bounds__(QG * KP * 64) prompt_attention_kernel(PromptArgs a) {
+  typedef typename Types<T>::v8 v8;
+  constexpr int kRows = 32 * QG, kTile = TK * D * 2, kStage = KP * 2 * kTile, kChunks = D / 8;
+  constexpr int kCopies = kTile / 1024 / QG;  // per wave, of a K tile and of a V tile
+  constexpr int kMergeF = 2 + D / 2;          // floats a lane hands over
+  static_assert(kTile / 1024 % QG == 0, "copies");
+  constexpr int kRing = ST * kStage, kMerge = (KP - 1) * QG * 64 * kMergeF * 4;
+  __shared__ __align__(1024) uint8_t ring[kRing > kMerge ? kRing : kMerge];
+  __shared__ OddValues<D> odd;
+
+  const int kvh = blockIdx.x % a.kv_heads, group = a.heads / a.kv_heads;
+  Job job;
+  if (!find_job<kRows>(a, blockIdx.x / a.kv_heads, CAUSAL, job)) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wq = wave % QG, part = wave / QG, lr = lane & 31, lg = lane >> 5;
+  // this lane's row (its last one for lanes past the end, which store nothing) and the last key it sees
+  const int row = job.row0 + 32 * wq + lr, at_row = min(row, job.rows - 1), query = at_row / group;
+  const int head = kvh * group + at_row % group;
+  const int seen0 = CAUSAL ? job.nk - job.nq : job.nk - 1;  // last key that query 0 sees
+  const int limit = CAUSAL ? seen0 + query : seen0;
+  const auto limit_of = [&](int r) { return CAUSAL ? seen0 + min(r, job.rows - 1) / group : seen0; };
+  const int wave_first = limit_of(job.row0 + 32 * wq), wave_last = limit_of(job.row0 + 32 * wq + 31);
+  const int block_first = limit_of(job.row0), block_last = limit_of(job.row0 + kRows - 1);
+
+  v8 q[D / 16];
+  const T* qp = static_cast<const T*>(a.q) + (job.q0 + query) * a.q_row + head * a.q_head + 8 * lg;
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j) q[j] = *reinterpret_cast<const v8*>(qp + 16 * j);
+  if (a.scale < 0.f) {  // scores are scaled by a positive factor after the product
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) q[j] = -q[j];
+  }
+  const float factor = fmaxf(__builtin_fabsf(a.scale) * kLog2e, 1e-30f);  // 0: so small that scores vanish
+
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ring));
+  const T* kbase = static_cast<const T*>(a.k) + job.k0 * a.k_row + kvh * a.k_head;
+  const T* vbase = static_cast<const T*>(a.v) + job.k0 * a.v_row + kvh * a.v_head;
+  const int tiles = block_last < 0 ? 0 : block_last / TK + 1, stages = (tiles + KP - 1) / KP;
+  const int crow = lane / kChunks, cslot = lane % kChunks;  // a copy fills 64 / kChunks rows
+  const auto issue = [&](int p) {
+    // a part whose tile is past the end copies the last one again: every wave issues the same number of copies
+    const int t = min(KP * p + part, tiles - 1), kv0 = t * TK, last = job.nk - 1 - kv0;
+    const uint32_t stage = lds0 + (p % ST) * kStage + part * 2 * kTile;
+    const T *kb = kbase + kv0 * a.k_row, *vb = vbase + kv0 * a.v_row;
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const int blk = kCopies * wq + i, r = blk * (64 / kChunks) + crow, rc = min(r, last);  // keys past the end: the last one
+      dma16_s(static_cast<uint32_t>(rc) * static_cast<uint32_t>(a.k_row * 2) + k_slot<D>(r, cslot) * 16, kb, stage + blk * 1024);
+    }
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const int blk = kCopies * wq + i, r = blk * (64 / kChunks) + crow, rc = min(r, last);
+      dma16_s(static_cast<uint32_t>(rc) * static_cast<uint32_t>(a.v_row * 2) + v_slot<D>(r, cslot) * 16, vb,
+              stage + kTile + blk * 1024);
+    }
+  };
+#pragma unroll
+  for (int p = 0; p < ST - 1; ++p)
+    if (p < stages) issue(p);
+
+  State<D> st;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) st.o[db][r] = 0.f;
+  st.m = -INFINITY;
+  st.l = 0.f;
+  for (int i = tid; i < 3 * D; i += QG * KP * 64) (&odd.first[0][0])[i] = kNoKey;
+  if (tid == 0) odd.any = 0;
+
+  for (int p = 0; p < stages; ++p) {
+    // stage p visible to every wave, every wave done with stage p - 1, whose slot takes stage p + ST - 1
+    wait_stages_ahead<2 * kCopies, ST - 1>(min(ST - 2, stages - 1 - p));
+    lds_barrier();
+    if (p + ST - 1 < stages) issue(p + ST - 1);
+    const int t = KP * p + part, kv0 = t * TK;
+    const uint32_t k = lds0 + (p % ST) * kStage + part * 2 * kTile, v = k + kTile;
+    if (KP * (p + 1) * TK - 1 > block_first) {  // some row of the block sees only a part of this stage
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        const int blk = kCopies * wq + i, r = blk * (64 / kChunks) + crow;
+        set_aside<T, D>(v + blk * 1024 + lane * 16, kv0 + r, v_slot<D>(r, cslot) * 8, odd);
+      }
+      lds_barrier();
+    }
+    if (kv0 <= wave_last) tile<T, D, TK>(k, v, q, factor, kv0, limit, kv0 + TK - 1 > wave_first, lane, st);
+  }
+
+  float m = st.m, l = st.l, scale_o = 1.f;
+  if constexpr (KP > 1) {
+    // parts 1 .. KP - 1 hand (m, l, O) through LDS to the wave of part 0 with the same rows
+    lds_barrier();  // every wave is done with the ring
+    float* mine = reinterpret_cast<float*>(ring) + (wq * 64 + lane) * kMergeF;
+    constexpr int kPartF = QG * 64 * kMergeF;
+    if (part > 0) {
+      float* to = mine + (part - 1) * kPartF;
+      to[0] = st.m;
+      to[1] = st.l;
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) to[2 + 16 * db + r] = st.o[db][r];
+    }
+    lds_barrier();
+    if (part > 0) return;
+#pragma unroll
+    for (int i = 0; i < KP - 1; ++i) m = fmaxf(m, mine[i * kPartF]);
+    scale_o = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m - m);
+    l *= scale_o;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) st.o[db][r] *= scale_o;
+#pragma unroll
+    for (int i = 0; i < KP - 1; ++i) {
+      const float* from = mine + i * kPartF;
+      const float e = from[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(from[0] - m);
+      l = fmaf(e, from[1], l);
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) st.o[db][r] = fmaf(e, from[2 + 16 * db + r], st.o[db][r]);
+    }
+  }
+  else {
+    lds_barrier();  // `odd` is complete and visible
+  }
+  if (row >= job.rows) return;
+  if (odd.any) {
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int d = 32 * db + 8 * (r >> 2) + 4 * lg + (r & 3);
+        if (odd.first[0][d] <= limit) st.o[db][r] += INFINITY;
+        if (odd.first[1][d] <= limit) st.o[db][r] -= INFINITY;
+        if (odd.first[2][d] <= limit) st.o[db][r] = __builtin_nanf("");
+      }
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;  // no key seen: zeros
+  T* op = static_cast<T*>(a.out) + (job.q0 + query) * a.o_row + head * a.o_head + 4 * lg;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      typedef T v4 __attribute__((ext_vector_type(4)));
+      v4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = static_cast<T>(st.o[db][4 * j + e] * inv);
+      *reinterpret_cast<v4*>(op + 32 * db + 8 * j) = x;
+    }
 }
 
 bool rows_ok(const void* p, int64_t row, int64_t head) {
@@ -75,17 +459,35 @@ extern "C" int fw_prompt_attention(const void* q, int64_t q_row, int64_t q_head,
   if ((q_rows > 0 && (!rows_ok(q, q_row, q_head) || !rows_ok(out, o_row, o_head))) ||
       (k_rows > 0 && (!rows_ok(k, k_row, k_head) || !rows_ok(v, v_row, v_head))))
     return fw_fail(FW_EINVAL, "prompt_attention: q, k, v and out must be 16-byte aligned with strides in multiples of 8");
+  // 64 rows of k and of v within the copies' 32-bit byte offsets; rows x heads of a sequence are counted in 32 bits
+  if (k_row < 0 || v_row < 0 || k_row >= (1 << 25) || v_row >= (1 << 25))
+    return fw_fail(FW_EINVAL, "prompt_attention: row strides of k and v must be below 2^25 elements");
+  if (q_rows * (heads / kv_heads) > 0x7FFFFF00 || k_rows > 0x7FFFFF00) return fw_fail(FW_EINVAL, "prompt_attention: too many rows");
   if (q_rows == 0) return FW_OK;
   const PromptArgs a{q, k, v, out, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, cu_q, cu_k, q_rows, k_rows, n_seq, heads, kv_heads, scale};
-  const int64_t blocks = (q_rows * heads + 3) / 4;
-  if (blocks > 0x7FFFFFFF) return fw_fail(FW_EINVAL, "prompt_attention: too many rows");
-  const auto launch = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, a);
+  const int64_t rows = q_rows * (heads / kv_heads);
+  int rc = FW_OK;
+  const auto launch = [&](auto kernel, int per_block, int threads) {
+    const int64_t blocks = (rows / per_block + n_seq) * kv_heads;  // a sequence's last block may be partial
+    if (blocks > 0x7FFFFFFF) rc = fw_fail(FW_EINVAL, "prompt_attention: too many rows");
+    else hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(threads), 0, stream, a);
   };
-  const auto by_mask = [&](auto full, auto masked) { causal ? launch(masked) : launch(full); };
-  if (dtype == FW_F16 && head_dim == 64) by_mask(prompt_attention_kernel<_Float16, 64, false>, prompt_attention_kernel<_Float16, 64, true>);
-  else if (dtype == FW_F16) by_mask(prompt_attention_kernel<_Float16, 128, false>, prompt_attention_kernel<_Float16, 128, true>);
-  else if (head_dim == 64) by_mask(prompt_attention_kernel<__bf16, 64, false>, prompt_attention_kernel<__bf16, 64, true>);
-  else by_mask(prompt_attention_kernel<__bf16, 128, false>, prompt_attention_kernel<__bf16, 128, true>);
-  return fw_check_launch("prompt_attention");
+#ifndef PA_CFG
+#define PA_CFG 0
+#endif
+  const auto by_rows = [&](auto t, auto d, auto mask) {
+    typedef decltype(t) T;
+    constexpr int D = decltype(d)::value;
+    constexpr bool M = decltype(mask)::value;
+    const int cfg = PA_CFG ? PA_CFG : rows / n_seq >= 512 ? 1 : rows / n_seq >= 256 ? 2 : 3;
+    if (cfg == 1) launch(prompt_attention_kernel<T, D, 8, 1, 64, 2, M>, 256, 512);
+    else if (cfg == 2) launch(prompt_attention_kernel<T, D, 4, 1, 64, 2, M>, 128, 256);
+    else launch(prompt_attention_kernel<T, D, 1, 4, 32, 2, M>, 32, 256);
+  };
+  const auto by_mask = [&](auto t, auto d) { causal ? by_rows(t, d, std::true_type()) : by_rows(t, d, std::false_type()); };
+  const std::integral_constant<int, 64> d64;
+  const std::integral_constant<int, 128> d128;
+  if (dtype == FW_F16) head_dim == 64 ? by_mask(_Float16(), d64) : by_mask(_Float16(), d128);
+  else head_dim == 64 ? by_mask(__bf16(), d64) : by_mask(__bf16(), d128);
+  return rc ? rc : fw_check_launch("prompt_attention");
 }

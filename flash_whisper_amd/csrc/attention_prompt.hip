@@ -69,10 +69,7 @@ struct PromptArgs {
 // ------------------------------------------------------------------------------------------
 constexpr float kSlack = 8.f;
 constexpr float kLog2e = 1.4426950408889634f;
-#ifndef PA_AHEAD
-#define PA_AHEAD 2
-#endif
-constexpr int kAhead = PA_AHEAD;
+constexpr int kAhead = 2;  // 1 to 4 measured within 2% of each other
 
 template <int D>
 __device__ __forceinline__ int k_slot(int row, int chunk) {
@@ -151,16 +148,32 @@ struct State {
   float m, l;
 };
 
-// V^T operand of dims 32 db .. and the 16 keys from row `key` of a staged V tile.
+// Byte offsets of a lane's operands in staged tiles, apart from the multiples of 8 and 32 rows that the reads add as
+// constants: K row lr, chunk 2 j + lg; V row 4 lg + i / 4, dims 32 db + 16 (lane / 16 % 2) + 4 (i % 4), for i =
+// lane % 16. The swizzles do not depend on those multiples.
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+typedef __attribute__((address_space(3))) s4v lds_s4;
+template <int D>
+struct Offsets {
+  uint32_t k[D / 16], v[D / 32];
+};
+template <int D>
+__device__ __forceinline__ Offsets<D> lane_offsets(int lane) {
+  Offsets<D> o;
+  const int lr = lane & 31, lg = lane >> 5, i = lane & 15, row = 4 * lg + (i >> 2);
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j) o.k[j] = lr * (2 * D) + k_slot<D>(lr, 2 * j + lg) * 16;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+    o.v[db] = row * (2 * D) + v_slot<D>(row, 4 * db + 2 * ((lane >> 4) & 1) + ((i >> 1) & 1)) * 16 + (i & 1) * 8;
+  return o;
+}
+
+// V^T operand of 32 dims and 16 keys: two transposing reads of 4 keys a lane half, 8 keys apart.
 template <class T, int D>
-__device__ __forceinline__ typename Types<T>::v8 read_vt(uint32_t v, int key, int db, int lane) {
-  const int i = lane & 15, row = key + 4 * (lane >> 5) + (i >> 2), chunk = 4 * db + 2 * ((lane >> 4) & 1) + ((i >> 1) & 1);
-  typedef __attribute__((address_space(3))) s4v lds_s4;
-  typedef short s8v __attribute__((ext_vector_type(8)));
-  const auto at = [&](int r) {
-    return reinterpret_cast<lds_s4*>(static_cast<uintptr_t>(v + r * (2 * D) + v_slot<D>(r, chunk) * 16 + (i & 1) * 8));
-  };
-  const s4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(row)), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(row + 8));
+__device__ __forceinline__ typename Types<T>::v8 read_vt(lds_u8* at) {
+  const s4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4*>(at));
+  const s4v b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4*>(at + 8 * 2 * D));
   return __builtin_bit_cast(typename Types<T>::v8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
@@ -196,11 +209,11 @@ __device__ __forceinline__ void set_aside(uint32_t at, int key, int d, OddValues
 // A wave's tile: K at LDS address k, V at v; keys kv0 .., of which the lane's row sees those up to `limit`; masked:
 // some row does not see all of them.
 template <class T, int D, int TK>
-__device__ __forceinline__ void tile(uint32_t k, uint32_t v, const typename Types<T>::v8 (&q)[D / 16], float factor, int kv0,
+__device__ __forceinline__ void tile(uint32_t k, uint32_t v, const Offsets<D>& off, const typename Types<T>::v8 (&q)[D / 16], float factor, int kv0,
                                      int limit, bool masked, int lane, State<D>& st) {
   typedef typename Types<T>::v8 v8;
   typedef typename Types<T>::v2 v2;
-  const int lr = lane & 31, lg = lane >> 5;
+  const int lg = lane >> 5;
   typedef __attribute__((address_space(3))) v8 lds_v8;
   constexpr int NB = TK / 32, NJ = D / 16, NP = TK / 16, ND = D / 32;
   f16v s[NB];
@@ -212,11 +225,9 @@ __device__ __forceinline__ void tile(uint32_t k, uint32_t v, const typename Type
   // since all of a tile's operands at once do not fit the registers.
   v8 kf[kAhead + 1][NB];
   const auto read_k = [&](int j) {
+    lds_u8* at = reinterpret_cast<lds_u8*>(static_cast<uintptr_t>(off.k[j] + k));
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const int row = 32 * b + lr;
-      kf[j % (kAhead + 1)][b] = *reinterpret_cast<lds_v8*>(static_cast<uintptr_t>(k + row * (2 * D) + k_slot<D>(row, 2 * j + lg) * 16));
-    }
+    for (int b = 0; b < NB; ++b) kf[j % (kAhead + 1)][b] = *reinterpret_cast<lds_v8*>(at + b * (32 * 2 * D));
   };
 #pragma unroll
   for (int j = 0; j < kAhead; ++j) read_k(j);
@@ -228,9 +239,12 @@ __device__ __forceinline__ void tile(uint32_t k, uint32_t v, const typename Type
     __builtin_amdgcn_sched_barrier(0);
   }
   v8 vf[2][ND];  // V^T operands: the first step's wait behind the softmax
+  lds_u8* vat[ND];
+#pragma unroll
+  for (int db = 0; db < ND; ++db) vat[db] = reinterpret_cast<lds_u8*>(static_cast<uintptr_t>(off.v[db] + v));
   const auto read_v = [&](int j) {
 #pragma unroll
-    for (int db = 0; db < ND; ++db) vf[j % 2][db] = read_vt<T, D>(v, 16 * j, db, lane);
+    for (int db = 0; db < ND; ++db) vf[j % 2][db] = read_vt<T, D>(vat[db] + j * (16 * 2 * D));
   };
   read_v(0);
   if (masked) {  // wave-uniform
@@ -245,7 +259,7 @@ __device__ __forceinline__ void tile(uint32_t k, uint32_t v, const typename Type
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
+    for (int r = 0; r < 16; ++r) top = __builtin_elementwise_maximum(top, s[b][r]);  // a NaN score: the row is NaN anyway
   top = xor_max<32>(top) * factor;
   if (__builtin_amdgcn_ballot_w64(top > st.m + kSlack)) {  // wave-uniform
     const float m_new = fmaxf(st.m, top);
@@ -283,7 +297,7 @@ __device__ __forceinline__ void tile(uint32_t k, uint32_t v, const typename Type
 }
 
 template <class T, int D, int QG, int KP, int TK, int ST, bool CAUSAL>
-__global__ void __launch_bounds__(QG * KP * 64) prompt_attention_kernel(PromptArgs a) {
+__global__ void __launch_bounds__(QG * KP * 64, 2) prompt_attention_kernel(PromptArgs a) {
   typedef typename Types<T>::v8 v8;
   constexpr int kRows = 32 * QG, kTile = TK * D * 2, kStage = KP * 2 * kTile, kChunks = D / 8;
   constexpr int kCopies = kTile / 1024 / QG;  // per wave, of a K tile and of a V tile
@@ -343,6 +357,7 @@ __global__ void __launch_bounds__(QG * KP * 64) prompt_attention_kernel(PromptAr
   for (int p = 0; p < ST - 1; ++p)
     if (p < stages) issue(p);
 
+  const Offsets<D> off = lane_offsets<D>(lane);
   State<D> st;
 #pragma unroll
   for (int db = 0; db < D / 32; ++db)
@@ -353,11 +368,24 @@ __global__ void __launch_bounds__(QG * KP * 64) prompt_attention_kernel(PromptAr
   for (int i = tid; i < 3 * D; i += QG * KP * 64) (&odd.first[0][0])[i] = kNoKey;
   if (tid == 0) odd.any = 0;
 
+  // Waves of a part share its tiles; with one wave a part the rings are the waves' own and nobody waits for others.
+  const auto sync = [&] {
+    if constexpr (QG > 1) lds_barrier();
+    else lds_reads_done();
+  };
+  if constexpr (QG == 1) lds_barrier();  // `odd` is cleared
   for (int p = 0; p < stages; ++p) {
-    // stage p visible to every wave, every wave done with stage p - 1, whose slot takes stage p + ST - 1
-    wait_stages_ahead<2 * kCopies, ST - 1>(min(ST - 2, stages - 1 - p));
-    lds_barrier();
-    if (p + ST - 1 < stages) issue(p + ST - 1);
+    // stage p visible to every wave of the part, every one done with stage p - 1, whose slot takes stage p + ST - 1
+    if constexpr (ST > 1) {
+      wait_stages_ahead<2 * kCopies, ST - 1>(min(ST - 2, stages - 1 - p));
+      sync();
+      if (p + ST - 1 < stages) issue(p + ST - 1);
+    } else {
+      sync();
+      issue(p);
+      wait_vmcnt<0>();
+      sync();
+    }
     const int t = KP * p + part, kv0 = t * TK;
     const uint32_t k = lds0 + (p % ST) * kStage + part * 2 * kTile, v = k + kTile;
     if (KP * (p + 1) * TK - 1 > block_first) {  // some row of the block sees only a part of this stage
@@ -366,9 +394,9 @@ __global__ void __launch_bounds__(QG * KP * 64) prompt_attention_kernel(PromptAr
         const int blk = kCopies * wq + i, r = blk * (64 / kChunks) + crow;
         set_aside<T, D>(v + blk * 1024 + lane * 16, kv0 + r, v_slot<D>(r, cslot) * 8, odd);
       }
-      lds_barrier();
+      sync();
     }
-    if (kv0 <= wave_last) tile<T, D, TK>(k, v, q, factor, kv0, limit, kv0 + TK - 1 > wave_first, lane, st);
+    if (kv0 <= wave_last) tile<T, D, TK>(k, v, off, q, factor, kv0, limit, kv0 + TK - 1 > wave_first, lane, st);
   }
 
   float m = st.m, l = st.l, scale_o = 1.f;
@@ -472,17 +500,21 @@ extern "C" int fw_prompt_attention(const void* q, int64_t q_row, int64_t q_head,
     if (blocks > 0x7FFFFFFF) rc = fw_fail(FW_EINVAL, "prompt_attention: too many rows");
     else hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(threads), 0, stream, a);
   };
-#ifndef PA_CFG
-#define PA_CFG 0
-#endif
   const auto by_rows = [&](auto t, auto d, auto mask) {
     typedef decltype(t) T;
     constexpr int D = decltype(d)::value;
     constexpr bool M = decltype(mask)::value;
-    const int cfg = PA_CFG ? PA_CFG : rows / n_seq >= 512 ? 1 : rows / n_seq >= 256 ? 2 : 3;
-    if (cfg == 1) launch(prompt_attention_kernel<T, D, 8, 1, 64, 2, M>, 256, 512);
-    else if (cfg == 2) launch(prompt_attention_kernel<T, D, 4, 1, 64, 2, M>, 128, 256);
-    else launch(prompt_attention_kernel<T, D, 1, 4, 32, 2, M>, 32, 256);
+    // Blocks of 128 rows stage every tile for four waves. They are the fastest where they fill the CUs; fewer rows
+    // are given to more blocks, and long chains of tiles to several waves, whose parts are then merged (us of 128 rows
+    // / 64 rows and 2 parts of 64 keys / of 32 keys / 32 rows and 8 parts, heads of 64 unless said: 1 x 4 queries x 20
+    // heads over 1500 keys 24.5 / 15.4 / 17.4 / 11.7; 1 x 1500 x 20, causal 27.1 / 18.4 / 19.9 / 24.9; 8 x 64 x 32 over
+    // 4000 keys and 8 heads of 128 84 / 68 / 79 / 87; 16 x 4 .. 224 x 20, causal 9.8 / 11.7 / 8.8 / 17.3, over 1500 keys
+    // 37.8 / 48.2 / 38.8 / 50.4).
+    const int64_t wide = (rows / 128 + n_seq) * kv_heads, keys = k_rows / n_seq;
+    if (wide <= 128 && keys >= 512) launch(prompt_attention_kernel<T, D, 1, 8, 32, 1, M>, 32, 512);
+    else if (wide <= 384 && keys >= 512) launch(prompt_attention_kernel<T, D, 2, 2, 64, 2, M>, 64, 256);
+    else if (wide <= 384 || keys < 256) launch(prompt_attention_kernel<T, D, 2, 2, 32, 2, M>, 64, 256);
+    else launch(prompt_attention_kernel<T, D, 4, 1, 64, 2, M>, 128, 256);
   };
   const auto by_mask = [&](auto t, auto d) { causal ? by_rows(t, d, std::true_type()) : by_rows(t, d, std::false_type()); };
   const std::integral_constant<int, 64> d64;

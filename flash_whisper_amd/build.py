@@ -4,7 +4,9 @@
 parallel, one object per source) and links them. The library exports the entry points declared in
 ``include/flash_whisper.h``. It also links the profiling build ``libflash_whisper_timeline.so``: the
 same objects with the decoder step compiled with FW_STEP_TIMELINE=1, which records the phase timeline
-that ``python -m flash_whisper_amd.step_timeline`` reads (selected with FW_LIBRARY; never the default). This replaces the reference's JIT extension build (custom/ext.py:13-18),
+that ``python -m flash_whisper_amd.step_timeline`` reads (selected with FW_LIBRARY; never the default), and
+the Python module ``_bind.so`` (csrc/bind.cpp), through which ext.py calls the ops whose kernels take less time than
+a ctypes call. This replaces the reference's JIT extension build (custom/ext.py:13-18),
 which ran nvcc through torch.utils.cpp_extension; here the build is ahead-of-time and in-tree so the
 built library travels with the source tree.
 """
@@ -23,6 +25,7 @@ BUILD_DIR = Path(os.environ.get('FW_BUILD_DIR', PKG / '_build'))
 LIB = PKG / 'libflash_whisper.so'
 TIMELINE_LIB = PKG / 'libflash_whisper_timeline.so'
 TIMELINE_SRC = 'decode_step.hip'  # the one source the profiling build compiles differently
+BIND_LIB = PKG / '_bind.so'  # the Python module of csrc/bind.cpp
 ARCH = os.environ.get('FW_OFFLOAD_ARCH', 'gfx950')
 HIPCC = os.environ.get('HIPCC', shutil.which('hipcc') or '/opt/rocm/bin/hipcc')
 
@@ -79,17 +82,40 @@ def _link(objs, lib, verbose):
     os.replace(tmp, lib)  # atomic: a process that already mapped the old file keeps it
 
 
+def _compile_bind(verbose):
+    """csrc/bind.cpp, host code on torch's and Python's headers, into the module _bind."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    tmp = BIND_LIB.with_suffix('.so.tmp')
+    cmd = [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared', '-Wall',
+           f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}', '-D__HIP_PLATFORM_AMD__=1',
+           *(f'-isystem{p}' for p in [*include_paths(), '/opt/rocm/include', sysconfig.get_paths()['include']]),
+           str(CSRC / 'bind.cpp'), '-o', str(tmp), *(f'-L{p}' for p in library_paths()), '-ltorch_python', '-ltorch_cpu',
+           '-lc10']
+    if verbose:
+        print(' '.join(cmd), flush=True)
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f'{cmd[0]} failed for bind.cpp:\n{proc.stdout}{proc.stderr}')
+    os.replace(tmp, BIND_LIB)
+
+
 def build(verbose=False, jobs=None):
-    """Compiles all sources and links the shared library and its phase-timeline profiling build. Always
-    rebuilds. Returns the product library's path."""
+    """Compiles all sources and links the shared library, its phase-timeline profiling build and the Python
+    module of the small ops' calls. Always rebuilds. Returns the product library's path."""
     BUILD_DIR.mkdir(parents=True, exist_ok=True)
     srcs = sources()
     tl_src = next(s for s in srcs if s.name == TIMELINE_SRC)
-    jobs = jobs or min(len(srcs) + 1, max(1, min(16, os.cpu_count() or 1)))
+    jobs = jobs or min(len(srcs) + 2, max(1, min(16, os.cpu_count() or 1)))
     with ThreadPoolExecutor(jobs) as pool:
+        bind = pool.submit(_compile_bind, verbose)
         tl_obj = pool.submit(_compile, tl_src, verbose, ('-DFW_STEP_TIMELINE=1',), '_timeline')
         objs = list(pool.map(lambda s: _compile(s, verbose), srcs))
         tl_obj = tl_obj.result()
+        bind.result()
     _link(objs, LIB, verbose)
     _link([tl_obj if o.stem == tl_src.stem else o for o in objs], TIMELINE_LIB, verbose)
     return LIB

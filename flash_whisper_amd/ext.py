@@ -24,6 +24,11 @@ from . import _lib
 from ._lib import ACT_GELU, ACT_NONE, EPI_BIAS  # noqa: F401  (re-exported constants)
 from .config import SPLIT_KEYS
 
+try:
+    from . import _bind  # the same calls without ctypes (built with the library); absent, they go through ctypes
+except ImportError:
+    _bind = None
+
 HIDDEN, HEAD_DIM = 1280, 64
 MAX_BATCH = 4  # decoder positions per batched launch (the prompt)
 WAVE_CHUNK = 240000  # samples per staged chunk of the waveform upload (half of 30 s: smaller chunks measured slower)
@@ -93,7 +98,7 @@ _DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 def _current_device():
     """The current device's index; before torch's first GPU call None, which no tensor is on."""
-    return _device() if torch.cuda.is_initialized() and _device is not None else None
+    return _device() if torch.cuda.is_initialized() and _device is not None and _raw_stream is not None else None
 
 
 def _heads_view(t, name, dtype, dev, heads, dim):
@@ -178,6 +183,10 @@ class WhisperExt:
 
     def __init__(self):
         self.lib = _lib.lib()
+        self._bind = _bind
+        if _bind is not None:
+            for name in ('fw_prompt_attention', 'fw_kv_q4_append', 'fw_kv_q4_read', 'fw_decode_attention_q4'):
+                _bind.set_entry(name, ctypes.cast(getattr(self.lib, name), ctypes.c_void_p).value)
 
     def _call(self, name, *args):
         status = getattr(self.lib, name)(*args)
@@ -398,6 +407,10 @@ class WhisperExt:
         the device). causal: a query sees the keys up to its own place counted from the end of both. A query that sees
         no key gets zeros; rows of out behind the last sequence are left as they are."""
         dev = _current_device()
+        # the compiled binding makes a valid call; what it refuses comes to the named checks below
+        if self._bind and dev is not None and self._bind.prompt_attention(q, k, v, out, cu_q, cu_k, scale, causal, dev,
+                                                                         _raw_stream(dev)):
+            return
         dtype = getattr(q, 'dtype', None)
         if dtype not in _DTYPES or q.dim() != 3 or q.size(2) not in (64, 128):
             raise RuntimeError('q must be fp16 or bf16 [rows, heads, 64 or 128]')
@@ -441,12 +454,18 @@ class WhisperExt:
     def kv_q4_append(self, k, v, cu, pos, cache):
         """Writes the packed rows cu[s] .. cu[s + 1] - 1 of k and v ([rows, kv_heads, head_dim], fp16 or bf16) into rows
         pos[s] .. of sequence s of the 4-bit cache (fw_kv_q4_append). Rows that fall outside it are dropped."""
+        dev = _current_device()
+        if self._bind and dev is not None and self._bind.kv_q4_append(k, v, cu, pos, cache, dev, _raw_stream(dev)):
+            return
         rows, arrays, sizes, places, dtype = self._packed(k, v, cu, pos, cache, _heads_view)
         self._call('fw_kv_q4_append', *rows, k.size(0), *places, *arrays, *sizes, _DTYPES[dtype], _stream())
 
     def kv_q4_read(self, cache, cu, pos, k, v):
         """The values that the cache holds for its rows pos[s] .. into rows cu[s] .. cu[s + 1] - 1 of k and v
         (fw_kv_q4_read): the counterpart of kv_q4_append, for a prompt that goes on where an earlier one ended."""
+        dev = _current_device()
+        if self._bind and dev is not None and self._bind.kv_q4_read(cache, cu, pos, k, v, dev, _raw_stream(dev)):
+            return
         rows, arrays, sizes, places, dtype = self._packed(k, v, cu, pos, cache, _out_view)
         self._call('fw_kv_q4_read', *arrays, *sizes, *places, k.size(0), *rows, _DTYPES[dtype], _stream())
 
@@ -463,6 +482,9 @@ class WhisperExt:
         (fw_decode_attention_q4). lens is int64 on the device and is not advanced; a negative one marks an idle
         sequence, which gets zeros and whose cache stays as it is."""
         dev = _current_device()
+        if self._bind and dev is not None and self._bind.decode_attention_q4(q, cache, lens, out, ws, scale, k_new, v_new,
+                                                                            dev, _raw_stream(dev)):
+            return
         n, kv_heads, max_len, dim = _cache_sizes(cache, dev)
         dtype = getattr(q, 'dtype', None)
         if dtype not in _DTYPES:

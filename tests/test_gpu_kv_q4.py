@@ -362,3 +362,35 @@ def test_prompt_then_tokens(ext, hip_device, kind, dim, heads, kv_heads):
             serving.write_row(want, s, now[s], new[1][0][s].float().numpy(), new[2][0][s].float().numpy())
         assert same_bits(cache, want) and lens.tolist() == [x + 1 for x in now]
         _check_decode(out.double().cpu().numpy(), new[0][1], want, [x + 1 for x in now], scale, dtype)
+
+
+@pytest.mark.parametrize('kind', ['fp16', 'bf16'])
+def test_compiled_binding_and_ctypes(ext, hip_device, kind):
+    """Every op through the compiled binding alone (a call that it leaves to ctypes fails here) and through ctypes alone:
+    the same bits, on a stream of its own each."""
+    from flash_whisper_amd.ext import WhisperExt
+
+    assert ext._bind is not None
+    dev, dtype, rng = hip_device, TYPES[kind], np.random.default_rng(15)
+    q, k, v = (rounded(rng, (40, h, 64), dtype)[0].to(dev) for h in (4, 2, 2))
+    cu, pos, one = starts([7, 33], dev), _index([3, 0], dev), _index([20, 33], dev)
+    results = []
+    for compiled in (True, False):
+        e = WhisperExt()
+        if compiled:
+            e._call = None
+        else:
+            e._bind = None
+        with torch.cuda.stream(torch.cuda.Stream()):
+            cache = e.kv_q4_cache(2, 2, 64, 64)
+            ws = e.decode_attention_q4_workspace(2, 4, cache)
+            outs = [torch.zeros_like(t) for t in (q, k, v)] + [torch.zeros(2, 4, 64, dtype=dtype, device=dev) for _ in range(2)]
+            e.prompt_attention(q, k, v, outs[0], cu, cu, 0.125)
+            e.prompt_attention(q, k, v, outs[0], cu, cu, 0.125, causal=False)
+            e.kv_q4_append(k, v, cu, pos, cache)
+            e.kv_q4_read(cache, cu, pos, outs[1], outs[2])
+            e.decode_attention_q4(q[:2], cache, pos, outs[3], ws, 0.125)
+            e.decode_attention_q4(q[:2], cache, one, outs[4], ws, 0.125, k[:2], v[:2])
+        torch.cuda.synchronize()
+        results.append(outs + list(cache))
+    assert all(torch.equal(a, b) for a, b in zip(*results))

@@ -140,3 +140,20 @@ def test_oracle_cache_rows(dim):
     serving.write_row(cache, 1, 7, x[2, 0], x[2, 1])
     k, _ = serving.read_rows(cache, 1, [7])
     assert np.isnan(k[0, 1, 32:64]).all() and np.isfinite(k[0, 1, :32]).all() and np.isfinite(k[0, 0]).all()
+
+
+def test_binding_refuses_without_a_call(built_lib):
+    """The compiled binding answers False, and makes no call, for anything that is not a valid call on the GPU named."""
+    from flash_whisper_amd import _bind
+    from flash_whisper_amd.ext import load_ext
+
+    cache = load_ext().kv_q4_cache(2, 2, 64, 64, device='cpu')
+    q, cu = torch.zeros(4, 2, 64, dtype=torch.float16), torch.zeros(3, dtype=torch.int64)
+    for args in ((), (q, q, q, q, cu, cu, 0.125, True, 0, 0), (q, q, q, q, cu, cu, 'x', True, 0, 0), (None,) * 10,
+                 (q, q, q, q, cu, cu, 0.125, True, 1 << 70, 0)):
+        assert _bind.prompt_attention(*args) is False
+    assert _bind.kv_q4_append(q, q, cu, cu[:2], cache, 0, 0) is False
+    assert _bind.kv_q4_read(cache, cu, cu[:2], q, q, 0, 0) is False and _bind.kv_q4_read(None, cu, cu[:2], q, q, 0, 0) is False
+    assert _bind.decode_attention_q4(q[:2], cache, cu[:2], q[:2], torch.zeros(4), 0.125, None, None, 0, 0) is False
+    with pytest.raises(ValueError):
+        _bind.set_entry('fw_other', 0)

@@ -4,6 +4,7 @@
 #include <type_traits>
 
 #include "lds_pipe.h"
+#include "packed_rows.h"
 
 namespace fw {
 namespace {
@@ -86,60 +87,26 @@ struct Job {
   int64_t q0, k0;
 };
 
-__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive sum over the wave
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const int x = __shfl_up(v, o);
-    if (lane >= o) v += x;
-  }
-  return v;
-}
-
-// Query rows of sequence s, its starts clamped to the rows there are.
+// Query or key rows of sequence s, its starts clamped to the rows there are.
 __device__ __forceinline__ int seq_rows(const int64_t* cu, int64_t rows, int s, int64_t& begin) {
-  begin = min(max(cu[s], int64_t{0}), rows);
-  return static_cast<int>(min(max(cu[s + 1], begin), rows) - begin);
+  begin = within(cu[s], 0, rows);
+  return static_cast<int>(within(cu[s + 1], begin, rows) - begin);
 }
 
-// Block `index` of the blocks that all sequences take; from the last one if `reverse`. False: there are fewer.
+// What the block of number `slot` does; false: nothing. Sequence s has the slots from cu_q[s] group / ROWS + s on:
+// one more than its rows fill, which its last block may need, and no sum over the sequences before it.
 template <int ROWS>
-__device__ __forceinline__ bool find_job(const PromptArgs& a, int index, bool reverse, Job& job) {
-  const int lane = threadIdx.x & 63, group = a.heads / a.kv_heads;
-  const auto blocks = [&](int s, int64_t& begin, int& nq) {
-    nq = s < a.n_seq ? seq_rows(a.cu_q, a.q_rows, s, begin) : 0;
-    return (nq * group + ROWS - 1) / ROWS;
-  };
-  if (reverse) {
-    int total = 0;
-    for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
-      int64_t begin;
-      int nq;
-      total += __builtin_amdgcn_readlane(wave_scan(blocks(s0 + lane, begin, nq), lane), 63);
-    }
-    index = total - 1 - index;
-    if (index < 0) return false;
-  }
-  for (int s0 = 0, sum = 0; s0 < a.n_seq; s0 += 64) {
-    int64_t begin = 0;
-    int nq;
-    const int n = blocks(s0 + lane, begin, nq), incl = wave_scan(n, lane) + sum;
-    const uint64_t past = __builtin_amdgcn_ballot_w64(incl > index);
-    if (past) {
-      const int at = __builtin_ctzll(past);
-      job.seq = s0 + at;
-      job.row0 = (index - (__builtin_amdgcn_readlane(incl, at) - __builtin_amdgcn_readlane(n, at))) * ROWS;
-      job.nq = __builtin_amdgcn_readlane(nq, at);
-      job.rows = job.nq * group;
-      int64_t q0, k0;
-      seq_rows(a.cu_q, a.q_rows, job.seq, q0);
-      job.nk = seq_rows(a.cu_k, a.k_rows, job.seq, k0);
-      job.q0 = q0;
-      job.k0 = k0;
-      return true;
-    }
-    sum = __builtin_amdgcn_readlane(incl, 63);
-  }
-  return false;
+__device__ __forceinline__ bool find_job(const PromptArgs& a, int64_t slot, Job& job) {
+  const int group = a.heads / a.kv_heads;
+  const auto start = [&](int s) { return within(a.cu_q[s], 0, a.q_rows) * group / ROWS + s; };
+  job.seq = last_started(a.n_seq, slot, start);
+  if (job.seq < 0) return false;
+  job.nq = seq_rows(a.cu_q, a.q_rows, job.seq, job.q0);
+  job.nk = seq_rows(a.cu_k, a.k_rows, job.seq, job.k0);
+  job.rows = job.nq * group;
+  const int64_t row0 = (slot - start(job.seq)) * ROWS;
+  job.row0 = static_cast<int>(row0);
+  return row0 < job.rows;
 }
 
 template <int D>
@@ -309,7 +276,9 @@ __global__ void __launch_bounds__(QG * KP * 64, 2) prompt_attention_kernel(Promp
 
   const int kvh = blockIdx.x % a.kv_heads, group = a.heads / a.kv_heads;
   Job job;
-  if (!find_job<kRows>(a, blockIdx.x / a.kv_heads, CAUSAL, job)) return;
+  // causal: from the last rows, whose blocks take longest
+  const unsigned slot = blockIdx.x / a.kv_heads, slots = gridDim.x / a.kv_heads;
+  if (!find_job<kRows>(a, CAUSAL ? slots - 1 - slot : slot, job)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wq = wave % QG, part = wave / QG, lr = lane & 31, lg = lane >> 5;
   // this lane's row (its last one for lanes past the end, which store nothing) and the last key it sees

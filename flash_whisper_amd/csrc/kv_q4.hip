@@ -9,7 +9,7 @@
 // A code c stands for fp16(low + step c), one rounding; 5 bits a value with step and low.
 #include <type_traits>
 
-#include "fw_common.h"
+#include "packed_rows.h"
 
 namespace fw {
 namespace {
@@ -51,31 +51,13 @@ struct Q4Slot {
   int64_t row;    // first cache row of the block, a multiple of 8 (may be negative or past the cache)
 };
 
-__device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {
-  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(v), lane);
-  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), lane);
-  return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
-}
-
 __device__ __forceinline__ Q4Slot q4_slot(const int64_t* cu, const int64_t* pos, int n_seq, int64_t rows, int64_t slot) {
-  const int lane = threadIdx.x & 63;
   Q4Slot r{-1, 0, 0, 0, 0};
-  int64_t p = 0;
-  for (int s0 = 0; s0 < n_seq; s0 += 64) {  // the last sequence whose slots begin at or before this one
-    const int s = min(s0 + lane, n_seq - 1);
-    const int64_t begin = min(max(cu[s], int64_t{0}), rows), end = min(max(cu[s + 1], begin), rows), place = pos[s];
-    const uint64_t at = __builtin_amdgcn_ballot_w64(s0 + lane < n_seq && begin / 8 + 2 * static_cast<int64_t>(s) <= slot);
-    if (at != 0) {  // the slots' begins do not fall while cu ascends; of one that does not, some sequence is taken
-      const int last = 63 - __builtin_clzll(at);
-      r.seq = s0 + last;
-      r.begin = lane_value(begin, last);
-      r.end = lane_value(end, last);
-      p = lane_value(place, last);
-    }
-    if (at != ~uint64_t{0}) break;
-  }
+  r.seq = last_started(n_seq, slot, [&](int s) { return within(cu[s], 0, rows) / 8 + 2 * static_cast<int64_t>(s); });
   if (r.seq < 0) return r;
-  const int64_t block = slot - (r.begin / 8 + 2 * static_cast<int64_t>(r.seq));
+  r.begin = within(cu[r.seq], 0, rows);
+  r.end = within(cu[r.seq + 1], r.begin, rows);
+  const int64_t p = pos[r.seq], block = slot - (r.begin / 8 + 2 * static_cast<int64_t>(r.seq));
   r.row = (p & ~int64_t{7}) + 8 * block;
   r.first = r.begin + (r.row - p);
   if (r.first >= r.end) r.seq = -1;
@@ -240,7 +222,7 @@ __global__ void __launch_bounds__(256) kv_q4_read_kernel(const int64_t* __restri
 // ------------------------------------------------------------------------------------------
 // Single-token attention. An item is a sequence, a key/value head and up to 16 of the query heads that read it;
 // S^T = K Q^T and O^T = V^T P^T are MFMAs of 16 keys or head dims by 16 query heads, so grouped heads share
-// every row that is read and dequantised. A wave takes 32 keys at a time, four waves a unit of 128 keys.
+// every row that is read and dequantised. A wave takes 32 keys at a time.
 //  - The scores' rows are assigned to keys so that lane group g = lane / 16 ends with the scores of keys
 //    8 g .. 8 g + 7 for query head lane % 16: row i of the first 16 is key 8 (i / 4) + i % 4, of the second 4
 //    more. These are the keys of one 16-byte unit of V, which the lane loads as the PV operand's source, so
@@ -250,8 +232,8 @@ __global__ void __launch_bounds__(256) kv_q4_read_kernel(const int64_t* __restri
 //    which masking a dword's nibbles yields pairs (0 4, 1 5, 2 6, 3 7).
 //  - The running maximum only moves when a score passes it by 2^kSlack (log2 units); weights stay within fp16.
 // A block takes a chunk of an item's keys; an item of one chunk is finished by its block, the chunks of a longer one
-// leave (m, l, O) in the workspace for the combine launch. Only the device knows the lengths: blocks without keys
-// end at once.
+// leave (m, l, O) in the workspace for the combine launch. Only the device knows the lengths: it puts full chunks
+// first (q4_piece), and blocks without keys end at once.
 // ------------------------------------------------------------------------------------------
 struct Q4Attn {
   const void* q;
@@ -559,8 +541,8 @@ __device__ __forceinline__ float q4_queries(const Q4Attn& a, const Q4Query<T, D>
 // Each half of a tile's registers is loaded again as soon as it is used up: K's while weights and values are worked
 // on, V's while the next tile's scores are.
 template <class T, int D>
-__device__ __forceinline__ void q4_tiles(const Q4Attn& a, int64_t hr, int first, int step, int end, int keys, int fresh,
-                                         const typename Vec8<T>::type& fresh_values, const h8v (&q)[D / 32], float factor,
+__device__ __forceinline__ void q4_tiles(const Q4Attn& a, int seq, int kvh, int first, int step, int end, int keys, int fresh,
+                                         const h8v (&q)[D / 32], float factor,
                                          int lane, Q4State<D>& st) {
 #pragma unroll
   for (int h = 0; h < D / 64; ++h)
@@ -570,6 +552,7 @@ __device__ __forceinline__ void q4_tiles(const Q4Attn& a, int64_t hr, int first,
   st.l = 0.f;
   const int all = (keys + kTileKeys - 1) / kTileKeys, tiles = min(end, all);
   if (first >= tiles) return;
+  const int64_t hr = (static_cast<int64_t>(seq) * a.c.heads + kvh) * a.c.max_len;
   const Q4Base b = q4_base<D>(a.c, hr, lane);
   Q4Tile<D> x;
   f4v s[2];
@@ -583,7 +566,7 @@ __device__ __forceinline__ void q4_tiles(const Q4Attn& a, int64_t hr, int first,
     q4_load_v<D>(b, t + step, x);
   }
   const int left = keys - t * kTileKeys;
-  if (fresh >= 0 && t == all - 1) q4_fresh<T, D>(a, fresh_values, hr, fresh, lane, x);
+  if (fresh >= 0 && t == all - 1) q4_fresh<T, D>(a, q4_fresh_values<T, D>(a, seq, kvh, lane), hr, fresh, lane, x);
   q4_scores<D>(x, q, s);
   if (left >= kTileKeys) q4_values<D, false>(x, s, factor, 0, lane, st);
   else q4_values<D, true>(x, s, factor, left, lane, st);
@@ -644,7 +627,51 @@ __device__ __forceinline__ Q4Item q4_item(const Q4Attn& a, int item) {
 
 template <class T>
 __device__ __forceinline__ void q4_store(const Q4Attn& a, int seq, int head, int d, float o, float l) {
-  static_cast<T*>(a.out)[seq * a.o_row + head * a.o_head + d] = static_cast<T>(l > 0.f ? o / l : 0.f);
+  static_cast<T*>(a.out)[seq * a.o_row + head * a.o_head + d] = static_cast<T>(l == 0.f ? 0.f : o / l);
+}
+
+__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive sum over the wave
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const int x = __shfl_up(v, o);
+    if (lane >= o) v += x;
+  }
+  return v;
+}
+
+// The piece of work of number `piece`: a sequence and the first key of its chunk; false where there is none. The full
+// chunks of all sequences come first and are spread over the CUs while these are empty; then the rest of every
+// sequence (or its zeros); blocks without work come last, behind everything.
+// (Chunk by chunk instead where there are too many sequences to look through: a round of loads for every 64.)
+constexpr int kLookThrough = 256;
+__device__ __forceinline__ bool q4_piece(const Q4Attn& a, int piece, int& seq, int& begin) {
+  const int lane = threadIdx.x & 63;
+  if (a.c.n_seq > kLookThrough) {
+    int fresh;
+    seq = piece % a.c.n_seq;
+    begin = piece / a.c.n_seq * a.chunk;
+    return begin == 0 || begin < q4_keys(a, seq, fresh);
+  }
+  int full = 0;  // chunks of the sequences so far
+  for (int s0 = 0; s0 < a.c.n_seq; s0 += 64) {
+    int fresh;
+    const int n = s0 + lane < a.c.n_seq ? q4_keys(a, s0 + lane, fresh) / a.chunk : 0;
+    const int incl = wave_scan(n, lane) + full;
+    const uint64_t past = __builtin_amdgcn_ballot_w64(incl > piece);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      seq = s0 + at;
+      begin = (piece - (__builtin_amdgcn_readlane(incl, at) - __builtin_amdgcn_readlane(n, at))) * a.chunk;
+      return true;
+    }
+    full = __builtin_amdgcn_readlane(incl, 63);
+  }
+  seq = piece - full;
+  if (seq >= a.c.n_seq) return false;
+  int fresh;
+  const int keys = q4_keys(a, seq, fresh), rest = keys % a.chunk;
+  begin = keys - rest;
+  return rest > 0 || keys == 0;
 }
 
 // The first arguments, which arrive in scalar registers, are what the way to the first tile needs; the rest of `a`
@@ -652,7 +679,7 @@ __device__ __forceinline__ void q4_store(const Q4Attn& a, int seq, int head, int
 template <class T, int D>
 __global__ void __launch_bounds__(512, 4) q4_attention_kernel(const int64_t* lens, uint8_t* k_codes, _Float16* k_meta,
                                                               uint8_t* v_codes, _Float16* v_meta, int max_len, int kv_heads,
-                                                              int heads, int chunk, Q4Attn a) {
+                                                              int heads, int chunk, int items, Q4Attn a) {
   extern __shared__ float lds[];
   a.lens = lens;
   a.c.k_codes = k_codes;
@@ -663,28 +690,27 @@ __global__ void __launch_bounds__(512, 4) q4_attention_kernel(const int64_t* len
   a.c.heads = kv_heads;
   a.heads = heads;
   a.chunk = chunk;
-  const int seq = blockIdx.y, waves = blockDim.x / 64, begin = static_cast<int>(gridDim.z - 1 - blockIdx.z) * a.chunk;
-  const Q4Item it = q4_item(a, blockIdx.x);
+  const int waves = blockDim.x / 64, item = blockIdx.x % items;
+  int seq = blockIdx.x / items, begin = 0;
+  if (a.chunks > 1 && !q4_piece(a, seq, seq, begin)) return;
+  const Q4Item it = q4_item(a, item);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int fresh;
-  if (begin > 0 && begin >= q4_keys(a, seq, fresh)) return;
   // requested before the length is known
   const Q4Query<T, D> query = q4_load_query<T, D>(a, seq, it.head + (lane & 15), (lane & 15) < it.cols, lane);
-  typename Vec8<T>::type fresh_values = {};
-  if (a.fresh.k) fresh_values = q4_fresh_values<T, D>(a, seq, it.kvh, lane);
   const int keys = q4_keys(a, seq, fresh);
   h8v q[D / 32];
   const float factor = q4_queries<T, D>(a, query, q);
   Q4State<D> st;
-  q4_tiles<T, D>(a, (static_cast<int64_t>(seq) * a.c.heads + it.kvh) * a.c.max_len, begin / kTileKeys + wave, waves,
-                 (begin + a.chunk) / kTileKeys, keys, fresh, fresh_values, q, factor, lane, st);
+  q4_tiles<T, D>(a, seq, it.kvh, begin / kTileKeys + wave, waves, (begin + a.chunk) / kTileKeys, keys, fresh, q, factor, lane,
+                 st);
   const Q4Merge<D> x(lds, waves, it.cols);
   q4_hand_in<D>(x, st, wave, it.cols, lane);
   __syncthreads();
   const bool whole = keys <= a.chunk;
-  const int64_t slot = (static_cast<int64_t>(seq) * gridDim.x + blockIdx.x) * a.chunks + begin / a.chunk;
+  const int64_t slot = (static_cast<int64_t>(seq) * items + item) * a.chunks + begin / a.chunk;
   const int cols = q4_cols(a);
-  float* ml = a.ws + static_cast<int64_t>(gridDim.x) * gridDim.y * a.chunks * cols * D + slot * cols * 2;
+  float* ml = a.ws + static_cast<int64_t>(items) * a.c.n_seq * a.chunks * cols * D + slot * cols * 2;
   for (int i = threadIdx.x; i < it.cols * D; i += blockDim.x) {
     float m, l;
     const int h = i / D, d = i % D;
@@ -701,53 +727,64 @@ __global__ void __launch_bounds__(512, 4) q4_attention_kernel(const int64_t* len
   }
 }
 
-// Block = (query head, sequence): joins the chunks of an item that has several.
-constexpr int kCombine = 256;
+// Joins the chunks of items that have several: block = (query head, sequence). The chunks' O are requested before
+// their weights are known. (A block for all query heads of an item is slower, its heads waiting for each other:
+// 7.7 us against 5.0 for 64 ragged sequences of 32 heads.)
+constexpr int kCombine = 256, kBatch = 8;
 template <class T, int D>
-__global__ void __launch_bounds__(kCombine) q4_combine_kernel(Q4Attn a) {
+__global__ void __launch_bounds__(kCombine) q4_combine_kernel(const int64_t* lens, int chunk, Q4Attn a) {
   constexpr int kLanes = kCombine / D;
-  __shared__ float red[kCombine / 64], part[kLanes][D];
+  __shared__ float red[2][kCombine / 64], part[kLanes][D];
   extern __shared__ float weight[];  // [chunks]
-  const int seq = blockIdx.y, head = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int seq = blockIdx.y, head = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid / 64, d = tid % D, from = tid / D;
+  a.lens = lens;
   int fresh;
-  const int keys = q4_keys(a, seq, fresh), n = (keys + a.chunk - 1) / a.chunk;
+  const int keys = q4_keys(a, seq, fresh), n = (keys + chunk - 1) / chunk;
   if (n <= 1) return;  // its block finished it
   const int group = a.heads / a.c.heads, parts = (group + kCols - 1) / kCols, items = a.c.heads * parts, cols = q4_cols(a);
   const int in_group = head % group, item = head / group * parts + in_group / kCols, h = in_group % kCols;
   const int64_t first = (static_cast<int64_t>(seq) * items + item) * a.chunks;
-  const float* ml = a.ws + static_cast<int64_t>(items) * a.c.n_seq * a.chunks * cols * D + (first * cols + h) * 2;
-  float m = -INFINITY;
+  const float2* ml = reinterpret_cast<const float2*>(a.ws + static_cast<int64_t>(items) * a.c.n_seq * a.chunks * cols * D) +
+                     first * cols + h;
+  const float* acc = a.ws + (first * cols + h) * D + d;
+  const auto load = [&](int i, float (&x)[kBatch]) {  // chunks i, i + kLanes, ..; past the end the last one
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) x[j] = acc[static_cast<int64_t>(min(i + j * kLanes, n - 1)) * (cols * D)];
+  };
+  float x[kBatch];
+  load(from, x);
+  float m = -INFINITY, l = 0.f;
   for (int i = tid; i < n; i += kCombine) {
-    weight[i] = ml[i * cols * 2];
+    weight[i] = ml[static_cast<int64_t>(i) * cols].x;
     m = fmaxf(m, weight[i]);
   }
   m = group_max<64>(m);
-  if (lane == 0) red[tid / 64] = m;
+  if (lane == 0) red[0][wave] = m;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kCombine / 64; ++i) m = fmaxf(m, red[i]);
-  float l = 0.f;
+  for (int i = 0; i < kCombine / 64; ++i) m = fmaxf(m, red[0][i]);
   for (int i = tid; i < n; i += kCombine) {
     weight[i] = __builtin_amdgcn_exp2f(weight[i] - m);
-    l = fmaf(weight[i], ml[i * cols * 2 + 1], l);
+    l = fmaf(weight[i], ml[static_cast<int64_t>(i) * cols].y, l);
   }
+  l = group_sum<64>(l);
+  if (lane == 0) red[1][wave] = l;
   __syncthreads();
-  l = block_sum_once<kCombine>(l, red);
-  const int d = tid % D, from = tid / D, step = cols * D;
-  const float* acc = a.ws + (first * cols + h) * D + d;
   float o = 0.f;
-  int i = from;
-  for (; i + 7 * kLanes < n; i += 8 * kLanes) {  // 8 loads in flight
-    float x[8];
+  for (int i = from;;) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = acc[static_cast<int64_t>(i + j * kLanes) * step];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) o = fmaf(weight[i + j * kLanes], x[j], o);
+    for (int j = 0; j < kBatch; ++j)
+      if (i + j * kLanes < n) o = fmaf(weight[i + j * kLanes], x[j], o);
+    i += kBatch * kLanes;
+    if (i >= n) break;
+    load(i, x);
   }
-  for (; i < n; i += kLanes) o = fmaf(weight[i], acc[static_cast<int64_t>(i) * step], o);
   part[from][d] = o;
   __syncthreads();
   if (tid >= D) return;
+  l = 0.f;
+#pragma unroll
+  for (int i = 0; i < kCombine / 64; ++i) l += red[1][i];
 #pragma unroll
   for (int j = 1; j < kLanes; ++j) o += part[j][d];
   q4_store<T>(a, seq, head, d, o, l);
@@ -758,7 +795,7 @@ __global__ void __launch_bounds__(kCombine) q4_combine_kernel(Q4Attn a) {
 // 14.4 us in one chunk, 19.2 shared out further). Longer ones are cut so that full lengths give about kWantBlocks
 // blocks, two a CU (131000 keys x 8 heads of 128: 42.7 us, with twice the blocks 48.4), into chunks of at most 256
 // keys a wave, which bounds how long a few long sequences among short ones keep their CUs (64 ragged sequences of
-// up to 8000 keys x 8 heads: 42 us, with 512 keys a wave 61), and of at least 1 / kMostBlocks of everything, which
+// up to 8000 keys x 8 heads: 39.5 us, with 512 keys a wave 61), and of at least 1 / kMostBlocks of everything, which
 // bounds the workspace. Blocks have 8 waves where items are few and 4 where they fill the CUs anyway (those 64
 // sequences: 33.5 us against 39.5; 64 x 20 heads of 64 over 700 keys 15.0 against 17.2, but 16 x 20 over 1500 keys as
 // two chunks of 4 waves 14.8 against 12.2), or where the merge of 16 heads of 128 would pass 64 KB of LDS.
@@ -912,18 +949,19 @@ extern "C" int fw_decode_attention_q4(const void* q, int64_t q_row, int64_t q_he
   if (!ws || ws_floats < need || !aligned(ws, 16))
     return fw_fail(FW_EINVAL, "decode_attention_q4: workspace needs %lld floats, 16-byte aligned", static_cast<long long>(need));
   const Q4Plan p = q4_plan(n_seq, heads, kv_heads, max_len, head_dim);
-  if (n_seq > 65535) return fw_fail(FW_EINVAL, "decode_attention_q4: too many sequences");
+  if (n_seq > 65535 || n_seq * p.parts() > 0x7FFFFFFF) return fw_fail(FW_EINVAL, "decode_attention_q4: too many sequences");
   const Q4Attn a{q, out, q_row, q_head, o_row, o_head, Q4Rows{k_new, v_new, k_row, k_head, v_row, v_head}, lens, c, heads, scale,
                  p.chunk, p.chunks, ws};
   const int lds = head_dim == 64 ? Q4Merge<64>::bytes(p.waves, p.cols) : Q4Merge<128>::bytes(p.waves, p.cols);
   q4_by_type(dtype, head_dim, [&](auto t, auto d) {
-    hipLaunchKernelGGL((q4_attention_kernel<decltype(t), d.value>), dim3(p.items, n_seq, p.chunks), dim3(64 * p.waves), lds,
-                       stream, lens, c.k_codes, c.k_meta, c.v_codes, c.v_meta, max_len, kv_heads, heads, p.chunk, a);
+    hipLaunchKernelGGL((q4_attention_kernel<decltype(t), d.value>), dim3(static_cast<unsigned>(n_seq * p.parts())), dim3(64 * p.waves), lds,
+                       stream, lens, c.k_codes, c.k_meta, c.v_codes, c.v_meta, max_len, kv_heads, heads, p.chunk, p.items, a);
   });
   if (const int rc = fw_check_launch("decode_attention_q4")) return rc;
   if (p.chunks == 1) return FW_OK;
   q4_by_type(dtype, head_dim, [&](auto t, auto d) {
-    hipLaunchKernelGGL((q4_combine_kernel<decltype(t), d.value>), dim3(heads, n_seq), dim3(kCombine), 4 * p.chunks, stream, a);
+    hipLaunchKernelGGL((q4_combine_kernel<decltype(t), d.value>), dim3(heads, n_seq), dim3(kCombine), 4 * p.chunks, stream, lens,
+                       p.chunk, a);
   });
   return fw_check_launch("decode_attention_q4 combine");
 }

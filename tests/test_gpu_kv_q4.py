@@ -394,3 +394,38 @@ def test_compiled_binding_and_ctypes(ext, hip_device, kind):
         torch.cuda.synchronize()
         results.append(outs + list(cache))
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize('n', [300, 5000])
+def test_many_sequences(ext, hip_device, n):
+    """More sequences than one, two or 64 rounds of looking for them: rows in and out, attention over caches of one chunk
+    and of several, prompts, each against the same done in calls of at most 50 sequences."""
+    dev, rng = hip_device, np.random.default_rng(n)
+    lengths = rng.integers(0, 4, n)
+    lengths[[3, n // 2, n - 1]] = 40, 0, 90
+    total = int(lengths.sum())
+    q, k, v = (rounded(rng, (total, h, 64), torch.float16)[0].to(dev) for h in (2, 1, 1))
+    cu, zero = starts(lengths, dev), torch.zeros(n, dtype=torch.int64, device=dev)
+    small, large = ext.kv_q4_cache(n, 1, 96, 64), ext.kv_q4_cache(n, 1, 2080, 64)
+    outs = [torch.full((total, 2, 64), 7.0, dtype=torch.float16, device=dev) for _ in range(2)]
+    decoded = [torch.full((n, 2, 64), 7.0, dtype=torch.float16, device=dev) for _ in range(3)]
+    q1, lens = rounded(rng, (n, 2, 64), torch.float16)[0].to(dev), torch.tensor(lengths, device=dev)
+    ext.prompt_attention(q, k, v, outs[0], cu, cu, 0.125)
+    for out, cache in zip(decoded, (small, large)):
+        ext.kv_q4_append(k, v, cu, zero, cache)
+        ext.decode_attention_q4(q1, cache, lens, out, ext.decode_attention_q4_workspace(n, 2, cache), 0.125)
+    back = [torch.zeros_like(k), torch.zeros_like(v)]
+    ext.kv_q4_read(large, cu, zero, *back)
+    for a in range(0, n, 50):
+        b, at = min(a + 50, n), cu[a:a + 51] - cu[a]
+        rows = slice(int(cu[a]), int(cu[b]))
+        ext.prompt_attention(q[rows], k[rows], v[rows], outs[1][rows], at, at, 0.125)
+        part = ext.kv_q4_cache(b - a, 1, 96, 64)
+        ext.kv_q4_append(k[rows], v[rows], at, zero[a:b], part)
+        assert all(torch.equal(x[a:b], y) for x, y in zip(small, part))
+        held = [torch.zeros_like(k[rows]), torch.zeros_like(k[rows])]
+        ext.kv_q4_read(part, at, zero[a:b], *held)
+        assert all(torch.equal(x[rows], y) for x, y in zip(back, held))
+        ext.decode_attention_q4(q1[a:b], part, lens[a:b], decoded[2][a:b], ext.decode_attention_q4_workspace(b - a, 2, part), 0.125)
+    assert torch.equal(*outs)
+    assert torch.equal(decoded[0], decoded[2]) and (decoded[1].float() - decoded[2].float()).abs().max() <= 2 ** -7

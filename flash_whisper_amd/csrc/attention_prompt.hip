@@ -474,13 +474,16 @@ extern "C" int fw_prompt_attention(const void* q, int64_t q_row, int64_t q_head,
     constexpr int D = decltype(d)::value;
     constexpr bool M = decltype(mask)::value;
     // Blocks of 128 rows stage every tile for four waves. They are the fastest where they fill the CUs; fewer rows
-    // are given to more blocks, and long chains of tiles to several waves, whose parts are then merged (us of 128 rows
-    // / 64 rows and 2 parts of 64 keys / of 32 keys / 32 rows and 8 parts, heads of 64 unless said: 1 x 4 queries x 20
-    // heads over 1500 keys 24.5 / 15.4 / 17.4 / 11.7; 1 x 1500 x 20, causal 27.1 / 18.4 / 19.9 / 24.9; 8 x 64 x 32 over
-    // 4000 keys and 8 heads of 128 84 / 68 / 79 / 87; 16 x 4 .. 224 x 20, causal 9.8 / 11.7 / 8.8 / 17.3, over 1500 keys
-    // 37.8 / 48.2 / 38.8 / 50.4).
+    // are given to more blocks, and long chains of tiles to several waves, whose parts are then merged; where a
+    // sequence is a tile or two, a wave works alone and many blocks share a CU (us of 128 rows / 64 rows and 2 parts
+    // of 64 keys / of 32 keys / 32 rows and 8 parts, heads of 64 unless said: 1 x 4 queries x 20 heads over 1500 keys
+    // 24.5 / 15.4 / 17.4 / 11.7; 1 x 1500 x 20, causal 27.1 / 18.4 / 19.9 / 24.9; 8 x 64 x 32 over 4000 keys and 8
+    // heads of 128 84 / 68 / 79 / 87; 16 x 4 .. 224 x 20, causal 9.8 / 11.7 / 8.8 / 17.3, over 1500 keys 37.8 / 48.2 /
+    // 38.8 / 50.4. Third form / one wave of 32 rows: 1 x 4 x 20 4.5 / 4.0; 2000 x 8 x 20 209 / 73; 64 x 64 x 20 15.9 /
+    // 13.3; 16 x 4 .. 224 x 20 8.0 / 10.5).
     const int64_t wide = (rows / 128 + n_seq) * kv_heads, keys = k_rows / n_seq;
     if (wide <= 128 && keys >= 512) launch(prompt_attention_kernel<T, D, 1, 8, 32, 1, M>, 32, 512);
+    else if (keys <= 64) launch(prompt_attention_kernel<T, D, 1, 1, 32, 1, M>, 32, 64);
     else if (wide <= 384 && keys >= 512) launch(prompt_attention_kernel<T, D, 2, 2, 64, 2, M>, 64, 256);
     else if (wide <= 384 || keys < 256) launch(prompt_attention_kernel<T, D, 2, 2, 32, 2, M>, 64, 256);
     else launch(prompt_attention_kernel<T, D, 4, 1, 64, 2, M>, 128, 256);

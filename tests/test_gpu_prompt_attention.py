@@ -190,3 +190,33 @@ def test_far_rows(ext, hip_device):
         t.copy_(x)
     ext.prompt_attention(q, k, v, out, starts([60, 40], dev), starts([60, 40], dev), 0.125)
     check_prompts(out.double().cpu().numpy(), *(x for _, x in h), [60, 40], [60, 40], 0.125, True, torch.float16)
+
+
+# every way of sharing out the rows, by the sizes that choose it: 128-row blocks, 64 rows and two parts of 64 or 32
+# keys, 32 rows and 8 parts, single waves; partial blocks and tiles in each
+FORMS = {'wide': ([500, 33, 700, 129], [500, 160, 700, 130], 40, 20), 'wide_long': ([1030, 40], [1500, 2100], 40, 20),
+         'two_parts': ([300, 70], [900, 601], 20, 20), 'two_short_parts': ([150, 33, 90], [150, 70, 210], 20, 20),
+         'eight_parts': ([4, 37, 1], [1000, 531, 777], 8, 2), 'single_waves': ([33, 8, 64, 1], [40, 20, 64, 64], 8, 4)}
+
+
+@pytest.mark.parametrize('kind, dim', [('fp16', 64), ('bf16', 64), ('fp16', 128), ('bf16', 128)])
+@pytest.mark.parametrize('causal', [True, False])
+@pytest.mark.parametrize('form', FORMS)
+def test_forms(ext, hip_device, form, causal, kind, dim):
+    nq, nk, heads, kv_heads = FORMS[form]
+    _run(ext, hip_device, nq, nk, heads, kv_heads, dim, kind, causal, seed=dim)
+
+
+@pytest.mark.parametrize('kind, dim', [('fp16', 64), ('bf16', 128)])
+@pytest.mark.parametrize('form', FORMS)
+def test_forms_values_not_seen(ext, hip_device, form, kind, dim):
+    """Infinities and NaN in the keys and values near each sequence's end: seen by its last queries, not by the others."""
+    nq, nk, heads, kv_heads = FORMS[form]
+
+    def edit(k, v):
+        for end in np.cumsum(nk):
+            k[end - 2, 0, 9] = float('inf')
+            v[end - 1, -1, 3], v[end - 3, -1, 4], v[end - 2, -1, dim - 1] = float('nan'), float('inf'), float('-inf')
+            v[end - 17, -1, 5] = float('inf')
+
+    _run(ext, hip_device, nq, nk, heads, kv_heads, dim, kind, True, seed=dim, edit=edit)

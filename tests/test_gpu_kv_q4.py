@@ -429,3 +429,40 @@ def test_many_sequences(ext, hip_device, n):
         ext.decode_attention_q4(q1[a:b], part, lens[a:b], decoded[2][a:b], ext.decode_attention_q4_workspace(b - a, 2, part), 0.125)
     assert torch.equal(*outs)
     assert torch.equal(decoded[0], decoded[2]) and (decoded[1].float() - decoded[2].float()).abs().max() <= 2 ** -7
+
+
+@pytest.mark.parametrize('kind, dim', [('fp16', 64), ('bf16', 128)])
+@pytest.mark.parametrize('scale', [0.0, -0.125, 1.0])
+def test_decode_scales(ext, hip_device, scale, kind, dim):
+    dev, dtype, rng = hip_device, TYPES[kind], np.random.default_rng(19)
+    lens = [70, 3]
+    want = _filled(rng, 2, 1, 96, dim, lens)
+    q, q64 = rounded(rng, (2, 2, dim), dtype)
+    cache, out = to_device(want, dev), torch.empty(2, 2, dim, dtype=dtype, device=dev)
+    ext.decode_attention_q4(q.to(dev), cache, _index(lens, dev), out, ext.decode_attention_q4_workspace(2, 2, cache), scale)
+    _check_decode(out.double().cpu().numpy(), q64, want, lens, scale, dtype)
+
+
+@pytest.mark.parametrize('max_len', [512, 4128])
+def test_decode_no_numbers(ext, hip_device, max_len):
+    """A query that is no number makes its own head NaN; a row of such keys every head that reads it; a value in such a
+    row its dims; the other sequence stays as it is."""
+    dev, rng = hip_device, np.random.default_rng(20)
+    lens = [max_len - 10, 300]
+    cache = to_device(_filled(rng, 2, 2, max_len, 64, lens), dev)
+    q, at = rounded(rng, (2, 4, 64), torch.float16)[0].to(dev), _index(lens, dev)
+    ws, want = ext.decode_attention_q4_workspace(2, 4, cache), torch.empty(2, 4, 64, dtype=torch.float16, device=dev)
+    ext.decode_attention_q4(q, cache, at, want, ws, 0.125)
+    bad, got = q.clone(), torch.empty_like(want)
+    bad[0, 1, 5] = float('nan')
+    ext.decode_attention_q4(bad, cache, at, got, ws, 0.125)
+    assert got[0, 1].isnan().all()
+    got[0, 1] = want[0, 1]
+    assert torch.equal(got, want)
+    k = torch.zeros(1, 2, 64, dtype=torch.float16, device=dev)
+    v = k.clone()
+    k[0, 0, 3], v[0, 1, 40] = float('inf'), float('nan')  # dims 0 .. 31 of head 0's key, 32 .. 63 of head 1's value
+    ext.kv_q4_append(k, v, starts([1, 0], dev), _index([150, 0], dev), cache)
+    ext.decode_attention_q4(q, cache, at, got, ws, 0.125)
+    assert got[0, :2].isnan().all() and got[0, 2:, 32:].isnan().all() and got[0, 2:, :32].isfinite().all()
+    assert torch.equal(got[1], want[1])

@@ -220,3 +220,42 @@ def test_forms_values_not_seen(ext, hip_device, form, kind, dim):
             v[end - 17, -1, 5] = float('inf')
 
     _run(ext, hip_device, nq, nk, heads, kv_heads, dim, kind, True, seed=dim, edit=edit)
+
+
+@pytest.mark.parametrize('kind, dim', [('fp16', 64), ('bf16', 128)])
+@pytest.mark.parametrize('scale', [0.0, -0.125, 1.0, -1e-3])
+def test_scales(ext, hip_device, scale, kind, dim):
+    """A scale of zero weighs all keys alike, a negative one turns the order of the scores round."""
+    dev, dtype, rng = hip_device, TYPES[kind], np.random.default_rng(17)
+    q, q64 = rounded(rng, (90, 2, dim), dtype)
+    k, k64 = rounded(rng, (90, 2, dim), dtype)
+    v, v64 = rounded(rng, (90, 2, dim), dtype)
+    out, cu = torch.empty(90, 2, dim, dtype=dtype, device=dev), starts([50, 40], dev)
+    ext.prompt_attention(q.to(dev), k.to(dev), v.to(dev), out, cu, cu, scale)
+    check_prompts(out.double().cpu().numpy(), q64, k64, v64, [50, 40], [50, 40], scale, True, dtype)
+
+
+def test_no_rows(ext, hip_device):
+    """No queries: nothing happens; no keys at all: zeros."""
+    dev = hip_device
+    q, none = torch.ones(6, 2, 64, dtype=torch.float16, device=dev), torch.empty(0, 2, 64, dtype=torch.float16, device=dev)
+    out, cu, cu0 = torch.ones_like(q), starts([2, 4], dev), starts([0, 0], dev)
+    ext.prompt_attention(none, q, q, none.clone(), cu0, cu, 0.125)
+    for causal in (True, False):
+        ext.prompt_attention(q, none, none, out.fill_(1), cu, cu0, 0.125, causal)
+        assert not out.any()
+
+
+@pytest.mark.parametrize('value', [float('nan'), float('inf')])
+def test_queries_that_are_no_numbers(ext, hip_device, value):
+    """They make their own row and head NaN, and no other."""
+    dev, rng = hip_device, np.random.default_rng(18)
+    q, k, v = (rounded(rng, (70, 2, 64), torch.float16)[0].to(dev) for _ in range(3))
+    cu, want = starts([70], dev), torch.empty(70, 2, 64, dtype=torch.float16, device=dev)
+    ext.prompt_attention(q, k, v, want, cu, cu, 0.125)
+    q[33, 1, 7] = value
+    got = torch.empty_like(want)
+    ext.prompt_attention(q, k, v, got, cu, cu, 0.125)
+    assert got[33, 1].isnan().all()
+    got[33, 1] = want[33, 1]
+    assert torch.equal(got, want)

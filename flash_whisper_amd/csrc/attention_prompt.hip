@@ -106,7 +106,7 @@ __device__ __forceinline__ bool find_job(const PromptArgs& a, int64_t slot, Job&
   job.rows = job.nq * group;
   const int64_t row0 = (slot - start(job.seq)) * ROWS;
   job.row0 = static_cast<int>(row0);
-  return row0 < job.rows;
+  return row0 >= 0 && row0 < job.rows;  // (negative: of starts that do not ascend)
 }
 
 template <int D>
@@ -456,6 +456,7 @@ extern "C" int fw_prompt_attention(const void* q, int64_t q_row, int64_t q_head,
   if ((q_rows > 0 && (!rows_ok(q, q_row, q_head) || !rows_ok(out, o_row, o_head))) ||
       (k_rows > 0 && (!rows_ok(k, k_row, k_head) || !rows_ok(v, v_row, v_head))))
     return fw_fail(FW_EINVAL, "prompt_attention: q, k, v and out must be 16-byte aligned with strides in multiples of 8");
+  if (!(__builtin_fabsf(scale) < INFINITY)) return fw_fail(FW_EINVAL, "prompt_attention: scale must be finite");
   // 64 rows of k and of v within the copies' 32-bit byte offsets; rows x heads of a sequence are counted in 32 bits
   if (k_row < 0 || v_row < 0 || k_row >= (1 << 25) || v_row >= (1 << 25))
     return fw_fail(FW_EINVAL, "prompt_attention: row strides of k and v must be below 2^25 elements");
@@ -466,7 +467,7 @@ extern "C" int fw_prompt_attention(const void* q, int64_t q_row, int64_t q_head,
   int rc = FW_OK;
   const auto launch = [&](auto kernel, int per_block, int threads) {
     const int64_t blocks = (rows / per_block + n_seq) * kv_heads;  // a sequence's last block may be partial
-    if (blocks > 0x7FFFFFFF) rc = fw_fail(FW_EINVAL, "prompt_attention: too many rows");
+    if (!grid_ok(blocks, threads)) rc = fw_fail(FW_EINVAL, "prompt_attention: too many rows");
     else hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(threads), 0, stream, a);
   };
   const auto by_rows = [&](auto t, auto d, auto mask) {

@@ -825,12 +825,15 @@ Q4Plan q4_plan(int n_seq, int heads, int kv_heads, int max_len, int dim) {
 
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
+constexpr int kMaxLen = 1 << 30;  // a row and a chunk further fit 32 bits
+
 // What every entry point asks of a cache; FW_OK or FW_EINVAL.
 int check_cache(const char* what, const Q4Cache& c, int dim) {
   if (!c.k_codes || !c.k_meta || !c.v_codes || !c.v_meta) return fw_fail(FW_EINVAL, "%s: null cache pointer", what);
   if (c.n_seq <= 0 || c.heads <= 0) return fw_fail(FW_EINVAL, "%s: n_seq and kv_heads must be positive", what);
   if (dim != 64 && dim != 128) return fw_fail(FW_EINVAL, "%s: head_dim must be 64 or 128", what);
-  if (c.max_len <= 0 || c.max_len % 32) return fw_fail(FW_EINVAL, "%s: max_len must be a positive multiple of 32", what);
+  if (c.max_len <= 0 || c.max_len % 32 || c.max_len > kMaxLen)
+    return fw_fail(FW_EINVAL, "%s: max_len must be a positive multiple of 32 up to 2^30", what);
   if (!aligned(c.k_codes, 16) || !aligned(c.k_meta, 16) || !aligned(c.v_codes, 16) || !aligned(c.v_meta, 16))
     return fw_fail(FW_EINVAL, "%s: the cache must be 16-byte aligned", what);
   return FW_OK;
@@ -878,7 +881,7 @@ int check_packed(const char* what, const Q4Rows& r, const int64_t* cu, const int
   if (rows > 0 && (!rows_ok(r.k, r.k_row, r.k_head) || !rows_ok(r.v, r.v_row, r.v_head)))
     return fw_fail(FW_EINVAL, "%s: k and v must be 16-byte aligned with strides in multiples of 8", what);
   // the grid: 4 waves a block, slots x heads x halves waves
-  if ((rows / 8 + 2 * static_cast<int64_t>(c.n_seq)) * c.heads * (dim / 64) > int64_t{4} * 0x7FFFFFFF)
+  if (rows > int64_t{1} << 40 || !grid_ok(((rows / 8 + 2 * static_cast<int64_t>(c.n_seq)) * c.heads * (dim / 64) + 3) / 4, 256))
     return fw_fail(FW_EINVAL, "%s: too many rows", what);
   return FW_OK;
 }
@@ -924,7 +927,7 @@ extern "C" int fw_kv_q4_read(const void* k_codes, const void* k_meta, const void
 
 extern "C" int64_t fw_decode_attention_q4_ws_floats(int n_seq, int heads, int kv_heads, int max_len, int head_dim) {
   if (n_seq <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_len <= 0 || max_len % 32 ||
-      (head_dim != 64 && head_dim != 128))
+      max_len > kMaxLen || (head_dim != 64 && head_dim != 128))
     return 0;
   const Q4Plan p = q4_plan(n_seq, heads, kv_heads, max_len, head_dim);
   return p.chunks == 1 ? 4 : (n_seq * p.parts() * p.cols * (head_dim + 2) + 3) / 4 * 4;
@@ -941,6 +944,7 @@ extern "C" int fw_decode_attention_q4(const void* q, int64_t q_row, int64_t q_he
   if (const int rc = check_cache("decode_attention_q4", c, head_dim)) return rc;
   if (dtype != FW_F16 && dtype != FW_BF16) return fw_fail(FW_EINVAL, "decode_attention_q4: dtype must be FW_F16 or FW_BF16");
   if (!q || !lens || !out) return fw_fail(FW_EINVAL, "decode_attention_q4: null pointer");
+  if (!(__builtin_fabsf(scale) < INFINITY)) return fw_fail(FW_EINVAL, "decode_attention_q4: scale must be finite");
   if (!k_new != !v_new) return fw_fail(FW_EINVAL, "decode_attention_q4: k_new and v_new must be given together");
   if (heads <= 0 || heads % kv_heads) return fw_fail(FW_EINVAL, "decode_attention_q4: heads must be a multiple of kv_heads");
   if (!rows_ok(q, q_row, q_head) || !rows_ok(out, o_row, o_head) || (k_new && (!rows_ok(k_new, k_row, k_head) || !rows_ok(v_new, v_row, v_head))))
@@ -949,7 +953,7 @@ extern "C" int fw_decode_attention_q4(const void* q, int64_t q_row, int64_t q_he
   if (!ws || ws_floats < need || !aligned(ws, 16))
     return fw_fail(FW_EINVAL, "decode_attention_q4: workspace needs %lld floats, 16-byte aligned", static_cast<long long>(need));
   const Q4Plan p = q4_plan(n_seq, heads, kv_heads, max_len, head_dim);
-  if (n_seq > 65535 || n_seq * p.parts() > 0x7FFFFFFF) return fw_fail(FW_EINVAL, "decode_attention_q4: too many sequences");
+  if (n_seq > 65535 || !grid_ok(n_seq * p.parts(), 64 * p.waves)) return fw_fail(FW_EINVAL, "decode_attention_q4: too many sequences");
   const Q4Attn a{q, out, q_row, q_head, o_row, o_head, Q4Rows{k_new, v_new, k_row, k_head, v_row, v_head}, lens, c, heads, scale,
                  p.chunk, p.chunks, ws};
   const int lds = head_dim == 64 ? Q4Merge<64>::bytes(p.waves, p.cols) : Q4Merge<128>::bytes(p.waves, p.cols);

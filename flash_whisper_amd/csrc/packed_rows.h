@@ -21,6 +21,9 @@ __device__ __forceinline__ int last_started(int n, int64_t slot, F start) {
   }
 }
 
+// Whether a launch of so many blocks stays within the 2^32 - 1 threads of a grid's axis.
+inline bool grid_ok(int64_t blocks, int threads) { return blocks <= 0xFFFFFFFFll / threads; }
+
 // A start or end within the rows there are.
 __device__ __forceinline__ int64_t within(int64_t x, int64_t low, int64_t rows) { return min(max(x, low), rows); }
 

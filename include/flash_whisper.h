@@ -435,14 +435,14 @@ int fw_cross_kv(const void* enc, int t, const void* w, const void* bias, void* c
  * key, each one before it a key less (j <= i + n_keys - n_queries, both counted within the sequence). A query that
  * sees no key gets zeros. What a query does not see does not reach its output, whatever it holds (infinities and NaN
  * too). Rows of out behind the last sequence are left as they are. Scores, softmax and sums are fp32; the weights
- * are rounded to the type for the product with v. out overlaps no input. */
+ * are rounded to the type for the product with v. out overlaps no input; scale is finite, here and below. */
 int fw_prompt_attention(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                         const void* v, int64_t v_row, int64_t v_head, void* out, int64_t o_row, int64_t o_head,
                         const int64_t* cu_q, const int64_t* cu_k, int n_seq, int64_t q_rows, int64_t k_rows, int heads,
                         int kv_heads, int head_dim, int dtype, float scale, int causal, hipStream_t stream);
 
-/* The 4-bit cache of n_seq sequences, kv_heads heads and max_len rows (a multiple of 32) of head_dim (64 or 128)
- * elements: 5 bits a value. 32 elements of a row share a step and a low value (fp16), and a code c of 0 .. 15 stands
+/* The 4-bit cache of n_seq sequences, kv_heads heads and max_len rows (a multiple of 32, at most 2^30) of head_dim (64
+ * or 128) elements: 5 bits a value. 32 elements of a row share a step and a low value (fp16), and a code c of 0 .. 15 stands
  * for fp16(low + step c). All four arrays are dense and 16-byte aligned:
  *   k_codes u8   [n_seq][kv_heads][max_len][head_dim / 2]          element d in byte d / 2, even d in the low bits
  *   k_meta  fp16 [n_seq][kv_heads][max_len][head_dim / 32][2]      step, low

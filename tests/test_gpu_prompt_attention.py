@@ -259,3 +259,15 @@ def test_queries_that_are_no_numbers(ext, hip_device, value):
     assert got[33, 1].isnan().all()
     got[33, 1] = want[33, 1]
     assert torch.equal(got, want)
+
+
+def test_starts_that_fall_and_rise(ext, hip_device):
+    """Starts must ascend; where they do not, no access leaves the rows: the ones around them stay as they were."""
+    dev = hip_device
+    x = torch.randn(1000, 2, 64, generator=torch.Generator().manual_seed(3)).half().to(dev)
+    for cu in ([300, 0, 50, 400], [390, 399, 10, 20], [200, 0, 0, 0]):
+        starts_of = torch.tensor(cu, dtype=torch.int64, device=dev)
+        for causal in (True, False):
+            out = torch.full_like(x, 3.0)
+            ext.prompt_attention(x[300:700], x[300:700], x[300:700], out[300:700], starts_of, starts_of, 0.125, causal)
+            assert (out[:300] == 3.0).all() and (out[700:] == 3.0).all() and not out.isnan().any()

@@ -157,3 +157,33 @@ def test_binding_refuses_without_a_call(built_lib):
     assert _bind.decode_attention_q4(q[:2], cache, cu[:2], q[:2], torch.zeros(4), 0.125, None, None, 0, 0) is False
     with pytest.raises(ValueError):
         _bind.set_entry('fw_other', 0)
+
+
+@pytest.mark.parametrize('scale', [float('inf'), float('-inf'), float('nan')])
+def test_scale_is_finite(built_lib, scale):
+    from flash_whisper_amd import _lib
+
+    strides = (1280, 64)
+    assert built_lib.fw_prompt_attention(D16, *strides, D16, *strides, D16, *strides, D16, *strides, D16, D16, 2, 8, 8, 20, 20, 64,
+                                         0, scale, 1, None) == _lib.FW_EINVAL
+    assert b'scale must be finite' in built_lib.fw_last_error()
+    assert built_lib.fw_decode_attention_q4(D16, *strides, *CACHE, D16, D16, *strides, None, *strides, None, *strides, 2, 20, 20,
+                                            448, 64, 0, scale, D16, 1 << 40, None) == _lib.FW_EINVAL
+    assert b'scale must be finite' in built_lib.fw_last_error()
+
+
+@pytest.mark.parametrize('call, what, message', [
+    (_prompt, dict(rows=1 << 31, heads=20, kv=20), b'too many rows'),          # rows of a sequence in 32 bits
+    (_prompt, dict(rows=1 << 30, heads=64, kv=64), b'too many rows'),          # 2^23 blocks x 64 heads x 256 threads
+    (_append, dict(rows=1 << 26, heads=8, dim=64), b'too many rows'),          # 2^23 x 8 waves of 64 threads: 2^32 and a few
+    (_read, dict(rows=1 << 28, heads=8, dim=128), b'too many rows'),
+    (_append, dict(rows=1 << 62), b'too many rows'),
+    (_append, dict(max_len=(1 << 30) + 32), b'up to 2^30'),
+    (_decode, dict(max_len=(1 << 30) + 32), b'up to 2^30'),
+    (_decode, dict(n=65536), b'too many sequences'),
+    (_decode, dict(n=65535, heads=512, kv=512), b'too many sequences')])       # 2^25 blocks of 256 threads
+def test_calls_past_a_grid(built_lib, call, what, message):
+    from flash_whisper_amd import _lib
+
+    assert call(built_lib, **what) == _lib.FW_EINVAL
+    assert message in built_lib.fw_last_error()

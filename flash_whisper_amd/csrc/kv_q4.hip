@@ -231,9 +231,13 @@ __global__ void __launch_bounds__(256) kv_q4_read_kernel(const int64_t* __restri
 //    step and low, which rounds once as the cache's definition does. Q's dims are permuted to the order in
 //    which masking a dword's nibbles yields pairs (0 4, 1 5, 2 6, 3 7).
 //  - The running maximum only moves when a score passes it by 2^kSlack (log2 units); weights stay within fp16.
+// Bound by memory where the lengths are alike (64 x 8000 keys x 8 heads of 128, 32 query heads: 131 us, 5.0 TB/s with
+// what the last-level cache gives; one of 131000: 43 us, 3.9 TB/s), by the longest block and the two launches' latency
+// where they are not (64 of 1 to 8000: 28.6 us, 3.0 TB/s), and by latency where there is little to read (300 keys x 20
+// heads: 4.8 us). Beside the loads the conversion of the codes takes most: 13 instructions for 8 codes.
 // A block takes a chunk of an item's keys; an item of one chunk is finished by its block, the chunks of a longer one
-// leave (m, l, O) in the workspace for the combine launch. Only the device knows the lengths: it puts full chunks
-// first (q4_piece), and blocks without keys end at once.
+// leave (m, l, O) in the workspace for the combine launch. Only the device knows the lengths: every block works out the
+// same chunk from them and finds its piece of work (q4_share, q4_piece); blocks without keys end at once.
 // ------------------------------------------------------------------------------------------
 struct Q4Attn {
   const void* q;
@@ -244,8 +248,10 @@ struct Q4Attn {
   Q4Cache c;
   int heads;  // query heads
   float scale;
-  int chunk, chunks;  // keys of a chunk (a multiple of kTileKeys), chunks of a full cache
-  float* ws;          // O [n_seq][items][chunks][cols][D], then (m, l) [n_seq][items][chunks][cols][2]
+  int chunk, most;  // keys of the largest chunk, the most chunks of a sequence
+  int unit;         // what chunks are multiples of; 0: all have the largest's size
+  int pieces;       // pieces of work per item number; 0: an item is one
+  float* ws;        // O [pieces][items][cols][D], then (m, l) [pieces][items][cols][2]
 };
 
 constexpr int kTileKeys = 32;
@@ -630,48 +636,101 @@ __device__ __forceinline__ void q4_store(const Q4Attn& a, int seq, int head, int
   static_cast<T*>(a.out)[seq * a.o_row + head * a.o_head + d] = static_cast<T>(l == 0.f ? 0.f : o / l);
 }
 
-__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive sum over the wave
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const int x = __shfl_up(v, o);
-    if (lane >= o) v += x;
-  }
+// Inclusive sum over the wave by DPP: within rows of 16 lanes, then row 0 to 1 and 2 to 3, then the lower half to the
+// upper. (Shuffles go through the LDS pipe: a microsecond in the 12000 blocks of 200 sequences.)
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);   // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);   // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);   // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);   // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 to rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 to rows 2 and 3
   return v;
+}
+__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
+
+// How the keys of all sequences are shared out: chunks so long that about kWantBlocks blocks have one (two a CU), at least
+// two tiles a wave and at most a.chunk. Lane i has the keys of sequences i, i + 64, .. Many items fill the CUs in any
+// case and get a.chunk, without the sum over the lengths; more sequences than kLookThrough nobody looks through at all.
+// (One sequence of 3000 keys in a cache for 131072, 8 heads of 128: 11.0 us, in chunks for a full cache 18.9; 8 of 2000
+// for 32768 12.3 against 17.1; 32 ragged ones of up to 4000 16.3 against 19.5; lengths near the full ones are alike.)
+constexpr int kLookThrough = 256, kRounds = kLookThrough / 64, kWantBlocks = 512;
+struct Q4Share {
+  int keys[kRounds], chunk;
+};
+__device__ __forceinline__ Q4Share q4_share(const Q4Attn& a, int items, int lane) {
+  Q4Share x;
+  x.chunk = a.chunk;
+  if (a.c.n_seq > kLookThrough) return x;
+  float all = 0.f;
+#pragma unroll
+  for (int j = 0; j < kRounds; ++j) {
+    int fresh;
+    x.keys[j] = 0;
+    if (64 * j < a.c.n_seq && 64 * j + lane < a.c.n_seq) x.keys[j] = q4_keys(a, 64 * j + lane, fresh);
+    all += static_cast<float>(x.keys[j]);
+  }
+  if (!a.unit) return x;
+  const float want = fminf(group_sum<64>(all) * static_cast<float>(items) * (1.0f / kWantBlocks), static_cast<float>(a.chunk));
+  x.chunk = min(max((static_cast<int>(want) / a.unit + 1) * a.unit, 2 * a.unit), a.chunk);
+  return x;
 }
 
 // The piece of work of number `piece`: a sequence and the first key of its chunk; false where there is none. The full
 // chunks of all sequences come first and are spread over the CUs while these are empty; then the rest of every
 // sequence (or its zeros); blocks without work come last, behind everything.
-// (Chunk by chunk instead where there are too many sequences to look through: a round of loads for every 64.)
-constexpr int kLookThrough = 256;
-__device__ __forceinline__ bool q4_piece(const Q4Attn& a, int piece, int& seq, int& begin) {
-  const int lane = threadIdx.x & 63;
-  if (a.c.n_seq > kLookThrough) {
-    int fresh;
+__device__ __forceinline__ bool q4_piece(const Q4Attn& a, const Q4Share& x, int piece, int lane, int& seq, int& begin) {
+  int fresh;
+  if (a.c.n_seq > kLookThrough) {  // chunk by chunk
     seq = piece % a.c.n_seq;
-    begin = piece / a.c.n_seq * a.chunk;
+    begin = piece / a.c.n_seq * x.chunk;
     return begin == 0 || begin < q4_keys(a, seq, fresh);
   }
   int full = 0;  // chunks of the sequences so far
-  for (int s0 = 0; s0 < a.c.n_seq; s0 += 64) {
-    int fresh;
-    const int n = s0 + lane < a.c.n_seq ? q4_keys(a, s0 + lane, fresh) / a.chunk : 0;
-    const int incl = wave_scan(n, lane) + full;
+#pragma unroll
+  for (int j = 0; j < kRounds; ++j) {
+    if (64 * j >= a.c.n_seq) break;
+    const int n = x.keys[j] / x.chunk, incl = wave_scan(n) + full;
     const uint64_t past = __builtin_amdgcn_ballot_w64(incl > piece);
     if (past) {
       const int at = __builtin_ctzll(past);
-      seq = s0 + at;
-      begin = (piece - (__builtin_amdgcn_readlane(incl, at) - __builtin_amdgcn_readlane(n, at))) * a.chunk;
+      seq = 64 * j + at;
+      begin = (piece - (__builtin_amdgcn_readlane(incl, at) - __builtin_amdgcn_readlane(n, at))) * x.chunk;
       return true;
     }
     full = __builtin_amdgcn_readlane(incl, 63);
   }
   seq = piece - full;
   if (seq >= a.c.n_seq) return false;
-  int fresh;
-  const int keys = q4_keys(a, seq, fresh), rest = keys % a.chunk;
+  const int keys = q4_keys(a, seq, fresh), rest = keys % x.chunk;
   begin = keys - rest;
   return rest > 0 || keys == 0;
+}
+
+// Where the chunks of a sequence are in the workspace: by their pieces' numbers, or, where all chunks have one size, by
+// sequence, so that nobody needs the other lengths.
+struct Q4Chunks {
+  int n, full, first, last;
+  __device__ int at(int i) const { return i < full ? first + i : last; }
+};
+__device__ __forceinline__ Q4Chunks q4_chunks(const Q4Attn& a, int items, int seq, int lane) {
+  int fresh;
+  const int keys = q4_keys(a, seq, fresh);
+  if (!a.unit) {
+    const int n = keys / a.chunk + (keys % a.chunk != 0);
+    return Q4Chunks{n, n, seq * a.most, 0};
+  }
+  const Q4Share x = q4_share(a, items, lane);
+  int before = 0, all = 0;
+#pragma unroll
+  for (int j = 0; j < kRounds; ++j) {
+    if (64 * j >= a.c.n_seq) break;
+    const int here = x.keys[j] / x.chunk;
+    before += 64 * j + lane < seq ? here : 0;
+    all += here;
+  }
+  const int full = keys / x.chunk;
+  return Q4Chunks{full + (keys % x.chunk != 0), full, wave_total(before), wave_total(all) + seq};
 }
 
 // The first arguments, which arrive in scalar registers, are what the way to the first tile needs; the rest of `a`
@@ -679,7 +738,7 @@ __device__ __forceinline__ bool q4_piece(const Q4Attn& a, int piece, int& seq, i
 template <class T, int D>
 __global__ void __launch_bounds__(512, 4) q4_attention_kernel(const int64_t* lens, uint8_t* k_codes, _Float16* k_meta,
                                                               uint8_t* v_codes, _Float16* v_meta, int max_len, int kv_heads,
-                                                              int heads, int chunk, int items, Q4Attn a) {
+                                                              int heads, int pieces, int items, Q4Attn a) {
   extern __shared__ float lds[];
   a.lens = lens;
   a.c.k_codes = k_codes;
@@ -689,12 +748,17 @@ __global__ void __launch_bounds__(512, 4) q4_attention_kernel(const int64_t* len
   a.c.max_len = max_len;
   a.c.heads = kv_heads;
   a.heads = heads;
-  a.chunk = chunk;
-  const int waves = blockDim.x / 64, item = blockIdx.x % items;
-  int seq = blockIdx.x / items, begin = 0;
-  if (a.chunks > 1 && !q4_piece(a, seq, seq, begin)) return;
+  a.pieces = pieces;
+  const int waves = blockDim.x / 64, item = blockIdx.x % items, piece = blockIdx.x / items;
+  const int lane = threadIdx.x & 63;
+  int seq = piece, begin = 0, chunk = max_len;
+  if (pieces) {
+    const Q4Share share = q4_share(a, items, lane);
+    if (!q4_piece(a, share, piece, lane, seq, begin)) return;
+    chunk = share.chunk;
+  }
   const Q4Item it = q4_item(a, item);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int fresh;
   // requested before the length is known
   const Q4Query<T, D> query = q4_load_query<T, D>(a, seq, it.head + (lane & 15), (lane & 15) < it.cols, lane);
@@ -702,15 +766,15 @@ __global__ void __launch_bounds__(512, 4) q4_attention_kernel(const int64_t* len
   h8v q[D / 32];
   const float factor = q4_queries<T, D>(a, query, q);
   Q4State<D> st;
-  q4_tiles<T, D>(a, seq, it.kvh, begin / kTileKeys + wave, waves, (begin + a.chunk) / kTileKeys, keys, fresh, q, factor, lane,
+  q4_tiles<T, D>(a, seq, it.kvh, begin / kTileKeys + wave, waves, (begin + chunk) / kTileKeys, keys, fresh, q, factor, lane,
                  st);
   const Q4Merge<D> x(lds, waves, it.cols);
   q4_hand_in<D>(x, st, wave, it.cols, lane);
   __syncthreads();
-  const bool whole = keys <= a.chunk;
-  const int64_t slot = (static_cast<int64_t>(seq) * items + item) * a.chunks + begin / a.chunk;
+  const bool whole = keys <= chunk;
+  const int64_t slot = static_cast<int64_t>(a.unit ? piece : seq * a.most + begin / chunk) * items + item;
   const int cols = q4_cols(a);
-  float* ml = a.ws + static_cast<int64_t>(items) * a.c.n_seq * a.chunks * cols * D + slot * cols * 2;
+  float* ml = a.ws + static_cast<int64_t>(pieces) * items * cols * D + slot * cols * 2;
   for (int i = threadIdx.x; i < it.cols * D; i += blockDim.x) {
     float m, l;
     const int h = i / D, d = i % D;
@@ -732,30 +796,29 @@ __global__ void __launch_bounds__(512, 4) q4_attention_kernel(const int64_t* len
 // 7.7 us against 5.0 for 64 ragged sequences of 32 heads.)
 constexpr int kCombine = 256, kBatch = 8;
 template <class T, int D>
-__global__ void __launch_bounds__(kCombine) q4_combine_kernel(const int64_t* lens, int chunk, Q4Attn a) {
+__global__ void __launch_bounds__(kCombine) q4_combine_kernel(const int64_t* lens, Q4Attn a) {
   constexpr int kLanes = kCombine / D;
   __shared__ float red[2][kCombine / 64], part[kLanes][D];
-  extern __shared__ float weight[];  // [chunks]
+  extern __shared__ float weight[];  // [the most chunks of a sequence]
   const int seq = blockIdx.y, head = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid / 64, d = tid % D, from = tid / D;
   a.lens = lens;
-  int fresh;
-  const int keys = q4_keys(a, seq, fresh), n = (keys + chunk - 1) / chunk;
-  if (n <= 1) return;  // its block finished it
   const int group = a.heads / a.c.heads, parts = (group + kCols - 1) / kCols, items = a.c.heads * parts, cols = q4_cols(a);
+  const Q4Chunks at = q4_chunks(a, items, seq, lane);
+  const int n = at.n;
+  if (n <= 1) return;  // its block finished it
   const int in_group = head % group, item = head / group * parts + in_group / kCols, h = in_group % kCols;
-  const int64_t first = (static_cast<int64_t>(seq) * items + item) * a.chunks;
-  const float2* ml = reinterpret_cast<const float2*>(a.ws + static_cast<int64_t>(items) * a.c.n_seq * a.chunks * cols * D) +
-                     first * cols + h;
-  const float* acc = a.ws + (first * cols + h) * D + d;
+  const float2* ml = reinterpret_cast<const float2*>(a.ws + static_cast<int64_t>(a.pieces) * items * cols * D) + item * cols + h;
+  const float* acc = a.ws + static_cast<int64_t>(item * cols + h) * D + d;
+  const auto slot = [&](int i) { return static_cast<int64_t>(at.at(i)) * (items * cols); };
   const auto load = [&](int i, float (&x)[kBatch]) {  // chunks i, i + kLanes, ..; past the end the last one
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) x[j] = acc[static_cast<int64_t>(min(i + j * kLanes, n - 1)) * (cols * D)];
+    for (int j = 0; j < kBatch; ++j) x[j] = acc[slot(min(i + j * kLanes, n - 1)) * D];
   };
   float x[kBatch];
   load(from, x);
   float m = -INFINITY, l = 0.f;
   for (int i = tid; i < n; i += kCombine) {
-    weight[i] = ml[static_cast<int64_t>(i) * cols].x;
+    weight[i] = ml[slot(i)].x;
     m = fmaxf(m, weight[i]);
   }
   m = group_max<64>(m);
@@ -765,7 +828,7 @@ __global__ void __launch_bounds__(kCombine) q4_combine_kernel(const int64_t* len
   for (int i = 0; i < kCombine / 64; ++i) m = fmaxf(m, red[0][i]);
   for (int i = tid; i < n; i += kCombine) {
     weight[i] = __builtin_amdgcn_exp2f(weight[i] - m);
-    l = fmaf(weight[i], ml[static_cast<int64_t>(i) * cols].y, l);
+    l = fmaf(weight[i], ml[slot(i)].y, l);
   }
   l = group_sum<64>(l);
   if (lane == 0) red[1][wave] = l;
@@ -790,20 +853,21 @@ __global__ void __launch_bounds__(kCombine) q4_combine_kernel(const int64_t* len
   q4_store<T>(a, seq, head, d, o, l);
 }
 
-// How a call is shared out, by sizes alone (the lengths are on the device). A cache of up to kOneChunk rows is one
+// What of a call goes by sizes alone (the lengths are on the device). A cache of up to kOneChunk rows is one
 // chunk: a second launch to join chunks costs more than it gains there (16 sequences x 20 heads of 64 over 1500 keys
-// 14.4 us in one chunk, 19.2 shared out further). Longer ones are cut so that full lengths give about kWantBlocks
-// blocks, two a CU (131000 keys x 8 heads of 128: 42.7 us, with twice the blocks 48.4), into chunks of at most 256
-// keys a wave, which bounds how long a few long sequences among short ones keep their CUs (64 ragged sequences of
-// up to 8000 keys x 8 heads: 39.5 us, with 512 keys a wave 61), and of at least 1 / kMostBlocks of everything, which
-// bounds the workspace. Blocks have 8 waves where items are few and 4 where they fill the CUs anyway (those 64
-// sequences: 33.5 us against 39.5; 64 x 20 heads of 64 over 700 keys 15.0 against 17.2, but 16 x 20 over 1500 keys as
-// two chunks of 4 waves 14.8 against 12.2), or where the merge of 16 heads of 128 would pass 64 KB of LDS.
+// 14.4 us in one chunk, 19.2 shared out further). Longer ones are cut. The largest chunk gives full lengths about
+// kWantBlocks blocks (131000 keys x 8 heads of 128: 42.8 us, with twice the blocks 51.7), but has at most kWaveKeys or
+// kManyWaveKeys keys a wave, which bounds how long a few long sequences among short ones keep their CUs (64 ragged
+// sequences of up to 8000 keys x 8 heads of 128 with 128 / 192 / 256 keys a wave: 29.4 / 28.6 / 30.6 us, 64 of 8000: 134.7 /
+// 131.9 / 129.9), and at least 1 / kMostBlocks of everything, which bounds the workspace. Blocks have 8 waves where items
+// are few and 4 where they fill the CUs anyway (those 64 ragged sequences: 33.5 us against 39.5; 64 x 20 heads of 64 over
+// 700 keys 15.0 against 17.2, but 16 x 20 over 1500 keys as two chunks of 4 waves 14.8 against 12.2), or where the merge of
+// 16 heads of 128 would pass 64 KB of LDS.
 struct Q4Plan {
-  int items, cols, waves, chunk, chunks;
-  int64_t parts() const { return static_cast<int64_t>(items) * chunks; }  // of a sequence
+  int items, cols, waves, chunk, most, unit, pieces;
+  int64_t blocks(int n_seq) const { return static_cast<int64_t>(items) * (pieces ? pieces : n_seq); }
 };
-constexpr int kOneChunk = 2048, kWaveKeys = 256, kWantBlocks = 512, kMostBlocks = 8192, kManyItems = 512;
+constexpr int kOneChunk = 2048, kWaveKeys = 256, kManyWaveKeys = 192, kMostBlocks = 8192, kManyItems = 512;
 
 Q4Plan q4_plan(int n_seq, int heads, int kv_heads, int max_len, int dim) {
   Q4Plan p;
@@ -814,12 +878,19 @@ Q4Plan q4_plan(int n_seq, int heads, int kv_heads, int max_len, int dim) {
   const bool many = static_cast<int64_t>(n_seq) * p.items >= kManyItems;
   p.waves = min(max_len / kTileKeys, many || lds8 > 65536 ? 4 : 8);
   p.chunk = max_len;
-  if (max_len > kOneChunk) {
-    const int64_t keys = static_cast<int64_t>(n_seq) * p.items * max_len, unit = kTileKeys * p.waves;
-    const int64_t want = max(min(keys / kWantBlocks, static_cast<int64_t>(kWaveKeys * p.waves)), keys / kMostBlocks);
-    p.chunk = static_cast<int>(min((want + unit) / unit * unit, static_cast<int64_t>(max_len)));
-  }
-  p.chunks = (max_len + p.chunk - 1) / p.chunk;
+  p.most = 1;
+  p.unit = p.pieces = 0;
+  if (max_len <= kOneChunk) return p;
+  const int64_t keys = static_cast<int64_t>(n_seq) * p.items * max_len, unit = kTileKeys * p.waves;
+  const int64_t want = max(min(keys / kWantBlocks, static_cast<int64_t>((many ? kManyWaveKeys : kWaveKeys) * p.waves)), keys / kMostBlocks);
+  p.chunk = static_cast<int>((want + unit) / unit * unit);
+  // full chunks: of the largest n_seq max_len / chunk, of smaller ones no more than kWantBlocks / items; a rest each
+  const int full = max_len / p.chunk, few = kWantBlocks / p.items + 1;
+  const bool by_length = !many && n_seq <= kLookThrough;
+  p.most = (by_length ? max(full, few) : full) + 1;
+  if (by_length) p.unit = static_cast<int>(unit);
+  const int64_t pieces = n_seq + (by_length ? max(static_cast<int64_t>(n_seq) * full, static_cast<int64_t>(few)) : static_cast<int64_t>(n_seq) * full);
+  p.pieces = static_cast<int>(min(pieces, static_cast<int64_t>(0x7FFFFFFF)));
   return p;
 }
 
@@ -930,7 +1001,7 @@ extern "C" int64_t fw_decode_attention_q4_ws_floats(int n_seq, int heads, int kv
       max_len > kMaxLen || (head_dim != 64 && head_dim != 128))
     return 0;
   const Q4Plan p = q4_plan(n_seq, heads, kv_heads, max_len, head_dim);
-  return p.chunks == 1 ? 4 : (n_seq * p.parts() * p.cols * (head_dim + 2) + 3) / 4 * 4;
+  return p.pieces ? (p.blocks(n_seq) * p.cols * (head_dim + 2) + 3) / 4 * 4 : 4;
 }
 
 extern "C" int fw_decode_attention_q4(const void* q, int64_t q_row, int64_t q_head, void* k_codes, void* k_meta,
@@ -953,19 +1024,18 @@ extern "C" int fw_decode_attention_q4(const void* q, int64_t q_row, int64_t q_he
   if (!ws || ws_floats < need || !aligned(ws, 16))
     return fw_fail(FW_EINVAL, "decode_attention_q4: workspace needs %lld floats, 16-byte aligned", static_cast<long long>(need));
   const Q4Plan p = q4_plan(n_seq, heads, kv_heads, max_len, head_dim);
-  if (n_seq > 65535 || !grid_ok(n_seq * p.parts(), 64 * p.waves)) return fw_fail(FW_EINVAL, "decode_attention_q4: too many sequences");
+  if (n_seq > 65535 || !grid_ok(p.blocks(n_seq), 64 * p.waves)) return fw_fail(FW_EINVAL, "decode_attention_q4: too many sequences");
   const Q4Attn a{q, out, q_row, q_head, o_row, o_head, Q4Rows{k_new, v_new, k_row, k_head, v_row, v_head}, lens, c, heads, scale,
-                 p.chunk, p.chunks, ws};
+                 p.chunk, p.most, p.unit, p.pieces, ws};
   const int lds = head_dim == 64 ? Q4Merge<64>::bytes(p.waves, p.cols) : Q4Merge<128>::bytes(p.waves, p.cols);
   q4_by_type(dtype, head_dim, [&](auto t, auto d) {
-    hipLaunchKernelGGL((q4_attention_kernel<decltype(t), d.value>), dim3(static_cast<unsigned>(n_seq * p.parts())), dim3(64 * p.waves), lds,
-                       stream, lens, c.k_codes, c.k_meta, c.v_codes, c.v_meta, max_len, kv_heads, heads, p.chunk, p.items, a);
+    hipLaunchKernelGGL((q4_attention_kernel<decltype(t), d.value>), dim3(static_cast<unsigned>(p.blocks(n_seq))), dim3(64 * p.waves), lds,
+                       stream, lens, c.k_codes, c.k_meta, c.v_codes, c.v_meta, max_len, kv_heads, heads, p.pieces, p.items, a);
   });
   if (const int rc = fw_check_launch("decode_attention_q4")) return rc;
-  if (p.chunks == 1) return FW_OK;
+  if (!p.pieces) return FW_OK;
   q4_by_type(dtype, head_dim, [&](auto t, auto d) {
-    hipLaunchKernelGGL((q4_combine_kernel<decltype(t), d.value>), dim3(heads, n_seq), dim3(kCombine), 4 * p.chunks, stream, lens,
-                       p.chunk, a);
+    hipLaunchKernelGGL((q4_combine_kernel<decltype(t), d.value>), dim3(heads, n_seq), dim3(kCombine), 4 * p.most, stream, lens, a);
   });
   return fw_check_launch("decode_attention_q4 combine");
 }

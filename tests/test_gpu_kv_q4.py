@@ -466,3 +466,38 @@ def test_decode_no_numbers(ext, hip_device, max_len):
     ext.decode_attention_q4(q, cache, at, got, ws, 0.125)
     assert got[0, :2].isnan().all() and got[0, 2:, 32:].isnan().all() and got[0, 2:, :32].isfinite().all()
     assert torch.equal(got[1], want[1])
+
+
+def _spread(n, high, few):
+    """n lengths, most of them short, every one of `few` among them."""
+    lens = [int(x) for x in np.random.default_rng(n).integers(0, high, n)]
+    for i, x in enumerate(few):
+        lens[(i * 37 + 5) % n] = x
+    return lens
+
+
+# Long caches are shared out in chunks. Few items: chunks by the lengths (one sequence, short and long; lengths at
+# multiples of a chunk; two to four rounds of 64 sequences); many items: chunks of one size; more sequences than are
+# looked through. The fresh row is at the end of a chunk, and the first of a new one.
+@pytest.mark.parametrize('fresh', [False, True])
+@pytest.mark.parametrize('kind, dim, heads, kv_heads, max_len, lens', [
+    ('fp16', 64, 4, 2, 16384, [3000]), ('fp16', 128, 2, 1, 16384, [511]), ('bf16', 128, 8, 1, 16384, [16384]), ('fp16', 64, 2, 2, 131072, [40000]),
+    ('bf16', 64, 17, 1, 8192, [8192, -1, 0, 512, 511, 513, 4096]), ('fp16', 64, 1, 1, 2080, _spread(70, 60, [2080, 2047, 0, 512])),
+    ('fp16', 64, 2, 1, 2080, _spread(256, 20, [2080, 1024, 1023, 0, -1])), ('bf16', 64, 1, 1, 2080, _spread(270, 20, [2080, 2048, 2047, 0, -1])),
+    ('fp16', 64, 20, 20, 2560, _spread(26, 60, [2560, 896, 895, 0, 1792, -1])), ('bf16', 128, 128, 32, 2560, _spread(16, 60, [2559, 896, 897, 0]))])
+def test_decode_shared_out(ext, hip_device, kind, dim, heads, kv_heads, max_len, lens, fresh):
+    dev, dtype, rng = hip_device, TYPES[kind], np.random.default_rng(max_len + len(lens))
+    n = len(lens)
+    want = _filled(rng, n, kv_heads, max_len, dim, lens)
+    cache = to_device(want, dev)
+    q, q64 = rounded(rng, (n, heads, dim), dtype)
+    k, v = (rounded(rng, (n, kv_heads, dim), dtype)[0] for _ in range(2))
+    out = torch.full((n, heads, dim), float('nan'), dtype=dtype, device=dev)
+    ws = torch.full_like(ext.decode_attention_q4_workspace(n, heads, cache), float('nan'))
+    ext.decode_attention_q4(q.to(dev), cache, _index(lens, dev), out, ws, dim ** -0.5, *((k.to(dev), v.to(dev)) if fresh else ()))
+    rows = [min(x, max_len - 1) for x in lens]
+    for s, row in enumerate(rows):
+        if fresh and row >= 0:
+            serving.write_row(want, s, row, k[s].float().numpy(), v[s].float().numpy())
+    assert same_bits(cache, want)
+    _check_decode(out.double().cpu().numpy(), q64, want, [r + 1 if r >= 0 else 0 for r in rows] if fresh else lens, dim ** -0.5, dtype)

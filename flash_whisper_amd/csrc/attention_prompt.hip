@@ -70,6 +70,10 @@ struct PromptArgs {
 //    whatever it is. A masked weight of 0 does not undo an infinity or NaN in V, so the block looks for them in
 //    the tile, puts zeros there, and keeps for each dim the first key with either infinity and with a NaN: a row sees
 //    the keys up to its limit, so at the end it gets those whose first key it sees.
+// Bound by the power that the products take for heads of 128 (8192 tokens of 32 heads, causal, bf16: 505 us, 1.09 PFLOP/s,
+// where a library product of 8192^3 reaches 1.2; with zeros as inputs 400 us), and for heads of 64, which have half the
+// products for every exponential, by the vector instructions beside them (8192 tokens of 20 heads: 203 us, 0.85 PFLOP/s:
+// 32 exponentials, 32 fused multiply-adds, 16 conversions and 16 sums for the 16 products of a wave's tile).
 // ------------------------------------------------------------------------------------------
 constexpr float kMost = 4096.f;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -179,8 +183,8 @@ __device__ __forceinline__ void set_aside(uint32_t at, int key, int d, OddValues
 // A wave's tile: K at LDS address k, V at v; keys kv0 .., of which the lane's row sees those up to `limit`; masked:
 // some row does not see all of them.
 template <class T, int D, int TK>
-__device__ __forceinline__ void tile(uint32_t k, uint32_t v, const Offsets<D>& off, const typename Types<T>::v8 (&q)[D / 16], float factor, int kv0,
-                                     int limit, bool masked, int lane, State<D>& st) {
+__device__ __forceinline__ void tile(uint32_t k, uint32_t v, const Offsets<D>& off, const typename Types<T>::v8 (&q)[D / 16],
+                                     float factor, int kv0, int limit, bool masked, int lane, State<D>& st) {
   typedef typename Types<T>::v8 v8;
   typedef typename Types<T>::v2 v2;
   const int lg = lane >> 5;
@@ -298,7 +302,8 @@ __global__ void __launch_bounds__(QG * KP * 64, 2) prompt_attention_kernel(Promp
   const int limit = CAUSAL ? seen0 + query : seen0;
   const auto limit_of = [&](int r) { return CAUSAL ? seen0 + min(r, job.rows - 1) / group : seen0; };
   // (a wave whose rows are all past the end takes part in the copies alone)
-  const int wave_row = job.row0 + 32 * wq, wave_first = limit_of(wave_row), wave_last = wave_row < job.rows ? limit_of(wave_row + 31) : -1;
+  const int wave_row = job.row0 + 32 * wq, wave_first = limit_of(wave_row);
+  const int wave_last = wave_row < job.rows ? limit_of(wave_row + 31) : -1;
   const int block_first = limit_of(job.row0), block_last = limit_of(job.row0 + kRows - 1);
 
   v8 q[D / 16];
@@ -445,6 +450,8 @@ __global__ void __launch_bounds__(QG * KP * 64, 2) prompt_attention_kernel(Promp
     }
 }
 
+constexpr int kCus = 256;
+
 bool rows_ok(const void* p, int64_t row, int64_t head) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && row % 8 == 0 && head % 8 == 0;
 }
@@ -459,8 +466,10 @@ extern "C" int fw_prompt_attention(const void* q, int64_t q_row, int64_t q_head,
                                    const int64_t* cu_q, const int64_t* cu_k, int n_seq, int64_t q_rows, int64_t k_rows,
                                    int heads, int kv_heads, int head_dim, int dtype, float scale, int causal,
                                    hipStream_t stream) {
-  if (n_seq <= 0 || q_rows < 0 || k_rows < 0) return fw_fail(FW_EINVAL, "prompt_attention: n_seq must be positive, rows not negative");
-  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads) return fw_fail(FW_EINVAL, "prompt_attention: heads must be a multiple of kv_heads");
+  if (n_seq <= 0 || q_rows < 0 || k_rows < 0)
+    return fw_fail(FW_EINVAL, "prompt_attention: n_seq must be positive, rows not negative");
+  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads)
+    return fw_fail(FW_EINVAL, "prompt_attention: heads must be a multiple of kv_heads");
   if (head_dim != 64 && head_dim != 128) return fw_fail(FW_EINVAL, "prompt_attention: head_dim must be 64 or 128");
   if (dtype != FW_F16 && dtype != FW_BF16) return fw_fail(FW_EINVAL, "prompt_attention: dtype must be FW_F16 or FW_BF16");
   if (!cu_q || !cu_k || (q_rows > 0 && (!q || !out)) || (k_rows > 0 && (!k || !v)))
@@ -474,7 +483,8 @@ extern "C" int fw_prompt_attention(const void* q, int64_t q_row, int64_t q_head,
     return fw_fail(FW_EINVAL, "prompt_attention: row strides of k and v must be below 2^25 elements");
   if (q_rows * (heads / kv_heads) > 0x7FFFFF00 || k_rows > 0x7FFFFF00) return fw_fail(FW_EINVAL, "prompt_attention: too many rows");
   if (q_rows == 0) return FW_OK;
-  const PromptArgs a{q, k, v, out, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, cu_q, cu_k, q_rows, k_rows, n_seq, heads, kv_heads, scale};
+  const PromptArgs a{q, k, v, out, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, cu_q, cu_k,
+                     q_rows, k_rows, n_seq, heads, kv_heads, scale};
   const int64_t rows = q_rows * (heads / kv_heads);
   int rc = FW_OK;
   const auto launch = [&](auto kernel, int per_block, int threads) {
@@ -486,19 +496,26 @@ extern "C" int fw_prompt_attention(const void* q, int64_t q_row, int64_t q_head,
     typedef decltype(t) T;
     constexpr int D = decltype(d)::value;
     constexpr bool M = decltype(mask)::value;
-    // Blocks of 128 rows stage every tile for four waves. They are the fastest where they fill the CUs; fewer rows
-    // are given to more blocks, and long chains of tiles to several waves, whose parts are then merged; where a
-    // sequence is a tile or two, a wave works alone and many blocks share a CU (us of 128 rows / 64 rows and 2 parts
-    // of 64 keys / of 32 keys / 32 rows and 8 parts, heads of 64 unless said: 1 x 4 queries x 20 heads over 1500 keys
-    // 24.5 / 15.4 / 17.4 / 11.7; 1 x 1500 x 20, causal 27.1 / 18.4 / 19.9 / 24.9; 8 x 64 x 32 over 4000 keys and 8
-    // heads of 128 84 / 68 / 79 / 87; 16 x 4 .. 224 x 20, causal 9.8 / 11.7 / 8.8 / 17.3, over 1500 keys 37.8 / 48.2 /
-    // 38.8 / 50.4. Third form / one wave of 32 rows: 1 x 4 x 20 4.5 / 4.0; 2000 x 8 x 20 209 / 73; 64 x 64 x 20 15.9 /
-    // 13.3; 16 x 4 .. 224 x 20 8.0 / 10.5).
-    const int64_t wide = (rows / 128 + n_seq) * kv_heads, keys = k_rows / n_seq;
-    if (wide <= 128 && keys >= 512) launch(prompt_attention_kernel<T, D, 1, 8, 32, 1, M>, 32, 512);
-    else if (keys <= 64) launch(prompt_attention_kernel<T, D, 1, 1, 32, 1, M>, 32, 64);
-    else if (wide <= 384 && keys >= 512) launch(prompt_attention_kernel<T, D, 2, 2, 64, 2, M>, 64, 256);
-    else if (wide <= 384 || keys < 256) launch(prompt_attention_kernel<T, D, 2, 2, 32, 2, M>, 64, 256);
+    // Blocks of 128 rows stage every tile for four waves and are the fastest where they fill the CUs. Few rows over many
+    // keys are given to several waves, whose parts of the keys are merged: 8 parts while blocks of 32 rows have a CU
+    // each, 2 parts of 64 keys while blocks of 64 rows are at most two a CU; then, and where the keys are few, 2 parts of
+    // 32 keys, up to 1.5 blocks of 128 rows a CU (2 where the keys are few and a block is over soon). Where a sequence is one
+    // tile, a wave works alone and many blocks share a CU. us of 128 rows / 64 rows, 2 parts of 32 keys / of 64 keys / 32
+    // rows, 8 parts:
+    //   heads of 64, 1 x 4 queries x 20 heads over 1500 keys 20.7 / 18.5 / 14.1 / 11.7; 6 x 4 likewise 21.7 / 19.5 / 15.3 /
+    //   13.8; 1 x 500 x 20, causal 11.1 / 9.4 / 8.3 / 10.9; 2 x 1500 x 20 31.2 / 29.3 / 27.3 / 49.7; 3 x 1500 x 20 41.1 /
+    //   39.8 / 40.2 / 72.5; 1 x 8192 x 20 204 / 257 / 234 / 386; 16 x 4 .. 224 x 20 9.4 / 8.3 / 11.5 / 20; over 1500
+    //   keys 35.9 / 39.4 / 46.5 / 57;
+    //   heads of 128 over 8 key/value heads, 4 x 32 x 32 over 4000 keys 86 / 72 / 57 / 33; 8 x 64 x 32 likewise 114 / 102 / 82 /
+    //   88; 1 x 1000 x 32, causal 27.1 / 23.9 / 26.2 / 47.4; 1 x 4096 x 32 157 / 183 / 224 / 314.
+    // Heads of 64, 128 rows / the single wave: 1 x 4 x 20 4.4 / 4.0; 2000 x 8 x 20 246 / 84; 64 x 64 x 20 14.9 / 13.9; 64 x 1
+    // .. 200 x 8 over 2 heads 7.0 / 8.5.
+    const int64_t keys = k_rows / n_seq;
+    const auto blocks_of = [&](int64_t n) { return (rows / n + n_seq) * kv_heads; };
+    if (blocks_of(32) <= kCus && keys >= 512) launch(prompt_attention_kernel<T, D, 1, 8, 32, 1, M>, 32, 512);
+    else if (keys <= 32) launch(prompt_attention_kernel<T, D, 1, 1, 32, 1, M>, 32, 64);
+    else if (blocks_of(64) <= 2 * kCus && keys >= 384) launch(prompt_attention_kernel<T, D, 2, 2, 64, 2, M>, 64, 256);
+    else if (blocks_of(128) <= (keys < 256 ? 2 * kCus : kCus * 3 / 2)) launch(prompt_attention_kernel<T, D, 2, 2, 32, 2, M>, 64, 256);
     else launch(prompt_attention_kernel<T, D, 4, 1, 64, 2, M>, 128, 256);
   };
   const auto by_mask = [&](auto t, auto d) { causal ? by_rows(t, d, std::true_type()) : by_rows(t, d, std::false_type()); };

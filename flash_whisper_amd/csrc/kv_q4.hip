@@ -421,7 +421,8 @@ __device__ __forceinline__ void q4_scores(const Q4Tile<D>& t, const h8v (&q)[D /
     for (int j = 0; j < D / 32; ++j) {
       h8v k;
       const uint32_t u = t.k[kt][j];
-      const h2v x[4] = {q4_pair<0>(u, step, low), q4_pair<1>(u, step, low), q4_pair<0>(u >> 8, step, low), q4_pair<1>(u >> 8, step, low)};
+      const h2v x[4] = {q4_pair<0>(u, step, low), q4_pair<1>(u, step, low), q4_pair<0>(u >> 8, step, low),
+                        q4_pair<1>(u >> 8, step, low)};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         k[2 * e] = x[e][0];
@@ -483,7 +484,8 @@ __device__ __forceinline__ void q4_values(const Q4Tile<D>& t, f4v (&s)[2], float
     for (int w = 0; w < 4; ++w) {
       const h2v step{vs[2 * w], vs[2 * w + 1]}, low{vl[2 * w], vl[2 * w + 1]};
       const uint32_t u = t.v[h][w];
-      const h2v x[4] = {q4_pair<0>(u, step, low), q4_pair<1>(u, step, low), q4_pair<0>(u >> 8, step, low), q4_pair<1>(u >> 8, step, low)};
+      const h2v x[4] = {q4_pair<0>(u, step, low), q4_pair<1>(u, step, low), q4_pair<0>(u >> 8, step, low),
+                        q4_pair<1>(u >> 8, step, low)};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         v[j][2 * w] = x[j][0];
@@ -882,14 +884,15 @@ Q4Plan q4_plan(int n_seq, int heads, int kv_heads, int max_len, int dim) {
   p.unit = p.pieces = 0;
   if (max_len <= kOneChunk) return p;
   const int64_t keys = static_cast<int64_t>(n_seq) * p.items * max_len, unit = kTileKeys * p.waves;
-  const int64_t want = max(min(keys / kWantBlocks, static_cast<int64_t>((many ? kManyWaveKeys : kWaveKeys) * p.waves)), keys / kMostBlocks);
+  const int64_t most = (many ? kManyWaveKeys : kWaveKeys) * p.waves, want = max(min(keys / kWantBlocks, most), keys / kMostBlocks);
   p.chunk = static_cast<int>((want + unit) / unit * unit);
   // full chunks: of the largest n_seq max_len / chunk, of smaller ones no more than kWantBlocks / items; a rest each
   const int full = max_len / p.chunk, few = kWantBlocks / p.items + 1;
   const bool by_length = !many && n_seq <= kLookThrough;
   p.most = (by_length ? max(full, few) : full) + 1;
   if (by_length) p.unit = static_cast<int>(unit);
-  const int64_t pieces = n_seq + (by_length ? max(static_cast<int64_t>(n_seq) * full, static_cast<int64_t>(few)) : static_cast<int64_t>(n_seq) * full);
+  const int64_t all_full = static_cast<int64_t>(n_seq) * full;
+  const int64_t pieces = n_seq + (by_length ? max(all_full, static_cast<int64_t>(few)) : all_full);
   p.pieces = static_cast<int>(min(pieces, static_cast<int64_t>(0x7FFFFFFF)));
   return p;
 }
@@ -973,7 +976,8 @@ extern "C" int fw_kv_q4_append(const void* k, int64_t k_row, int64_t k_head, con
   if (rows == 0) return FW_OK;
   const Q4Grid g = q4_grid(rows, n_seq, kv_heads, head_dim, 1);
   q4_by_type(dtype, head_dim, [&](auto t, auto d) {
-    hipLaunchKernelGGL((kv_q4_append_kernel<decltype(t), d.value>), dim3(g.blocks), dim3(256), 0, stream, cu, pos, rows, g.slots, n_seq, kv_heads, r, c);
+    hipLaunchKernelGGL((kv_q4_append_kernel<decltype(t), d.value>), dim3(g.blocks), dim3(256), 0, stream, cu, pos, rows, g.slots,
+                       n_seq, kv_heads, r, c);
   });
   return fw_check_launch("kv_q4_append");
 }
@@ -1018,19 +1022,22 @@ extern "C" int fw_decode_attention_q4(const void* q, int64_t q_row, int64_t q_he
   if (!(__builtin_fabsf(scale) < INFINITY)) return fw_fail(FW_EINVAL, "decode_attention_q4: scale must be finite");
   if (!k_new != !v_new) return fw_fail(FW_EINVAL, "decode_attention_q4: k_new and v_new must be given together");
   if (heads <= 0 || heads % kv_heads) return fw_fail(FW_EINVAL, "decode_attention_q4: heads must be a multiple of kv_heads");
-  if (!rows_ok(q, q_row, q_head) || !rows_ok(out, o_row, o_head) || (k_new && (!rows_ok(k_new, k_row, k_head) || !rows_ok(v_new, v_row, v_head))))
-    return fw_fail(FW_EINVAL, "decode_attention_q4: q, out, k_new and v_new must be 16-byte aligned with strides in multiples of 8");
+  if (!rows_ok(q, q_row, q_head) || !rows_ok(out, o_row, o_head) ||
+      (k_new && (!rows_ok(k_new, k_row, k_head) || !rows_ok(v_new, v_row, v_head))))
+    return fw_fail(FW_EINVAL,
+                   "decode_attention_q4: q, out, k_new and v_new must be 16-byte aligned with strides in multiples of 8");
   const int64_t need = fw_decode_attention_q4_ws_floats(n_seq, heads, kv_heads, max_len, head_dim);
   if (!ws || ws_floats < need || !aligned(ws, 16))
     return fw_fail(FW_EINVAL, "decode_attention_q4: workspace needs %lld floats, 16-byte aligned", static_cast<long long>(need));
   const Q4Plan p = q4_plan(n_seq, heads, kv_heads, max_len, head_dim);
-  if (n_seq > 65535 || !grid_ok(p.blocks(n_seq), 64 * p.waves)) return fw_fail(FW_EINVAL, "decode_attention_q4: too many sequences");
+  if (n_seq > 65535 || !grid_ok(p.blocks(n_seq), 64 * p.waves))
+    return fw_fail(FW_EINVAL, "decode_attention_q4: too many sequences");
   const Q4Attn a{q, out, q_row, q_head, o_row, o_head, Q4Rows{k_new, v_new, k_row, k_head, v_row, v_head}, lens, c, heads, scale,
                  p.chunk, p.most, p.unit, p.pieces, ws};
   const int lds = head_dim == 64 ? Q4Merge<64>::bytes(p.waves, p.cols) : Q4Merge<128>::bytes(p.waves, p.cols);
   q4_by_type(dtype, head_dim, [&](auto t, auto d) {
-    hipLaunchKernelGGL((q4_attention_kernel<decltype(t), d.value>), dim3(static_cast<unsigned>(p.blocks(n_seq))), dim3(64 * p.waves), lds,
-                       stream, lens, c.k_codes, c.k_meta, c.v_codes, c.v_meta, max_len, kv_heads, heads, p.pieces, p.items, a);
+    hipLaunchKernelGGL((q4_attention_kernel<decltype(t), d.value>), dim3(static_cast<unsigned>(p.blocks(n_seq))),
+                       dim3(64 * p.waves), lds, stream, lens, c.k_codes, c.k_meta, c.v_codes, c.v_meta, max_len, kv_heads, heads, p.pieces, p.items, a);
   });
   if (const int rc = fw_check_launch("decode_attention_q4")) return rc;
   if (!p.pieces) return FW_OK;

@@ -271,3 +271,18 @@ def test_starts_that_fall_and_rise(ext, hip_device):
             out = torch.full_like(x, 3.0)
             ext.prompt_attention(x[300:700], x[300:700], x[300:700], out[300:700], starts_of, starts_of, 0.125, causal)
             assert (out[:300] == 3.0).all() and (out[700:] == 3.0).all() and not out.isnan().any()
+
+
+# sizes on either side of where one way of sharing out the rows takes over from another
+SIDES = {'full_blocks': ([700, 33, 900], [700, 160, 900], 40, 20), 'few_full_blocks': ([640, 129], [700, 130], 40, 20),
+         'one_tile': ([32, 8, 2, 1], [32, 20, 4, 7], 8, 4), 'past_one_tile': ([33, 8, 64, 1], [33, 31, 64, 4], 8, 4),
+         'keys_383': ([383], [383], 8, 8), 'keys_384': ([384], [384], 8, 8), 'keys_511': ([40], [511], 8, 4), 'keys_512': ([40], [512], 8, 4),
+         'eight_parts_full': ([200, 31], [600, 600], 26, 26), 'past_eight_parts': ([225, 31], [600, 600], 26, 26)}
+
+
+@pytest.mark.parametrize('kind, dim', [('fp16', 64), ('bf16', 128)])
+@pytest.mark.parametrize('causal', [True, False])
+@pytest.mark.parametrize('sides', SIDES)
+def test_sides_of_forms(ext, hip_device, sides, causal, kind, dim):
+    nq, nk, heads, kv_heads = SIDES[sides]
+    _run(ext, hip_device, nq, nk, heads, kv_heads, dim, kind, causal, seed=dim + 1)

@@ -498,12 +498,14 @@ extern "C" int fw_prompt_attention(const void* q, int64_t q_row, int64_t q_head,
     constexpr bool M = decltype(mask)::value;
     // Blocks of 128 rows stage every tile for four waves and are the fastest where they fill the CUs. Few rows over many
     // keys are given to several waves, whose parts of the keys are merged: 8 parts while blocks of 32 rows have a CU
-    // each, 2 parts of 64 keys while blocks of 64 rows are at most two a CU; then, and where the keys are few, 2 parts of
+    // each, 2 parts of 64 keys while blocks of 64 rows are at most two a CU (causal ones of heads of 64, which end at
+    // different times and of which a CU holds two, four); then, and where the keys are few, 2 parts of
     // 32 keys, up to 1.5 blocks of 128 rows a CU (2 where the keys are few and a block is over soon). Where a sequence is one
     // tile, a wave works alone and many blocks share a CU. us of 128 rows / 64 rows, 2 parts of 32 keys / of 64 keys / 32
     // rows, 8 parts:
     //   heads of 64, 1 x 4 queries x 20 heads over 1500 keys 20.7 / 18.5 / 14.1 / 11.7; 6 x 4 likewise 21.7 / 19.5 / 15.3 /
-    //   13.8; 1 x 500 x 20, causal 11.1 / 9.4 / 8.3 / 10.9; 2 x 1500 x 20 31.2 / 29.3 / 27.3 / 49.7; 3 x 1500 x 20 41.1 /
+    //   13.8; 1 x 500 x 20, causal 11.1 / 9.4 / 8.3 / 10.9; 1 x 2000 x 20 30.9 / 26.9 / 22.6 / 38.5; 2 x 1500 x 20 31.2 / 29.3 /
+    //   27.3 / 49.7; 3 x 1500 x 20 41.1 /
     //   39.8 / 40.2 / 72.5; 1 x 8192 x 20 204 / 257 / 234 / 386; 16 x 4 .. 224 x 20 9.4 / 8.3 / 11.5 / 20; over 1500
     //   keys 35.9 / 39.4 / 46.5 / 57;
     //   heads of 128 over 8 key/value heads, 4 x 32 x 32 over 4000 keys 86 / 72 / 57 / 33; 8 x 64 x 32 likewise 114 / 102 / 82 /
@@ -514,7 +516,7 @@ extern "C" int fw_prompt_attention(const void* q, int64_t q_row, int64_t q_head,
     const auto blocks_of = [&](int64_t n) { return (rows / n + n_seq) * kv_heads; };
     if (blocks_of(32) <= kCus && keys >= 512) launch(prompt_attention_kernel<T, D, 1, 8, 32, 1, M>, 32, 512);
     else if (keys <= 32) launch(prompt_attention_kernel<T, D, 1, 1, 32, 1, M>, 32, 64);
-    else if (blocks_of(64) <= 2 * kCus && keys >= 384) launch(prompt_attention_kernel<T, D, 2, 2, 64, 2, M>, 64, 256);
+    else if (blocks_of(64) <= (M && D == 64 ? 4 : 2) * kCus && keys >= 384) launch(prompt_attention_kernel<T, D, 2, 2, 64, 2, M>, 64, 256);
     else if (blocks_of(128) <= (keys < 256 ? 2 * kCus : kCus * 3 / 2)) launch(prompt_attention_kernel<T, D, 2, 2, 32, 2, M>, 64, 256);
     else launch(prompt_attention_kernel<T, D, 4, 1, 64, 2, M>, 128, 256);
   };

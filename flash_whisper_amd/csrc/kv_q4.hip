@@ -796,8 +796,11 @@ __global__ void __launch_bounds__(512, 4) q4_attention_kernel(const int64_t* len
 // Joins the chunks of items that have several: block = (query head, sequence). The chunks' O are requested before
 // their weights are known. (A block for all query heads of an item is slower, its heads waiting for each other:
 // 7.7 us against 5.0 for 64 ragged sequences of 32 heads.)
-constexpr int kCombine = 256, kBatch = 8;
-template <class T, int D>
+// 512 threads where the blocks are at most one a CU, so that twice the chunks are on their way (2 sequences of 39000 keys,
+// one key/value head: the call takes 14.8 us instead of 18.4; 1024 threads 14.2, but 10.3 instead of 9.6 where
+// there are fewer chunks), else 256 (64 ragged sequences of 32 heads 28.5 against 30.2).
+constexpr int kBatch = 8;
+template <class T, int D, int kCombine>
 __global__ void __launch_bounds__(kCombine) q4_combine_kernel(const int64_t* lens, Q4Attn a) {
   constexpr int kLanes = kCombine / D;
   __shared__ float red[2][kCombine / 64], part[kLanes][D];
@@ -1041,8 +1044,10 @@ extern "C" int fw_decode_attention_q4(const void* q, int64_t q_row, int64_t q_he
   });
   if (const int rc = fw_check_launch("decode_attention_q4")) return rc;
   if (!p.pieces) return FW_OK;
+  const int threads = heads * static_cast<int64_t>(n_seq) <= 256 ? 512 : 256;
   q4_by_type(dtype, head_dim, [&](auto t, auto d) {
-    hipLaunchKernelGGL((q4_combine_kernel<decltype(t), d.value>), dim3(heads, n_seq), dim3(kCombine), 4 * p.most, stream, lens, a);
+    const auto kernel = threads == 512 ? q4_combine_kernel<decltype(t), d.value, 512> : q4_combine_kernel<decltype(t), d.value, 256>;
+    hipLaunchKernelGGL(kernel, dim3(heads, n_seq), dim3(threads), 4 * p.most, stream, lens, a);
   });
   return fw_check_launch("decode_attention_q4 combine");
 }

@@ -503,8 +503,8 @@ extern "C" int fw_prompt_attention(const void* q, int64_t q_row, int64_t q_head,
     // 32 keys, up to 1.5 blocks of 128 rows a CU (2 where the keys are few and a block is over soon). Where a sequence is one
     // tile, a wave works alone and many blocks share a CU. us of 128 rows / 64 rows, 2 parts of 32 keys / of 64 keys / 32
     // rows, 8 parts:
-    //   heads of 64, 1 x 4 queries x 20 heads over 1500 keys 20.7 / 18.5 / 14.1 / 11.7; 6 x 4 likewise 21.7 / 19.5 / 15.3 /
-    //   13.8; 1 x 500 x 20, causal 11.1 / 9.4 / 8.3 / 10.9; 1 x 2000 x 20 30.9 / 26.9 / 22.6 / 38.5; 2 x 1500 x 20 31.2 / 29.3 /
+    //   heads of 64, 1 x 4 queries x 20 heads over 1500 keys 20.7 / 18.5 / 14.1 / 11.3; 6 x 4 likewise 21.7 / 19.5 / 15.3 /
+    //   13.5; 1 x 500 x 20, causal 11.1 / 9.4 / 8.3 / 10.9; 1 x 2000 x 20 30.9 / 26.9 / 22.6 / 38.5; 2 x 1500 x 20 31.2 / 29.3 /
     //   27.3 / 49.7; 3 x 1500 x 20 41.1 /
     //   39.8 / 40.2 / 72.5; 1 x 8192 x 20 204 / 257 / 234 / 386; 16 x 4 .. 224 x 20 9.4 / 8.3 / 11.5 / 20; over 1500
     //   keys 35.9 / 39.4 / 46.5 / 57;
@@ -514,7 +514,9 @@ extern "C" int fw_prompt_attention(const void* q, int64_t q_row, int64_t q_head,
     // .. 200 x 8 over 2 heads 7.0 / 8.5.
     const int64_t keys = k_rows / n_seq;
     const auto blocks_of = [&](int64_t n) { return (rows / n + n_seq) * kv_heads; };
-    if (blocks_of(32) <= kCus && keys >= 512) launch(prompt_attention_kernel<T, D, 1, 8, 32, 1, M>, 32, 512);
+    // (8 parts with a second stage where the LDS holds it: 1 x 4 queries x 20 heads over 1500 keys 11.3 us against 12.1, 5 x 8
+    // x 20 over 2705 16.5 against 17.7.)
+    if (blocks_of(32) <= kCus && keys >= 512) launch(prompt_attention_kernel<T, D, 1, 8, 32, D == 64 ? 2 : 1, M>, 32, 512);
     else if (keys <= 32) launch(prompt_attention_kernel<T, D, 1, 1, 32, 1, M>, 32, 64);
     else if (blocks_of(64) <= (M && D == 64 ? 4 : 2) * kCus && keys >= 384) launch(prompt_attention_kernel<T, D, 2, 2, 64, 2, M>, 64, 256);
     else if (blocks_of(128) <= (keys < 256 ? 2 * kCus : kCus * 3 / 2)) launch(prompt_attention_kernel<T, D, 2, 2, 32, 2, M>, 64, 256);

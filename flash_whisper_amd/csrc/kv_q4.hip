@@ -860,7 +860,9 @@ __global__ void __launch_bounds__(kCombine) q4_combine_kernel(const int64_t* len
 
 // What of a call goes by sizes alone (the lengths are on the device). A cache of up to kOneChunk rows is one
 // chunk: a second launch to join chunks costs more than it gains there (16 sequences x 20 heads of 64 over 1500 keys
-// 14.4 us in one chunk, 19.2 shared out further). Longer ones are cut. The largest chunk gives full lengths about
+// 14.4 us in one chunk, 19.2 shared out further; 1 x 20 7.8 and 8.7). For heads of 128, which take a wave twice as long, half
+// of that where the items fill a quarter of the CUs at most (2000 keys x 8 heads: 9.5 us, in one chunk 13.2; 32 x 8 heads over
+// 1536 keys 20.1, in one 13.4). Longer ones are cut. The largest chunk gives full lengths about
 // kWantBlocks blocks (131000 keys x 8 heads of 128: 42.8 us, with twice the blocks 51.7), but has at most kWaveKeys or
 // kManyWaveKeys keys a wave, which bounds how long a few long sequences among short ones keep their CUs (64 ragged
 // sequences of up to 8000 keys x 8 heads of 128 with 128 / 192 / 256 keys a wave: 29.4 / 28.6 / 30.6 us, 64 of 8000: 134.7 /
@@ -885,7 +887,8 @@ Q4Plan q4_plan(int n_seq, int heads, int kv_heads, int max_len, int dim) {
   p.chunk = max_len;
   p.most = 1;
   p.unit = p.pieces = 0;
-  if (max_len <= kOneChunk) return p;
+  const bool few_items = static_cast<int64_t>(n_seq) * p.items <= 64;
+  if (max_len <= (dim == 128 && few_items ? kOneChunk / 2 : kOneChunk)) return p;
   const int64_t keys = static_cast<int64_t>(n_seq) * p.items * max_len, unit = kTileKeys * p.waves;
   const int64_t most = (many ? kManyWaveKeys : kWaveKeys) * p.waves, want = max(min(keys / kWantBlocks, most), keys / kMostBlocks);
   p.chunk = static_cast<int>((want + unit) / unit * unit);

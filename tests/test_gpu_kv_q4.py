@@ -501,3 +501,16 @@ def test_decode_shared_out(ext, hip_device, kind, dim, heads, kv_heads, max_len,
             serving.write_row(want, s, row, k[s].float().numpy(), v[s].float().numpy())
     assert same_bits(cache, want)
     _check_decode(out.double().cpu().numpy(), q64, want, [r + 1 if r >= 0 else 0 for r in rows] if fresh else lens, dim ** -0.5, dtype)
+
+
+@pytest.mark.parametrize('n, heads, kv_heads, max_len', [(8, 8, 8, 1024), (8, 8, 8, 1056), (9, 8, 8, 1056), (1, 20, 4, 2048), (1, 20, 4, 2080)])
+def test_decode_sides_of_one_chunk(ext, hip_device, n, heads, kv_heads, max_len):
+    """Heads of 128: caches that are one chunk, and those next to them that are shared out."""
+    dev, rng = hip_device, np.random.default_rng(max_len + n)
+    lens = [max_len - 3, 512, 513, 511, 0, 1024, 100, 1, 900][:n]
+    want = _filled(rng, n, kv_heads, max_len, 128, lens)
+    cache = to_device(want, dev)
+    q, q64 = rounded(rng, (n, heads, 128), torch.float16)
+    out = torch.full((n, heads, 128), float('nan'), dtype=torch.float16, device=dev)
+    ext.decode_attention_q4(q.to(dev), cache, _index(lens, dev), out, ext.decode_attention_q4_workspace(n, heads, cache), 128 ** -0.5)
+    _check_decode(out.double().cpu().numpy(), q64, want, lens, 128 ** -0.5, torch.float16)

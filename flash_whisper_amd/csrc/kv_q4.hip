@@ -500,7 +500,9 @@ __device__ __forceinline__ void q4_values(const Q4Tile<D>& t, f4v (&s)[2], float
 // The item's queries as the products' operand, lane (h, g): dims D / 4 g + 8 j .. in the order of q4_pair's
 // pairs, and the factor from raw scores to log2 units. A bf16 query is scaled by a power of two to fit fp16 (its
 // elements 2^-24 of the largest and less lose bits); the factor undoes it. A negative scale negates the query,
-// a zero one becomes so small that scores vanish.
+// a zero one becomes so small that scores vanish. The factor of the scaled query is kept a positive number: against one of
+// zero a masked score (-infinity), against an infinite one a score of zero would be NaN. (Raised to 1e-30, scores, of at most
+// 2^39, vanish all the same; lowered to the largest number, every score but zero is past 2^79, which fp32 does not resolve.)
 template <class T, int D>
 struct Q4Query {
   typename Vec8<T>::type x[D / 32];
@@ -525,7 +527,7 @@ __device__ __forceinline__ float q4_queries(const Q4Attn& a, const Q4Query<T, D>
       big = fmaxf(big, __builtin_fabsf(f[j][e]));
     }
   }
-  float factor = fmaxf(__builtin_fabsf(a.scale) * kLog2e, 1e-30f);
+  float factor = __builtin_fabsf(a.scale);
   if constexpr (!__is_same(T, _Float16)) {
     big = xor_max<32>(xor_max<16>(big));
     const int ex = big < INFINITY ? __builtin_amdgcn_frexp_expf(big) : 0;
@@ -535,6 +537,7 @@ __device__ __forceinline__ float q4_queries(const Q4Attn& a, const Q4Query<T, D>
       for (int e = 0; e < 8; ++e) f[j][e] = __builtin_amdgcn_ldexpf(f[j][e], -ex);
     factor = __builtin_amdgcn_ldexpf(factor, ex);
   }
+  factor = fminf(fmaxf(factor * kLog2e, 1e-30f), __FLT_MAX__);
 #pragma unroll
   for (int j = 0; j < D / 32; ++j)
 #pragma unroll

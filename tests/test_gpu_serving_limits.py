@@ -1,0 +1,61 @@
+"""The prompt attention and the 4-bit cache at the ends of what their entry points take: scales, values and sizes."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import serving
+from serving_tools import check_attention, check_prompts, rounded, starts, to_device
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope='module')
+def ext(hip_device):
+    from flash_whisper_amd.ext import load_ext
+
+    return load_ext()
+
+
+def _index(x, dev):
+    return torch.tensor(x, dtype=torch.int64, device=dev)
+
+
+def _cache_of(k, v, max_len, dim, dev):
+    """A cache whose one sequence holds rows k, v [rows, heads, dim], on the device and as the oracle's arrays."""
+    want = serving.empty_cache(1, k.shape[1], max_len, dim, fill=0xFF)
+    for i in range(len(k)):
+        serving.write_row(want, 0, i, k[i].float().numpy(), v[i].float().numpy())
+    return to_device(want, dev), want
+
+
+@pytest.mark.parametrize('keys', [1, 32, 37, 300])
+@pytest.mark.parametrize('exponent', [-126, -60, 0, 100])
+def test_decode_scale_of_zero(ext, hip_device, exponent, keys):
+    """A scale of zero weighs all keys alike, however small or large a bf16 query is, and where the last tile is not whole."""
+    dev, rng = hip_device, np.random.default_rng(keys)
+    k, v = (rounded(rng, (keys, 1, 64), torch.float16)[0] for _ in range(2))
+    cache, want = _cache_of(k, v, 320, 64, dev)
+    q = (rounded(rng, (1, 2, 64), torch.bfloat16)[0].float() * 2.0 ** exponent).bfloat16()
+    out = torch.full((1, 2, 64), 9.0, dtype=torch.bfloat16, device=dev)
+    ext.decode_attention_q4(q.to(dev), cache, _index([keys], dev), out, ext.decode_attention_q4_workspace(1, 2, cache), 0.0)
+    k64, v64 = serving.read_rows(want, 0, range(keys))
+    o, spread, size = serving.attend(q.double().numpy(), k64, v64, 0.0, False)
+    check_attention(out.double().cpu().numpy(), o, spread, size, np.abs(v64.astype(np.float64)).max(), keys, torch.bfloat16)
+
+
+@pytest.mark.parametrize('scale', [1.0, -1.0, 0.125])
+def test_decode_large_queries(ext, hip_device, scale):
+    """The largest bf16 queries over keys that are zero where they are not: scores of zero stay zero, all keys weigh alike."""
+    dev, rng = hip_device, np.random.default_rng(2)
+    k, v = (rounded(rng, (37, 1, 64), torch.float16)[0] for _ in range(2))
+    k[:, :, :32] = 0
+    cache, want = _cache_of(k, v, 64, 64, dev)
+    q = torch.zeros(1, 2, 64, dtype=torch.bfloat16)
+    q[:, :, 3] = 3e38
+    out = torch.full((1, 2, 64), 9.0, dtype=torch.bfloat16, device=dev)
+    ext.decode_attention_q4(q.to(dev), cache, _index([37], dev), out, ext.decode_attention_q4_workspace(1, 2, cache), scale)
+    k64, v64 = serving.read_rows(want, 0, range(37))
+    o, spread, size = serving.attend(q.double().numpy(), k64, v64, scale, False)
+    assert not size.any()
+    check_attention(out.double().cpu().numpy(), o, spread, size, np.abs(v64.astype(np.float64)).max(), 37, torch.bfloat16)

@@ -314,7 +314,13 @@ __global__ void __launch_bounds__(QG * KP * 64, 2) prompt_attention_kernel(Promp
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) q[j] = -q[j];
   }
-  const float factor = fmaxf(__builtin_fabsf(a.scale) * kLog2e, 1e-30f);  // 0: so small that scores vanish
+  // A scale of zero makes the queries zero instead (a bf16 score may be as large as any factor is small), so that the
+  // factor is never one: a masked score (-infinity) times zero is NaN.
+  if (a.scale == 0.f) {
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) q[j] *= static_cast<T>(0.f);
+  }
+  const float factor = fmaxf(__builtin_fabsf(a.scale) * kLog2e, __FLT_MIN__);
 
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ring));
   const T* kbase = static_cast<const T*>(a.k) + job.k0 * a.k_row + kvh * a.k_head;
@@ -477,7 +483,8 @@ extern "C" int fw_prompt_attention(const void* q, int64_t q_row, int64_t q_head,
   if ((q_rows > 0 && (!rows_ok(q, q_row, q_head) || !rows_ok(out, o_row, o_head))) ||
       (k_rows > 0 && (!rows_ok(k, k_row, k_head) || !rows_ok(v, v_row, v_head))))
     return fw_fail(FW_EINVAL, "prompt_attention: q, k, v and out must be 16-byte aligned with strides in multiples of 8");
-  if (!(__builtin_fabsf(scale) < INFINITY)) return fw_fail(FW_EINVAL, "prompt_attention: scale must be finite");
+  if (!(__builtin_fabsf(scale) * kLog2e < INFINITY))
+    return fw_fail(FW_EINVAL, "prompt_attention: scale must be finite (and below 2.3e38 in size)");
   // 64 rows of k and of v within the copies' 32-bit byte offsets; rows x heads of a sequence are counted in 32 bits
   if (k_row < 0 || v_row < 0 || k_row >= (1 << 25) || v_row >= (1 << 25))
     return fw_fail(FW_EINVAL, "prompt_attention: row strides of k and v must be below 2^25 elements");

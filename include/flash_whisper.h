@@ -435,7 +435,7 @@ int fw_cross_kv(const void* enc, int t, const void* w, const void* bias, void* c
  * key, each one before it a key less (j <= i + n_keys - n_queries, both counted within the sequence). A query that
  * sees no key gets zeros. What a query does not see does not reach its output, whatever it holds (infinities and NaN
  * too). Rows of out behind the last sequence are left as they are. Scores, softmax and sums are fp32; the weights
- * are rounded to the type for the product with v. out overlaps no input; scale is finite, here and below;
+ * are rounded to the type for the product with v. out overlaps no input; scale is finite, here (and below 2.3e38 in size) and below;
  * where a score passes 2^27 in size (scale q . k log2(e)), which fp32 resolves to 16, the result is not defined. */
 int fw_prompt_attention(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                         const void* v, int64_t v_row, int64_t v_head, void* out, int64_t o_row, int64_t o_head,

@@ -59,3 +59,28 @@ def test_decode_large_queries(ext, hip_device, scale):
     o, spread, size = serving.attend(q.double().numpy(), k64, v64, scale, False)
     assert not size.any()
     check_attention(out.double().cpu().numpy(), o, spread, size, np.abs(v64.astype(np.float64)).max(), 37, torch.bfloat16)
+
+
+@pytest.mark.parametrize('dim', [64, 128])
+@pytest.mark.parametrize('causal', [True, False])
+@pytest.mark.parametrize('scale', [0.0, -0.0, 2.0 ** -119, -2.0 ** -119])
+def test_prompt_small_scales_of_large_scores(ext, hip_device, scale, causal, dim):
+    """bf16 queries and keys whose products are near 2^120: a scale of zero weighs all keys alike all the same, and one of
+    2^-119 gives ordinary scores."""
+    dev, rng = hip_device, np.random.default_rng(dim)
+    q, k = ((rounded(rng, (90, 2, dim), torch.bfloat16)[0].float() * 2.0 ** 57).bfloat16() for _ in range(2))
+    v, v64 = rounded(rng, (90, 2, dim), torch.bfloat16)
+    out, cu = torch.empty(90, 2, dim, dtype=torch.bfloat16, device=dev), starts([50, 40], dev)
+    ext.prompt_attention(q.to(dev), k.to(dev), v.to(dev), out, cu, cu, scale, causal)
+    check_prompts(out.double().cpu().numpy(), q.double().numpy(), k.double().numpy(), v64, [50, 40], [50, 40], scale, causal, torch.bfloat16)
+
+
+def test_prompt_scale_of_zero_no_numbers(ext, hip_device):
+    """A scale of zero does not turn a query that is no number into one."""
+    dev, rng = hip_device, np.random.default_rng(6)
+    q, k, v = (rounded(rng, (40, 2, 64), torch.float16)[0].to(dev) for _ in range(3))
+    q[3, 1, 5], q[4, 0, 6] = float('nan'), float('inf')
+    out, cu = torch.empty_like(q), starts([40], dev)
+    ext.prompt_attention(q, k, v, out, cu, cu, 0.0)
+    bad = out.isnan().all(-1)
+    assert bad[3, 1] and bad[4, 0] and bad.sum() == 2 and out.isnan().sum() == 128

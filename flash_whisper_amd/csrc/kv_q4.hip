@@ -66,7 +66,8 @@ __device__ __forceinline__ Q4Slot q4_slot(const int64_t* cu, const int64_t* pos,
 
 // A group's step and low from its smallest and largest value: the step rounded towards zero, so that
 // low + 15 step stays within the group's values and no finite value reads back as an infinity. A group
-// holding a NaN or an infinity gets a NaN step and reads back as NaN.
+// holding a NaN, an infinity or a bf16 value that fp16 rounds to one gets a NaN step and reads back as NaN.
+constexpr float kPastHalf = 65520.f;
 __device__ __forceinline__ void q4_meta(float lo, float hi, bool finite, _Float16& step, _Float16& low) {
   const auto rtz = __builtin_amdgcn_cvt_pkrtz((hi - lo) * (1.0f / 15.0f), 0.f);
   step = finite ? static_cast<_Float16>(rtz[0]) : static_cast<_Float16>(__builtin_nanf(""));
@@ -91,7 +92,7 @@ __device__ __forceinline__ uint32_t q4_pack8(const typename Vec8<T>::type& x, _F
   hi = __builtin_elementwise_maximum(hi, xor_lane<1>(hi));
   lo = __builtin_elementwise_minimum(lo, xor_lane<2>(lo));
   hi = __builtin_elementwise_maximum(hi, xor_lane<2>(hi));
-  q4_meta(lo, hi, lo > -INFINITY && hi < INFINITY, step, low);
+  q4_meta(lo, hi, lo > -kPastHalf && hi < kPastHalf, step, low);
   const float s = h2f(step), l = h2f(low), inverse = 1.0f / s;
   uint32_t codes = 0;
 #pragma unroll

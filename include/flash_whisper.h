@@ -454,7 +454,8 @@ int fw_prompt_attention(const void* q, int64_t q_row, int64_t q_head, const void
  * fw_prompt_attention) into the cache rows pos[s] .. of sequence s (cu, pos int64, device); rows that fall outside
  * [0, max_len) are dropped, every other row of the cache is left as it is. Per group: low = fp16(min), step =
  * (max - min) / 15 in fp16 rounded towards zero, c = the code nearest to (x - low) / step, ties to even. A group
- * holding a NaN or an infinity reads back as NaN; bf16 values beyond fp16's range read back as non-finite ones. */
+ * holding a NaN, an infinity or a value of 65520 or more in size (bf16) reads back as NaN. Steps and values are no finer
+ * than fp16's, 2^-24: bf16 values below 2^-25 read back as zeros, a range below 2^-10 costs up to 2^-20 beside half a step. */
 int fw_kv_q4_append(const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head,
                     int64_t rows, const int64_t* cu, const int64_t* pos, void* k_codes, void* k_meta, void* v_codes,
                     void* v_meta, int n_seq, int kv_heads, int max_len, int head_dim, int dtype, hipStream_t stream);

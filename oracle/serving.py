@@ -46,7 +46,7 @@ def quantise(x):
     """(step, low) fp16 [..., dim / 32] and codes uint8 [..., dim] of rows x [..., dim]."""
     g = np.asarray(x, np.float32).reshape(*x.shape[:-1], -1, GROUP)
     with np.errstate(invalid='ignore', over='ignore', divide='ignore'):
-        finite = np.isfinite(g).all(-1)
+        finite = (np.abs(g) < 65520).all(-1)  # what fp16 rounds to a number
         low32, high = g.min(-1), g.max(-1)
         step = np.where(finite, half_down(np.where(finite, (high - low32) * np.float32(1 / 15), 0)), np.float16(np.nan))
         low = np.float16(low32)

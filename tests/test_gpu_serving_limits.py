@@ -84,3 +84,31 @@ def test_prompt_scale_of_zero_no_numbers(ext, hip_device):
     ext.prompt_attention(q, k, v, out, cu, cu, 0.0)
     bad = out.isnan().all(-1)
     assert bad[3, 1] and bad[4, 0] and bad.sum() == 2 and out.isnan().sum() == 128
+
+
+@pytest.mark.parametrize('fresh', [False, True])
+@pytest.mark.parametrize('values, good', [([65280.0, -65280.0, 1.0], True), ([65536.0, 0.0, 1.0], False), ([1e6, 7e4, 9e4, 100.0], False),
+                                          ([-65536.0, 5.0], False), ([-3e38, 3e38], False), ([1e-30, -2e-9], True), ([3e-5, 0.0, 1e-5], True)])
+def test_cache_bf16_past_fp16(ext, hip_device, values, good, fresh):
+    """A bf16 group whose values fp16 does not reach reads back as NaN, none of it as other numbers, and as what the codes
+    stand for below; the row's other group and the other head stay what they are. By an append, and by the decode's fresh row."""
+    dev = hip_device
+    x = torch.zeros(1, 2, 64, dtype=torch.bfloat16)
+    x[0, 0, :len(values)] = torch.tensor(values, dtype=torch.bfloat16)
+    x[0, 0, 32:], x[0, 1] = torch.arange(32) / 8, torch.arange(64) / 16
+    cache, cu, pos = ext.kv_q4_cache(1, 2, 32, 64), starts([1], dev), _index([0], dev)
+    if fresh:
+        out = torch.empty_like(x, device=dev)
+        ext.decode_attention_q4(torch.zeros_like(x, device=dev), cache, pos, out, ext.decode_attention_q4_workspace(1, 2, cache), 0.125,
+                                x.to(dev), x.to(dev))
+    else:
+        ext.kv_q4_append(x.to(dev), x.to(dev), cu, pos, cache)
+    want = serving.empty_cache(1, 2, 32, 64)
+    serving.write_row(want, 0, 0, x[0].float().numpy(), x[0].float().numpy())
+    got = torch.empty_like(x, device=dev), torch.empty_like(x, device=dev)
+    ext.kv_q4_read(cache, cu, pos, *got)
+    for g, w in zip(got, serving.read_rows(want, 0, [0])):
+        g, w = g.cpu(), torch.from_numpy(w).to(torch.bfloat16)
+        bad = torch.zeros(1, 2, 64, dtype=torch.bool)
+        bad[0, 0, :32] = not good
+        assert torch.equal(w.isnan(), bad) and torch.equal(g.isnan(), bad) and torch.equal(g[~bad], w[~bad])

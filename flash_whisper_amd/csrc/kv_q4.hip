@@ -7,6 +7,7 @@
 //                                          one 16-byte load holds a lane's 8 keys of the P V products
 //   v_meta  [seq][head][L / 8][D / 32] {step of 8 rows, low of 8 rows}
 // A code c stands for fp16(low + step c), one rounding; 5 bits a value with step and low.
+#include <algorithm>
 #include <type_traits>
 
 #include "packed_rows.h"
@@ -894,7 +895,8 @@ Q4Plan q4_plan(int n_seq, int heads, int kv_heads, int max_len, int dim) {
   const bool few_items = static_cast<int64_t>(n_seq) * p.items <= 64;
   if (max_len <= (dim == 128 && few_items ? kOneChunk / 2 : kOneChunk)) return p;
   const int64_t keys = static_cast<int64_t>(n_seq) * p.items * max_len, unit = kTileKeys * p.waves;
-  const int64_t most = (many ? kManyWaveKeys : kWaveKeys) * p.waves, want = max(min(keys / kWantBlocks, most), keys / kMostBlocks);
+  const int64_t most = (many ? kManyWaveKeys : kWaveKeys) * p.waves;  // (std:: below: the unqualified ones take ints on the host)
+  const int64_t want = std::min<int64_t>(std::max(std::min(keys / kWantBlocks, most), keys / kMostBlocks), max_len);
   p.chunk = static_cast<int>((want + unit) / unit * unit);
   // full chunks: of the largest n_seq max_len / chunk, of smaller ones no more than kWantBlocks / items; a rest each
   const int full = max_len / p.chunk, few = kWantBlocks / p.items + 1;
@@ -902,8 +904,8 @@ Q4Plan q4_plan(int n_seq, int heads, int kv_heads, int max_len, int dim) {
   p.most = (by_length ? max(full, few) : full) + 1;
   if (by_length) p.unit = static_cast<int>(unit);
   const int64_t all_full = static_cast<int64_t>(n_seq) * full;
-  const int64_t pieces = n_seq + (by_length ? max(all_full, static_cast<int64_t>(few)) : all_full);
-  p.pieces = static_cast<int>(min(pieces, static_cast<int64_t>(0x7FFFFFFF)));
+  const int64_t pieces = n_seq + (by_length ? std::max<int64_t>(all_full, few) : all_full);
+  p.pieces = static_cast<int>(std::min<int64_t>(pieces, 0x7FFFFFFF));
   return p;
 }
 

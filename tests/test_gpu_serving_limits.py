@@ -112,3 +112,25 @@ def test_cache_bf16_past_fp16(ext, hip_device, values, good, fresh):
         bad = torch.zeros(1, 2, 64, dtype=torch.bool)
         bad[0, 0, :32] = not good
         assert torch.equal(w.isnan(), bad) and torch.equal(g.isnan(), bad) and torch.equal(g[~bad], w[~bad])
+
+
+def test_decode_heads_times_rows(ext, hip_device):
+    """2^20 query heads over one key/value head of 2^28 rows: 2^44 keys in all items, the chunk still a number of rows."""
+    dev, rng = hip_device, np.random.default_rng(7)
+    rows = 1 << 28
+    empty = lambda dtype, *shape: torch.empty(1, 1, *shape, dtype=dtype, device=dev)
+    cache = (empty(torch.uint8, rows, 32), empty(torch.float16, rows, 2, 2), empty(torch.uint8, rows // 8, 16, 16),
+             empty(torch.float16, rows // 8, 2, 2, 8))
+    k, v = (rounded(rng, (70, 1, 64), torch.float16)[0] for _ in range(2))
+    ext.kv_q4_append(k.to(dev), v.to(dev), starts([70], dev), _index([0], dev), cache)
+    want = serving.empty_cache(1, 1, 96, 64)
+    for i in range(70):
+        serving.write_row(want, 0, i, k[i].float().numpy(), v[i].float().numpy())
+    few, q64 = rounded(rng, (1, 16, 64), torch.float16)
+    q = few.to(dev).repeat(1, 1 << 16, 1)
+    out = torch.full_like(q, 9.0)
+    ext.decode_attention_q4(q, cache, _index([70], dev), out, ext.decode_attention_q4_workspace(1, 1 << 20, cache), 0.125)
+    o, spread, size = serving.attend(q64, *serving.read_rows(want, 0, range(70)), 0.125, False)
+    got = out.view(1, 1 << 16, 16, 64)
+    assert torch.equal(got, got[:, :1].expand_as(got))
+    check_attention(got[0, :1].double().cpu().numpy(), o, spread, size, np.abs(v.double().numpy()).max() * 1.1, 70, torch.float16)

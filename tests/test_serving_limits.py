@@ -20,3 +20,13 @@ def test_prompt_scale_past_the_exponent(built_lib, scale):
 
     assert _prompt(built_lib, scale=scale) == _lib.FW_EINVAL
     assert b'scale must be finite' in built_lib.fw_last_error()
+
+
+@pytest.mark.parametrize('n, heads, kv, max_len, dim', [(1, 1 << 20, 1, 1 << 28, 64), (1, 1 << 18, 1, 1 << 30, 64), (4, 1 << 20, 4, 1 << 28, 128),
+                                                        (1, 16, 1, 1 << 30, 64), (4096, 64, 8, 1 << 17, 128), (64, 32, 8, 131072, 128)])
+def test_decode_workspace_is_bounded(built_lib, n, heads, kv, max_len, dim):
+    """However many keys there are in all items, they are at most 8192 chunks and one more an item: (m, l, O) of each."""
+    group = heads // kv
+    items, cols = kv * -(-group // 16), min(16, group)
+    floats = built_lib.fw_decode_attention_q4_ws_floats(n, heads, kv, max_len, dim)
+    assert 0 < floats <= (8192 + n * items) * cols * (dim + 2) + 4

@@ -488,7 +488,7 @@ extern "C" int fw_prompt_attention(const void* q, int64_t q_row, int64_t q_head,
   // 64 rows of k and of v within the copies' 32-bit byte offsets; rows x heads of a sequence are counted in 32 bits
   if (k_row < 0 || v_row < 0 || k_row >= (1 << 25) || v_row >= (1 << 25))
     return fw_fail(FW_EINVAL, "prompt_attention: row strides of k and v must be below 2^25 elements");
-  if (q_rows * (heads / kv_heads) > 0x7FFFFF00 || k_rows > 0x7FFFFF00) return fw_fail(FW_EINVAL, "prompt_attention: too many rows");
+  if (q_rows > 0x7FFFFF00 / (heads / kv_heads) || k_rows > 0x7FFFFF00) return fw_fail(FW_EINVAL, "prompt_attention: too many rows");
   if (q_rows == 0) return FW_OK;
   const PromptArgs a{q, k, v, out, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, cu_q, cu_k,
                      q_rows, k_rows, n_seq, heads, kv_heads, scale};

@@ -30,3 +30,12 @@ def test_decode_workspace_is_bounded(built_lib, n, heads, kv, max_len, dim):
     items, cols = kv * -(-group // 16), min(16, group)
     floats = built_lib.fw_decode_attention_q4_ws_floats(n, heads, kv, max_len, dim)
     assert 0 < floats <= (8192 + n * items) * cols * (dim + 2) + 4
+
+
+@pytest.mark.parametrize('rows, heads, kv', [(1 << 62, 80, 20), (1 << 61, 8, 1), (0x7FFFFF01, 20, 20), (0x7FFFFF00 // 4 + 1, 80, 20)])
+def test_prompt_rows_times_heads(built_lib, rows, heads, kv):
+    """The rows of a group's heads are counted in 32 bits; more are refused however large, also where the product wraps round."""
+    from flash_whisper_amd import _lib
+
+    assert _prompt(built_lib, q_rows=rows, heads=heads, kv=kv) == _lib.FW_EINVAL
+    assert b'too many rows' in built_lib.fw_last_error()

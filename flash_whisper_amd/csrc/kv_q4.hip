@@ -966,8 +966,9 @@ int check_packed(const char* what, const Q4Rows& r, const int64_t* cu, const int
   if (!cu || !pos || (rows > 0 && (!r.k || !r.v))) return fw_fail(FW_EINVAL, "%s: null pointer", what);
   if (rows > 0 && (!rows_ok(r.k, r.k_row, r.k_head) || !rows_ok(r.v, r.v_row, r.v_head)))
     return fw_fail(FW_EINVAL, "%s: k and v must be 16-byte aligned with strides in multiples of 8", what);
-  // the grid: 4 waves a block, slots x heads x halves waves
-  if (rows > int64_t{1} << 40 || !grid_ok(((rows / 8 + 2 * static_cast<int64_t>(c.n_seq)) * c.heads * (dim / 64) + 3) / 4, 256))
+  // the grid: 4 waves a block, slots x heads x halves waves (a quotient: their product may pass 64 bits)
+  const int64_t slots = rows / 8 + 2 * static_cast<int64_t>(c.n_seq), per_slot = static_cast<int64_t>(c.heads) * (dim / 64);
+  if (slots > 0xFFFFFFFFll / 256 * 4 / per_slot)
     return fw_fail(FW_EINVAL, "%s: too many rows", what);
   return FW_OK;
 }

@@ -39,3 +39,16 @@ def test_prompt_rows_times_heads(built_lib, rows, heads, kv):
 
     assert _prompt(built_lib, q_rows=rows, heads=heads, kv=kv) == _lib.FW_EINVAL
     assert b'too many rows' in built_lib.fw_last_error()
+
+
+@pytest.mark.parametrize('rows, heads, dim', [((1 << 40) - 32, 1 << 27, 64), ((1 << 40) - 32, 1 << 26, 128), (1 << 62, 1 << 30, 128), (1 << 10, 1 << 30, 128),
+                                              (1 << 62, 1, 64)])
+def test_cache_rows_times_heads(built_lib, rows, heads, dim):
+    """An append or a read of more waves than a grid has is refused, also where their number wraps round 64 bits."""
+    from flash_whisper_amd import _lib
+
+    strides, cache, sizes = (64, 64), (D16, D16, D16, D16), (2, heads, 32, dim)
+    assert built_lib.fw_kv_q4_append(D16, *strides, D16, *strides, rows, D16, D16, *cache, *sizes, 0, None) == _lib.FW_EINVAL
+    assert b'too many rows' in built_lib.fw_last_error()
+    assert built_lib.fw_kv_q4_read(*cache, *sizes, D16, D16, rows, D16, *strides, D16, *strides, 0, None) == _lib.FW_EINVAL
+    assert b'too many rows' in built_lib.fw_last_error()

@@ -1045,6 +1045,8 @@ extern "C" int fw_decode_attention_q4(const void* q, int64_t q_row, int64_t q_he
   const Q4Plan p = q4_plan(n_seq, heads, kv_heads, max_len, head_dim);
   if (n_seq > 65535 || !grid_ok(p.blocks(n_seq), 64 * p.waves))
     return fw_fail(FW_EINVAL, "decode_attention_q4: too many sequences");
+  const int threads = heads * static_cast<int64_t>(n_seq) <= 256 ? 512 : 256;  // of the combine launch
+  if (p.pieces && !grid_ok(heads, threads)) return fw_fail(FW_EINVAL, "decode_attention_q4: too many heads");
   const Q4Attn a{q, out, q_row, q_head, o_row, o_head, Q4Rows{k_new, v_new, k_row, k_head, v_row, v_head}, lens, c, heads, scale,
                  p.chunk, p.most, p.unit, p.pieces, ws};
   const int lds = head_dim == 64 ? Q4Merge<64>::bytes(p.waves, p.cols) : Q4Merge<128>::bytes(p.waves, p.cols);
@@ -1054,7 +1056,6 @@ extern "C" int fw_decode_attention_q4(const void* q, int64_t q_row, int64_t q_he
   });
   if (const int rc = fw_check_launch("decode_attention_q4")) return rc;
   if (!p.pieces) return FW_OK;
-  const int threads = heads * static_cast<int64_t>(n_seq) <= 256 ? 512 : 256;
   q4_by_type(dtype, head_dim, [&](auto t, auto d) {
     const auto kernel = threads == 512 ? q4_combine_kernel<decltype(t), d.value, 512> : q4_combine_kernel<decltype(t), d.value, 256>;
     hipLaunchKernelGGL(kernel, dim3(heads, n_seq), dim3(threads), 4 * p.most, stream, lens, a);

@@ -52,3 +52,13 @@ def test_cache_rows_times_heads(built_lib, rows, heads, dim):
     assert b'too many rows' in built_lib.fw_last_error()
     assert built_lib.fw_kv_q4_read(*cache, *sizes, D16, D16, rows, D16, *strides, D16, *strides, 0, None) == _lib.FW_EINVAL
     assert b'too many rows' in built_lib.fw_last_error()
+
+
+def test_decode_heads_past_a_grid(built_lib):
+    """More heads than the joining launch has blocks for are refused before anything is launched."""
+    from flash_whisper_amd import _lib
+
+    strides = (64, 64)
+    assert built_lib.fw_decode_attention_q4(D16, *strides, D16, D16, D16, D16, D16, D16, *strides, None, *strides, None, *strides, 1, 1 << 25, 1,
+                                            4096, 64, 0, 0.125, D16, 1 << 60, None) == _lib.FW_EINVAL
+    assert b'too many heads' in built_lib.fw_last_error()

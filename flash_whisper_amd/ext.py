@@ -140,9 +140,15 @@ class KvQ4Cache(NamedTuple):
     v_meta: torch.Tensor   # fp16 [n_seq, kv_heads, max_len / 8, head_dim / 32, 2, 8]
 
 
+def _cache_arrays(cache):
+    if not (isinstance(cache, (tuple, list)) and len(cache) == 4 and all(isinstance(t, torch.Tensor) for t in cache)):
+        raise RuntimeError('the cache must be a KvQ4Cache: k_codes, k_meta, v_codes, v_meta')
+    return cache
+
+
 def _cache_sizes(cache, dev):
     """Checks the four arrays of a cache; returns n_seq, kv_heads, max_len, head_dim."""
-    k_codes, k_meta, v_codes, v_meta = cache
+    k_codes, k_meta, v_codes, v_meta = _cache_arrays(cache)
     for t, dtype, name in ((k_codes, torch.uint8, 'k_codes'), (k_meta, _F16, 'k_meta'), (v_codes, torch.uint8, 'v_codes'),
                            (v_meta, _F16, 'v_meta')):
         if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev and t.is_contiguous()):
@@ -471,10 +477,12 @@ class WhisperExt:
 
     def decode_attention_q4_workspace(self, n_seq, heads, cache):
         """Workspace of decode_attention_q4 for n_seq sequences and `heads` query heads over `cache` (one per stream)."""
-        _, kv_heads, max_len, half = cache[0].shape
+        codes = _cache_arrays(cache)[0]
+        _require(codes.dim() == 4, 'k_codes must be [n_seq, kv_heads, max_len, head_dim / 2]')
+        _, kv_heads, max_len, half = codes.shape
         n = self.lib.fw_decode_attention_q4_ws_floats(int(n_seq), int(heads), kv_heads, max_len, 2 * half)
         _require(n > 0, 'decode_attention_q4: heads must be a multiple of the cache\'s heads')
-        return torch.empty(n, dtype=torch.float32, device=cache[0].device)
+        return torch.empty(n, dtype=torch.float32, device=codes.device)
 
     def decode_attention_q4(self, q, cache, lens, out, ws, scale, k_new=None, v_new=None):
         """One query a sequence, q and out [n_seq, heads, head_dim], over the first lens[s] rows of the 4-bit cache; with

@@ -3,6 +3,7 @@
 import ctypes
 
 import pytest
+import torch
 
 D16 = ctypes.c_void_p(16)
 
@@ -62,3 +63,17 @@ def test_decode_heads_past_a_grid(built_lib):
     assert built_lib.fw_decode_attention_q4(D16, *strides, D16, D16, D16, D16, D16, D16, *strides, None, *strides, None, *strides, 1, 1 << 25, 1,
                                             4096, 64, 0, 0.125, D16, 1 << 60, None) == _lib.FW_EINVAL
     assert b'too many heads' in built_lib.fw_last_error()
+
+
+@pytest.mark.parametrize('cache', [None, (), 7, (torch.zeros(1, 1, 32, 32),) * 3, (None,) * 4, [None] * 4])
+def test_not_a_cache(built_lib, cache):
+    """Anything but a cache's four arrays is a RuntimeError, as every invalid argument is."""
+    from flash_whisper_amd.ext import load_ext
+
+    ext = load_ext()
+    x, cu = torch.zeros(4, 2, 64, dtype=torch.float16), torch.zeros(2, dtype=torch.int64)
+    for call in (lambda: ext.kv_q4_append(x, x, cu, cu[:1], cache), lambda: ext.kv_q4_read(cache, cu, cu[:1], x, x),
+                 lambda: ext.decode_attention_q4(x[:1], cache, cu[:1], x[:1], torch.zeros(4), 0.125),
+                 lambda: ext.decode_attention_q4_workspace(1, 2, cache)):
+        with pytest.raises(RuntimeError):
+            call()

@@ -658,7 +658,8 @@ __device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readl
 
 // How the keys of all sequences are shared out: chunks so long that about kWantBlocks blocks have one (two a CU), at least
 // two tiles a wave and at most a.chunk. Lane i has the keys of sequences i, i + 64, .. Many items fill the CUs in any
-// case and get a.chunk, without the sum over the lengths; more sequences than kLookThrough nobody looks through at all.
+// case and get a.chunk, without the sum over the lengths, unless the cache is so long that it makes a.chunk long (q4_plan);
+// more sequences than kLookThrough nobody looks through at all.
 // (One sequence of 3000 keys in a cache for 131072, 8 heads of 128: 11.0 us, in chunks for a full cache 18.9; 8 of 2000
 // for 32768 12.3 against 17.1; 32 ragged ones of up to 4000 16.3 against 19.5; lengths near the full ones are alike.)
 constexpr int kLookThrough = 256, kRounds = kLookThrough / 64, kWantBlocks = 512;
@@ -871,7 +872,11 @@ __global__ void __launch_bounds__(kCombine) q4_combine_kernel(const int64_t* len
 // kWantBlocks blocks (131000 keys x 8 heads of 128: 42.8 us, with twice the blocks 51.7), but has at most kWaveKeys or
 // kManyWaveKeys keys a wave, which bounds how long a few long sequences among short ones keep their CUs (64 ragged
 // sequences of up to 8000 keys x 8 heads of 128 with 128 / 192 / 256 keys a wave: 29.4 / 28.6 / 30.6 us, 64 of 8000: 134.7 /
-// 131.9 / 129.9), and at least 1 / kMostBlocks of everything, which bounds the workspace. Blocks have 8 waves where items
+// 131.9 / 129.9). The chunk is at least 1 / kMostBlocks of everything, which bounds the workspace and comes before that; where
+// this makes it kLoose times as long as the bound for many items, up to kLookThrough sequences get chunks by their lengths (64
+// ragged sequences x 8 heads of 128 in caches of 16384 / 32768 / 49152 / 131072 rows, 1.3 / 2.7 / 4 / 11 times the bound: 25.5 /
+// 32.0 / 31.2 / 53.2 us, by length 26.3 / 26.9 / 26.5 / 26.8; all of 1000 keys 22.1 / 23.5 / 22.4 / 28.7 and 24.8 / 25.9 / 25.1 /
+// 26.6; 250 x 4 heads, one of 8000 keys, 2.6 / 5.2 / 10 times: 25.0 / 29.6 / 49.7, by length 28.5 / 28.7 / 28.7). Blocks have 8 waves where items
 // are few and 4 where they fill the CUs anyway (those 64 ragged sequences: 33.5 us against 39.5; 64 x 20 heads of 64 over
 // 700 keys 15.0 against 17.2, but 16 x 20 over 1500 keys as two chunks of 4 waves 14.8 against 12.2), or where the merge of
 // 16 heads of 128 would pass 64 KB of LDS.
@@ -879,7 +884,7 @@ struct Q4Plan {
   int items, cols, waves, chunk, most, unit, pieces;
   int64_t blocks(int n_seq) const { return static_cast<int64_t>(items) * (pieces ? pieces : n_seq); }
 };
-constexpr int kOneChunk = 2048, kWaveKeys = 256, kManyWaveKeys = 192, kMostBlocks = 8192, kManyItems = 512;
+constexpr int kOneChunk = 2048, kWaveKeys = 256, kManyWaveKeys = 192, kMostBlocks = 8192, kManyItems = 512, kLoose = 3;
 
 Q4Plan q4_plan(int n_seq, int heads, int kv_heads, int max_len, int dim) {
   Q4Plan p;
@@ -900,7 +905,7 @@ Q4Plan q4_plan(int n_seq, int heads, int kv_heads, int max_len, int dim) {
   p.chunk = static_cast<int>((want + unit) / unit * unit);
   // full chunks: of the largest n_seq max_len / chunk, of smaller ones no more than kWantBlocks / items; a rest each
   const int full = max_len / p.chunk, few = kWantBlocks / p.items + 1;
-  const bool by_length = !many && n_seq <= kLookThrough;
+  const bool by_length = n_seq <= kLookThrough && (!many || want > kLoose * most);
   p.most = (by_length ? max(full, few) : full) + 1;
   if (by_length) p.unit = static_cast<int>(unit);
   const int64_t all_full = static_cast<int64_t>(n_seq) * full;

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from oracle import serving
-from serving_tools import check_attention, check_prompts, rounded, starts, to_device
+from serving_tools import TYPES, check_attention, check_prompts, rounded, starts, to_device
 
 pytestmark = pytest.mark.gpu
 
@@ -134,3 +134,50 @@ def test_decode_heads_times_rows(ext, hip_device):
     got = out.view(1, 1 << 16, 16, 64)
     assert torch.equal(got, got[:, :1].expand_as(got))
     check_attention(got[0, :1].double().cpu().numpy(), o, spread, size, np.abs(v.double().numpy()).max() * 1.1, 70, torch.float16)
+
+
+@pytest.mark.parametrize('fresh', [False, True])
+@pytest.mark.parametrize('kind, dim, n, heads, kv_heads, max_len', [('fp16', 64, 32, 256, 1, 40960), ('bf16', 128, 130, 8, 4, 40960),
+                                                                    ('fp16', 64, 256, 32, 2, 40960)])
+def test_decode_many_items_in_long_caches(ext, hip_device, kind, dim, n, heads, kv_heads, max_len, fresh):
+    """512 items and more whose capacity would make chunks long: the few long sequences among them in chunks by the lengths,
+    the fresh row at a chunk's end and the first of one; a captured call replayed with other lengths gives the bits of an eager
+    one, and both the float64 values."""
+    dev, dtype, rng = hip_device, TYPES[kind], np.random.default_rng(n)
+    cache = ext.kv_q4_cache(n, kv_heads, max_len, dim)
+    ws = torch.full_like(ext.decode_attention_q4_workspace(n, heads, cache), float('nan'))
+    q, q64 = rounded(rng, (n, heads, dim), dtype)
+    k1, v1 = (torch.zeros(n, kv_heads, dim, dtype=dtype, device=dev) for _ in range(2))
+    q, lens, out = q.to(dev), torch.full((n,), -1, dtype=torch.int64, device=dev), torch.empty(n, heads, dim, dtype=dtype, device=dev)
+    call = lambda: ext.decode_attention_q4(q, cache, lens, out, ws, dim ** -0.5, *((k1, v1) if fresh else ()))
+    rows = [3000, 5] + [int(x) for x in rng.integers(0, 40, n - 2)]
+    rows[n // 2], rows[n - 1] = 9000, 2047
+    k, v = (rounded(rng, (sum(rows), kv_heads, dim), dtype)[0].to(dev) for _ in range(2))
+    ext.kv_q4_append(k, v, starts(rows, dev), torch.zeros_like(lens), cache)
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    held_k, held_v = torch.empty_like(k, dtype=torch.float16), torch.empty_like(v, dtype=torch.float16)
+    ext.kv_q4_read(cache, starts(rows, dev), torch.zeros_like(lens), held_k, held_v)
+    for few in (0, 256, 255, 1 << 20):  # the long ones cut to some rows, or not at all
+        now = [min(x, few) if x > 2047 else x for x in rows]
+        now[3] = -1
+        lens.copy_(_index([x - 1 if fresh and x > 0 else x for x in now], dev))
+        if fresh:  # the row that is there already, written again
+            for s, (x, at) in enumerate(zip(now, np.cumsum([0] + rows[:-1]))):
+                k1[s], v1[s] = (k[at + x - 1], v[at + x - 1]) if x > 0 else (0, 0)
+            lens[[s for s, x in enumerate(now) if x == 0]] = -1
+        out.fill_(9.0)
+        graph.replay()
+        got = out.clone()
+        out.fill_(7.0)
+        call()
+        torch.cuda.synchronize()
+        assert torch.equal(got, out)
+        got = got.double().cpu().numpy()
+        for s in {0, 1, 2, 3, 4, n // 2, n - 2, n - 1}:
+            a, x = sum(rows[:s]), max(now[s], 0)
+            ks, vs = (h[a:a + x].double().cpu().numpy() for h in (held_k, held_v))
+            o, spread, size = serving.attend(q64[s][None], ks, vs, dim ** -0.5, False)
+            check_attention(got[s][None], o, spread, size, np.abs(vs).max(initial=0), x, dtype)

@@ -866,7 +866,7 @@ __global__ void __launch_bounds__(kCombine) q4_combine_kernel(const int64_t* len
 
 // What of a call goes by sizes alone (the lengths are on the device). A cache of up to kOneChunk rows is one
 // chunk: a second launch to join chunks costs more than it gains there (16 sequences x 20 heads of 64 over 1500 keys
-// 14.4 us in one chunk, 19.2 shared out further; 1 x 20 7.8 and 8.7). For heads of 128, which take a wave twice as long, half
+// 13.6 us in one chunk, 18.9 shared out further; 1 x 20 8.4 and 9.3). For heads of 128, which take a wave twice as long, half
 // of that where the items fill a quarter of the CUs at most (2000 keys x 8 heads: 9.5 us, in one chunk 13.2; 32 x 8 heads over
 // 1536 keys 20.1, in one 13.4). Longer ones are cut. The largest chunk gives full lengths about
 // kWantBlocks blocks (131000 keys x 8 heads of 128: 42.8 us, with twice the blocks 51.7), but has at most kWaveKeys or
@@ -878,7 +878,7 @@ __global__ void __launch_bounds__(kCombine) q4_combine_kernel(const int64_t* len
 // 32.0 / 31.2 / 53.2 us, by length 26.3 / 26.9 / 26.5 / 26.8; all of 1000 keys 22.1 / 23.5 / 22.4 / 28.7 and 24.8 / 25.9 / 25.1 /
 // 26.6; 250 x 4 heads, one of 8000 keys, 2.6 / 5.2 / 10 times: 25.0 / 29.6 / 49.7, by length 28.5 / 28.7 / 28.7). Blocks have 8 waves where items
 // are few and 4 where they fill the CUs anyway (those 64 ragged sequences: 33.5 us against 39.5; 64 x 20 heads of 64 over
-// 700 keys 15.0 against 17.2, but 16 x 20 over 1500 keys as two chunks of 4 waves 14.8 against 12.2), or where the merge of
+// 700 keys 15.0 against 17.2, but 16 x 20 over 1500 keys as two chunks of 4 waves 16.3 against 13.6), or where the merge of
 // 16 heads of 128 would pass 64 KB of LDS.
 struct Q4Plan {
   int items, cols, waves, chunk, most, unit, pieces;

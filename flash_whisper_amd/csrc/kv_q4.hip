@@ -903,8 +903,9 @@ Q4Plan q4_plan(int n_seq, int heads, int kv_heads, int max_len, int dim) {
   const int64_t most = (many ? kManyWaveKeys : kWaveKeys) * p.waves;  // (std:: below: the unqualified ones take ints on the host)
   const int64_t want = std::min<int64_t>(std::max(std::min(keys / kWantBlocks, most), keys / kMostBlocks), max_len);
   p.chunk = static_cast<int>((want + unit) / unit * unit);
-  // full chunks: of the largest n_seq max_len / chunk, of smaller ones no more than kWantBlocks / items; a rest each
-  const int full = max_len / p.chunk, few = kWantBlocks / p.items + 1;
+  // full chunks: of the largest n_seq max_len / chunk, of smaller ones no more than kWantBlocks / items (none of more
+  // items than that: a chunk is then longer than all sequences); a rest each
+  const int full = max_len / p.chunk, few = p.items > kWantBlocks ? 0 : kWantBlocks / p.items + 1;
   const bool by_length = n_seq <= kLookThrough && (!many || want > kLoose * most);
   p.most = (by_length ? max(full, few) : full) + 1;
   if (by_length) p.unit = static_cast<int>(unit);

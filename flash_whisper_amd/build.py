@@ -5,8 +5,8 @@ parallel, one object per source) and links them. The library exports the entry p
 ``include/flash_whisper.h``. It also links the profiling build ``libflash_whisper_timeline.so``: the
 same objects with the decoder step compiled with FW_STEP_TIMELINE=1, which records the phase timeline
 that ``python -m flash_whisper_amd.step_timeline`` reads (selected with FW_LIBRARY; never the default), and
-the Python module ``_bind.so`` (csrc/bind.cpp), through which ext.py calls the ops whose kernels take less time than
-a ctypes call. This replaces the reference's JIT extension build (custom/ext.py:13-18),
+the Python module ``_bind.so`` (csrc/bind.cpp, with g++ or $CXX), through which ext.py calls the ops whose kernels take
+less time than a ctypes call; where that cannot be compiled the build says so and goes on. This replaces the reference's JIT extension build (custom/ext.py:13-18),
 which ran nvcc through torch.utils.cpp_extension; here the build is ahead-of-time and in-tree so the
 built library travels with the source tree.
 """
@@ -83,24 +83,33 @@ def _link(objs, lib, verbose):
 
 
 def _compile_bind(verbose):
-    """csrc/bind.cpp, host code on torch's and Python's headers, into the module _bind."""
-    import sysconfig
+    """csrc/bind.cpp, host code on torch's and Python's headers, into the module _bind; returns whether there is one. The
+    library does not need it: without a C++ compiler or the headers ext.py makes the same calls through ctypes."""
+    try:
+        import sysconfig
 
-    import torch
-    from torch.utils.cpp_extension import include_paths, library_paths
+        import torch
+        from torch.utils.cpp_extension import include_paths, library_paths
 
-    tmp = BIND_LIB.with_suffix('.so.tmp')
-    cmd = [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared', '-Wall',
-           f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}', '-D__HIP_PLATFORM_AMD__=1',
-           *(f'-isystem{p}' for p in [*include_paths(), '/opt/rocm/include', sysconfig.get_paths()['include']]),
-           str(CSRC / 'bind.cpp'), '-o', str(tmp), *(f'-L{p}' for p in library_paths()), '-ltorch_python', '-ltorch_cpu',
-           '-lc10']
-    if verbose:
-        print(' '.join(cmd), flush=True)
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError(f'{cmd[0]} failed for bind.cpp:\n{proc.stdout}{proc.stderr}')
-    os.replace(tmp, BIND_LIB)
+        tmp = BIND_LIB.with_suffix('.so.tmp')
+        rocm = os.environ.get('ROCM_PATH') or Path(HIPCC).resolve().parents[1]
+        cmd = [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared', '-Wall',
+               f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}', '-D__HIP_PLATFORM_AMD__=1',
+               *(f'-isystem{p}' for p in [*include_paths(), f'{rocm}/include', sysconfig.get_paths()['include']]),
+               str(CSRC / 'bind.cpp'), '-o', str(tmp), *(f'-L{p}' for p in library_paths()), '-ltorch_python',
+               '-ltorch_cpu', '-lc10']
+        if verbose:
+            print(' '.join(cmd), flush=True)
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+        why = f'{cmd[0]} failed for bind.cpp:\n{proc.stdout}{proc.stderr}' if proc.returncode else ''
+    except (ImportError, OSError) as e:
+        why = str(e)
+    if not why:
+        os.replace(tmp, BIND_LIB)
+        return True
+    BIND_LIB.unlink(missing_ok=True)  # an earlier build's need not fit this library
+    print(f'{BIND_LIB.name} is not built, its calls go through ctypes: {why}', file=sys.stderr, flush=True)
+    return False
 
 
 def build(verbose=False, jobs=None):

@@ -77,3 +77,21 @@ def test_not_a_cache(built_lib, cache):
                  lambda: ext.decode_attention_q4_workspace(1, 2, cache)):
         with pytest.raises(RuntimeError):
             call()
+
+
+@pytest.mark.parametrize('missing', ['compiler', 'headers', 'torch'])
+def test_build_without_the_binding(monkeypatch, tmp_path, capsys, missing):
+    """No C++ compiler, one that fails, no torch to compile against: the build says so, leaves no binding of an earlier one
+    behind and goes on."""
+    import sys
+
+    from flash_whisper_amd import build
+
+    monkeypatch.setattr(build, 'BIND_LIB', tmp_path / '_bind.so')
+    (tmp_path / '_bind.so').write_bytes(b'an earlier one')
+    if missing == 'torch':
+        monkeypatch.setitem(sys.modules, 'torch.utils.cpp_extension', None)
+    else:
+        monkeypatch.setenv('CXX', str(tmp_path / 'none') if missing == 'compiler' else 'false')
+    assert build._compile_bind(False) is False
+    assert not list(tmp_path.iterdir()) and 'ctypes' in capsys.readouterr().err

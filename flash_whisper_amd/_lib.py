@@ -18,6 +18,7 @@ FW_OK, FW_EINVAL, FW_EHIP = 0, -1, -2
 NOALLOC_ATTN_SLOTS = 2048  # FW_NOALLOC_ATTN_SLOTS
 ACT_NONE, ACT_GELU = 0, 1
 F16, BF16 = 0, 1  # FW_F16, FW_BF16
+PROMPT_128_ROWS, PROMPT_2_PARTS, PROMPT_2_SHORT_PARTS, PROMPT_8_PARTS, PROMPT_WAVES = range(5)  # FW_PROMPT_*
 EPI_BIAS, EPI_BIAS_GELU, EPI_BIAS_RESID, EPI_BIAS_RESID_CLAMP, EPI_BIAS_GELU_POS, EPI_SCALE_Q = range(6)
 
 P = c_void_p
@@ -62,6 +63,7 @@ SIGNATURES = {
     'fw_cross_kv': (c_int, [P, c_int, P, P, P, c_int, c_int, P]),
     'fw_prompt_attention': (c_int, [P, c_int64, c_int64, P, c_int64, c_int64, P, c_int64, c_int64, P, c_int64, c_int64,
                                     P, P, c_int, c_int64, c_int64, c_int, c_int, c_int, c_int, c_float, c_int, P]),
+    'fw_prompt_attention_form': (c_int, [c_int, c_int64, c_int64, c_int, c_int, c_int, c_int]),
     'fw_kv_q4_append': (c_int, [P, c_int64, c_int64, P, c_int64, c_int64, c_int64, P, P, P, P, P, P, c_int, c_int, c_int,
                                 c_int, c_int, P]),
     'fw_kv_q4_read': (c_int, [P, P, P, P, c_int, c_int, c_int, c_int, P, P, c_int64, P, c_int64, c_int64, P, c_int64,

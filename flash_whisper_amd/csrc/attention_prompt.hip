@@ -458,6 +458,49 @@ __global__ void __launch_bounds__(QG * KP * 64, 2) prompt_attention_kernel(Promp
 
 constexpr int kCus = 256;
 
+// How a call shares out its rows, FW_PROMPT_*.
+// Blocks of 128 rows stage every tile for four waves and are the fastest where they fill the CUs. Few rows over many
+// keys are given to several waves, whose parts of the keys are merged: 8 parts while blocks of 32 rows have a CU
+// each, 2 parts of 64 keys while blocks of 64 rows are at most two a CU (causal ones of heads of 64, which end at
+// different times and of which a CU holds two, four); then, and where the keys are few, 2 parts of
+// 32 keys, up to 1.5 blocks of 128 rows a CU (2 where the keys are few and a block is over soon). Where the keys are a
+// tile a sequence, a wave works alone and many blocks share a CU. Keys a sequence are the average, since only the device
+// has the lengths: one long prompt among many of a token runs in single waves (63 x 1 token and 1900 x 20 heads of 64
+// 48 us, the 1900 alone 22.5; 255 x 1 and 4096 122 and 67), where 2000 prompts of 8 tokens are three times as fast.
+// us of 128 rows / 64 rows, 2 parts of 32 keys / of 64 keys / 32 rows, 8 parts:
+//   heads of 64, 1 x 4 queries x 20 heads over 1500 keys 20.7 / 18.5 / 14.1 / 11.3; 6 x 4 likewise 21.7 / 19.5 / 15.3 /
+//   13.5; 1 x 500 x 20, causal 11.1 / 9.4 / 8.3 / 10.9; 1 x 2000 x 20 30.9 / 26.9 / 22.6 / 38.5; 2 x 1500 x 20 31.2 / 29.3 /
+//   27.3 / 49.7; 3 x 1500 x 20 41.1 /
+//   39.8 / 40.2 / 72.5; 1 x 8192 x 20 204 / 257 / 234 / 386; 16 x 4 .. 224 x 20 9.4 / 8.3 / 11.5 / 20; over 1500
+//   keys 35.9 / 39.4 / 46.5 / 57;
+//   heads of 128 over 8 key/value heads, 4 x 32 x 32 over 4000 keys 86 / 72 / 57 / 33; 8 x 64 x 32 likewise 114 / 102 / 82 /
+//   88; 1 x 1000 x 32, causal 27.1 / 23.9 / 26.2 / 47.4; 1 x 4096 x 32 157 / 183 / 224 / 314.
+// Heads of 64, 128 rows / the single wave: 1 x 4 x 20 4.4 / 4.0; 2000 x 8 x 20 246 / 84; 64 x 64 x 20 14.9 / 13.9; 64 x 1
+// .. 200 x 8 over 2 heads 7.0 / 8.5.
+// (8 parts with a second stage where the LDS holds it: 1 x 4 queries x 20 heads over 1500 keys 11.3 us against 12.1, 5 x 8
+// x 20 over 2705 16.5 against 17.7.)
+int prompt_form(int n_seq, int64_t rows, int64_t k_rows, int kv_heads, int dim, bool causal) {
+  const int64_t keys = k_rows / n_seq;
+  const auto blocks_of = [&](int64_t n) { return (rows / n + n_seq) * kv_heads; };
+  if (blocks_of(32) <= kCus && keys >= 512) return FW_PROMPT_8_PARTS;
+  if (keys <= 32) return FW_PROMPT_WAVES;
+  if (blocks_of(64) <= (causal && dim == 64 ? 4 : 2) * kCus && keys >= 384) return FW_PROMPT_2_PARTS;
+  if (blocks_of(128) <= (keys < 256 ? 2 * kCus : kCus * 3 / 2)) return FW_PROMPT_2_SHORT_PARTS;
+  return FW_PROMPT_128_ROWS;
+}
+
+// What a call asks of its sizes; FW_OK or FW_EINVAL.
+int check_sizes(int n_seq, int64_t q_rows, int64_t k_rows, int heads, int kv_heads, int head_dim) {
+  if (n_seq <= 0 || q_rows < 0 || k_rows < 0)
+    return fw_fail(FW_EINVAL, "prompt_attention: n_seq must be positive, rows not negative");
+  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads)
+    return fw_fail(FW_EINVAL, "prompt_attention: heads must be a multiple of kv_heads");
+  if (head_dim != 64 && head_dim != 128) return fw_fail(FW_EINVAL, "prompt_attention: head_dim must be 64 or 128");
+  // rows x heads of a sequence are counted in 32 bits
+  if (q_rows > 0x7FFFFF00 / (heads / kv_heads) || k_rows > 0x7FFFFF00) return fw_fail(FW_EINVAL, "prompt_attention: too many rows");
+  return FW_OK;
+}
+
 bool rows_ok(const void* p, int64_t row, int64_t head) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && row % 8 == 0 && head % 8 == 0;
 }
@@ -467,16 +510,18 @@ bool rows_ok(const void* p, int64_t row, int64_t head) {
 
 using namespace fw;
 
+extern "C" int fw_prompt_attention_form(int n_seq, int64_t q_rows, int64_t k_rows, int heads, int kv_heads, int head_dim,
+                                        int causal) {
+  if (const int rc = check_sizes(n_seq, q_rows, k_rows, heads, kv_heads, head_dim)) return rc;
+  return prompt_form(n_seq, q_rows * (heads / kv_heads), k_rows, kv_heads, head_dim, causal);
+}
+
 extern "C" int fw_prompt_attention(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                                    const void* v, int64_t v_row, int64_t v_head, void* out, int64_t o_row, int64_t o_head,
                                    const int64_t* cu_q, const int64_t* cu_k, int n_seq, int64_t q_rows, int64_t k_rows,
                                    int heads, int kv_heads, int head_dim, int dtype, float scale, int causal,
                                    hipStream_t stream) {
-  if (n_seq <= 0 || q_rows < 0 || k_rows < 0)
-    return fw_fail(FW_EINVAL, "prompt_attention: n_seq must be positive, rows not negative");
-  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads)
-    return fw_fail(FW_EINVAL, "prompt_attention: heads must be a multiple of kv_heads");
-  if (head_dim != 64 && head_dim != 128) return fw_fail(FW_EINVAL, "prompt_attention: head_dim must be 64 or 128");
+  if (const int rc = check_sizes(n_seq, q_rows, k_rows, heads, kv_heads, head_dim)) return rc;
   if (dtype != FW_F16 && dtype != FW_BF16) return fw_fail(FW_EINVAL, "prompt_attention: dtype must be FW_F16 or FW_BF16");
   if (!cu_q || !cu_k || (q_rows > 0 && (!q || !out)) || (k_rows > 0 && (!k || !v)))
     return fw_fail(FW_EINVAL, "prompt_attention: null pointer");
@@ -485,14 +530,14 @@ extern "C" int fw_prompt_attention(const void* q, int64_t q_row, int64_t q_head,
     return fw_fail(FW_EINVAL, "prompt_attention: q, k, v and out must be 16-byte aligned with strides in multiples of 8");
   if (!(__builtin_fabsf(scale) * kLog2e < INFINITY))
     return fw_fail(FW_EINVAL, "prompt_attention: scale must be finite (and below 2.3e38 in size)");
-  // 64 rows of k and of v within the copies' 32-bit byte offsets; rows x heads of a sequence are counted in 32 bits
+  // 64 rows of k and of v within the copies' 32-bit byte offsets
   if (k_row < 0 || v_row < 0 || k_row >= (1 << 25) || v_row >= (1 << 25))
     return fw_fail(FW_EINVAL, "prompt_attention: row strides of k and v must be below 2^25 elements");
-  if (q_rows > 0x7FFFFF00 / (heads / kv_heads) || k_rows > 0x7FFFFF00) return fw_fail(FW_EINVAL, "prompt_attention: too many rows");
   if (q_rows == 0) return FW_OK;
   const PromptArgs a{q, k, v, out, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, cu_q, cu_k,
                      q_rows, k_rows, n_seq, heads, kv_heads, scale};
   const int64_t rows = q_rows * (heads / kv_heads);
+  const int form = prompt_form(n_seq, rows, k_rows, kv_heads, head_dim, causal);
   int rc = FW_OK;
   const auto launch = [&](auto kernel, int per_block, int threads) {
     const int64_t blocks = (rows / per_block + n_seq) * kv_heads;  // a sequence's last block may be partial
@@ -503,31 +548,13 @@ extern "C" int fw_prompt_attention(const void* q, int64_t q_row, int64_t q_head,
     typedef decltype(t) T;
     constexpr int D = decltype(d)::value;
     constexpr bool M = decltype(mask)::value;
-    // Blocks of 128 rows stage every tile for four waves and are the fastest where they fill the CUs. Few rows over many
-    // keys are given to several waves, whose parts of the keys are merged: 8 parts while blocks of 32 rows have a CU
-    // each, 2 parts of 64 keys while blocks of 64 rows are at most two a CU (causal ones of heads of 64, which end at
-    // different times and of which a CU holds two, four); then, and where the keys are few, 2 parts of
-    // 32 keys, up to 1.5 blocks of 128 rows a CU (2 where the keys are few and a block is over soon). Where a sequence is one
-    // tile, a wave works alone and many blocks share a CU. us of 128 rows / 64 rows, 2 parts of 32 keys / of 64 keys / 32
-    // rows, 8 parts:
-    //   heads of 64, 1 x 4 queries x 20 heads over 1500 keys 20.7 / 18.5 / 14.1 / 11.3; 6 x 4 likewise 21.7 / 19.5 / 15.3 /
-    //   13.5; 1 x 500 x 20, causal 11.1 / 9.4 / 8.3 / 10.9; 1 x 2000 x 20 30.9 / 26.9 / 22.6 / 38.5; 2 x 1500 x 20 31.2 / 29.3 /
-    //   27.3 / 49.7; 3 x 1500 x 20 41.1 /
-    //   39.8 / 40.2 / 72.5; 1 x 8192 x 20 204 / 257 / 234 / 386; 16 x 4 .. 224 x 20 9.4 / 8.3 / 11.5 / 20; over 1500
-    //   keys 35.9 / 39.4 / 46.5 / 57;
-    //   heads of 128 over 8 key/value heads, 4 x 32 x 32 over 4000 keys 86 / 72 / 57 / 33; 8 x 64 x 32 likewise 114 / 102 / 82 /
-    //   88; 1 x 1000 x 32, causal 27.1 / 23.9 / 26.2 / 47.4; 1 x 4096 x 32 157 / 183 / 224 / 314.
-    // Heads of 64, 128 rows / the single wave: 1 x 4 x 20 4.4 / 4.0; 2000 x 8 x 20 246 / 84; 64 x 64 x 20 14.9 / 13.9; 64 x 1
-    // .. 200 x 8 over 2 heads 7.0 / 8.5.
-    const int64_t keys = k_rows / n_seq;
-    const auto blocks_of = [&](int64_t n) { return (rows / n + n_seq) * kv_heads; };
-    // (8 parts with a second stage where the LDS holds it: 1 x 4 queries x 20 heads over 1500 keys 11.3 us against 12.1, 5 x 8
-    // x 20 over 2705 16.5 against 17.7.)
-    if (blocks_of(32) <= kCus && keys >= 512) launch(prompt_attention_kernel<T, D, 1, 8, 32, D == 64 ? 2 : 1, M>, 32, 512);
-    else if (keys <= 32) launch(prompt_attention_kernel<T, D, 1, 1, 32, 1, M>, 32, 64);
-    else if (blocks_of(64) <= (M && D == 64 ? 4 : 2) * kCus && keys >= 384) launch(prompt_attention_kernel<T, D, 2, 2, 64, 2, M>, 64, 256);
-    else if (blocks_of(128) <= (keys < 256 ? 2 * kCus : kCus * 3 / 2)) launch(prompt_attention_kernel<T, D, 2, 2, 32, 2, M>, 64, 256);
-    else launch(prompt_attention_kernel<T, D, 4, 1, 64, 2, M>, 128, 256);
+    switch (form) {
+      case FW_PROMPT_8_PARTS: launch(prompt_attention_kernel<T, D, 1, 8, 32, D == 64 ? 2 : 1, M>, 32, 512); break;
+      case FW_PROMPT_WAVES: launch(prompt_attention_kernel<T, D, 1, 1, 32, 1, M>, 32, 64); break;
+      case FW_PROMPT_2_PARTS: launch(prompt_attention_kernel<T, D, 2, 2, 64, 2, M>, 64, 256); break;
+      case FW_PROMPT_2_SHORT_PARTS: launch(prompt_attention_kernel<T, D, 2, 2, 32, 2, M>, 64, 256); break;
+      default: launch(prompt_attention_kernel<T, D, 4, 1, 64, 2, M>, 128, 256);
+    }
   };
   const auto by_mask = [&](auto t, auto d) { causal ? by_rows(t, d, std::true_type()) : by_rows(t, d, std::false_type()); };
   const std::integral_constant<int, 64> d64;

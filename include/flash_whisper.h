@@ -442,6 +442,15 @@ int fw_prompt_attention(const void* q, int64_t q_row, int64_t q_head, const void
                         const int64_t* cu_q, const int64_t* cu_k, int n_seq, int64_t q_rows, int64_t k_rows, int heads,
                         int kv_heads, int head_dim, int dtype, float scale, int causal, hipStream_t stream);
 
+/* How such a call shares out its work, by its sizes alone: blocks of 128 rows; of 64 rows with the keys in 2 parts, 64 or 32 at a
+ * time; of 32 rows with the keys in 8 parts; single waves of 32 rows. FW_EINVAL for sizes that it refuses. */
+#define FW_PROMPT_128_ROWS 0
+#define FW_PROMPT_2_PARTS 1
+#define FW_PROMPT_2_SHORT_PARTS 2
+#define FW_PROMPT_8_PARTS 3
+#define FW_PROMPT_WAVES 4
+int fw_prompt_attention_form(int n_seq, int64_t q_rows, int64_t k_rows, int heads, int kv_heads, int head_dim, int causal);
+
 /* The 4-bit cache of n_seq sequences, kv_heads heads and max_len rows (a multiple of 32, at most 2^30) of head_dim (64
  * or 128) elements: 5 bits a value. 32 elements of a row share a step and a low value (fp16), and a code c of 0 .. 15 stands
  * for fp16(low + step c). All four arrays are dense and 16-byte aligned:

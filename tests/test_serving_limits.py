@@ -95,3 +95,17 @@ def test_build_without_the_binding(monkeypatch, tmp_path, capsys, missing):
         monkeypatch.setenv('CXX', str(tmp_path / 'none') if missing == 'compiler' else 'false')
     assert build._compile_bind(False) is False
     assert not list(tmp_path.iterdir()) and 'ctypes' in capsys.readouterr().err
+
+
+def test_prompt_forms(built_lib):
+    """What the library says of sizes on either side of its rule, and of sizes that it refuses."""
+    from flash_whisper_amd import _lib
+
+    form = built_lib.fw_prompt_attention_form
+    assert form(1, 4, 4, 20, 20, 64, 1) == _lib.PROMPT_WAVES and form(64, 64 * 32, 64 * 32, 20, 20, 64, 1) == _lib.PROMPT_WAVES
+    assert form(64, 64 * 33, 64 * 33, 20, 20, 64, 1) == _lib.PROMPT_128_ROWS and form(4, 4 * 33, 4 * 33, 20, 20, 64, 1) == _lib.PROMPT_2_SHORT_PARTS
+    assert form(1, 4, 1500, 20, 20, 64, 0) == _lib.PROMPT_8_PARTS and form(1, 4, 511, 20, 20, 64, 0) == _lib.PROMPT_2_PARTS
+    assert form(1, 2000, 2000, 20, 20, 64, 1) == _lib.PROMPT_2_PARTS and form(1, 2000, 2000, 20, 20, 64, 0) == _lib.PROMPT_2_SHORT_PARTS
+    assert form(1, 8192, 8192, 32, 8, 128, 1) == _lib.PROMPT_128_ROWS
+    for bad in ((0, 4, 4, 20, 20, 64), (1, -1, 4, 20, 20, 64), (1, 4, 4, 20, 8, 64), (1, 4, 4, 20, 20, 80), (1, 1 << 31, 4, 20, 20, 64)):
+        assert form(*bad, 1) == _lib.FW_EINVAL

@@ -314,13 +314,9 @@ __global__ void __launch_bounds__(QG * KP * 64, 2) prompt_attention_kernel(Promp
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) q[j] = -q[j];
   }
-  // A scale of zero makes the queries zero instead (a bf16 score may be as large as any factor is small), so that the
-  // factor is never one: a masked score (-infinity) times zero is NaN.
-  if (a.scale == 0.f) {
-#pragma unroll
-    for (int j = 0; j < D / 16; ++j) q[j] *= static_cast<T>(0.f);
-  }
-  const float factor = fmaxf(__builtin_fabsf(a.scale) * kLog2e, __FLT_MIN__);
+  // 0: the smallest number instead, against which the largest bf16 score, below 2^128, vanishes too; a masked score
+  // (-infinity) times zero would be NaN. fp32 keeps subnormal numbers here.
+  const float factor = fmaxf(__builtin_fabsf(a.scale) * kLog2e, __FLT_DENORM_MIN__);
 
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ring));
   const T* kbase = static_cast<const T*>(a.k) + job.k0 * a.k_row + kvh * a.k_head;

@@ -181,3 +181,65 @@ def test_decode_many_items_in_long_caches(ext, hip_device, kind, dim, n, heads, 
             ks, vs = (h[a:a + x].double().cpu().numpy() for h in (held_k, held_v))
             o, spread, size = serving.attend(q64[s][None], ks, vs, dim ** -0.5, False)
             check_attention(got[s][None], o, spread, size, np.abs(vs).max(initial=0), x, dtype)
+
+
+@pytest.mark.parametrize('causal', [True, False])
+def test_rows_before_the_first_sequence(ext, hip_device, causal):
+    """Starts need not begin at the first row: rows before it are neither read into a sequence nor written, by any of the ops."""
+    dev, rng, at = hip_device, np.random.default_rng(8), [37, 40, 40, 140]
+    q, q64 = rounded(rng, (150, 4, 64), torch.float16)
+    k, k64 = rounded(rng, (150, 2, 64), torch.float16)
+    v, v64 = rounded(rng, (150, 2, 64), torch.float16)
+    k[:37], v[:37], k[140:], v[140:] = float('nan'), float('inf'), float('inf'), float('nan')
+    cu, k, v, out = _index(at, dev), k.to(dev), v.to(dev), torch.full((150, 4, 64), 5.0, dtype=torch.float16, device=dev)
+    ext.prompt_attention(q.to(dev), k, v, out, cu, cu, 0.125, causal)
+    got = out.double().cpu().numpy()
+    assert (got[:37] == 5.0).all() and (got[140:] == 5.0).all()
+    check_prompts(got[37:140], q64[37:], k64[37:], v64[37:], [3, 0, 100], [3, 0, 100], 0.125, causal, torch.float16)
+    cache, want = ext.kv_q4_cache(3, 2, 128, 64), ext.kv_q4_cache(3, 2, 128, 64)
+    pos = _index([125, 0, 9], dev)
+    ext.kv_q4_append(k, v, cu, pos, cache)
+    ext.kv_q4_append(k[37:140], v[37:140], cu - 37, pos, want)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(cache, want))
+    back = [torch.full_like(k, 5.0) for _ in range(2)]
+    ext.kv_q4_read(cache, cu, pos, *back)
+    held = [torch.zeros_like(k[37:140]) for _ in range(2)]
+    ext.kv_q4_read(want, cu - 37, pos, *held)
+    for b, h in zip(back, held):
+        assert torch.equal(b[37:140], h) and (b[:37] == 5.0).all() and (b[140:] == 5.0).all()
+
+
+def test_calls_of_two_threads(ext, hip_device):
+    """Two threads that call the ops at once, a stream and a workspace each: the bits of calls one after another."""
+    import threading
+
+    dev, sets = hip_device, []
+    for seed in range(2):
+        rng = np.random.default_rng(seed)
+        q, k, v = (rounded(rng, (200, h, 64), torch.float16)[0].to(dev) for h in (4, 2, 2))
+        cache = ext.kv_q4_cache(3, 2, 4128, 64)
+        sets.append((q, k, v, cache, ext.decode_attention_q4_workspace(3, 4, cache), starts([100, 0, 100 - seed], dev), _index([4000, 0, 7], dev)))
+    torch.cuda.synchronize()
+
+    def run(s, turns):
+        q, k, v, cache, ws, cu, pos = s
+        out, one = torch.zeros_like(q), torch.zeros(3, 4, 64, dtype=torch.float16, device=dev)
+        for _ in range(turns):
+            ext.prompt_attention(q, k, v, out, cu, cu, 0.125)
+            ext.kv_q4_append(k, v, cu, pos, cache)
+            ext.decode_attention_q4(q[:3], cache, pos + 50, one, ws, 0.125)
+        torch.cuda.current_stream().synchronize()
+        return out, one
+
+    want, got = [run(s, 1) for s in sets], [None, None]
+
+    def thread(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got[i] = run(sets[i], 20)
+
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(a, b) for w, g in zip(want, got) for a, b in zip(w, g))

@@ -232,7 +232,10 @@ __global__ void __launch_bounds__(256) kv_q4_read_kernel(const int64_t* __restri
 //  - Codes become fp16 by or-ing them into 1024's mantissa (1024 + c), subtracting 1024, and one packed fma with
 //    step and low, which rounds once as the cache's definition does. Q's dims are permuted to the order in
 //    which masking a dword's nibbles yields pairs (0 4, 1 5, 2 6, 3 7).
-//  - The running maximum only moves when a score passes it by 2^kSlack (log2 units); weights stay within fp16.
+//  - The running maximum only moves when a score passes it by kSlack (log2 units), so weights are at most 2^8. They are
+//    rounded to fp16 for bf16 callers too: the values are fp16, one matrix instruction takes both, and 2^-11 of a weight is
+//    an eighth of what a bf16 output is rounded by (64 ragged sequences x 32 heads of 128, bf16: 1.656e-3 rms off the values in 64
+//    bits, rounding those to bf16 1.655e-3). Their sum, in fp32, is over the rounded ones, as the products are.
 // Bound by memory where the lengths are alike (64 x 8000 keys x 8 heads of 128, 32 query heads: 131 us, 5.0 TB/s with
 // what the last-level cache gives; one of 131000: 43 us, 3.9 TB/s), by the longest block and the two launches' latency
 // where they are not (64 of 1 to 8000: 28.6 us, 3.0 TB/s), and by latency where there is little to read (300 keys x 20
@@ -501,7 +504,7 @@ __device__ __forceinline__ void q4_values(const Q4Tile<D>& t, f4v (&s)[2], float
 
 // The item's queries as the products' operand, lane (h, g): dims D / 4 g + 8 j .. in the order of q4_pair's
 // pairs, and the factor from raw scores to log2 units. A bf16 query is scaled by a power of two to fit fp16 (its
-// elements 2^-24 of the largest and less lose bits); the factor undoes it. A negative scale negates the query,
+// 8 bits do down to 2^-17 of the largest element; what is lost below is at most 2^-25 of it); the factor undoes it. A negative scale negates the query,
 // a zero one becomes so small that scores vanish. The factor of the scaled query is kept a positive number: against one of
 // zero a masked score (-infinity), against an infinite one a score of zero would be NaN. (Raised to 1e-30, scores, of at most
 // 2^39, vanish all the same; lowered to the largest number, every score but zero is past 2^79, which fp32 does not resolve.)

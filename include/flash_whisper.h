@@ -434,9 +434,10 @@ int fw_cross_kv(const void* enc, int t, const void* w, const void* bias, void* c
  * out[i] <- sum_j softmax_j(scale q[i] . k[j]) v[j] over the keys j of i's sequence; causal: the last query sees every
  * key, each one before it a key less (j <= i + n_keys - n_queries, both counted within the sequence). A query that
  * sees no key gets zeros. What a query does not see does not reach its output, whatever it holds (infinities and NaN
- * too). Rows of out behind the last sequence are left as they are. Scores, softmax and sums are fp32; the weights
- * are rounded to the type for the product with v. out overlaps no input; scale is finite, here (and below 2.3e38 in size) and below;
- * where a score passes 2^27 in size (scale q . k log2(e)), which fp32 resolves to 16, the result is not defined. */
+ * too). Rows of out before the first and behind the last sequence are left as they are. Scores, softmax and sums are fp32;
+ * the weights are rounded to the type for their sum and the product with v (fp16 ones below 2^-25 of the largest are lost), and
+ * the division comes last, so |v| x keys has to stay below 2^116 (bf16). out overlaps no input. scale is finite and below
+ * 2.3e38 in size. Where scale q . k log2(e) passes 2^27 in size, which fp32 resolves to 16, the result is not defined. */
 int fw_prompt_attention(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                         const void* v, int64_t v_row, int64_t v_head, void* out, int64_t o_row, int64_t o_head,
                         const int64_t* cu_q, const int64_t* cu_k, int n_seq, int64_t q_rows, int64_t k_rows, int heads,
@@ -480,7 +481,10 @@ int fw_kv_q4_read(const void* k_codes, const void* k_meta, const void* v_codes, 
  * most max_len). With them ([n_seq, kv_heads, head_dim]; both or neither) their row is written to cache row lens[s]
  * first, as fw_kv_q4_append would, and lens[s] + 1 rows are attended to; at lens[s] >= max_len the last row is
  * overwritten. A sequence without rows, and an idle one (lens[s] < 0: nothing is written to its cache), gets zeros.
- * lens is not advanced. ws: fw_decode_attention_q4_ws_floats floats, 16-byte aligned, uninitialised; calls that may
+ * lens is not advanced. Scores, softmax and sums are fp32, with scale and scores within the limits of fw_prompt_attention (any
+ * finite scale). Weights are rounded to fp16 for their sum and the product with the values, of which those below 2^-25 of
+ * the largest are lost; a head's bf16 query is taken in fp16 at its own power of two: elements below 2^-17 of the head's largest
+ * lose bits, below 2^-25 all. ws: fw_decode_attention_q4_ws_floats floats, 16-byte aligned, uninitialised; calls that may
  * overlap need one each. */
 int fw_decode_attention_q4(const void* q, int64_t q_row, int64_t q_head, void* k_codes, void* k_meta, void* v_codes,
                            void* v_meta, const int64_t* lens, void* out, int64_t o_row, int64_t o_head,

@@ -6,9 +6,9 @@ parallel, one object per source) and links them. The library exports the entry p
 same objects with the decoder step compiled with FW_STEP_TIMELINE=1, which records the phase timeline
 that ``python -m flash_whisper_amd.step_timeline`` reads (selected with FW_LIBRARY; never the default), and
 the Python module ``_bind.so`` (csrc/bind.cpp, with g++ or $CXX), through which ext.py calls the ops whose kernels take
-less time than a ctypes call; where that cannot be compiled the build says so and goes on. This replaces the reference's JIT extension build (custom/ext.py:13-18),
-which ran nvcc through torch.utils.cpp_extension; here the build is ahead-of-time and in-tree so the
-built library travels with the source tree.
+less time than a ctypes call; where that cannot be compiled the build says so and goes on. This replaces the
+reference's JIT extension build (custom/ext.py:13-18), which ran nvcc through torch.utils.cpp_extension; here the build
+is ahead-of-time and in-tree so the built library travels with the source tree.
 """
 
 import argparse

@@ -464,8 +464,8 @@ constexpr int kCus = 256;
 // each, 2 parts of 64 keys while blocks of 64 rows are at most two a CU (causal ones of heads of 64, which end at
 // different times and of which a CU holds two, four); then, and where the keys are few, 2 parts of
 // 32 keys, up to 1.5 blocks of 128 rows a CU (2 where the keys are few and a block is over soon). Where the keys are a
-// tile a sequence, a wave works alone and many blocks share a CU. Keys a sequence are the average, since only the device
-// has the lengths: one long prompt among many of a token runs in single waves (63 x 1 token and 1900 x 20 heads of 64
+// tile a sequence, a wave works alone and many blocks share a CU. Keys a sequence are the average of all rows there are,
+// behind the last sequence too, since only the device has the lengths: one long prompt among many of a token runs in single waves (63 x 1 token and 1900 x 20 heads of 64
 // 48 us, the 1900 alone 22.5; 255 x 1 and 4096 122 and 67), where 2000 prompts of 8 tokens are three times as fast.
 // us of 128 rows / 64 rows, 2 parts of 32 keys / of 64 keys / 32 rows, 8 parts:
 //   heads of 64, 1 x 4 queries x 20 heads over 1500 keys 20.7 / 18.5 / 14.1 / 11.3; 6 x 4 likewise 21.7 / 19.5 / 15.3 /

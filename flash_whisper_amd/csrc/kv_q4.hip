@@ -504,8 +504,8 @@ __device__ __forceinline__ void q4_values(const Q4Tile<D>& t, f4v (&s)[2], float
 
 // The item's queries as the products' operand, lane (h, g): dims D / 4 g + 8 j .. in the order of q4_pair's
 // pairs, and the factor from raw scores to log2 units. A bf16 query is scaled by a power of two to fit fp16 (its
-// 8 bits do down to 2^-17 of the largest element; what is lost below is at most 2^-25 of it); the factor undoes it. A negative scale negates the query,
-// a zero one becomes so small that scores vanish. The factor of the scaled query is kept a positive number: against one of
+// 8 bits do down to 2^-17 of the largest element; what is lost below is at most 2^-25 of it); the factor undoes it. A
+// negative scale negates the query, a zero one becomes so small that scores vanish. The factor of the scaled query is kept a positive number: against one of
 // zero a masked score (-infinity), against an infinite one a score of zero would be NaN. (Raised to 1e-30, scores, of at most
 // 2^39, vanish all the same; lowered to the largest number, every score but zero is past 2^79, which fp32 does not resolve.)
 template <class T, int D>
@@ -879,8 +879,8 @@ __global__ void __launch_bounds__(kCombine) q4_combine_kernel(const int64_t* len
 // this makes it kLoose times as long as the bound for many items, up to kLookThrough sequences get chunks by their lengths (64
 // ragged sequences x 8 heads of 128 in caches of 16384 / 32768 / 49152 / 131072 rows, 1.3 / 2.7 / 4 / 11 times the bound: 25.5 /
 // 32.0 / 31.2 / 53.2 us, by length 26.3 / 26.9 / 26.5 / 26.8; all of 1000 keys 22.1 / 23.5 / 22.4 / 28.7 and 24.8 / 25.9 / 25.1 /
-// 26.6; 250 x 4 heads, one of 8000 keys, 2.6 / 5.2 / 10 times: 25.0 / 29.6 / 49.7, by length 28.5 / 28.7 / 28.7). Blocks have 8 waves where items
-// are few and 4 where they fill the CUs anyway (those 64 ragged sequences: 33.5 us against 39.5; 64 x 20 heads of 64 over
+// 26.6; 250 x 4 heads, one of 8000 keys, 2.6 / 5.2 / 10 times: 25.0 / 29.6 / 49.7, by length 28.5 / 28.7 / 28.7). Blocks
+// have 8 waves where items are few and 4 where they fill the CUs anyway (those 64 ragged sequences: 33.5 us against 39.5; 64 x 20 heads of 64 over
 // 700 keys 15.0 against 17.2, but 16 x 20 over 1500 keys as two chunks of 4 waves 16.3 against 13.6), or where the merge of
 // 16 heads of 128 would pass 64 KB of LDS.
 struct Q4Plan {

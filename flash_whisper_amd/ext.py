@@ -103,10 +103,12 @@ def _current_device():
 
 def _heads_view(t, name, dtype, dev, heads, dim):
     """Checks a [rows, heads, dim] CUDA view of `dtype` with unit element stride and strides in multiples of 8 (heads
-    None: any count); returns its row and head strides (0 where there is one row or head)."""
+    None: any count); returns its row and head strides (0 where there is one row or head, or none: then they mean nothing)."""
     if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.dim() == 3 and t.get_device() == dev):
         (rows, h, d), (sr, sh, sd) = t.shape, t.stride()
-        if d == dim and sd == 1 and (heads is None or h == heads):
+        if d == dim and (sd == 1 or rows == 0) and (heads is None or h == heads):
+            if rows == 0:
+                return 0, 0
             sr, sh = sr if rows > 1 else 0, sh if h > 1 else 0
             if (sr | sh) & 7 == 0 and t.data_ptr() & 15 == 0:
                 return sr, sh
@@ -118,6 +120,8 @@ def _out_view(t, name, dtype, dev, heads, dim):
     """_heads_view of a tensor that is written: its rows must not overlap each other."""
     sr, sh = _heads_view(t, name, dtype, dev, heads, dim)
     rows, h, _ = t.shape
+    if rows == 0:
+        return sr, sh
     if rows > 1 and h > 1:
         apart = min(sr, sh) >= dim and (sr >= (h - 1) * sh + dim or sh >= (rows - 1) * sr + dim)
     else:

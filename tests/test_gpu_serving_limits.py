@@ -243,3 +243,17 @@ def test_calls_of_two_threads(ext, hip_device):
     for t in threads:
         t.join()
     assert all(torch.equal(a, b) for w, g in zip(want, got) for a, b in zip(w, g))
+
+
+def test_tensors_without_rows(ext, hip_device):
+    """Empty tensors of any strides: an append, a read and queries of no rows do nothing, keys of no rows give zeros."""
+    dev = hip_device
+    none = torch.empty(0, dtype=torch.float16, device=dev).as_strided((0, 2, 64), (1, 3, 2))
+    cache, cu, pos = ext.kv_q4_cache(2, 2, 32, 64), _index([0, 0, 0], dev), _index([3, 0], dev)
+    q, out = torch.ones(2, 2, 64, dtype=torch.float16, device=dev), torch.full((2, 2, 64), 5.0, dtype=torch.float16, device=dev)
+    ext.kv_q4_append(none, none, cu, pos, cache)
+    ext.kv_q4_read(cache, cu, pos, none, none)
+    ext.prompt_attention(none, q, q, none, cu, _index([0, 1, 2], dev), 0.125)
+    assert not any(t.any() for t in cache)
+    ext.prompt_attention(q, none, none, out, _index([0, 1, 2], dev), cu, 0.125)
+    assert not out.any()

@@ -109,3 +109,17 @@ def test_prompt_forms(built_lib):
     assert form(1, 8192, 8192, 32, 8, 128, 1) == _lib.PROMPT_128_ROWS
     for bad in ((0, 4, 4, 20, 20, 64), (1, -1, 4, 20, 20, 64), (1, 4, 4, 20, 8, 64), (1, 4, 4, 20, 20, 80), (1, 1 << 31, 4, 20, 20, 64)):
         assert form(*bad, 1) == _lib.FW_EINVAL
+
+
+def test_views_without_rows():
+    """The strides of a tensor without rows mean nothing; its heads, head size and type are still asked for."""
+    from flash_whisper_amd import ext
+
+    none, f16 = torch.empty(0).half().as_strided((0, 2, 64), (1, 3, 2)), torch.float16
+    for view in (ext._heads_view, ext._out_view):
+        assert view(none, 'k', f16, -1, 2, 64) == (0, 0) and view(none, 'k', f16, -1, None, 64) == (0, 0)
+        for args in ((f16, -1, 3, 64), (f16, -1, 2, 128), (torch.bfloat16, -1, 2, 64), (f16, 0, 2, 64)):
+            with pytest.raises(RuntimeError):
+                view(none, 'k', *args)
+        with pytest.raises(RuntimeError):
+            view(torch.zeros(400, dtype=f16).as_strided((1, 2, 64), (1, 3, 2)), 'k', f16, -1, 2, 64)

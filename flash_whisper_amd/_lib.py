@@ -17,7 +17,7 @@ LIB_PATH = Path(os.environ.get('FW_LIBRARY') or Path(__file__).resolve().parent 
 FW_OK, FW_EINVAL, FW_EHIP = 0, -1, -2
 NOALLOC_ATTN_SLOTS = 2048  # FW_NOALLOC_ATTN_SLOTS
 ACT_NONE, ACT_GELU = 0, 1
-F16, BF16 = 0, 1  # FW_F16, FW_BF16
+F16, BF16, F32 = 0, 1, 2  # FW_F16, FW_BF16, FW_F32
 PROMPT_128_ROWS, PROMPT_2_PARTS, PROMPT_2_SHORT_PARTS, PROMPT_8_PARTS, PROMPT_WAVES = range(5)  # FW_PROMPT_*
 EPI_BIAS, EPI_BIAS_GELU, EPI_BIAS_RESID, EPI_BIAS_RESID_CLAMP, EPI_BIAS_GELU_POS, EPI_SCALE_Q = range(6)
 
@@ -72,6 +72,13 @@ SIGNATURES = {
                                        c_int64, c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_float, P, c_int64,
                                        P]),
     'fw_decode_attention_q4_ws_floats': (c_int64, [c_int, c_int, c_int, c_int, c_int]),
+    'fw_kv_page_map': (c_int, [P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int64, c_int64, c_int, P]),
+    'fw_kv_page_append': (c_int, [P, c_int64, c_int64, P, c_int64, c_int64, P, c_int64, P, P, c_int, c_int, c_int, c_int, P]),
+    'fw_decode_attention_paged': (c_int, [P, c_int64, c_int64, P, P, P, P, P, P, P, c_int64, c_int64, c_int, c_int, c_int,
+                                          c_int, c_int, c_int, c_int, c_int, c_int, c_float, P, c_int64, P]),
+    'fw_decode_attention_paged_ws_floats': (c_int64, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    'fw_logits_rules': (c_int, [P, c_int64, P, c_int64, c_int, c_int, c_int, P, c_int64, P, P, P, P, P, P, P, c_int64, P, P,
+                                c_int64, c_int, P, P]),
     'fw_synth_normal_f16': (c_int, [P, c_int64, c_int64, c_uint64, c_uint64, c_float, c_float, P]),
     'fw_synth_normal_f16_host': (c_int, [P, c_int64, c_int64, c_uint64, c_uint64, c_float, c_float]),
     'fw_decoder_step_workspace_bytes': (ctypes.c_size_t, [c_int]),

@@ -44,6 +44,7 @@ PER_FILE_FLAGS = {
     'attention_enc.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form', *PRELOAD],
     'attention_prompt.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form', *PRELOAD],
     'decode.hip': PRELOAD,
+    'attention_paged.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form', *PRELOAD],
     'kv_q4.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form', *PRELOAD],
     'encoder.hip': PRELOAD,
     'logmel.hip': PRELOAD,

@@ -1,0 +1,680 @@
+// Single-token attention over a key/value cache in pages (pages.h) for gfx950, the rows that a group of sequences shares
+// read once for all of it. Built with MFMA results in VGPRs, as the other attentions.
+#include <algorithm>
+#include <type_traits>
+
+#include "packed_rows.h"
+#include "pages.h"
+
+namespace fw {
+namespace {
+
+typedef __bf16 b8v __attribute__((ext_vector_type(8)));
+typedef __bf16 b2v __attribute__((ext_vector_type(2)));
+
+template <class T>
+struct Types;
+template <>
+struct Types<_Float16> {
+  typedef h8v v8;
+  typedef h2v v2;
+};
+template <>
+struct Types<__bf16> {
+  typedef b8v v8;
+  typedef b2v v2;
+};
+
+__device__ __forceinline__ f4v mfma16(const h8v& a, const h8v& b, const f4v& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f4v mfma16(const b8v& a, const b8v& b, const f4v& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ float add_pair(h2v x, float s) {
+  return __builtin_amdgcn_fdot2(x, h2v{static_cast<_Float16>(1.f), static_cast<_Float16>(1.f)}, s, false);
+}
+__device__ __forceinline__ float add_pair(b2v x, float s) {
+  return __builtin_amdgcn_fdot2_f32_bf16(x, b2v{static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)}, s, false);
+}
+
+// ------------------------------------------------------------------------------------------
+// A piece of work is a run of keys of one sequence's table and the columns that see them: a column is a query head of a
+// sequence, and the `group` heads that share a key/value head, of the sequence alone or of all sequences of its group one after
+// another, are the columns of the products S^T = K Q^T and O^T = V^T P^T (16 keys or head dims by 16 columns). A wave takes
+// 32 keys at a time, straight from the pages into the operands' registers:
+//  - K: row i of the first 16 is key 8 (i / 4) + i % 4, of the second 4 more, so that lane group g = lane / 16 ends with the
+//    scores of keys 8 g .. 8 g + 7 for column lane % 16: what the P V products take from it, without crossing lanes.
+//  - V: a lane's 8 keys of a dim are 16 bytes of a page.
+//  - The running maximum only moves when a score passes it by kSlack (log2 units), so weights are at most 2^8; they are
+//    rounded to the type, which the matrix instructions take, and their sum, in fp32, is over the rounded ones.
+// ------------------------------------------------------------------------------------------
+struct PagedArgs {
+  const void *q, *k, *v;
+  void* out;
+  int64_t q_row, q_head, o_row, o_head;
+  const int32_t* table;
+  const int64_t *lens, *cu_g, *shared;
+  int n_seq, heads, kv_heads, groups, width, n_pages, page_shift;
+  float scale;
+  int cols;           // columns of a piece of a group's shared keys, at most
+  int want;           // pieces that all keys are to make, about
+  int most;           // pieces there may be; 0: each sequence is a piece, and nothing is shared
+  int* plan;          // Header, Pieces, Owners, Groups, the group of each sequence
+  float *part, *ml;   // O [slot][kv head][16][D], (m, l) [slot][kv head][16][2]
+};
+
+constexpr int kTileKeys = 32;
+constexpr int kCols = 16;
+constexpr float kSlack = 8.f;
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Columns [col, col + cols) of the sequences from `seq` on see keys [begin, end) of seq's table.
+struct __align__(16) Piece {
+  int seq, col, cols, begin;
+  int end, slot;  // where 16 columns' results go, cols / 16 slots; -1: they are the whole, and go to `out`
+  int pad[2];
+};
+// What the pieces of a sequence left: of its group's shared keys, its columns from `col` on in runs of `step` slots, and its own.
+struct __align__(16) Owner {
+  int shared_slot, shared_n, shared_step, col;
+  int slot, n;
+  int pad[2];
+};
+// A group's shared rows, its first sequence, and where the pieces of its shared keys leave their results.
+struct __align__(16) Group {
+  int rows, begin, slot, n;
+  int step, whole;  // whole: no sequence of it sees more
+  int pad[2];
+};
+struct __align__(16) Header {
+  int pieces, pad[3];
+};
+
+__device__ __forceinline__ int paged_keys(const PagedArgs& a, int seq) {
+  return static_cast<int>(within(a.lens[seq], 0, static_cast<int64_t>(a.width) << a.page_shift));
+}
+
+template <class T, int D, int CT>
+struct PagedState {
+  f4v o[CT][D / 16];  // lane (column, g), register r: dim 16 db + 4 g + r
+  float m[CT], l[CT];  // l: this lane's keys only
+};
+
+template <class T, int D>
+struct PagedTile {
+  typename Types<T>::v8 k[2][D / 32], v[D / 16];
+};
+
+// Where the pages of a wave's next 64 tiles are, lane l its l-th; a page of 16 rows is half a tile. -1: no page.
+struct PagedPages {
+  int lo, hi;
+};
+__device__ __forceinline__ PagedPages paged_pages(const PagedArgs& a, const int32_t* table, int tile, int end) {
+  const int row = tile * kTileKeys;
+  PagedPages p{-1, -1};
+  if (row >= 0 && row < end) p.lo = table[row >> a.page_shift];
+  if (a.page_shift == 4 && row >= 0 && row + 16 < end) p.hi = table[(row >> 4) + 1];
+  if (a.page_shift != 4) p.hi = p.lo;
+  if (p.lo < 0 || p.lo >= a.n_pages) p.lo = -1;
+  if (p.hi < 0 || p.hi >= a.n_pages) p.hi = -1;
+  return p;
+}
+
+// A lane's addresses in a tile whose rows lie in pages lo and hi: of its two K rows and of its V unit.
+template <class T, int D>
+__device__ __forceinline__ void paged_load_k(const PagedArgs& a, int kvh, int tile, int lo, int hi, int lane, PagedTile<T, D>& t) {
+  typedef typename Types<T>::v8 v8;
+  const int i = lane & 15, g = lane >> 4, page = i < 8 ? lo : hi, rows = 1 << a.page_shift;
+  const int row = (tile * kTileKeys + 8 * (i >> 2) + (i & 3)) & (rows - 1);
+  const T* at = static_cast<const T*>(a.k) + ((static_cast<int64_t>(max(page, 0)) * a.kv_heads + kvh) * rows + row) * D + 8 * g;
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) t.k[s][j] = *reinterpret_cast<const v8*>(at + 4 * s * D + 32 * j);
+}
+template <class T, int D>
+__device__ __forceinline__ void paged_load_v(const PagedArgs& a, int kvh, int tile, int lo, int hi, int lane, PagedTile<T, D>& t) {
+  typedef typename Types<T>::v8 v8;
+  const int i = lane & 15, g = lane >> 4, page = g < 2 ? lo : hi, rows = 1 << a.page_shift;
+  const int row = (tile * kTileKeys + 8 * g) & (rows - 1);
+  const T* at = static_cast<const T*>(a.v) + ((static_cast<int64_t>(max(page, 0)) * a.kv_heads + kvh) * rows + row) * D + 8 * i;
+#pragma unroll
+  for (int db = 0; db < D / 16; ++db) t.v[db] = *reinterpret_cast<const v8*>(at + 128 * db);
+}
+
+// A tile's scores for the columns; masked: only the first `left` of the lane's 8 keys count.
+template <class T, int D, int CT>
+__device__ __forceinline__ void paged_scores(const PagedTile<T, D>& t, const typename Types<T>::v8 (&q)[CT][D / 32], f4v (&s)[CT][2]) {
+#pragma unroll
+  for (int c = 0; c < CT; ++c)
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) s[c][kt] = f4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) s[c][kt] = mfma16(t.k[kt][j], q[c][j], s[c][kt]);
+}
+
+template <class T, int D, int CT, bool MASKED>
+__device__ __forceinline__ void paged_values(PagedTile<T, D>& t, f4v (&s)[CT][2], float factor, int left, PagedState<T, D, CT>& st) {
+  typedef typename Types<T>::v8 v8;
+  typedef typename Types<T>::v2 v2;
+  v8 p[CT];
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (MASKED && 4 * kt + r >= left) s[c][kt][r] = -INFINITY;
+        top = __builtin_elementwise_maximum(top, s[c][kt][r]);  // a NaN stays: its column is NaN anyway
+      }
+    top = xor_max<32>(xor_max<16>(top)) * factor;
+    if (__builtin_amdgcn_ballot_w64(top > st.m[c] + kSlack)) {
+      const float m_new = fmaxf(st.m[c], top), corr = st.m[c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m[c] - m_new);
+      st.l[c] *= corr;
+#pragma unroll
+      for (int db = 0; db < D / 16; ++db) st.o[c][db] *= corr;
+      st.m[c] = m_new;
+    }
+    const float m = st.m[c] == -INFINITY ? 0.f : st.m[c];  // no key seen yet: the weights are 0
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int r = 0; r < 4; r += 2) {
+        v2 x;
+        x[0] = static_cast<T>(__builtin_amdgcn_exp2f(fmaf(s[c][kt][r], factor, -m)));
+        x[1] = static_cast<T>(__builtin_amdgcn_exp2f(fmaf(s[c][kt][r + 1], factor, -m)));
+        st.l[c] = add_pair(x, st.l[c]);
+        p[c][4 * kt + r] = x[0];
+        p[c][4 * kt + r + 1] = x[1];
+      }
+  }
+#pragma unroll
+  for (int db = 0; db < D / 16; ++db) {
+    if constexpr (MASKED) {  // whatever the hidden rows hold, their values count as zeros
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e >= left) t.v[db][e] = static_cast<T>(0.f);
+    }
+#pragma unroll
+    for (int c = 0; c < CT; ++c) st.o[c][db] = mfma16(t.v[db], p[c], st.o[c][db]);
+  }
+}
+
+// Tiles first, first + step, .. of the keys below `end` of a table. Each half of a tile's registers is loaded again as
+// soon as it is used up.
+template <class T, int D, int CT>
+__device__ __forceinline__ void paged_tiles(const PagedArgs& a, const int32_t* table, int kvh, int first, int step, int end,
+                                            const typename Types<T>::v8 (&q)[CT][D / 32], float factor, int lane,
+                                            PagedState<T, D, CT>& st) {
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) st.o[c][db] = f4v{0.f, 0.f, 0.f, 0.f};
+    st.m[c] = -INFINITY;
+    st.l[c] = 0.f;
+  }
+  const int tiles = (end + kTileKeys - 1) / kTileKeys;
+  if (first >= tiles) return;
+  PagedPages pages = paged_pages(a, table, first + lane * step, end);
+  int lo = __builtin_amdgcn_readlane(pages.lo, 0), hi = __builtin_amdgcn_readlane(pages.hi, 0);
+  PagedTile<T, D> x;
+  f4v s[CT][2];
+  paged_load_k<T, D>(a, kvh, first, lo, hi, lane, x);
+  paged_load_v<T, D>(a, kvh, first, lo, hi, lane, x);
+  int t = first, n = 1;
+  for (; t + step < tiles; t += step, ++n) {
+    if ((n & 63) == 0) pages = paged_pages(a, table, t + step + lane * step, end);
+    const int lo1 = __builtin_amdgcn_readlane(pages.lo, n & 63), hi1 = __builtin_amdgcn_readlane(pages.hi, n & 63);
+    paged_scores<T, D, CT>(x, q, s);
+    paged_load_k<T, D>(a, kvh, t + step, lo1, hi1, lane, x);
+    if ((lo | hi) >= 0) paged_values<T, D, CT, false>(x, s, factor, 8, st);
+    else paged_values<T, D, CT, true>(x, s, factor, (lane < 32 ? lo : hi) >= 0 ? 8 : 0, st);
+    paged_load_v<T, D>(a, kvh, t + step, lo1, hi1, lane, x);
+    lo = lo1;
+    hi = hi1;
+  }
+  paged_scores<T, D, CT>(x, q, s);
+  const int left = end - t * kTileKeys;
+  if (left >= kTileKeys && (lo | hi) >= 0) paged_values<T, D, CT, false>(x, s, factor, 8, st);
+  else paged_values<T, D, CT, true>(x, s, factor, (lane < 32 ? lo : hi) >= 0 ? left - 8 * (lane >> 4) : 0, st);
+}
+
+// The waves' results of 16 columns meet in LDS: O [wave][column][D + 4], m and l [wave][column].
+template <int D>
+struct PagedMerge {
+  static constexpr int kPitch = D + 4;
+  float *m, *l, *acc;
+  int cols;
+  __device__ PagedMerge(float* lds, int waves, int c) : m(lds), l(lds + waves * kCols), acc(lds + 2 * waves * kCols), cols(c) {}
+  static constexpr int bytes(int waves, int cols) { return 4 * waves * (2 * kCols + cols * kPitch); }
+};
+
+template <class T, int D, int CT>
+__device__ __forceinline__ void paged_piece(const PagedArgs& a, const Piece& p, int kvh, const int32_t* table, float* lds) {
+  typedef typename Types<T>::v8 v8;
+  const int waves = blockDim.x / 64, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = lane & 15, g = lane >> 4, group = a.heads / a.kv_heads;
+  v8 q[CT][D / 32];
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    const int col = p.col + min(16 * c + i, p.cols - 1);  // columns past the end repeat the last one
+    const T* at = static_cast<const T*>(a.q) + (p.seq + col / group) * a.q_row + (kvh * group + col % group) * a.q_head + 8 * g;
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+      q[c][j] = *reinterpret_cast<const v8*>(at + 32 * j);
+      if (a.scale < 0.f) q[c][j] = -q[c][j];  // scores are scaled by a positive factor after the product
+    }
+  }
+  // 0: the smallest number instead; a hidden score (-infinity) times zero would be NaN
+  const float factor = fmaxf(__builtin_fabsf(a.scale) * kLog2e, __FLT_DENORM_MIN__);
+  PagedState<T, D, CT> st;
+  paged_tiles<T, D, CT>(a, table, kvh, p.begin / kTileKeys + wave, waves, p.end, q, factor, lane, st);
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    const int cols = min(kCols, p.cols - kCols * c);
+    if (cols <= 0) break;
+    const PagedMerge<D> x(lds, waves, cols);
+    const float own_l = xor_add<32>(xor_add<16>(st.l[c]));
+    if (c > 0) __syncthreads();
+    if (i < cols) {
+      if (g == 0) {
+        x.m[wave * kCols + i] = st.m[c];
+        x.l[wave * kCols + i] = own_l;
+      }
+      float* to = x.acc + (wave * cols + i) * PagedMerge<D>::kPitch + 4 * g;
+#pragma unroll
+      for (int db = 0; db < D / 16; ++db) *reinterpret_cast<f4v*>(to + 16 * db) = st.o[c][db];
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < cols * D; e += blockDim.x) {
+      const int col = e / D, d = e % D;
+      float m = -INFINITY, l = 0.f, o = 0.f;
+      for (int w = 0; w < waves; ++w) m = fmaxf(m, x.m[w * kCols + col]);
+      for (int w = 0; w < waves; ++w) {
+        const float mw = x.m[w * kCols + col], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - m);
+        l = fmaf(f, x.l[w * kCols + col], l);
+        o = fmaf(f, x.acc[(w * cols + col) * PagedMerge<D>::kPitch + d], o);
+      }
+      if (p.slot < 0) {
+        const int at = p.col + kCols * c + col, seq = p.seq + at / group, head = kvh * group + at % group;
+        // (an idle sequence of a group sees nothing, whatever its group sees)
+        const float y = l == 0.f || a.lens[seq] <= 0 ? 0.f : o / l;
+        static_cast<T*>(a.out)[seq * a.o_row + head * a.o_head + d] = static_cast<T>(y);
+      } else {
+        const int64_t at = (static_cast<int64_t>(p.slot + c) * a.kv_heads + kvh) * kCols + col;
+        a.part[at * D + d] = o;
+        if (d == 0) {
+          a.ml[2 * at] = m;
+          a.ml[2 * at + 1] = l;
+        }
+      }
+    }
+  }
+}
+
+// Direct: a block for each sequence, key/value head and 16 of its columns. Else a block for each piece and key/value head.
+template <class T, int D, int CT>
+__global__ void __launch_bounds__(512, 2) paged_attention_kernel(PagedArgs a) {
+  extern __shared__ float lds[];
+  const int kvh = blockIdx.x % a.kv_heads;
+  const unsigned at = blockIdx.x / a.kv_heads;
+  if constexpr (CT == 0) {
+    const int group = a.heads / a.kv_heads, parts = (group + kCols - 1) / kCols, col = static_cast<int>(at % parts) * kCols;
+    const int seq = static_cast<int>(at / parts);
+    const Piece p{seq, col, min(kCols, group - col), 0, paged_keys(a, seq), -1, {}};
+    paged_piece<T, D, 1>(a, p, kvh, a.table + static_cast<int64_t>(seq) * a.width, lds);
+  } else {
+    if (static_cast<int>(at) >= reinterpret_cast<const Header*>(a.plan)->pieces) return;
+    const Piece p = (reinterpret_cast<const Piece*>(a.plan + 4))[at];
+    const int32_t* table = a.table + static_cast<int64_t>(p.seq) * a.width;
+    if (CT == 1 || p.cols <= kCols) paged_piece<T, D, 1>(a, p, kvh, table, lds);
+    else paged_piece<T, D, CT>(a, p, kvh, table, lds);
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// The plan: one block turns the lengths into pieces. A group's shared rows are those that all its live sequences have, cut to
+// whole tiles unless they are all that any of them has. All keys, times the runs of columns that see them, make about `want`
+// pieces, a multiple of a tile for each wave; the pieces of one run of keys are alike.
+// ------------------------------------------------------------------------------------------
+constexpr int kPlanThreads = 1024, kSerial = 32;
+
+__device__ __forceinline__ int64_t plan_sum(int64_t v, int64_t* part) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0;
+  for (int w = 0; w < kPlanThreads / 64; ++w) v += part[w];
+  return v;
+}
+// Exclusive sum over the block; total: of all.
+__device__ __forceinline__ int plan_scan(int v, int* part, int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mine = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(v, o);
+    if (lane >= o) v += x;
+  }
+  __syncthreads();
+  if (lane == 63) part[wave] = v;
+  __syncthreads();
+  total = 0;
+  for (int w = 0; w < kPlanThreads / 64; ++w) {
+    if (w < wave) v += part[w];
+    total += part[w];
+  }
+  return v - mine;
+}
+
+struct Members {
+  int begin, end;
+};
+__device__ __forceinline__ Members members_of(const PagedArgs& a, int g) {
+  const int64_t b = within(a.cu_g[g], 0, a.n_seq);
+  return Members{static_cast<int>(b), static_cast<int>(within(a.cu_g[g + 1], b, a.n_seq))};
+}
+// Shared rows of a group whose live sequences have `low` to `high` keys (high 0: none is live, or none has keys).
+__device__ __forceinline__ int shared_rows(const PagedArgs& a, int g, int low, int high) {
+  if (high <= 0) return 0;
+  const int64_t most = within(a.shared[g], 0, low);
+  return static_cast<int>(most == high ? most : most & ~int64_t{kTileKeys - 1});
+}
+// Keys of one piece, of `keys` in pieces of at most `chunk`.
+__device__ __forceinline__ int piece_keys(int keys, int n) {
+  return n ? ((keys + n - 1) / n + kTileKeys - 1) / kTileKeys * kTileKeys : 0;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedArgs a, int unit) {
+  __shared__ int64_t sums[kPlanThreads / 64];
+  __shared__ int scans[kPlanThreads / 64];
+  const int tid = threadIdx.x, lane = tid & 63, group = a.heads / a.kv_heads, parts = (group + kCols - 1) / kCols;
+  Piece* pieces = reinterpret_cast<Piece*>(a.plan + 4);
+  Owner* owners = reinterpret_cast<Owner*>(pieces + a.most);
+  Group* of = reinterpret_cast<Group*>(owners + a.n_seq);
+  int* group_of = reinterpret_cast<int*>(of + a.groups);  // by sequence; -1: none, or nothing is shared
+  for (int s = tid; s < a.n_seq; s += kPlanThreads) group_of[s] = -1;
+  // groups whose starts do not ascend would overlap: none is one
+  int descends = 0;
+  for (int g = tid; g < a.groups; g += kPlanThreads) descends |= a.cu_g[g] > a.cu_g[g + 1];
+  const int groups = __syncthreads_or(descends) ? 0 : a.groups;
+  // shared rows of every group: the sequences of a small group by a thread, of a large one by a wave
+  int64_t work = 0;
+  const auto runs_of = [&](const Members& m) { return ((m.end - m.begin) * group + a.cols - 1) / a.cols; };
+  for (int g0 = tid & ~63; g0 < groups; g0 += kPlanThreads) {
+    const int g = g0 + lane;
+    Members m{0, 0};
+    int low = 0x7FFFFFFF, high = 0;
+    if (g < groups) m = members_of(a, g);
+    const int count = m.end - m.begin;
+    for (int s = m.begin; count <= kSerial && s < m.end; ++s) {
+      if (a.lens[s] < 0) continue;
+      const int keys = paged_keys(a, s);
+      low = min(low, keys);
+      high = max(high, keys);
+    }
+    for (uint64_t big = __builtin_amdgcn_ballot_w64(count > kSerial); big; big &= big - 1) {
+      const int l = __builtin_ctzll(big), b = __builtin_amdgcn_readlane(m.begin, l), e = __builtin_amdgcn_readlane(m.end, l);
+      int lo = 0x7FFFFFFF, hi = 0;
+      for (int s = b + lane; s < e; s += 64) {
+        if (a.lens[s] < 0) continue;
+        const int keys = paged_keys(a, s);
+        lo = min(lo, keys);
+        hi = max(hi, keys);
+      }
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        lo = min(lo, __shfl_xor(lo, o));
+        hi = max(hi, __shfl_xor(hi, o));
+      }
+      if (lane == l) {
+        low = lo;
+        high = hi;
+      }
+    }
+    const int rows = g < groups && count > 1 ? shared_rows(a, g, low, high) : 0;
+    if (g < groups) of[g] = Group{rows, m.begin, -1, 0, 0, rows == high, {}};
+    work += static_cast<int64_t>(rows) * runs_of(m);
+    if (rows && count <= kSerial)
+      for (int s = m.begin; s < m.end; ++s) group_of[s] = g;
+    for (uint64_t big = __builtin_amdgcn_ballot_w64(rows && count > kSerial); big; big &= big - 1) {
+      const int l = __builtin_ctzll(big), b = __builtin_amdgcn_readlane(m.begin, l), e = __builtin_amdgcn_readlane(m.end, l);
+      for (int s = b + lane; s < e; s += 64) group_of[s] = g0 + l;
+    }
+  }
+  __syncthreads();
+  const auto shared_of = [&](int s) { return group_of[s] < 0 ? 0 : of[group_of[s]].rows; };
+  for (int s = tid; s < a.n_seq; s += kPlanThreads) work += static_cast<int64_t>(max(paged_keys(a, s) - shared_of(s), 0)) * parts;
+  work = plan_sum(work, sums);
+  const int64_t chunk = (work / a.want / unit + 1) * unit;
+  const auto count_of = [&](int keys) { return static_cast<int>((keys + chunk - 1) / chunk); };
+  // pieces of the groups, then of the sequences
+  int next = 0, slot = 0;
+  const int tiles = a.cols / kCols;
+  for (int g0 = 0; g0 < groups; g0 += kPlanThreads) {
+    const int g = g0 + tid;
+    Group x{};
+    Members m{0, 0};
+    int runs = 0;
+    if (g < groups) {
+      m = members_of(a, g);
+      x = of[g];
+      x.n = count_of(x.rows);
+      runs = x.n ? runs_of(m) : 0;
+    }
+    const bool whole = x.whole && x.n == 1;
+    int total;
+    const int before = plan_scan(x.n * runs, scans, total), size = piece_keys(x.rows, x.n);
+    for (int y = 0; y < x.n * runs; ++y) {
+      const int i = y / runs, r = y % runs, at = next + before + y, left = (m.end - m.begin) * group - r * a.cols;
+      if (at < a.most)
+        pieces[at] = Piece{m.begin, r * a.cols, min(a.cols, left), i * size, min((i + 1) * size, x.rows),
+                           whole ? -1 : slot + (before + y) * tiles, {}};
+    }
+    if (g < groups) {
+      x.slot = whole ? -1 : slot + before * tiles;
+      x.step = runs * tiles;
+      of[g] = x;
+    }
+    next += total;
+    slot += total * tiles;
+  }
+  __syncthreads();
+  for (int s0 = 0; s0 < a.n_seq; s0 += kPlanThreads) {
+    const int s = s0 + tid;
+    Owner o{};
+    int keys = 0, begin = 0;
+    if (s < a.n_seq) {
+      if (group_of[s] >= 0) {
+        const Group x = of[group_of[s]];
+        begin = x.rows;
+        o = Owner{x.slot, x.n, x.step, (s - x.begin) * group, 0, 0, {}};
+      }
+      keys = max(paged_keys(a, s) - begin, 0);
+      o.n = count_of(keys);
+      if (begin == 0 && o.n == 0) o.n = 1;  // its zeros
+    }
+    int total;
+    const int before = plan_scan(o.n * parts, scans, total), size = piece_keys(keys, o.n);
+    o.slot = begin == 0 && o.n == 1 ? -1 : slot + before;
+    for (int y = 0; y < o.n * parts; ++y) {
+      const int i = y / parts, r = y % parts, at = next + before + y;
+      if (at < a.most)
+        pieces[at] = Piece{s, r * kCols, min(kCols, group - r * kCols), begin + i * size, begin + min((i + 1) * size, keys),
+                           o.slot < 0 ? -1 : o.slot + y, {}};
+    }
+    if (s < a.n_seq) owners[s] = o;
+    next += total;
+    slot += total;
+  }
+  if (tid == 0) reinterpret_cast<Header*>(a.plan)->pieces = min(next, a.most);
+}
+
+// Joins what the pieces of a sequence left: block = (query head, sequence).
+constexpr int kCombine = 256, kMostParts = 2112;
+template <class T, int D>
+__global__ void __launch_bounds__(kCombine) paged_combine_kernel(PagedArgs a) {
+  constexpr int kLanes = kCombine / D, kBatch = 8;
+  __shared__ float weight[kMostParts], red[2][kCombine / 64], sum[kLanes][D];
+  const int seq = blockIdx.y, head = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid / 64, d = tid % D, from = tid / D;
+  const Owner o = (reinterpret_cast<const Owner*>(a.plan + 4 + 8 * static_cast<int64_t>(a.most)))[seq];
+  const int n = min(o.shared_n + o.n, kMostParts);
+  if ((o.shared_n == 0 || o.shared_slot < 0) && (o.n == 0 || o.slot < 0)) return;  // its block finished it
+  const int group = a.heads / a.kv_heads, kvh = head / group, col = head % group;
+  const auto slot = [&](int i) {
+    const int c = i < o.shared_n ? o.col + col : col;
+    const int at = i < o.shared_n ? o.shared_slot + i * o.shared_step : o.slot + (i - o.shared_n) * ((group + kCols - 1) / kCols);
+    return (static_cast<int64_t>(at + c / kCols) * a.kv_heads + kvh) * kCols + c % kCols;
+  };
+  const auto load = [&](int i, float (&x)[kBatch]) {  // chunks i, i + kLanes, ..; past the end the last one
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) x[j] = a.part[slot(min(i + j * kLanes, n - 1)) * D + d];
+  };
+  float x[kBatch];
+  load(from, x);
+  float m = -INFINITY, l = 0.f;
+  for (int i = tid; i < n; i += kCombine) {
+    weight[i] = a.ml[2 * slot(i)];
+    m = fmaxf(m, weight[i]);
+  }
+  m = group_max<64>(m);
+  if (lane == 0) red[0][wave] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kCombine / 64; ++i) m = fmaxf(m, red[0][i]);
+  for (int i = tid; i < n; i += kCombine) {
+    weight[i] = weight[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(weight[i] - m);
+    l = fmaf(weight[i], a.ml[2 * slot(i) + 1], l);
+  }
+  l = group_sum<64>(l);
+  if (lane == 0) red[1][wave] = l;
+  __syncthreads();
+  float y = 0.f;
+  for (int i = from;;) {
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      if (i + j * kLanes < n) y = fmaf(weight[i + j * kLanes], x[j], y);
+    i += kBatch * kLanes;
+    if (i >= n) break;
+    load(i, x);
+  }
+  sum[from][d] = y;
+  __syncthreads();
+  if (tid >= D) return;
+  l = 0.f;
+#pragma unroll
+  for (int i = 0; i < kCombine / 64; ++i) l += red[1][i];
+#pragma unroll
+  for (int j = 1; j < kLanes; ++j) y += sum[j][d];
+  static_cast<T*>(a.out)[seq * a.o_row + head * a.o_head + d] = static_cast<T>(l == 0.f || a.lens[seq] <= 0 ? 0.f : y / l);
+}
+
+// What of a call goes by sizes alone (the lengths are on the device).
+struct PagedSizes {
+  int cols, want, waves, direct_waves;
+  int64_t most, slots, ints, floats;  // pieces, 16-column results, the plan's words, workspace
+};
+constexpr int kDirectRows = 1024, kWantBlocks = 1024;
+
+PagedSizes paged_sizes(int n_seq, int heads, int kv_heads, int64_t capacity, int groups, int dim) {
+  PagedSizes p = {};
+  const int64_t group = heads / kv_heads, parts = (group + kCols - 1) / kCols;
+  p.direct_waves = static_cast<int>(std::min<int64_t>(8, (capacity + kTileKeys - 1) / kTileKeys));
+  p.waves = 4;
+  if (capacity <= kDirectRows) {
+    p.floats = 4;
+    return p;
+  }
+  p.cols = groups && (n_seq + groups - 1) / groups * group > kCols ? 2 * kCols : kCols;
+  p.want = std::max(1, kWantBlocks / kv_heads);
+  // each run of columns has the pieces that fill its share of `want`, and one more
+  const int64_t runs = groups ? n_seq * group / p.cols + groups : 0;
+  p.most = p.want + runs + n_seq * parts + 1;
+  p.slots = p.cols / kCols * (p.want + runs) + n_seq * parts + 1;
+  p.ints = 4 + 8 * p.most + 8 * static_cast<int64_t>(n_seq) + 8 * static_cast<int64_t>(groups) + n_seq;
+  p.ints = (p.ints + 3) / 4 * 4;
+  p.floats = p.ints + p.slots * kv_heads * kCols * (dim + 2);
+  return p;
+}
+
+bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+bool rows_ok(const void* p, int64_t row, int64_t head) { return aligned(p, 16) && row % 8 == 0 && head % 8 == 0; }
+
+// What every call asks of its sizes; FW_OK or FW_EINVAL.
+int check_paged(int n_seq, int heads, int kv_heads, int width, int page, int groups, int head_dim) {
+  const char* what = "decode_attention_paged";
+  if (page_shift_of(page) < 0) return fw_fail(FW_EINVAL, "%s: page must be 16, 32, 64, 128 or 256 rows", what);
+  if (head_dim != 64 && head_dim != 128) return fw_fail(FW_EINVAL, "%s: head_dim must be 64 or 128", what);
+  if (n_seq <= 0 || width <= 0 || groups < 0) return fw_fail(FW_EINVAL, "%s: n_seq and width must be positive, groups not negative", what);
+  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads) return fw_fail(FW_EINVAL, "%s: heads must be a multiple of kv_heads", what);
+  if (static_cast<int64_t>(width) * page > (1 << 30)) return fw_fail(FW_EINVAL, "%s: at most 2^30 rows a sequence", what);
+  if (n_seq > 65535 || groups > 65535) return fw_fail(FW_EINVAL, "%s: too many sequences", what);
+  if (heads > (1 << 14)) return fw_fail(FW_EINVAL, "%s: too many heads", what);  // columns of a group in 32 bits
+  return FW_OK;
+}
+
+}  // namespace
+}  // namespace fw
+
+using namespace fw;
+
+extern "C" int64_t fw_decode_attention_paged_ws_floats(int n_seq, int heads, int kv_heads, int width, int page, int groups,
+                                                       int head_dim) {
+  if (check_paged(n_seq, heads, kv_heads, width, page, groups, head_dim)) return 0;
+  return paged_sizes(n_seq, heads, kv_heads, static_cast<int64_t>(width) * page, groups, head_dim).floats;
+}
+
+extern "C" int fw_decode_attention_paged(const void* q, int64_t q_row, int64_t q_head, const void* k_pages, const void* v_pages,
+                                         const int32_t* table, const int64_t* lens, const int64_t* cu_groups,
+                                         const int64_t* shared, void* out, int64_t o_row, int64_t o_head, int n_seq, int heads,
+                                         int kv_heads, int n_pages, int page, int width, int groups, int head_dim, int dtype,
+                                         float scale, float* ws, int64_t ws_floats, hipStream_t stream) {
+  const char* what = "decode_attention_paged";
+  if (const int rc = check_paged(n_seq, heads, kv_heads, width, page, groups, head_dim)) return rc;
+  if (n_pages <= 0) return fw_fail(FW_EINVAL, "%s: n_pages must be positive", what);
+  if (dtype != FW_F16 && dtype != FW_BF16) return fw_fail(FW_EINVAL, "%s: dtype must be FW_F16 or FW_BF16", what);
+  if (!q || !k_pages || !v_pages || !table || !lens || !out || (groups > 0 && (!cu_groups || !shared)))
+    return fw_fail(FW_EINVAL, "%s: null pointer", what);
+  if (!(__builtin_fabsf(scale) * kLog2e < INFINITY))
+    return fw_fail(FW_EINVAL, "%s: scale must be finite (and below 2.3e38 in size)", what);
+  if (!rows_ok(q, q_row, q_head) || !rows_ok(out, o_row, o_head) || !aligned(k_pages, 16) || !aligned(v_pages, 16))
+    return fw_fail(FW_EINVAL, "%s: q, out and the pages must be 16-byte aligned with strides in multiples of 8", what);
+  const PagedSizes p = paged_sizes(n_seq, heads, kv_heads, static_cast<int64_t>(width) * page, groups, head_dim);
+  if (!ws || ws_floats < p.floats || !aligned(ws, 16))
+    return fw_fail(FW_EINVAL, "%s: workspace needs %lld floats, 16-byte aligned", what, static_cast<long long>(p.floats));
+  const int group = heads / kv_heads, parts = (group + kCols - 1) / kCols;
+  const int waves = p.most ? p.waves : p.direct_waves, cols = p.cols ? kCols : std::min(kCols, group);
+  const int64_t blocks = kv_heads * (p.most ? p.most : static_cast<int64_t>(n_seq) * parts);
+  if (!grid_ok(blocks, 64 * waves) || p.slots > 0x7FFFFFFF / kCols) return fw_fail(FW_EINVAL, "%s: too many sequences", what);
+  PagedArgs a{q, k_pages, v_pages, out, q_row, q_head, o_row, o_head, table, lens, cu_groups, shared, n_seq, heads, kv_heads,
+              groups, width, n_pages, page_shift_of(page), scale, p.cols, p.want, static_cast<int>(p.most),
+              reinterpret_cast<int*>(ws), ws + p.ints, nullptr};
+  a.ml = a.part + p.slots * kv_heads * kCols * head_dim;
+  const int lds = head_dim == 64 ? PagedMerge<64>::bytes(waves, cols) : PagedMerge<128>::bytes(waves, cols);
+  if (p.most) {
+    hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, a, kTileKeys * waves);
+    if (const int rc = fw_check_launch(what)) return rc;
+  }
+  const auto run = [&](auto t, auto d) {
+    typedef decltype(t) T;
+    constexpr int D = decltype(d)::value;
+    const auto kernel = !p.most ? paged_attention_kernel<T, D, 0>
+                        : p.cols == kCols ? paged_attention_kernel<T, D, 1> : paged_attention_kernel<T, D, 2>;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(64 * waves), lds, stream, a);
+    if (const int rc = fw_check_launch(what)) return rc;
+    if (!p.most) return static_cast<int>(FW_OK);
+    hipLaunchKernelGGL((paged_combine_kernel<T, D>), dim3(heads, n_seq), dim3(kCombine), 0, stream, a);
+    return fw_check_launch("decode_attention_paged combine");
+  };
+  const std::integral_constant<int, 64> d64;
+  const std::integral_constant<int, 128> d128;
+  if (dtype == FW_F16) return head_dim == 64 ? run(_Float16(), d64) : run(_Float16(), d128);
+  return head_dim == 64 ? run(__bf16(), d64) : run(__bf16(), d128);
+}

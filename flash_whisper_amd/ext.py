@@ -31,10 +31,11 @@ except ImportError:
 
 HIDDEN, HEAD_DIM = 1280, 64
 MAX_BATCH = 4  # decoder positions per batched launch (the prompt)
+PAGES = (16, 32, 64, 128, 256)  # rows that a page of a cache may have
 WAVE_CHUNK = 240000  # samples per staged chunk of the waveform upload (half of 30 s: smaller chunks measured slower)
 
 
-_F16, _F32, _I64 = torch.float16, torch.float32, torch.int64
+_F16, _F32, _I64, _I32 = torch.float16, torch.float32, torch.int64, torch.int32
 # absent from a torch without GPU support
 _device = getattr(torch._C, '_cuda_getDevice', None)
 _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
@@ -94,6 +95,7 @@ def _check(t, name, dtype, what):
 
 # The prompt attention and the 4-bit cache take fp16 or bf16 rows of any strides that keep 16-byte pieces whole.
 _DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+_LOGITS = {**_DTYPES, torch.float32: _lib.F32}
 
 
 def _current_device():
@@ -166,6 +168,40 @@ def _cache_sizes(cache, dev):
             or v_meta.shape != (n, heads, max_len // 8, half // 16, 2, 8)):
         raise RuntimeError('the arrays of the cache do not belong together')
     return n, heads, max_len, 2 * half
+
+
+class KvPages(NamedTuple):
+    """A key/value cache in pages (layout: fw_kv_page_map in include/flash_whisper.h)."""
+    k: torch.Tensor  # fp16 or bf16 [n_pages, kv_heads, page, head_dim]
+    v: torch.Tensor  # of its type [n_pages, kv_heads, page / 8, head_dim, 8]
+
+
+def _page_arrays(cache):
+    if not (isinstance(cache, (tuple, list)) and len(cache) == 2 and all(isinstance(t, torch.Tensor) for t in cache)):
+        raise RuntimeError('the cache must be KvPages: k, v')
+    return cache
+
+
+def _page_sizes(cache, dev):
+    """Checks the two arrays of a cache in pages; returns n_pages, kv_heads, page, head_dim, dtype."""
+    k, v = _page_arrays(cache)
+    for t, name in ((k, 'k'), (v, 'v')):
+        if not (t.dtype in _DTYPES and t.dtype is k.dtype and t.get_device() == dev and t.is_contiguous()):
+            raise RuntimeError(f'{name} of the cache must be contiguous fp16 or bf16, both alike, on the current device')
+    if k.dim() != 4 or k.size(2) not in PAGES or k.size(3) not in (64, 128):
+        raise RuntimeError(f'k of the cache must be [n_pages, kv_heads, page, head_dim], page one of {PAGES}, head_dim 64 or 128')
+    n, heads, page, dim = k.shape
+    if v.shape != (n, heads, page // 8, dim, 8):
+        raise RuntimeError('the arrays of the cache do not belong together')
+    return n, heads, page, dim, k.dtype
+
+
+def _dense(t, name, dtype, shape, dev):
+    """Checks a contiguous tensor of `dtype` and shape (None: any size) on the current device."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev and t.is_contiguous()
+            and t.dim() == len(shape) and all(n is None or n == m for n, m in zip(shape, t.shape))):
+        sizes = ', '.join('any' if n is None else str(n) for n in shape)
+        raise RuntimeError(f'{name} must be contiguous {dtype} [{sizes}] on the current device')
 
 
 class HostTokens:
@@ -522,6 +558,138 @@ class WhisperExt:
         self._call('fw_decode_attention_q4', q.data_ptr(), q_row, q_head, k_codes.data_ptr(), k_meta.data_ptr(),
                    v_codes.data_ptr(), v_meta.data_ptr(), lens.data_ptr(), out.data_ptr(), o_row, o_head, *fresh, n, heads,
                    kv_heads, max_len, dim, _DTYPES[dtype], float(scale), ws.data_ptr(), ws.numel(), _stream())
+
+    # ---- several answers to one prompt: a cache in pages, and rules on logits -----------------
+    def kv_pages(self, n_pages, kv_heads, page, head_dim, dtype=torch.float16, device='cuda'):
+        """An empty KvPages of n_pages pages of `page` rows (16, 32, 64, 128 or 256)."""
+        _require(n_pages > 0 and kv_heads > 0 and page in PAGES and head_dim in (64, 128) and dtype in _DTYPES,
+                 f'n_pages and kv_heads must be positive, page one of {PAGES}, head_dim 64 or 128, dtype fp16 or bf16')
+        return KvPages(torch.zeros(n_pages, kv_heads, page, head_dim, dtype=dtype, device=device),
+                       torch.zeros(n_pages, kv_heads, page // 8, head_dim, 8, dtype=dtype, device=device))
+
+    def kv_page_map(self, pos, cu, table, held, stack, count, slots, page, own=None, held_out=None, count_out=None):
+        """Brings the page tables up to the sequences' lengths, and finds the slots of their new rows (fw_kv_page_map).
+        Sequence s holds the pages table[s, :held[s]] (table int32 [n_seq, width], held int64 [n_seq]) and gets the packed
+        rows cu[s] .. cu[s + 1] - 1 as its rows pos[s] .. (int64, pos < 0: idle). Pages past its last row, from entry own[s]
+        on, go back onto the stack of free pages (stack int32, count int64 [2]: pages on it, pages that were missing), new ones
+        are taken from its top; slots[r] (int64) is the place of packed row r, -1 where it has none. held_out and count_out
+        default to held and count."""
+        dev = _current_device()
+        _dense(table, 'table', _I32, (None, None), dev)
+        n, width = table.shape
+        held_out, count_out = held if held_out is None else held_out, count if count_out is None else count_out
+        _index(pos, 'pos', n, dev)
+        _index(cu, 'cu', n + 1, dev)
+        for t, name in ((held, 'held'), (held_out, 'held_out')) + (() if own is None else ((own, 'own'),)):
+            _index(t, name, n, dev)
+        _index(count, 'count', 2, dev)
+        _index(count_out, 'count_out', 2, dev)
+        _dense(stack, 'stack', _I32, (None,), dev)
+        _dense(slots, 'slots', _I64, (None,), dev)
+        self._call('fw_kv_page_map', pos.data_ptr(), cu.data_ptr(), table.data_ptr(), held.data_ptr(), _ptr(own),
+                   stack.data_ptr(), count.data_ptr(), held_out.data_ptr(), count_out.data_ptr(), slots.data_ptr(), n, width,
+                   stack.numel(), slots.numel(), int(page), _stream())
+
+    def kv_page_append(self, k, v, slots, cache):
+        """Writes rows r of k and v ([rows, kv_heads, head_dim] of the cache's type) to slot slots[r] (int64) of a cache in
+        pages (fw_kv_page_append). Rows whose slot is negative or past the pages are dropped; no slot may occur twice."""
+        dev = _current_device()
+        n, heads, page, dim, dtype = _page_sizes(cache, dev)
+        strides = (*_heads_view(k, 'k', dtype, dev, heads, dim), *_heads_view(v, 'v', dtype, dev, heads, dim))
+        if k.size(0) != v.size(0):
+            raise RuntimeError('k and v must have the same rows')
+        _index(slots, 'slots', k.size(0), dev)
+        self._call('fw_kv_page_append', k.data_ptr(), *strides[:2], v.data_ptr(), *strides[2:], slots.data_ptr(), k.size(0),
+                   cache[0].data_ptr(), cache[1].data_ptr(), n, heads, page, dim, _stream())
+
+    def decode_attention_paged_workspace(self, n_seq, heads, cache, width, groups=0):
+        """Workspace of decode_attention_paged for n_seq sequences with tables of `width` pages and `heads` query heads in
+        `groups` groups over `cache` (one per stream)."""
+        k, _ = _page_arrays(cache)
+        _require(k.dim() == 4, 'k of the cache must be [n_pages, kv_heads, page, head_dim]')
+        n = self.lib.fw_decode_attention_paged_ws_floats(int(n_seq), int(heads), k.size(1), int(width), k.size(2), int(groups),
+                                                         k.size(3))
+        if n <= 0:
+            raise RuntimeError(f'decode_attention_paged_workspace: {self.lib.fw_last_error().decode(errors="replace")}')
+        return torch.empty(n, dtype=torch.float32, device=k.device)
+
+    def decode_attention_paged(self, q, cache, table, lens, out, ws, scale, cu_groups=None, shared=None):
+        """One query a sequence, q and out [n_seq, heads, head_dim], over the first lens[s] rows (int64) of the pages
+        table[s] (int32 [n_seq, width]) (fw_decode_attention_paged); a sequence without rows, or idle (lens[s] < 0), gets
+        zeros. The sequences cu_groups[g] .. cu_groups[g + 1] - 1 have their first shared[g] rows in common (int64): these are
+        read once for all of them, from the first one's table."""
+        dev = _current_device()
+        n_pages, kv_heads, page, dim, dtype = _page_sizes(cache, dev)
+        q_row, q_head = _heads_view(q, 'q', dtype, dev, None, dim)
+        n, heads = q.size(0), q.size(1)
+        o_row, o_head = _out_view(out, 'out', dtype, dev, heads, dim)
+        if out.size(0) != n:
+            raise RuntimeError('out must have the rows of q')
+        _dense(table, 'table', _I32, (n, None), dev)
+        _index(lens, 'lens', n, dev)
+        _dense(ws, 'the workspace', _F32, (None,), dev)
+        groups = 0
+        if cu_groups is not None or shared is not None:
+            if cu_groups is None or shared is None:
+                raise RuntimeError('cu_groups and shared must be given together')
+            _index(shared, 'shared', None, dev)
+            groups = shared.size(0)
+            _index(cu_groups, 'cu_groups', groups + 1, dev)
+        self._call('fw_decode_attention_paged', q.data_ptr(), q_row, q_head, cache[0].data_ptr(), cache[1].data_ptr(),
+                   table.data_ptr(), lens.data_ptr(), _ptr(cu_groups), _ptr(shared), out.data_ptr(), o_row, o_head, n, heads,
+                   kv_heads, n_pages, page, table.size(1), groups, dim, _DTYPES[dtype], float(scale), ws.data_ptr(),
+                   ws.numel(), _stream())
+
+    def logits_rules(self, logits, out, tokens=None, cu=None, prompt=None, repetition=None, presence=None, frequency=None,
+                     bias_ids=None, bias=None, cu_bias=None, masks=None, mask_of=None):
+        """Penalties, biases and masks on logits [rows, vocab] (fp16, bf16 or fp32), into out, which may be logits itself
+        (fw_logits_rules). The history of row r is tokens[cu[r]:cu[r + 1]] (int64), its first prompt[r] the prompt: a token of it
+        is divided by repetition[r] if positive, else multiplied; one that comes c times behind the prompt loses frequency[r] c +
+        presence[r] (fp32 [rows] each). Then bias[j] (fp32) is added to token bias_ids[j] for the j from cu_bias[r] to
+        cu_bias[r + 1] (of a token's, the last), and tokens whose bit in the row's mask (int32 [sets, words], bit i % 32 of
+        word i / 32; set mask_of[r], -1: none; without mask_of one for all or for each row) is 0 get -infinity."""
+        dev = _current_device()
+        for t, name in ((logits, 'logits'), (out, 'out')):
+            if not (isinstance(t, torch.Tensor) and t.dtype in _LOGITS and t.dtype is logits.dtype and t.get_device() == dev
+                    and t.dim() == 2 and t.size(1) > 0 and (t.stride(1) == 1 or t.size(1) == 1 or t.size(0) == 0)):
+                raise RuntimeError(f'{name} must be [rows, vocab] fp16, bf16 or fp32 (both alike) on the current device with '
+                                   'unit column stride')
+        rows, vocab = logits.shape
+        if out.shape != logits.shape or (rows > 1 and out.stride(0) < vocab):
+            raise RuntimeError('out must have the shape of logits, its rows apart')
+        history = tokens is not None or cu is not None
+        if history:
+            _index(cu, 'cu', rows + 1, dev)
+            _dense(tokens, 'tokens', _I64, (None,), dev)
+        elif any(t is not None for t in (prompt, repetition, presence, frequency)):
+            raise RuntimeError('penalties need tokens and cu')
+        if prompt is not None:
+            _index(prompt, 'prompt', rows, dev)
+        for t, name in ((repetition, 'repetition'), (presence, 'presence'), (frequency, 'frequency')):
+            if t is not None:
+                _dense(t, name, _F32, (rows,), dev)
+        if not (bias_ids is None) == (bias is None) == (cu_bias is None):
+            raise RuntimeError('bias_ids, bias and cu_bias must be given together')
+        if bias_ids is not None:
+            _dense(bias_ids, 'bias_ids', _I64, (None,), dev)
+            _dense(bias, 'bias', _F32, (bias_ids.size(0),), dev)
+            _index(cu_bias, 'cu_bias', rows + 1, dev)
+        sets = words = 0
+        if masks is not None:
+            _dense(masks, 'masks', _I32, (None, None), dev)
+            sets, words = masks.shape
+            if sets == 0:
+                raise RuntimeError('masks must hold a set')
+        if mask_of is not None:
+            _index(mask_of, 'mask_of', rows, dev)
+        # an empty history or list is none (its tensor has no address)
+        met = (tokens, cu, prompt, repetition, presence, frequency) if history and tokens.numel() else (None,) * 6
+        listed = (bias_ids, bias, cu_bias) if bias_ids is not None and bias_ids.numel() else (None,) * 3
+        self._call('fw_logits_rules', logits.data_ptr(), logits.stride(0) if rows > 1 else 0, out.data_ptr(),
+                   out.stride(0) if rows > 1 else 0, rows, vocab, _LOGITS[logits.dtype], _ptr(met[0]),
+                   0 if met[0] is None else tokens.numel(), *(_ptr(t) for t in met[1:]), _ptr(listed[0]), _ptr(listed[1]),
+                   0 if listed[0] is None else bias.numel(), _ptr(listed[2]), _ptr(masks), words, sets, _ptr(mask_of),
+                   _stream())
 
     # ---- the decoder layers of one token in one launch --------------------------------------
     def decoder_step_supported(self, n_layers, vocab, max_pos, enc_len, prompt=False):

@@ -42,6 +42,7 @@ extern "C" {
 /* Element types of the prompt attention and the 4-bit cache. */
 #define FW_F16 0
 #define FW_BF16 1
+#define FW_F32 2 /* fw_logits_rules alone */
 
 const char* fw_last_error(void);
 int fw_version(void);
@@ -493,6 +494,75 @@ int fw_decode_attention_q4(const void* q, int64_t q_row, int64_t q_head, void* k
                            float scale, float* ws, int64_t ws_floats, hipStream_t stream);
 /* Floats of its workspace (0 for sizes it refuses). */
 int64_t fw_decode_attention_q4_ws_floats(int n_seq, int heads, int kv_heads, int max_len, int head_dim);
+
+/* ---- several answers to one prompt: a key/value cache in pages, and rules on logits (no reference counterpart) ----
+ *
+ * Keys and values are held in n_pages pages of `page` rows (16, 32, 64, 128 or 256), of kv_heads heads of head_dim (64 or
+ * 128) 16-bit elements; both arrays are dense and 16-byte aligned:
+ *   k_pages [n_pages][kv_heads][page][head_dim]
+ *   v_pages [n_pages][kv_heads][page / 8][head_dim][8]   row t, element d at [t / 8][d][t % 8]
+ * Row j of sequence s is row j % page of page table[s][j / page] (int32, device, [n_seq][width]); slot x is row x % page of
+ * page x / page. Sequences may list the same pages: rows that they share are held once.
+ *
+ * fw_kv_page_map brings the tables up to the sequences' lengths. Sequence s holds the pages table[s][0 .. held[s] - 1]; its
+ * cu[s + 1] - cu[s] new packed rows become its rows pos[s] .. (pos, cu, held, own, count, slots: int64, device), and it
+ * wants the pages of rows 0 .. pos[s] + new - 1, at most `width`. Pages that it holds beyond those, from entry own[s] on (own
+ * null: 0), are put on the stack of free pages, stack[0 .. count[0] - 1] (int32, device, room for stack_size), in the order of
+ * sequences and entries; entries before own[s] belong to others and are only dropped. Then pages are taken from the stack's
+ * top, in the same order, while there are any. held_out[s] <- the pages that s holds now; count_out[0] <- the pages on the
+ * stack, count_out[1] <- the pages that were wanted and not there (the stack was empty, or the table is too narrow).
+ * slots[r] <- the slot of packed row r, -1 where it has no page. pos[s] < 0: an idle sequence, which keeps its pages and whose
+ * rows get -1. Rows of slots outside the sequences are left as they are. held_out may be held, and count_out count; a call with
+ * others can be repeated and does the same again. cu ascends; entries outside the rows are clamped to them. width is at most
+ * 2^20. Up to 1024 sequences and 8192 rows take one launch, else two. */
+int fw_kv_page_map(const int64_t* pos, const int64_t* cu, int32_t* table, const int64_t* held, const int64_t* own,
+                   int32_t* stack, const int64_t* count, int64_t* held_out, int64_t* count_out, int64_t* slots, int n_seq,
+                   int width, int64_t stack_size, int64_t rows, int page, hipStream_t stream);
+
+/* Rows r of k and v ([rows, kv_heads, head_dim], 16-bit elements, strides as in fw_prompt_attention) to slot slots[r]
+ * (int64, device). Rows with a slot that there is not (negative, or past the pages) are dropped; every other row of the cache is
+ * left as it is. No slot may occur twice. */
+int fw_kv_page_append(const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head,
+                      const int64_t* slots, int64_t rows, void* k_pages, void* v_pages, int n_pages, int kv_heads, int page,
+                      int head_dim, hipStream_t stream);
+
+/* Attention of one query a sequence over a cache in pages: q, out [n_seq, heads, head_dim] with strides, heads grouped as in
+ * fw_prompt_attention; sequence s attends to its first lens[s] rows (int64, device; at most width x page). One without rows and
+ * an idle one (lens[s] < 0) get zeros. A table entry outside the pages hides its rows, as if they were not there.
+ * The sequences cu_groups[g] .. cu_groups[g + 1] - 1 (int64, device, groups + 1 entries, ascending) form a group, whose first
+ * shared[g] rows (int64, device) are the same, keys and values, in the tables of all its sequences that are not idle: the result
+ * is that of each sequence alone, but those rows are read from the first sequence's table, once for all, as far as the
+ * shortest sequence has them. The first sequence may be idle; its table then lists them all the same. groups 0: cu_groups and
+ * shared may be null. Sequences outside the groups share nothing; starts that do not ascend make no groups.
+ * Scores, softmax and sums are fp32; the weights are rounded to the type for their sum and the product with v, of which fp16
+ * ones below 2^-25 of the largest are lost. Rows that are not seen do not reach the output, whatever they hold; those that are
+ * seen are finite. scale and scores are within the limits of fw_prompt_attention. out overlaps no input. At most 65535 sequences,
+ * 65535 groups, 16384 heads and 2^30 rows a sequence. ws: fw_decode_attention_paged_ws_floats floats, 16-byte aligned,
+ * uninitialised; calls that may overlap need one each. */
+int fw_decode_attention_paged(const void* q, int64_t q_row, int64_t q_head, const void* k_pages, const void* v_pages,
+                              const int32_t* table, const int64_t* lens, const int64_t* cu_groups, const int64_t* shared,
+                              void* out, int64_t o_row, int64_t o_head, int n_seq, int heads, int kv_heads, int n_pages,
+                              int page, int width, int groups, int head_dim, int dtype, float scale, float* ws,
+                              int64_t ws_floats, hipStream_t stream);
+/* Floats of its workspace (0 for sizes it refuses). */
+int64_t fw_decode_attention_paged_ws_floats(int n_seq, int heads, int kv_heads, int width, int page, int groups,
+                                            int head_dim);
+
+/* Rules on logits x [rows, vocab] (FW_F16, FW_BF16 or FW_F32; rows x_row elements apart) into out, of the same type, rows
+ * o_row apart; out may be x itself, else overlaps no input. Of row r and token i, in fp32, in this order, rounded once at the end:
+ *   - i is in the row's history, tokens[cu[r] .. cu[r + 1] - 1] (int64, device): x / repetition[r] if x > 0, else x repetition[r];
+ *   - and c > 0 times among them behind the first prompt[r] (int64; null: 0): x - frequency[r] c - presence[r];
+ *   - i is in the row's list bias_ids[cu_bias[r] .. cu_bias[r + 1] - 1] (int64, device): x + the bias at its last place there;
+ *   - bit i % 32 of word i / 32 of the row's mask is 0: -infinity, whatever x was.
+ * repetition, presence, frequency (fp32, device, [rows]) may be null each: 1, 0, 0. masks: int32, device, n_sets sets of words
+ * mask_row apart; row r has set mask_of[r] (int64, device; one outside the sets: no mask), or without mask_of the only set, or
+ * set r of `rows` or more. tokens (n_tokens of them), bias_ids (n_bias) and masks may be null, then their rule is left out. Ids
+ * outside the vocabulary are passed over; starts are clamped as in fw_prompt_attention. */
+int fw_logits_rules(const void* x, int64_t x_row, void* out, int64_t o_row, int rows, int vocab, int dtype,
+                    const int64_t* tokens, int64_t n_tokens, const int64_t* cu, const int64_t* prompt, const float* repetition,
+                    const float* presence, const float* frequency, const int64_t* bias_ids, const float* bias, int64_t n_bias,
+                    const int64_t* cu_bias, const int32_t* masks, int64_t mask_row, int n_sets, const int64_t* mask_of,
+                    hipStream_t stream);
 
 /* ---- seeded synthetic weights (the random-init N(mean, std) fp16 generator) -------------- */
 

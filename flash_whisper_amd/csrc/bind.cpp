@@ -13,6 +13,10 @@ decltype(&fw_prompt_attention) prompt_attention_entry = nullptr;
 decltype(&fw_kv_q4_append) kv_q4_append_entry = nullptr;
 decltype(&fw_kv_q4_read) kv_q4_read_entry = nullptr;
 decltype(&fw_decode_attention_q4) decode_attention_q4_entry = nullptr;
+decltype(&fw_kv_page_map) kv_page_map_entry = nullptr;
+decltype(&fw_kv_page_append) kv_page_append_entry = nullptr;
+decltype(&fw_decode_attention_paged) decode_attention_paged_entry = nullptr;
+decltype(&fw_logits_rules) logits_rules_entry = nullptr;
 
 // A tensor argument on GPU `dev`, or null.
 const at::Tensor* tensor(PyObject* o, int64_t dev) {
@@ -179,6 +183,156 @@ PyObject* decode_attention_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
       static_cast<int>(c.dim), dtype, scale, static_cast<float*>(ws->data_ptr()), ws->numel(), stream_of(a[9])));
 }
 
+// The contiguous tensor of a type and dimension, or null.
+const at::Tensor* dense(PyObject* o, int64_t dev, at::ScalarType type, int64_t dims) {
+  const at::Tensor* t = tensor(o, dev);
+  return t && t->scalar_type() == type && t->dim() == dims && t->is_contiguous() ? t : nullptr;
+}
+// Data of a contiguous [n] tensor of `type`, or of None; false for anything else.
+template <class P>
+bool optional(PyObject* o, int64_t dev, at::ScalarType type, int64_t n, P*& p) {
+  p = nullptr;
+  if (o == Py_None) return true;
+  const at::Tensor* t = dense(o, dev, type, 1);
+  if (!t || t->size(0) != n) return false;
+  p = static_cast<P*>(t->data_ptr());
+  return true;
+}
+
+// kv_page_map(pos, cu, table, held, stack, count, slots, page, own, held_out, count_out, device, stream)
+PyObject* kv_page_map(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t dev, page;
+  if (n != 13 || !kv_page_map_entry || !integer(a[11], dev) || !integer(a[7], page) || !fits(page)) Py_RETURN_FALSE;
+  const at::Tensor *table = dense(a[2], dev, at::kInt, 2), *stack = dense(a[4], dev, at::kInt, 1), *slots = dense(a[6], dev, at::kLong, 1);
+  if (!table || !stack || !slots) Py_RETURN_FALSE;
+  const int64_t seqs = table->size(0);
+  const int64_t *pos = index(tensor(a[0], dev), seqs), *cu = index(tensor(a[1], dev), seqs + 1), *held = index(tensor(a[3], dev), seqs);
+  const int64_t *count = index(tensor(a[5], dev), 2), *own;
+  int64_t* held_out = const_cast<int64_t*>(a[9] == Py_None ? held : index(tensor(a[9], dev), seqs));
+  int64_t* count_out = const_cast<int64_t*>(a[10] == Py_None ? count : index(tensor(a[10], dev), 2));
+  if (!pos || !cu || !held || !count || !held_out || !count_out || !optional(a[8], dev, at::kLong, seqs, own) || !fits(seqs) ||
+      !fits(table->size(1)))
+    Py_RETURN_FALSE;
+  return made(kv_page_map_entry(pos, cu, static_cast<int32_t*>(table->data_ptr()), held, own, static_cast<int32_t*>(stack->data_ptr()),
+                                count, held_out, count_out, static_cast<int64_t*>(slots->data_ptr()), static_cast<int>(seqs),
+                                static_cast<int>(table->size(1)), stack->size(0), slots->size(0), static_cast<int>(page),
+                                stream_of(a[12])));
+}
+
+struct Pages {
+  void *k, *v;
+  int64_t n, heads, page, dim;
+  at::ScalarType type;
+};
+bool pages(PyObject* o, int64_t dev, Pages& p) {
+  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 2) return false;
+  const at::Tensor* k = tensor(PyTuple_GET_ITEM(o, 0), dev);
+  if (!k || dtype_of(*k) < 0 || k->dim() != 4 || !k->is_contiguous()) return false;
+  p.type = k->scalar_type();
+  const at::Tensor* v = dense(PyTuple_GET_ITEM(o, 1), dev, p.type, 5);
+  p.n = k->size(0);
+  p.heads = k->size(1);
+  p.page = k->size(2);
+  p.dim = k->size(3);
+  if (!v || v->sizes() != at::IntArrayRef({p.n, p.heads, p.page / 8, p.dim, 8}) || !fits(p.n) || !fits(p.heads) || !fits(p.page))
+    return false;
+  p.k = k->data_ptr();
+  p.v = v->data_ptr();
+  return true;
+}
+
+// kv_page_append(k, v, slots, cache, device, stream)
+PyObject* kv_page_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t dev;
+  Pages c;
+  View k, v;
+  if (n != 6 || !kv_page_append_entry || !integer(a[4], dev) || !pages(a[3], dev, c) || !view(tensor(a[0], dev), c.type, c.dim, k) ||
+      !view(tensor(a[1], dev), c.type, c.dim, v) || k.rows != v.rows || k.heads != c.heads || v.heads != c.heads)
+    Py_RETURN_FALSE;
+  const int64_t* slots = index(tensor(a[2], dev), k.rows);
+  if (!slots) Py_RETURN_FALSE;
+  return made(kv_page_append_entry(k.p, k.row, k.head, v.p, v.row, v.head, slots, k.rows, c.k, c.v, static_cast<int>(c.n),
+                                   static_cast<int>(c.heads), static_cast<int>(c.page), static_cast<int>(c.dim), stream_of(a[5])));
+}
+
+// decode_attention_paged(q, cache, table, lens, out, ws, scale, cu_groups, shared, device, stream)
+PyObject* decode_attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t dev;
+  float scale;
+  Pages c;
+  View q, out;
+  if (n != 11 || !decode_attention_paged_entry || !integer(a[9], dev) || !number(a[6], scale) || !pages(a[1], dev, c)) Py_RETURN_FALSE;
+  const at::Tensor *table = dense(a[2], dev, at::kInt, 2), *ws = dense(a[5], dev, at::kFloat, 1);
+  if (!table || !ws || !view(tensor(a[0], dev), c.type, c.dim, q) || !view(tensor(a[4], dev), c.type, c.dim, out) || !apart(out, c.dim) ||
+      out.rows != q.rows || out.heads != q.heads || table->size(0) != q.rows)
+    Py_RETURN_FALSE;
+  const int64_t *lens = index(tensor(a[3], dev), q.rows), *cu = nullptr, *shared = nullptr;
+  int64_t groups = 0;
+  if ((a[7] == Py_None) != (a[8] == Py_None)) Py_RETURN_FALSE;
+  if (a[7] != Py_None) {
+    const at::Tensor* t = dense(a[8], dev, at::kLong, 1);
+    if (!t) Py_RETURN_FALSE;
+    groups = t->size(0);
+    shared = static_cast<const int64_t*>(t->data_ptr());
+    cu = index(tensor(a[7], dev), groups + 1);
+    if (!cu) Py_RETURN_FALSE;
+  }
+  if (!lens || !fits(q.rows) || !fits(q.heads) || !fits(table->size(1)) || !fits(groups)) Py_RETURN_FALSE;
+  return made(decode_attention_paged_entry(
+      q.p, q.row, q.head, c.k, c.v, static_cast<const int32_t*>(table->data_ptr()), lens, cu, shared, out.p, out.row, out.head,
+      static_cast<int>(q.rows), static_cast<int>(q.heads), static_cast<int>(c.heads), static_cast<int>(c.n), static_cast<int>(c.page),
+      static_cast<int>(table->size(1)), static_cast<int>(groups), static_cast<int>(c.dim), c.type == at::kHalf ? FW_F16 : FW_BF16, scale,
+      static_cast<float*>(ws->data_ptr()), ws->numel(), stream_of(a[10])));
+}
+
+// logits_rules(logits, out, tokens, cu, prompt, repetition, presence, frequency, bias_ids, bias, cu_bias, masks, mask_of,
+//              device, stream)
+PyObject* logits_rules(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t dev;
+  if (n != 15 || !logits_rules_entry || !integer(a[13], dev)) Py_RETURN_FALSE;
+  const at::Tensor *x = tensor(a[0], dev), *out = tensor(a[1], dev);
+  if (!x || !out || x->dim() != 2 || x->sizes() != out->sizes() || x->scalar_type() != out->scalar_type()) Py_RETURN_FALSE;
+  const int dtype = x->scalar_type() == at::kFloat ? FW_F32 : dtype_of(*x);
+  const int64_t rows = x->size(0), vocab = x->size(1);
+  if (dtype < 0 || rows == 0 || vocab == 0 || !fits(rows) || !fits(vocab) || (vocab > 1 && (x->stride(1) != 1 || out->stride(1) != 1)) ||
+      (rows > 1 && out->stride(0) < vocab))
+    Py_RETURN_FALSE;
+  const int64_t *tokens = nullptr, *cu = nullptr, *prompt = nullptr, *ids = nullptr, *cu_bias = nullptr, *of = nullptr;
+  const float *repetition = nullptr, *presence = nullptr, *frequency = nullptr, *bias = nullptr;
+  int64_t n_tokens = 0, n_bias = 0, words = 0, sets = 0;
+  const int32_t* masks = nullptr;
+  if (a[2] != Py_None || a[3] != Py_None) {
+    const at::Tensor* t = dense(a[2], dev, at::kLong, 1);
+    if (!t || t->size(0) == 0) Py_RETURN_FALSE;
+    n_tokens = t->size(0);
+    tokens = static_cast<const int64_t*>(t->data_ptr());
+    if (!(cu = index(tensor(a[3], dev), rows + 1))) Py_RETURN_FALSE;
+  }
+  if (!optional(a[4], dev, at::kLong, rows, prompt) || !optional(a[5], dev, at::kFloat, rows, repetition) ||
+      !optional(a[6], dev, at::kFloat, rows, presence) || !optional(a[7], dev, at::kFloat, rows, frequency))
+    Py_RETURN_FALSE;
+  if (a[8] != Py_None || a[9] != Py_None || a[10] != Py_None) {
+    const at::Tensor *t = dense(a[8], dev, at::kLong, 1), *b = dense(a[9], dev, at::kFloat, 1);
+    if (!t || !b || t->size(0) == 0 || b->size(0) != t->size(0)) Py_RETURN_FALSE;
+    n_bias = t->size(0);
+    ids = static_cast<const int64_t*>(t->data_ptr());
+    bias = static_cast<const float*>(b->data_ptr());
+    if (!(cu_bias = index(tensor(a[10], dev), rows + 1))) Py_RETURN_FALSE;
+  }
+  if (a[11] != Py_None) {
+    const at::Tensor* t = dense(a[11], dev, at::kInt, 2);
+    if (!t || t->size(0) == 0 || !fits(t->size(0))) Py_RETURN_FALSE;
+    sets = t->size(0);
+    words = t->size(1);
+    masks = static_cast<const int32_t*>(t->data_ptr());
+  }
+  if (!optional(a[12], dev, at::kLong, rows, of)) Py_RETURN_FALSE;
+  return made(logits_rules_entry(x->data_ptr(), rows > 1 ? x->stride(0) : 0, out->data_ptr(), rows > 1 ? out->stride(0) : 0,
+                                 static_cast<int>(rows), static_cast<int>(vocab), dtype, tokens, n_tokens, cu, prompt, repetition,
+                                 presence, frequency, ids, bias, n_bias, cu_bias, masks, words, static_cast<int>(sets), of,
+                                 stream_of(a[14])));
+}
+
 // set_entry(name, address)
 PyObject* set_entry(PyObject*, PyObject* args) {
   const char* name;
@@ -189,6 +343,10 @@ PyObject* set_entry(PyObject*, PyObject* args) {
   else if (is("fw_kv_q4_append")) kv_q4_append_entry = reinterpret_cast<decltype(&fw_kv_q4_append)>(address);
   else if (is("fw_kv_q4_read")) kv_q4_read_entry = reinterpret_cast<decltype(&fw_kv_q4_read)>(address);
   else if (is("fw_decode_attention_q4")) decode_attention_q4_entry = reinterpret_cast<decltype(&fw_decode_attention_q4)>(address);
+  else if (is("fw_kv_page_map")) kv_page_map_entry = reinterpret_cast<decltype(&fw_kv_page_map)>(address);
+  else if (is("fw_kv_page_append")) kv_page_append_entry = reinterpret_cast<decltype(&fw_kv_page_append)>(address);
+  else if (is("fw_decode_attention_paged")) decode_attention_paged_entry = reinterpret_cast<decltype(&fw_decode_attention_paged)>(address);
+  else if (is("fw_logits_rules")) logits_rules_entry = reinterpret_cast<decltype(&fw_logits_rules)>(address);
   else return PyErr_Format(PyExc_ValueError, "no entry point %s", name);
   Py_RETURN_NONE;
 }
@@ -205,6 +363,7 @@ PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
 
 #define FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<f>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(prompt_attention), FAST(kv_q4_append), FAST(kv_q4_read), FAST(decode_attention_q4),
+                         FAST(kv_page_map), FAST(kv_page_append), FAST(decode_attention_paged), FAST(logits_rules),
                          {"set_entry", set_entry, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bind", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

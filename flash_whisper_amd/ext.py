@@ -231,7 +231,8 @@ class WhisperExt:
         self.lib = _lib.lib()
         self._bind = _bind
         if _bind is not None:
-            for name in ('fw_prompt_attention', 'fw_kv_q4_append', 'fw_kv_q4_read', 'fw_decode_attention_q4'):
+            for name in ('fw_prompt_attention', 'fw_kv_q4_append', 'fw_kv_q4_read', 'fw_decode_attention_q4', 'fw_kv_page_map',
+                         'fw_kv_page_append', 'fw_decode_attention_paged', 'fw_logits_rules'):
                 _bind.set_entry(name, ctypes.cast(getattr(self.lib, name), ctypes.c_void_p).value)
 
     def _call(self, name, *args):
@@ -575,6 +576,9 @@ class WhisperExt:
         are taken from its top; slots[r] (int64) is the place of packed row r, -1 where it has none. held_out and count_out
         default to held and count."""
         dev = _current_device()
+        if self._bind and dev is not None and self._bind.kv_page_map(pos, cu, table, held, stack, count, slots, page, own, held_out,
+                                                                    count_out, dev, _raw_stream(dev)):
+            return
         _dense(table, 'table', _I32, (None, None), dev)
         n, width = table.shape
         held_out, count_out = held if held_out is None else held_out, count if count_out is None else count_out
@@ -594,6 +598,8 @@ class WhisperExt:
         """Writes rows r of k and v ([rows, kv_heads, head_dim] of the cache's type) to slot slots[r] (int64) of a cache in
         pages (fw_kv_page_append). Rows whose slot is negative or past the pages are dropped; no slot may occur twice."""
         dev = _current_device()
+        if self._bind and dev is not None and self._bind.kv_page_append(k, v, slots, cache, dev, _raw_stream(dev)):
+            return
         n, heads, page, dim, dtype = _page_sizes(cache, dev)
         strides = (*_heads_view(k, 'k', dtype, dev, heads, dim), *_heads_view(v, 'v', dtype, dev, heads, dim))
         if k.size(0) != v.size(0):
@@ -619,6 +625,9 @@ class WhisperExt:
         zeros. The sequences cu_groups[g] .. cu_groups[g + 1] - 1 have their first shared[g] rows in common (int64): these are
         read once for all of them, from the first one's table."""
         dev = _current_device()
+        if self._bind and dev is not None and self._bind.decode_attention_paged(q, cache, table, lens, out, ws, scale, cu_groups,
+                                                                               shared, dev, _raw_stream(dev)):
+            return
         n_pages, kv_heads, page, dim, dtype = _page_sizes(cache, dev)
         q_row, q_head = _heads_view(q, 'q', dtype, dev, None, dim)
         n, heads = q.size(0), q.size(1)
@@ -649,6 +658,10 @@ class WhisperExt:
         cu_bias[r + 1] (of a token's, the last), and tokens whose bit in the row's mask (int32 [sets, words], bit i % 32 of
         word i / 32; set mask_of[r], -1: none; without mask_of one for all or for each row) is 0 get -infinity."""
         dev = _current_device()
+        if self._bind and dev is not None and self._bind.logits_rules(logits, out, tokens, cu, prompt, repetition, presence, frequency,
+                                                                     bias_ids, bias, cu_bias, masks, mask_of, dev,
+                                                                     _raw_stream(dev)):
+            return
         for t, name in ((logits, 'logits'), (out, 'out')):
             if not (isinstance(t, torch.Tensor) and t.dtype in _LOGITS and t.dtype is logits.dtype and t.get_device() == dev
                     and t.dim() == 2 and t.size(1) > 0 and (t.stride(1) == 1 or t.size(1) == 1 or t.size(0) == 0)):

@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "lds_pipe.h"
 #include "packed_rows.h"
 #include "pages.h"
 
@@ -57,10 +58,10 @@ struct PagedArgs {
   const int64_t *lens, *cu_g, *shared;
   int n_seq, heads, kv_heads, groups, width, n_pages, page_shift;
   float scale;
-  int cols;           // columns of a piece of a group's shared keys, at most
+  int cols;           // columns of a piece of a group's shared keys, at most: 16, or 64 or 128 in wide ones
   int want;           // pieces that all keys are to make, about
   int most;           // pieces there may be; 0: each sequence is a piece, and nothing is shared
-  int* plan;          // Header, Pieces, Owners, Groups, the group of each sequence
+  int* plan;          // Header, Pieces, Owners, and the plan's arrays where LDS does not hold them
   float *part, *ml;   // O [slot][kv head][16][D], (m, l) [slot][kv head][16][2]
 };
 
@@ -79,12 +80,6 @@ struct __align__(16) Piece {
 struct __align__(16) Owner {
   int shared_slot, shared_n, shared_step, col;
   int slot, n;
-  int pad[2];
-};
-// A group's shared rows, its first sequence, and where the pieces of its shared keys leave their results.
-struct __align__(16) Group {
-  int rows, begin, slot, n;
-  int step, whole;  // whole: no sequence of it sees more
   int pad[2];
 };
 struct __align__(16) Header {
@@ -318,13 +313,127 @@ __device__ __forceinline__ void paged_piece(const PagedArgs& a, const Piece& p, 
   }
 }
 
-// Direct: a block for each sequence, key/value head and 16 of its columns. Else a block for each piece and key/value head.
+// A piece of many columns: wave w has columns 16 CT w .. and all of the keys, which arrive in LDS by direct copies, a ring of
+// kStages tiles, so that a row of K and V is read once for 64 CT columns. A tile of a page is contiguous, V's just as the operands
+// are read; K's 16-byte chunks are swapped within a row so that the 16 rows of a read lie in different banks.
+constexpr int kStages = 4, kWaves = 4;
+template <int D>
+__device__ __forceinline__ int wide_swap(int row) {
+  return D == 128 ? (row & 3) | ((row >> 3) & 3) << 2 : ((row >> 1) & 1) | ((row >> 3) & 3) << 1;
+}
+
 template <class T, int D, int CT>
-__global__ void __launch_bounds__(512, 2) paged_attention_kernel(PagedArgs a) {
-  extern __shared__ float lds[];
+__device__ __forceinline__ void paged_wide(const PagedArgs& a, const Piece& p, int kvh, const int32_t* table, float* lds) {
+  typedef typename Types<T>::v8 v8;
+  typedef __attribute__((address_space(3))) v8 lds_v8;
+  constexpr int kHalf = kTileKeys * D * 2, kStage = 2 * kHalf;  // bytes of a tile of K or V, of both
+  constexpr int kCopies = kHalf / 1024 / kWaves;                // of K, and of V, a wave
+  constexpr int kRowBytes = 2 * D, kCopyRows = 1024 / kRowBytes;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = lane & 15, g = lane >> 4, group = a.heads / a.kv_heads, col0 = kCols * CT * wave;
+  const bool live = col0 < p.cols;
+  const uint32_t ring = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
+  const int first = p.begin / kTileKeys, tiles = (p.end + kTileKeys - 1) / kTileKeys - first, rows = 1 << a.page_shift;
+  PagedPages pages = paged_pages(a, table, first + lane, p.end);
+  uint32_t ok = 0;  // two bits a stage: the pages of its tile's halves
+  const auto issue = [&](int n) {
+    if (n && (n & 63) == 0) pages = paged_pages(a, table, first + n + lane, p.end);
+    const int lo = __builtin_amdgcn_readlane(pages.lo, n & 63), hi = __builtin_amdgcn_readlane(pages.hi, n & 63), s = n % kStages;
+    ok = (ok & ~(3u << (2 * s))) | static_cast<uint32_t>((lo >= 0) | (hi >= 0) << 1) << (2 * s);
+    const uint32_t to = ring + s * kStage;
+    const int row = ((first + n) * kTileKeys) & (rows - 1);
+    const int64_t at_lo = ((static_cast<int64_t>(max(lo, 0)) * a.kv_heads + kvh) * rows + row) * kRowBytes;
+    // (a page of 16 rows: the second half begins another page's rows)
+    const int64_t at_hi = a.page_shift == 4 ? (static_cast<int64_t>(max(hi, 0)) * a.kv_heads + kvh) * rows * kRowBytes - kHalf / 2 : at_lo;
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) {
+      const int blk = kCopies * wave + c, r = blk * kCopyRows + lane / (D / 8), chunk = (lane % (D / 8)) ^ wide_swap<D>(r);
+      const int64_t at = blk * 1024 < kHalf / 2 ? at_lo : at_hi;
+      dma16_s(static_cast<uint32_t>(r * kRowBytes + chunk * 16), static_cast<const uint8_t*>(a.k) + at, to + blk * 1024);
+      dma16_s(static_cast<uint32_t>(blk * 1024 + lane * 16), static_cast<const uint8_t*>(a.v) + at, to + kHalf + blk * 1024);
+    }
+  };
+#pragma unroll
+  for (int n = 0; n < kStages - 1; ++n)
+    if (n < tiles) issue(n);
+  v8 q[CT][D / 32];
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    const int col = p.col + min(col0 + kCols * c + i, p.cols - 1);  // columns past the end repeat the last one
+    const T* at = static_cast<const T*>(a.q) + (p.seq + col / group) * a.q_row + (kvh * group + col % group) * a.q_head + 8 * g;
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+      q[c][j] = *reinterpret_cast<const v8*>(at + 32 * j);
+      if (a.scale < 0.f) q[c][j] = -q[c][j];
+    }
+  }
+  const float factor = fmaxf(__builtin_fabsf(a.scale) * kLog2e, __FLT_DENORM_MIN__);
+  PagedState<T, D, CT> st;
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) st.o[c][db] = f4v{0.f, 0.f, 0.f, 0.f};
+    st.m[c] = -INFINITY;
+    st.l[c] = 0.f;
+  }
+  const uint32_t k_row = (8 * (i >> 2) + (i & 3)) * kRowBytes, v_at = kHalf + (g * D + i) * 16;
+  for (int n = 0; n < tiles; ++n) {
+    // tile n visible to every wave, every one done with tile n - 1, whose place tile n + kStages - 1 takes
+    wait_stages_ahead<2 * kCopies, kStages - 1>(min(kStages - 2, tiles - 1 - n));
+    lds_barrier();
+    const uint32_t at = ring + n % kStages * kStage, has = (ok >> (2 * (n % kStages))) & 3;
+    if (n + kStages - 1 < tiles) issue(n + kStages - 1);
+    if (!live) continue;
+    PagedTile<T, D> x;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j)
+        x.k[kt][j] = *reinterpret_cast<lds_v8*>(
+            static_cast<uintptr_t>(at + k_row + 4 * kt * kRowBytes + ((4 * j + g) ^ wide_swap<D>(8 * (i >> 2) + (i & 3))) * 16));
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) x.v[db] = *reinterpret_cast<lds_v8*>(static_cast<uintptr_t>(at + v_at + db * 256));
+    f4v s[CT][2];
+    paged_scores<T, D, CT>(x, q, s);
+    const int left = p.end - (first + n) * kTileKeys;
+    if (left >= kTileKeys && has == 3) paged_values<T, D, CT, false>(x, s, factor, 8, st);
+    else paged_values<T, D, CT, true>(x, s, factor, has >> (lane >> 5) & 1 ? left - 8 * g : 0, st);
+  }
+  if (!live) return;
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    const float l = xor_add<32>(xor_add<16>(st.l[c]));
+    const int col = col0 + kCols * c + i;
+    if (col >= p.cols) continue;
+    if (p.slot < 0) {
+      typedef T v4 __attribute__((ext_vector_type(4)));
+      const int seq = p.seq + (p.col + col) / group, head = kvh * group + (p.col + col) % group;
+      const float inv = l == 0.f || a.lens[seq] <= 0 ? 0.f : 1.0f / l;
+      T* to = static_cast<T*>(a.out) + seq * a.o_row + head * a.o_head + 4 * g;
+#pragma unroll
+      for (int db = 0; db < D / 16; ++db) {
+        v4 y;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[r] = static_cast<T>(inv == 0.f ? 0.f : st.o[c][db][r] * inv);
+        *reinterpret_cast<v4*>(to + 16 * db) = y;
+      }
+    } else {
+      const int64_t to = (static_cast<int64_t>(p.slot + col / kCols) * a.kv_heads + kvh) * kCols + i;
+      if (g == 0) *reinterpret_cast<float2*>(a.ml + 2 * to) = make_float2(st.m[c], l);
+#pragma unroll
+      for (int db = 0; db < D / 16; ++db) *reinterpret_cast<f4v*>(a.part + to * D + 16 * db + 4 * g) = st.o[c][db];
+    }
+  }
+}
+
+// CT < 0: a block for each sequence, key/value head and 16 of its columns. Else a block for each piece and key/value head; CT > 0:
+// those of more than 16 columns are wide.
+template <class T, int D, int CT>
+__global__ void __launch_bounds__(CT < 0 ? 512 : 64 * kWaves, 2) paged_attention_kernel(PagedArgs a) {
+  extern __shared__ __align__(1024) float lds[];
   const int kvh = blockIdx.x % a.kv_heads;
   const unsigned at = blockIdx.x / a.kv_heads;
-  if constexpr (CT == 0) {
+  if constexpr (CT < 0) {
     const int group = a.heads / a.kv_heads, parts = (group + kCols - 1) / kCols, col = static_cast<int>(at % parts) * kCols;
     const int seq = static_cast<int>(at / parts);
     const Piece p{seq, col, min(kCols, group - col), 0, paged_keys(a, seq), -1, {}};
@@ -333,25 +442,31 @@ __global__ void __launch_bounds__(512, 2) paged_attention_kernel(PagedArgs a) {
     if (static_cast<int>(at) >= reinterpret_cast<const Header*>(a.plan)->pieces) return;
     const Piece p = (reinterpret_cast<const Piece*>(a.plan + 4))[at];
     const int32_t* table = a.table + static_cast<int64_t>(p.seq) * a.width;
-    if (CT == 1 || p.cols <= kCols) paged_piece<T, D, 1>(a, p, kvh, table, lds);
-    else paged_piece<T, D, CT>(a, p, kvh, table, lds);
+    if constexpr (CT > 0) {
+      if (p.cols > kCols) {
+        paged_wide<T, D, CT>(a, p, kvh, table, lds);
+        return;
+      }
+    }
+    paged_piece<T, D, 1>(a, p, kvh, table, lds);
   }
 }
 
 // ------------------------------------------------------------------------------------------
 // The plan: one block turns the lengths into pieces. A group's shared rows are those that all its live sequences have, cut to
 // whole tiles unless they are all that any of them has. All keys, times the runs of columns that see them, make about `want`
-// pieces, a multiple of a tile for each wave; the pieces of one run of keys are alike.
+// pieces, a multiple of a tile for each wave; the pieces of one run of keys are alike, those of groups come first. Bound by
+// latency: up to kPlanLds sequences and groups everything but the lengths and the pieces stays in LDS.
 // ------------------------------------------------------------------------------------------
-constexpr int kPlanThreads = 1024, kSerial = 32;
+constexpr int kPlanThreads = 1024, kPlanLds = 1024;
 
 __device__ __forceinline__ int64_t plan_sum(int64_t v, int64_t* part) {
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
-  __syncthreads();
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
   __syncthreads();
   v = 0;
+#pragma unroll
   for (int w = 0; w < kPlanThreads / 64; ++w) v += part[w];
   return v;
 }
@@ -367,6 +482,7 @@ __device__ __forceinline__ int plan_scan(int v, int* part, int& total) {
   if (lane == 63) part[wave] = v;
   __syncthreads();
   total = 0;
+#pragma unroll
   for (int w = 0; w < kPlanThreads / 64; ++w) {
     if (w < wave) v += part[w];
     total += part[w];
@@ -374,147 +490,128 @@ __device__ __forceinline__ int plan_scan(int v, int* part, int& total) {
   return v - mine;
 }
 
-struct Members {
-  int begin, end;
-};
-__device__ __forceinline__ Members members_of(const PagedArgs& a, int g) {
-  const int64_t b = within(a.cu_g[g], 0, a.n_seq);
-  return Members{static_cast<int>(b), static_cast<int>(within(a.cu_g[g + 1], b, a.n_seq))};
-}
-// Shared rows of a group whose live sequences have `low` to `high` keys (high 0: none is live, or none has keys).
-__device__ __forceinline__ int shared_rows(const PagedArgs& a, int g, int low, int high) {
-  if (high <= 0) return 0;
-  const int64_t most = within(a.shared[g], 0, low);
-  return static_cast<int>(most == high ? most : most & ~int64_t{kTileKeys - 1});
-}
-// Keys of one piece, of `keys` in pieces of at most `chunk`.
-__device__ __forceinline__ int piece_keys(int keys, int n) {
-  return n ? ((keys + n - 1) / n + kTileKeys - 1) / kTileKeys * kTileKeys : 0;
+// The last of n ascending values that is <= x, or -1.
+__device__ __forceinline__ int plan_find(const int* at, int n, int x) {
+  int lo = -1, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (at[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedArgs a, int unit) {
+// Words of the plan's arrays: keys, groups of n sequences; starts, rows, low, high of the groups; the first piece of each.
+__host__ __device__ constexpr int64_t plan_words(int64_t n, int64_t groups) { return 2 * n + 4 * groups + 1 + (n + groups + 1); }
+
+__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedArgs a, int unit, int weight) {
   __shared__ int64_t sums[kPlanThreads / 64];
-  __shared__ int scans[kPlanThreads / 64];
-  const int tid = threadIdx.x, lane = tid & 63, group = a.heads / a.kv_heads, parts = (group + kCols - 1) / kCols;
+  __shared__ int scans[kPlanThreads / 64], local[plan_words(kPlanLds, kPlanLds)];
+  const int tid = threadIdx.x, n_seq = a.n_seq, group = a.heads / a.kv_heads, parts = (group + kCols - 1) / kCols;
   Piece* pieces = reinterpret_cast<Piece*>(a.plan + 4);
   Owner* owners = reinterpret_cast<Owner*>(pieces + a.most);
-  Group* of = reinterpret_cast<Group*>(owners + a.n_seq);
-  int* group_of = reinterpret_cast<int*>(of + a.groups);  // by sequence; -1: none, or nothing is shared
-  for (int s = tid; s < a.n_seq; s += kPlanThreads) group_of[s] = -1;
-  // groups whose starts do not ascend would overlap: none is one
-  int descends = 0;
-  for (int g = tid; g < a.groups; g += kPlanThreads) descends |= a.cu_g[g] > a.cu_g[g + 1];
+  int* keys = n_seq <= kPlanLds && a.groups <= kPlanLds ? local : reinterpret_cast<int*>(owners + n_seq);  // -1: idle
+  int *of = keys + n_seq, *starts = of + n_seq, *rows = starts + a.groups + 1;
+  int *low = rows + a.groups, *high = low + a.groups, *before = high + a.groups;
+  for (int s = tid; s < n_seq; s += kPlanThreads) keys[s] = a.lens[s] < 0 ? -1 : paged_keys(a, s);
+  int descends = 0;  // groups whose starts do not ascend would overlap: none is one
+  for (int g = tid; g <= a.groups && a.groups; g += kPlanThreads) {
+    const int64_t start = a.cu_g[g];
+    starts[g] = static_cast<int>(within(start, 0, n_seq));
+    if (g == a.groups) break;
+    descends |= start > a.cu_g[g + 1];
+    rows[g] = static_cast<int>(within(a.shared[g], 0, 1 << 30));
+    low[g] = 0x7FFFFFFF;
+    high[g] = 0;
+  }
   const int groups = __syncthreads_or(descends) ? 0 : a.groups;
-  // shared rows of every group: the sequences of a small group by a thread, of a large one by a wave
-  int64_t work = 0;
-  const auto runs_of = [&](const Members& m) { return ((m.end - m.begin) * group + a.cols - 1) / a.cols; };
-  for (int g0 = tid & ~63; g0 < groups; g0 += kPlanThreads) {
-    const int g = g0 + lane;
-    Members m{0, 0};
-    int low = 0x7FFFFFFF, high = 0;
-    if (g < groups) m = members_of(a, g);
-    const int count = m.end - m.begin;
-    for (int s = m.begin; count <= kSerial && s < m.end; ++s) {
-      if (a.lens[s] < 0) continue;
-      const int keys = paged_keys(a, s);
-      low = min(low, keys);
-      high = max(high, keys);
+  // the fewest and most keys of a group's live sequences; a wave of one group asks once
+  for (int s0 = tid & ~63; s0 < n_seq; s0 += kPlanThreads) {
+    const int s = s0 + (tid & 63);
+    int g = -1, lo = 0x7FFFFFFF, hi = 0;
+    if (s < n_seq) {
+      g = plan_find(starts, groups, s);
+      if (g >= 0 && s >= starts[g + 1]) g = -1;
+      of[s] = g;
+      if (keys[s] >= 0) lo = hi = keys[s];
     }
-    for (uint64_t big = __builtin_amdgcn_ballot_w64(count > kSerial); big; big &= big - 1) {
-      const int l = __builtin_ctzll(big), b = __builtin_amdgcn_readlane(m.begin, l), e = __builtin_amdgcn_readlane(m.end, l);
-      int lo = 0x7FFFFFFF, hi = 0;
-      for (int s = b + lane; s < e; s += 64) {
-        if (a.lens[s] < 0) continue;
-        const int keys = paged_keys(a, s);
-        lo = min(lo, keys);
-        hi = max(hi, keys);
-      }
+    const int one = __builtin_amdgcn_readfirstlane(g);
+    if (__builtin_amdgcn_ballot_w64(g == one) == __builtin_amdgcn_ballot_w64(true)) {
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
         lo = min(lo, __shfl_xor(lo, o));
         hi = max(hi, __shfl_xor(hi, o));
       }
-      if (lane == l) {
-        low = lo;
-        high = hi;
-      }
+      if ((tid & 63) != 0) g = -1;
     }
-    const int rows = g < groups && count > 1 ? shared_rows(a, g, low, high) : 0;
-    if (g < groups) of[g] = Group{rows, m.begin, -1, 0, 0, rows == high, {}};
-    work += static_cast<int64_t>(rows) * runs_of(m);
-    if (rows && count <= kSerial)
-      for (int s = m.begin; s < m.end; ++s) group_of[s] = g;
-    for (uint64_t big = __builtin_amdgcn_ballot_w64(rows && count > kSerial); big; big &= big - 1) {
-      const int l = __builtin_ctzll(big), b = __builtin_amdgcn_readlane(m.begin, l), e = __builtin_amdgcn_readlane(m.end, l);
-      for (int s = b + lane; s < e; s += 64) group_of[s] = g0 + l;
+    if (g >= 0) {
+      atomicMin(&low[g], lo);
+      atomicMax(&high[g], hi);
     }
   }
   __syncthreads();
-  const auto shared_of = [&](int s) { return group_of[s] < 0 ? 0 : of[group_of[s]].rows; };
-  for (int s = tid; s < a.n_seq; s += kPlanThreads) work += static_cast<int64_t>(max(paged_keys(a, s) - shared_of(s), 0)) * parts;
+  int64_t work = 0;
+  const int wide = a.cols > kCols ? weight : 1;  // a wide piece's tile takes so many of others
+  const auto runs_of = [&](int g) { return ((starts[g + 1] - starts[g]) * group + a.cols - 1) / a.cols; };
+  for (int g = tid; g < groups; g += kPlanThreads) {
+    const int most = starts[g + 1] - starts[g] > 1 && high[g] > 0 ? min(rows[g], low[g]) : 0, whole = most == high[g];
+    rows[g] = whole ? most : most & ~(kTileKeys - 1);
+    low[g] = whole;  // from here on: whether no sequence of it sees more
+    work += static_cast<int64_t>(rows[g]) * runs_of(g) * wide;
+  }
+  __syncthreads();
+  const auto begin_of = [&](int s) { return of[s] < 0 ? 0 : rows[of[s]]; };
+  for (int s = tid; s < n_seq; s += kPlanThreads) work += static_cast<int64_t>(max(keys[s] - begin_of(s), 0)) * parts;
   work = plan_sum(work, sums);
-  const int64_t chunk = (work / a.want / unit + 1) * unit;
-  const auto count_of = [&](int keys) { return static_cast<int>((keys + chunk - 1) / chunk); };
-  // pieces of the groups, then of the sequences
-  int next = 0, slot = 0;
-  const int tiles = a.cols / kCols;
-  for (int g0 = 0; g0 < groups; g0 += kPlanThreads) {
-    const int g = g0 + tid;
-    Group x{};
-    Members m{0, 0};
-    int runs = 0;
-    if (g < groups) {
-      m = members_of(a, g);
-      x = of[g];
-      x.n = count_of(x.rows);
-      runs = x.n ? runs_of(m) : 0;
-    }
-    const bool whole = x.whole && x.n == 1;
-    int total;
-    const int before = plan_scan(x.n * runs, scans, total), size = piece_keys(x.rows, x.n);
-    for (int y = 0; y < x.n * runs; ++y) {
-      const int i = y / runs, r = y % runs, at = next + before + y, left = (m.end - m.begin) * group - r * a.cols;
-      if (at < a.most)
-        pieces[at] = Piece{m.begin, r * a.cols, min(a.cols, left), i * size, min((i + 1) * size, x.rows),
-                           whole ? -1 : slot + (before + y) * tiles, {}};
-    }
-    if (g < groups) {
-      x.slot = whole ? -1 : slot + before * tiles;
-      x.step = runs * tiles;
-      of[g] = x;
-    }
-    next += total;
-    slot += total * tiles;
+  const uint32_t chunk = static_cast<uint32_t>(min((work / a.want / unit + 1) * unit, int64_t{1} << 30));
+  const uint32_t shared_chunk = (chunk / wide + kTileKeys - 1) / kTileKeys * kTileKeys;
+  const auto count = [](int x, uint32_t each) { return static_cast<int>((x + each - 1) / each); };
+  // pieces of the groups, then of the sequences; one without keys has one, for its zeros
+  int pieces_n = 0;
+  for (int e0 = 0; e0 < groups + n_seq; e0 += kPlanThreads) {
+    const int e = e0 + tid, s = e - groups;
+    int n = 0, total;
+    if (s < 0) n = count(rows[e], shared_chunk) * runs_of(e);
+    else if (s < n_seq) n = max(count(max(keys[s] - begin_of(s), 0), chunk), begin_of(s) == 0) * parts;
+    const int sum = plan_scan(n, scans, total);
+    if (s < n_seq) before[e] = pieces_n + sum;
+    pieces_n += total;
   }
+  if (tid == 0) before[groups + n_seq] = pieces_n;
   __syncthreads();
-  for (int s0 = 0; s0 < a.n_seq; s0 += kPlanThreads) {
-    const int s = s0 + tid;
-    Owner o{};
-    int keys = 0, begin = 0;
-    if (s < a.n_seq) {
-      if (group_of[s] >= 0) {
-        const Group x = of[group_of[s]];
-        begin = x.rows;
-        o = Owner{x.slot, x.n, x.step, (s - x.begin) * group, 0, 0, {}};
-      }
-      keys = max(paged_keys(a, s) - begin, 0);
-      o.n = count_of(keys);
-      if (begin == 0 && o.n == 0) o.n = 1;  // its zeros
+  const int of_groups = before[groups], tiles = a.cols / kCols;
+  // a piece of a group has `tiles` slots, one of a sequence has one
+  const auto slot_of = [&](int at) { return at < of_groups ? at * tiles : of_groups * tiles + (at - of_groups); };
+  for (int at = tid; at < min(pieces_n, a.most); at += kPlanThreads) {
+    const int e = plan_find(before, groups + n_seq, at), s = e - groups, x = at - before[e];
+    Piece p;
+    if (s < 0) {
+      const int n = count(rows[e], shared_chunk), runs = runs_of(e), i = x / runs, r = x % runs;
+      const int size = ((rows[e] + n - 1) / n + kTileKeys - 1) / kTileKeys * kTileKeys;
+      p = Piece{starts[e], r * a.cols, min(a.cols, (starts[e + 1] - starts[e]) * group - r * a.cols), i * size,
+                min((i + 1) * size, rows[e]), low[e] && n == 1 ? -1 : slot_of(at), {}};
+    } else {
+      const int n = (before[e + 1] - before[e]) / parts, begin = begin_of(s), mine = max(keys[s] - begin, 0), i = x / parts, r = x % parts;
+      const int size = ((mine + n - 1) / n + kTileKeys - 1) / kTileKeys * kTileKeys;
+      p = Piece{s, r * kCols, min(kCols, group - r * kCols), begin + i * size, begin + min((i + 1) * size, mine),
+                begin == 0 && n == 1 ? -1 : slot_of(at), {}};
     }
-    int total;
-    const int before = plan_scan(o.n * parts, scans, total), size = piece_keys(keys, o.n);
-    o.slot = begin == 0 && o.n == 1 ? -1 : slot + before;
-    for (int y = 0; y < o.n * parts; ++y) {
-      const int i = y / parts, r = y % parts, at = next + before + y;
-      if (at < a.most)
-        pieces[at] = Piece{s, r * kCols, min(kCols, group - r * kCols), begin + i * size, begin + min((i + 1) * size, keys),
-                           o.slot < 0 ? -1 : o.slot + y, {}};
-    }
-    if (s < a.n_seq) owners[s] = o;
-    next += total;
-    slot += total;
+    pieces[at] = p;
   }
-  if (tid == 0) reinterpret_cast<Header*>(a.plan)->pieces = min(next, a.most);
+  for (int s = tid; s < n_seq; s += kPlanThreads) {
+    Owner o{};
+    const int g = of[s], begin = begin_of(s), e = groups + s;
+    if (begin) {
+      o.shared_n = count(rows[g], shared_chunk);
+      o.shared_slot = low[g] && o.shared_n == 1 ? -1 : slot_of(before[g]);
+      o.shared_step = runs_of(g) * tiles;
+      o.col = (s - starts[g]) * group;
+    }
+    o.n = (before[e + 1] - before[e]) / parts;
+    o.slot = begin == 0 && o.n == 1 ? -1 : slot_of(before[e]);
+    owners[s] = o;
+  }
+  if (tid == 0) reinterpret_cast<Header*>(a.plan)->pieces = min(pieces_n, a.most);
 }
 
 // Joins what the pieces of a sequence left: block = (query head, sequence).
@@ -587,18 +684,19 @@ PagedSizes paged_sizes(int n_seq, int heads, int kv_heads, int64_t capacity, int
   PagedSizes p = {};
   const int64_t group = heads / kv_heads, parts = (group + kCols - 1) / kCols;
   p.direct_waves = static_cast<int>(std::min<int64_t>(8, (capacity + kTileKeys - 1) / kTileKeys));
-  p.waves = 4;
+  p.waves = kWaves;
   if (capacity <= kDirectRows) {
     p.floats = 4;
     return p;
   }
-  p.cols = groups && (n_seq + groups - 1) / groups * group > kCols ? 2 * kCols : kCols;
+  const int64_t columns = groups ? (n_seq + groups - 1) / groups * group : 0;  // of an average group
+  p.cols = columns > 64 ? 128 : columns > kCols ? 64 : kCols;
   p.want = std::max(1, kWantBlocks / kv_heads);
   // each run of columns has the pieces that fill its share of `want`, and one more
   const int64_t runs = groups ? n_seq * group / p.cols + groups : 0;
   p.most = p.want + runs + n_seq * parts + 1;
   p.slots = p.cols / kCols * (p.want + runs) + n_seq * parts + 1;
-  p.ints = 4 + 8 * p.most + 8 * static_cast<int64_t>(n_seq) + 8 * static_cast<int64_t>(groups) + n_seq;
+  p.ints = 4 + 8 * p.most + 8 * static_cast<int64_t>(n_seq) + (n_seq <= kPlanLds && groups <= kPlanLds ? 0 : plan_words(n_seq, groups));
   p.ints = (p.ints + 3) / 4 * 4;
   p.floats = p.ints + p.slots * kv_heads * kCols * (dim + 2);
   return p;
@@ -657,16 +755,17 @@ extern "C" int fw_decode_attention_paged(const void* q, int64_t q_row, int64_t q
               groups, width, n_pages, page_shift_of(page), scale, p.cols, p.want, static_cast<int>(p.most),
               reinterpret_cast<int*>(ws), ws + p.ints, nullptr};
   a.ml = a.part + p.slots * kv_heads * kCols * head_dim;
-  const int lds = head_dim == 64 ? PagedMerge<64>::bytes(waves, cols) : PagedMerge<128>::bytes(waves, cols);
+  int lds = head_dim == 64 ? PagedMerge<64>::bytes(waves, cols) : PagedMerge<128>::bytes(waves, cols);
+  if (p.cols > kCols) lds = std::max(lds, kStages * 2 * kTileKeys * head_dim * 2);
   if (p.most) {
-    hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, a, kTileKeys * waves);
+    hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, a, kTileKeys * waves, p.cols > 64 ? 3 : 2);
     if (const int rc = fw_check_launch(what)) return rc;
   }
   const auto run = [&](auto t, auto d) {
     typedef decltype(t) T;
     constexpr int D = decltype(d)::value;
-    const auto kernel = !p.most ? paged_attention_kernel<T, D, 0>
-                        : p.cols == kCols ? paged_attention_kernel<T, D, 1> : paged_attention_kernel<T, D, 2>;
+    const auto kernel = !p.most ? paged_attention_kernel<T, D, -1> : p.cols == kCols ? paged_attention_kernel<T, D, 0>
+                        : p.cols == 64 ? paged_attention_kernel<T, D, 1> : paged_attention_kernel<T, D, 2>;
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(64 * waves), lds, stream, a);
     if (const int rc = fw_check_launch(what)) return rc;
     if (!p.most) return static_cast<int>(FW_OK);

@@ -60,6 +60,8 @@ struct PagedArgs {
   float scale;
   int cols;           // columns of a piece of a group's shared keys, at most: 16, or 64 or 128 in wide ones
   int want;           // pieces that all keys are to make, about
+  uint32_t unit, least;  // what a chunk of keys is a multiple of, and at least
+  int weight;         // what a tile takes in a piece of a group, of what it takes in others
   int most;           // pieces there may be; 0: each sequence is a piece, and nothing is shared
   int* plan;          // Header, Pieces, Owners, and the plan's arrays where LDS does not hold them
   float *part, *ml;   // O [slot][kv head][16][D], (m, l) [slot][kv head][16][2]
@@ -82,10 +84,6 @@ struct __align__(16) Owner {
   int slot, n;
   int pad[2];
 };
-struct __align__(16) Header {
-  int pieces, pad[3];
-};
-
 __device__ __forceinline__ int paged_keys(const PagedArgs& a, int seq) {
   return static_cast<int>(within(a.lens[seq], 0, static_cast<int64_t>(a.width) << a.page_shift));
 }
@@ -248,6 +246,293 @@ struct PagedMerge {
   int cols;
   __device__ PagedMerge(float* lds, int waves, int c) : m(lds), l(lds + waves * kCols), acc(lds + 2 * waves * kCols), cols(c) {}
   static constexpr int bytes(int waves, int cols) { return 4 * waves * (2 * kCols + cols * kPitch); }
+};
+
+__device__ __forceinline__ Piece* pieces_of(const PagedArgs& a) { return reinterpret_cast<Piece*>(a.plan + 4); }
+__device__ __forceinline__ Owner* owners_of(const PagedArgs& a) { return reinterpret_cast<Owner*>(pieces_of(a) + a.most); }
+
+// Inclusive sum over the wave by DPP: within rows of 16 lanes, then row 0 to 1 and 2 to 3, then the lower half to the upper.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);   // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);   // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);   // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);   // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 to rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 to rows 2 and 3
+  return v;
+}
+
+// ------------------------------------------------------------------------------------------
+// The plan turns the lengths into pieces. A group's shared rows are those that all its live sequences have, cut to whole
+// tiles unless they are all that any of them has. All keys, times the runs of columns that see them, make about `want` pieces, a
+// multiple of a tile for each wave; the pieces of one run of keys are alike, those of groups come first. Bound by latency, and a
+// launch of its own costs as much as a small call's attention: up to 64 sequences and groups every wave of the attention makes
+// the plan for itself, a sequence a lane, without barriers, and finds its block's piece in it (WavePlan); more of them are planned by
+// one block, which leaves it in the workspace.
+// ------------------------------------------------------------------------------------------
+constexpr int kPlanThreads = 1024, kPlanLds = 1024;
+
+// Words of its arrays: keys, groups of n sequences; starts, rows, low, high of the groups; the first piece of each.
+__host__ __device__ constexpr int64_t plan_words(int64_t n, int64_t groups) { return 2 * n + 4 * groups + 1 + (n + groups + 1); }
+
+struct Plan {
+  const PagedArgs& a;
+  int *keys, *of, *starts, *rows, *low, *high, *before;  // low: the fewest keys, in the end whether no sequence sees more
+  int groups, group, parts, total;
+  uint32_t chunk, shared_chunk;
+
+  __device__ static int count(int x, uint32_t each) { return static_cast<int>((x + each - 1) / each); }
+  __device__ int runs_of(int g) const { return ((starts[g + 1] - starts[g]) * group + a.cols - 1) / a.cols; }
+  __device__ int begin_of(int s) const { return of[s] < 0 ? 0 : rows[of[s]]; }  // the sequence's first own row
+  // where 16 columns' results of a piece go: one of a group has cols / 16 slots, one of a sequence one
+  __device__ int slot_of(int at) const {
+    const int shared = before[groups];
+    return at < shared ? at * (a.cols / kCols) : shared * (a.cols / kCols) + (at - shared);
+  }
+  __device__ static int size_of(int keys, int n) { return ((keys + n - 1) / n + kTileKeys - 1) / kTileKeys * kTileKeys; }
+  __device__ Piece piece(int at) const {
+    const int e = find(before, groups + a.n_seq, at), s = e - groups, x = at - before[e];
+    if (s < 0) {
+      const int n = count(rows[e], shared_chunk), runs = runs_of(e), i = x / runs, r = x % runs, size = size_of(rows[e], n);
+      return Piece{starts[e], r * a.cols, min(a.cols, (starts[e + 1] - starts[e]) * group - r * a.cols), i * size,
+                   min((i + 1) * size, rows[e]), low[e] && n == 1 ? -1 : slot_of(at), {}};
+    }
+    const int n = (before[e + 1] - before[e]) / parts, begin = begin_of(s), mine = max(keys[s] - begin, 0), i = x / parts, r = x % parts;
+    const int size = size_of(mine, n);
+    return Piece{s, r * kCols, min(kCols, group - r * kCols), begin + i * size, begin + min((i + 1) * size, mine),
+                 begin == 0 && n == 1 ? -1 : slot_of(at), {}};
+  }
+  __device__ Owner owner(int s) const {
+    Owner o{};
+    const int g = of[s], begin = begin_of(s), e = groups + s;
+    if (begin) {
+      o.shared_n = count(rows[g], shared_chunk);
+      o.shared_slot = low[g] && o.shared_n == 1 ? -1 : slot_of(before[g]);
+      o.shared_step = runs_of(g) * (a.cols / kCols);
+      o.col = (s - starts[g]) * group;
+    }
+    o.n = (before[e + 1] - before[e]) / parts;
+    o.slot = begin == 0 && o.n == 1 ? -1 : slot_of(before[e]);
+    return o;
+  }
+  // The last of n ascending values that is <= x, or -1.
+  __device__ static int find(const int* at, int n, int x) {
+    int lo = -1, hi = n;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (at[mid] <= x) lo = mid;
+      else hi = mid;
+    }
+    return lo;
+  }
+};
+
+// The plan by a block, its arrays in `mem`.
+__device__ __forceinline__ Plan make_plan(const PagedArgs& a, int* mem) {
+  constexpr int threads = kPlanThreads, waves = threads / 64;
+  __shared__ int64_t sums[waves];
+  __shared__ int scans[waves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n_seq = a.n_seq;
+  Plan p{a, mem};
+  p.of = p.keys + n_seq;
+  p.starts = p.of + n_seq;
+  p.rows = p.starts + a.groups + 1;
+  p.low = p.rows + a.groups;
+  p.high = p.low + a.groups;
+  p.before = p.high + a.groups;
+  p.group = a.heads / a.kv_heads;
+  p.parts = (p.group + kCols - 1) / kCols;
+  for (int s = tid; s < n_seq; s += threads) p.keys[s] = a.lens[s] < 0 ? -1 : paged_keys(a, s);  // -1: idle
+  int descends = 0;  // groups whose starts do not ascend would overlap: none is one
+  for (int g = tid; g <= a.groups && a.groups; g += threads) {
+    const int64_t start = a.cu_g[g], next = a.cu_g[min(g + 1, a.groups)];
+    p.starts[g] = static_cast<int>(within(start, 0, n_seq));
+    if (g == a.groups) break;
+    descends |= start > next;
+    p.rows[g] = static_cast<int>(within(a.shared[g], 0, 1 << 30));
+    p.low[g] = 0x7FFFFFFF;
+    p.high[g] = 0;
+  }
+  p.groups = __syncthreads_or(descends) ? 0 : a.groups;
+  // the fewest and most keys of a group's live sequences; a wave of one group asks once
+  for (int s0 = tid & ~63; s0 < n_seq; s0 += threads) {
+    const int s = s0 + lane;
+    int g = -1, lo = 0x7FFFFFFF, hi = 0;
+    if (s < n_seq) {
+      g = Plan::find(p.starts, p.groups, s);
+      if (g >= 0 && s >= p.starts[g + 1]) g = -1;
+      p.of[s] = g;
+      if (p.keys[s] >= 0) lo = hi = p.keys[s];
+    }
+    const int one = __builtin_amdgcn_readfirstlane(g);
+    if (__builtin_amdgcn_ballot_w64(g == one) == __builtin_amdgcn_ballot_w64(true)) {
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        lo = min(lo, __shfl_xor(lo, o));
+        hi = max(hi, __shfl_xor(hi, o));
+      }
+      if (lane != 0) g = -1;
+    }
+    if (g >= 0) {
+      atomicMin(&p.low[g], lo);
+      atomicMax(&p.high[g], hi);
+    }
+  }
+  __syncthreads();
+  int64_t work = 0;
+  for (int g = tid; g < p.groups; g += threads) {
+    const int most = p.starts[g + 1] - p.starts[g] > 1 && p.high[g] > 0 ? min(p.rows[g], p.low[g]) : 0, whole = most == p.high[g];
+    p.rows[g] = whole ? most : most & ~(kTileKeys - 1);
+    p.low[g] = whole;
+    work += static_cast<int64_t>(p.rows[g]) * (p.runs_of(g) * a.weight);
+  }
+  if (p.groups) __syncthreads();
+  for (int s = tid; s < n_seq; s += threads) work += static_cast<int64_t>(max(p.keys[s] - p.begin_of(s), 0)) * p.parts;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) work += __shfl_xor(work, o);
+  if (lane == 0) sums[wave] = work;
+  __syncthreads();
+  work = 0;
+  for (int w = 0; w < waves; ++w) work += sums[w];
+  // (rounded up past what fp32 may lose of it: a chunk is no less than its share)
+  const float share = static_cast<float>(work) * 1.000001f / static_cast<float>(a.want);
+  p.chunk = max((static_cast<uint32_t>(fminf(share, 1 << 30)) / a.unit + 1) * a.unit, a.least);
+  p.shared_chunk = (p.chunk / a.weight + kTileKeys - 1) / kTileKeys * kTileKeys;
+  // pieces of the groups, then of the sequences; one without keys has one, for its zeros
+  p.total = 0;
+  for (int e0 = 0; e0 < p.groups + n_seq; e0 += threads) {
+    const int e = e0 + tid, s = e - p.groups;
+    int n = 0;
+    if (s < 0) n = Plan::count(p.rows[e], p.shared_chunk) * p.runs_of(e);
+    else if (s < n_seq) n = max(Plan::count(max(p.keys[s] - p.begin_of(s), 0), p.chunk), p.begin_of(s) == 0 ? 1 : 0) * p.parts;
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(sum, o);
+      if (lane >= o) sum += x;
+    }
+    if (e0) __syncthreads();
+    if (lane == 63) scans[wave] = sum;
+    __syncthreads();
+    int all = 0;
+    for (int w = 0; w < waves; ++w) {
+      if (w < wave) sum += scans[w];
+      all += scans[w];
+    }
+    if (s < n_seq) p.before[e] = p.total + sum - n;
+    p.total += all;
+  }
+  if (tid == 0) p.before[p.groups + n_seq] = p.total;
+  __syncthreads();
+  p.total = min(p.total, a.most);
+  return p;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedArgs a) {
+  __shared__ int local[plan_words(kPlanLds, kPlanLds)];
+  Owner* owners = owners_of(a);
+  const Plan p = make_plan(a, a.n_seq <= kPlanLds && a.groups <= kPlanLds ? local : reinterpret_cast<int*>(owners + a.n_seq));
+  for (int at = threadIdx.x; at < p.total; at += kPlanThreads) pieces_of(a)[at] = p.piece(at);
+  for (int s = threadIdx.x; s < a.n_seq; s += kPlanThreads) owners[s] = p.owner(s);
+  if (threadIdx.x == 0) a.plan[0] = p.total;
+}
+
+// The same plan by a wave: lane s has sequence s, and for its group the numbers of its first sequence's lane.
+constexpr int kWavePlan = 64;
+struct WavePlan {
+  int keys, start, members;       // the lane's sequence; its group's first one (itself: none)
+  int rows, whole, shared_n;      // its group's shared rows, whether they are all, and their pieces a run
+  int n, shared_before, before;   // its own pieces a run; pieces up to the end of its group's (in the first lane), and of its own
+  int of_groups, total;           // (in every lane)
+
+  __device__ __forceinline__ static int lane_of(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+  __device__ __forceinline__ void make(const PagedArgs& a, int lane) {
+    const int group = a.heads / a.kv_heads, parts = (group + kCols - 1) / kCols;
+    int64_t len = -1, begin = 0, end = 0, want = 0;
+    if (lane < a.n_seq) len = a.lens[lane];
+    if (lane < a.groups) {
+      begin = a.cu_g[lane];
+      end = a.cu_g[lane + 1];
+      want = a.shared[lane];
+    }
+    keys = static_cast<int>(within(len, -1, static_cast<int64_t>(a.width) << a.page_shift));
+    start = lane;
+    members = 1;
+    rows = whole = shared_n = 0;
+    // (groups whose starts do not ascend would overlap: none is one)
+    if (a.groups && !__builtin_amdgcn_ballot_w64(begin > end)) {
+      const int b = static_cast<int>(within(begin, 0, a.n_seq)), e = static_cast<int>(within(end, b, a.n_seq));
+      // a group of several tells its first sequence's lane its number; the others look there
+      const int told = __builtin_amdgcn_ds_permute(4 * (e - b > 1 ? b : 63), e - b > 1 ? lane + 1 : 0);
+      // (lane 63 begins no group of several, so what the others tell it is nothing)
+      const uint64_t firsts = __builtin_amdgcn_ballot_w64(told > 0 && lane < 63) & (~uint64_t{0} >> (63 - lane));
+      const int first = firsts ? 63 - __builtin_clzll(firsts) : lane, g = __shfl(told, first) - 1;
+      const int last = __shfl(e, max(g, 0)), most = static_cast<int>(within(__shfl(static_cast<int>(within(want, 0, 1 << 30)), max(g, 0)), 0, 1 << 30));
+      const bool in = firsts && lane < last;
+      if (in) {
+        start = first;
+        members = last - first;
+      }
+      int low = keys < 0 ? 0x7FFFFFFF : keys, high = max(keys, 0);
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(low, o), y = __shfl_up(high, o);
+        if (lane - o >= start) {
+          low = min(low, x);
+          high = max(high, y);
+        }
+      }
+      low = __shfl(low, start + members - 1);
+      high = __shfl(high, start + members - 1);
+      if (in && high > 0) {
+        const int have = min(most, low);
+        whole = have == high;
+        rows = whole ? have : have & ~(kTileKeys - 1);
+      }
+    }
+    const int mine = max(keys - rows, 0), runs = (members * group + a.cols - 1) / a.cols;
+    const float work = static_cast<float>(mine) * parts + (lane == start ? static_cast<float>(rows) * (runs * a.weight) : 0.f);
+    const float share = group_sum<64>(work) * 1.0001f / static_cast<float>(a.want);  // (no less than its share)
+    const uint32_t chunk = max((static_cast<uint32_t>(fminf(share, 1 << 30)) / a.unit + 1) * a.unit, a.least);
+    const uint32_t shared_chunk = (chunk / a.weight + kTileKeys - 1) / kTileKeys * kTileKeys;
+    shared_n = Plan::count(rows, shared_chunk);
+    n = lane < a.n_seq ? max(Plan::count(mine, chunk), rows == 0 ? 1 : 0) : 0;
+    shared_before = wave_scan(lane == start ? shared_n * runs : 0);
+    of_groups = lane_of(shared_before, 63);
+    before = of_groups + wave_scan(n * parts);
+    total = min(lane_of(before, 63), a.most);
+  }
+  // (every lane asks for the same piece)
+  __device__ __forceinline__ Piece piece(const PagedArgs& a, int at) const {
+    const int group = a.heads / a.kv_heads, parts = (group + kCols - 1) / kCols, tiles = a.cols / kCols;
+    if (at < of_groups) {
+      const int s = __builtin_ctzll(__builtin_amdgcn_ballot_w64(shared_before > at));
+      const int columns = lane_of(members, s) * group, runs = (columns + a.cols - 1) / a.cols, k = lane_of(rows, s), pieces = lane_of(shared_n, s);
+      const int x = at - (lane_of(shared_before, s) - pieces * runs), i = x / runs, r = x % runs, size = Plan::size_of(k, pieces);
+      return Piece{s, r * a.cols, min(a.cols, columns - r * a.cols), i * size, min((i + 1) * size, k),
+                   lane_of(whole, s) && pieces == 1 ? -1 : at * tiles, {}};
+    }
+    const int s = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before > at)), pieces = lane_of(n, s), begin = lane_of(rows, s);
+    const int mine = max(lane_of(keys, s) - begin, 0), x = at - (lane_of(before, s) - pieces * parts), i = x / parts, r = x % parts;
+    const int size = Plan::size_of(mine, pieces);
+    return Piece{s, r * kCols, min(kCols, group - r * kCols), begin + i * size, begin + min((i + 1) * size, mine),
+                 begin == 0 && pieces == 1 ? -1 : of_groups * tiles + (at - of_groups), {}};
+  }
+  // Of the lane's own sequence.
+  __device__ __forceinline__ Owner owner(const PagedArgs& a, int lane) const {
+    const int group = a.heads / a.kv_heads, parts = (group + kCols - 1) / kCols, tiles = a.cols / kCols;
+    const int runs = (members * group + a.cols - 1) / a.cols, end = __shfl(shared_before, start);
+    Owner o{};
+    if (rows) {
+      o.shared_n = shared_n;
+      o.shared_slot = whole && shared_n == 1 ? -1 : (end - shared_n * runs) * tiles;
+      o.shared_step = runs * tiles;
+      o.col = (lane - start) * group;
+    }
+    o.n = n;
+    o.slot = rows == 0 && n == 1 ? -1 : of_groups * tiles + (before - n * parts - of_groups);
+    return o;
+  }
 };
 
 template <class T, int D, int CT>
@@ -439,8 +724,17 @@ __global__ void __launch_bounds__(CT < 0 ? 512 : 64 * kWaves, 2) paged_attention
     const Piece p{seq, col, min(kCols, group - col), 0, paged_keys(a, seq), -1, {}};
     paged_piece<T, D, 1>(a, p, kvh, a.table + static_cast<int64_t>(seq) * a.width, lds);
   } else {
-    if (static_cast<int>(at) >= reinterpret_cast<const Header*>(a.plan)->pieces) return;
-    const Piece p = (reinterpret_cast<const Piece*>(a.plan + 4))[at];
+    Piece p;
+    if (a.n_seq <= kWavePlan && a.groups <= kWavePlan) {
+      WavePlan plan;
+      plan.make(a, threadIdx.x & 63);
+      if (blockIdx.x == 0 && static_cast<int>(threadIdx.x) < a.n_seq) owners_of(a)[threadIdx.x] = plan.owner(a, threadIdx.x);
+      if (static_cast<int>(at) >= plan.total) return;
+      p = plan.piece(a, at);
+    } else {
+      if (static_cast<int>(at) >= a.plan[0]) return;
+      p = pieces_of(a)[at];
+    }
     const int32_t* table = a.table + static_cast<int64_t>(p.seq) * a.width;
     if constexpr (CT > 0) {
       if (p.cols > kCols) {
@@ -452,168 +746,6 @@ __global__ void __launch_bounds__(CT < 0 ? 512 : 64 * kWaves, 2) paged_attention
   }
 }
 
-// ------------------------------------------------------------------------------------------
-// The plan: one block turns the lengths into pieces. A group's shared rows are those that all its live sequences have, cut to
-// whole tiles unless they are all that any of them has. All keys, times the runs of columns that see them, make about `want`
-// pieces, a multiple of a tile for each wave; the pieces of one run of keys are alike, those of groups come first. Bound by
-// latency: up to kPlanLds sequences and groups everything but the lengths and the pieces stays in LDS.
-// ------------------------------------------------------------------------------------------
-constexpr int kPlanThreads = 1024, kPlanLds = 1024;
-
-__device__ __forceinline__ int64_t plan_sum(int64_t v, int64_t* part) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = 0;
-#pragma unroll
-  for (int w = 0; w < kPlanThreads / 64; ++w) v += part[w];
-  return v;
-}
-// Exclusive sum over the block; total: of all.
-__device__ __forceinline__ int plan_scan(int v, int* part, int& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mine = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int x = __shfl_up(v, o);
-    if (lane >= o) v += x;
-  }
-  __syncthreads();
-  if (lane == 63) part[wave] = v;
-  __syncthreads();
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kPlanThreads / 64; ++w) {
-    if (w < wave) v += part[w];
-    total += part[w];
-  }
-  return v - mine;
-}
-
-// The last of n ascending values that is <= x, or -1.
-__device__ __forceinline__ int plan_find(const int* at, int n, int x) {
-  int lo = -1, hi = n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (at[mid] <= x) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
-
-// Words of the plan's arrays: keys, groups of n sequences; starts, rows, low, high of the groups; the first piece of each.
-__host__ __device__ constexpr int64_t plan_words(int64_t n, int64_t groups) { return 2 * n + 4 * groups + 1 + (n + groups + 1); }
-
-__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedArgs a, int unit, int weight) {
-  __shared__ int64_t sums[kPlanThreads / 64];
-  __shared__ int scans[kPlanThreads / 64], local[plan_words(kPlanLds, kPlanLds)];
-  const int tid = threadIdx.x, n_seq = a.n_seq, group = a.heads / a.kv_heads, parts = (group + kCols - 1) / kCols;
-  Piece* pieces = reinterpret_cast<Piece*>(a.plan + 4);
-  Owner* owners = reinterpret_cast<Owner*>(pieces + a.most);
-  int* keys = n_seq <= kPlanLds && a.groups <= kPlanLds ? local : reinterpret_cast<int*>(owners + n_seq);  // -1: idle
-  int *of = keys + n_seq, *starts = of + n_seq, *rows = starts + a.groups + 1;
-  int *low = rows + a.groups, *high = low + a.groups, *before = high + a.groups;
-  for (int s = tid; s < n_seq; s += kPlanThreads) keys[s] = a.lens[s] < 0 ? -1 : paged_keys(a, s);
-  int descends = 0;  // groups whose starts do not ascend would overlap: none is one
-  for (int g = tid; g <= a.groups && a.groups; g += kPlanThreads) {
-    const int64_t start = a.cu_g[g];
-    starts[g] = static_cast<int>(within(start, 0, n_seq));
-    if (g == a.groups) break;
-    descends |= start > a.cu_g[g + 1];
-    rows[g] = static_cast<int>(within(a.shared[g], 0, 1 << 30));
-    low[g] = 0x7FFFFFFF;
-    high[g] = 0;
-  }
-  const int groups = __syncthreads_or(descends) ? 0 : a.groups;
-  // the fewest and most keys of a group's live sequences; a wave of one group asks once
-  for (int s0 = tid & ~63; s0 < n_seq; s0 += kPlanThreads) {
-    const int s = s0 + (tid & 63);
-    int g = -1, lo = 0x7FFFFFFF, hi = 0;
-    if (s < n_seq) {
-      g = plan_find(starts, groups, s);
-      if (g >= 0 && s >= starts[g + 1]) g = -1;
-      of[s] = g;
-      if (keys[s] >= 0) lo = hi = keys[s];
-    }
-    const int one = __builtin_amdgcn_readfirstlane(g);
-    if (__builtin_amdgcn_ballot_w64(g == one) == __builtin_amdgcn_ballot_w64(true)) {
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        lo = min(lo, __shfl_xor(lo, o));
-        hi = max(hi, __shfl_xor(hi, o));
-      }
-      if ((tid & 63) != 0) g = -1;
-    }
-    if (g >= 0) {
-      atomicMin(&low[g], lo);
-      atomicMax(&high[g], hi);
-    }
-  }
-  __syncthreads();
-  int64_t work = 0;
-  const int wide = a.cols > kCols ? weight : 1;  // a wide piece's tile takes so many of others
-  const auto runs_of = [&](int g) { return ((starts[g + 1] - starts[g]) * group + a.cols - 1) / a.cols; };
-  for (int g = tid; g < groups; g += kPlanThreads) {
-    const int most = starts[g + 1] - starts[g] > 1 && high[g] > 0 ? min(rows[g], low[g]) : 0, whole = most == high[g];
-    rows[g] = whole ? most : most & ~(kTileKeys - 1);
-    low[g] = whole;  // from here on: whether no sequence of it sees more
-    work += static_cast<int64_t>(rows[g]) * runs_of(g) * wide;
-  }
-  __syncthreads();
-  const auto begin_of = [&](int s) { return of[s] < 0 ? 0 : rows[of[s]]; };
-  for (int s = tid; s < n_seq; s += kPlanThreads) work += static_cast<int64_t>(max(keys[s] - begin_of(s), 0)) * parts;
-  work = plan_sum(work, sums);
-  const uint32_t chunk = static_cast<uint32_t>(min((work / a.want / unit + 1) * unit, int64_t{1} << 30));
-  const uint32_t shared_chunk = (chunk / wide + kTileKeys - 1) / kTileKeys * kTileKeys;
-  const auto count = [](int x, uint32_t each) { return static_cast<int>((x + each - 1) / each); };
-  // pieces of the groups, then of the sequences; one without keys has one, for its zeros
-  int pieces_n = 0;
-  for (int e0 = 0; e0 < groups + n_seq; e0 += kPlanThreads) {
-    const int e = e0 + tid, s = e - groups;
-    int n = 0, total;
-    if (s < 0) n = count(rows[e], shared_chunk) * runs_of(e);
-    else if (s < n_seq) n = max(count(max(keys[s] - begin_of(s), 0), chunk), begin_of(s) == 0) * parts;
-    const int sum = plan_scan(n, scans, total);
-    if (s < n_seq) before[e] = pieces_n + sum;
-    pieces_n += total;
-  }
-  if (tid == 0) before[groups + n_seq] = pieces_n;
-  __syncthreads();
-  const int of_groups = before[groups], tiles = a.cols / kCols;
-  // a piece of a group has `tiles` slots, one of a sequence has one
-  const auto slot_of = [&](int at) { return at < of_groups ? at * tiles : of_groups * tiles + (at - of_groups); };
-  for (int at = tid; at < min(pieces_n, a.most); at += kPlanThreads) {
-    const int e = plan_find(before, groups + n_seq, at), s = e - groups, x = at - before[e];
-    Piece p;
-    if (s < 0) {
-      const int n = count(rows[e], shared_chunk), runs = runs_of(e), i = x / runs, r = x % runs;
-      const int size = ((rows[e] + n - 1) / n + kTileKeys - 1) / kTileKeys * kTileKeys;
-      p = Piece{starts[e], r * a.cols, min(a.cols, (starts[e + 1] - starts[e]) * group - r * a.cols), i * size,
-                min((i + 1) * size, rows[e]), low[e] && n == 1 ? -1 : slot_of(at), {}};
-    } else {
-      const int n = (before[e + 1] - before[e]) / parts, begin = begin_of(s), mine = max(keys[s] - begin, 0), i = x / parts, r = x % parts;
-      const int size = ((mine + n - 1) / n + kTileKeys - 1) / kTileKeys * kTileKeys;
-      p = Piece{s, r * kCols, min(kCols, group - r * kCols), begin + i * size, begin + min((i + 1) * size, mine),
-                begin == 0 && n == 1 ? -1 : slot_of(at), {}};
-    }
-    pieces[at] = p;
-  }
-  for (int s = tid; s < n_seq; s += kPlanThreads) {
-    Owner o{};
-    const int g = of[s], begin = begin_of(s), e = groups + s;
-    if (begin) {
-      o.shared_n = count(rows[g], shared_chunk);
-      o.shared_slot = low[g] && o.shared_n == 1 ? -1 : slot_of(before[g]);
-      o.shared_step = runs_of(g) * tiles;
-      o.col = (s - starts[g]) * group;
-    }
-    o.n = (before[e + 1] - before[e]) / parts;
-    o.slot = begin == 0 && o.n == 1 ? -1 : slot_of(before[e]);
-    owners[s] = o;
-  }
-  if (tid == 0) reinterpret_cast<Header*>(a.plan)->pieces = min(pieces_n, a.most);
-}
-
 // Joins what the pieces of a sequence left: block = (query head, sequence).
 constexpr int kCombine = 256, kMostParts = 2112;
 template <class T, int D>
@@ -621,7 +753,7 @@ __global__ void __launch_bounds__(kCombine) paged_combine_kernel(PagedArgs a) {
   constexpr int kLanes = kCombine / D, kBatch = 8;
   __shared__ float weight[kMostParts], red[2][kCombine / 64], sum[kLanes][D];
   const int seq = blockIdx.y, head = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid / 64, d = tid % D, from = tid / D;
-  const Owner o = (reinterpret_cast<const Owner*>(a.plan + 4 + 8 * static_cast<int64_t>(a.most)))[seq];
+  const Owner o = owners_of(a)[seq];
   const int n = min(o.shared_n + o.n, kMostParts);
   if ((o.shared_n == 0 || o.shared_slot < 0) && (o.n == 0 || o.slot < 0)) return;  // its block finished it
   const int group = a.heads / a.kv_heads, kvh = head / group, col = head % group;
@@ -752,13 +884,14 @@ extern "C" int fw_decode_attention_paged(const void* q, int64_t q_row, int64_t q
   const int64_t blocks = kv_heads * (p.most ? p.most : static_cast<int64_t>(n_seq) * parts);
   if (!grid_ok(blocks, 64 * waves) || p.slots > 0x7FFFFFFF / kCols) return fw_fail(FW_EINVAL, "%s: too many sequences", what);
   PagedArgs a{q, k_pages, v_pages, out, q_row, q_head, o_row, o_head, table, lens, cu_groups, shared, n_seq, heads, kv_heads,
-              groups, width, n_pages, page_shift_of(page), scale, p.cols, p.want, static_cast<int>(p.most),
+              groups, width, n_pages, page_shift_of(page), scale, p.cols, p.want, static_cast<uint32_t>(kTileKeys * p.waves),
+              static_cast<uint32_t>(kTileKeys * p.waves), p.cols > 64 ? 3 : p.cols > kCols ? 2 : 1, static_cast<int>(p.most),
               reinterpret_cast<int*>(ws), ws + p.ints, nullptr};
   a.ml = a.part + p.slots * kv_heads * kCols * head_dim;
   int lds = head_dim == 64 ? PagedMerge<64>::bytes(waves, cols) : PagedMerge<128>::bytes(waves, cols);
   if (p.cols > kCols) lds = std::max(lds, kStages * 2 * kTileKeys * head_dim * 2);
-  if (p.most) {
-    hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, a, kTileKeys * waves, p.cols > 64 ? 3 : 2);
+  if (p.most && (n_seq > kWavePlan || groups > kWavePlan)) {
+    hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, a);
     if (const int rc = fw_check_launch(what)) return rc;
   }
   const auto run = [&](auto t, auto d) {

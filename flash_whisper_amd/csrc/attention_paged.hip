@@ -61,7 +61,6 @@ struct PagedArgs {
   int cols;           // columns of a piece of a group's shared keys, at most: 16, or 64 or 128 in wide ones
   int want;           // pieces that all keys are to make, about
   uint32_t unit, least;  // what a chunk of keys is a multiple of, and at least
-  int weight;         // what a tile takes in a piece of a group, of what it takes in others
   int most;           // pieces there may be; 0: each sequence is a piece, and nothing is shared
   int* plan;          // Header, Pieces, Owners, and the plan's arrays where LDS does not hold them
   float *part, *ml;   // O [slot][kv head][16][D], (m, l) [slot][kv head][16][2]
@@ -279,7 +278,7 @@ struct Plan {
   const PagedArgs& a;
   int *keys, *of, *starts, *rows, *low, *high, *before;  // low: the fewest keys, in the end whether no sequence sees more
   int groups, group, parts, total;
-  uint32_t chunk, shared_chunk;
+  uint32_t chunk;
 
   __device__ static int count(int x, uint32_t each) { return static_cast<int>((x + each - 1) / each); }
   __device__ int runs_of(int g) const { return ((starts[g + 1] - starts[g]) * group + a.cols - 1) / a.cols; }
@@ -293,7 +292,7 @@ struct Plan {
   __device__ Piece piece(int at) const {
     const int e = find(before, groups + a.n_seq, at), s = e - groups, x = at - before[e];
     if (s < 0) {
-      const int n = count(rows[e], shared_chunk), runs = runs_of(e), i = x / runs, r = x % runs, size = size_of(rows[e], n);
+      const int n = count(rows[e], chunk), runs = runs_of(e), i = x / runs, r = x % runs, size = size_of(rows[e], n);
       return Piece{starts[e], r * a.cols, min(a.cols, (starts[e + 1] - starts[e]) * group - r * a.cols), i * size,
                    min((i + 1) * size, rows[e]), low[e] && n == 1 ? -1 : slot_of(at), {}};
     }
@@ -306,7 +305,7 @@ struct Plan {
     Owner o{};
     const int g = of[s], begin = begin_of(s), e = groups + s;
     if (begin) {
-      o.shared_n = count(rows[g], shared_chunk);
+      o.shared_n = count(rows[g], chunk);
       o.shared_slot = low[g] && o.shared_n == 1 ? -1 : slot_of(before[g]);
       o.shared_step = runs_of(g) * (a.cols / kCols);
       o.col = (s - starts[g]) * group;
@@ -384,7 +383,7 @@ __device__ __forceinline__ Plan make_plan(const PagedArgs& a, int* mem) {
     const int most = p.starts[g + 1] - p.starts[g] > 1 && p.high[g] > 0 ? min(p.rows[g], p.low[g]) : 0, whole = most == p.high[g];
     p.rows[g] = whole ? most : most & ~(kTileKeys - 1);
     p.low[g] = whole;
-    work += static_cast<int64_t>(p.rows[g]) * (p.runs_of(g) * a.weight);
+    work += static_cast<int64_t>(p.rows[g]) * p.runs_of(g);
   }
   if (p.groups) __syncthreads();
   for (int s = tid; s < n_seq; s += threads) work += static_cast<int64_t>(max(p.keys[s] - p.begin_of(s), 0)) * p.parts;
@@ -397,13 +396,12 @@ __device__ __forceinline__ Plan make_plan(const PagedArgs& a, int* mem) {
   // (rounded up past what fp32 may lose of it: a chunk is no less than its share)
   const float share = static_cast<float>(work) * 1.000001f / static_cast<float>(a.want);
   p.chunk = max((static_cast<uint32_t>(fminf(share, 1 << 30)) / a.unit + 1) * a.unit, a.least);
-  p.shared_chunk = (p.chunk / a.weight + kTileKeys - 1) / kTileKeys * kTileKeys;
   // pieces of the groups, then of the sequences; one without keys has one, for its zeros
   p.total = 0;
   for (int e0 = 0; e0 < p.groups + n_seq; e0 += threads) {
     const int e = e0 + tid, s = e - p.groups;
     int n = 0;
-    if (s < 0) n = Plan::count(p.rows[e], p.shared_chunk) * p.runs_of(e);
+    if (s < 0) n = Plan::count(p.rows[e], p.chunk) * p.runs_of(e);
     else if (s < n_seq) n = max(Plan::count(max(p.keys[s] - p.begin_of(s), 0), p.chunk), p.begin_of(s) == 0 ? 1 : 0) * p.parts;
     int sum = n;
 #pragma unroll
@@ -491,11 +489,10 @@ struct WavePlan {
       }
     }
     const int mine = max(keys - rows, 0), runs = (members * group + a.cols - 1) / a.cols;
-    const float work = static_cast<float>(mine) * parts + (lane == start ? static_cast<float>(rows) * (runs * a.weight) : 0.f);
+    const float work = static_cast<float>(mine) * parts + (lane == start ? static_cast<float>(rows) * runs : 0.f);
     const float share = group_sum<64>(work) * 1.0001f / static_cast<float>(a.want);  // (no less than its share)
     const uint32_t chunk = max((static_cast<uint32_t>(fminf(share, 1 << 30)) / a.unit + 1) * a.unit, a.least);
-    const uint32_t shared_chunk = (chunk / a.weight + kTileKeys - 1) / kTileKeys * kTileKeys;
-    shared_n = Plan::count(rows, shared_chunk);
+    shared_n = Plan::count(rows, chunk);
     n = lane < a.n_seq ? max(Plan::count(mine, chunk), rows == 0 ? 1 : 0) : 0;
     shared_before = wave_scan(lane == start ? shared_n * runs : 0);
     of_groups = lane_of(shared_before, 63);
@@ -810,7 +807,7 @@ struct PagedSizes {
   int cols, want, waves, direct_waves;
   int64_t most, slots, ints, floats;  // pieces, 16-column results, the plan's words, workspace
 };
-constexpr int kDirectRows = 1024, kWantBlocks = 1024;
+constexpr int kDirectRows = 1024, kWantBlocks = 512;
 
 PagedSizes paged_sizes(int n_seq, int heads, int kv_heads, int64_t capacity, int groups, int dim) {
   PagedSizes p = {};
@@ -885,7 +882,7 @@ extern "C" int fw_decode_attention_paged(const void* q, int64_t q_row, int64_t q
   if (!grid_ok(blocks, 64 * waves) || p.slots > 0x7FFFFFFF / kCols) return fw_fail(FW_EINVAL, "%s: too many sequences", what);
   PagedArgs a{q, k_pages, v_pages, out, q_row, q_head, o_row, o_head, table, lens, cu_groups, shared, n_seq, heads, kv_heads,
               groups, width, n_pages, page_shift_of(page), scale, p.cols, p.want, static_cast<uint32_t>(kTileKeys * p.waves),
-              static_cast<uint32_t>(kTileKeys * p.waves), p.cols > 64 ? 3 : p.cols > kCols ? 2 : 1, static_cast<int>(p.most),
+              static_cast<uint32_t>(kTileKeys * p.waves), static_cast<int>(p.most),
               reinterpret_cast<int*>(ws), ws + p.ints, nullptr};
   a.ml = a.part + p.slots * kv_heads * kCols * head_dim;
   int lds = head_dim == 64 ? PagedMerge<64>::bytes(waves, cols) : PagedMerge<128>::bytes(waves, cols);

@@ -60,7 +60,7 @@ struct PagedArgs {
   float scale;
   int cols;           // columns of a piece of a group's shared keys, at most: 16, or 64 or 128 in wide ones
   int want;           // pieces that all keys are to make, about
-  uint32_t unit, least;  // what a chunk of keys is a multiple of, and at least
+  uint32_t unit;      // what a chunk of keys is a multiple of: a tile for each wave
   int most;           // pieces there may be; 0: each sequence is a piece, and nothing is shared
   int* plan;          // Header, Pieces, Owners, and the plan's arrays where LDS does not hold them
   float *part, *ml;   // O [slot][kv head][16][D], (m, l) [slot][kv head][16][2]
@@ -395,7 +395,7 @@ __device__ __forceinline__ Plan make_plan(const PagedArgs& a, int* mem) {
   for (int w = 0; w < waves; ++w) work += sums[w];
   // (rounded up past what fp32 may lose of it: a chunk is no less than its share)
   const float share = static_cast<float>(work) * 1.000001f / static_cast<float>(a.want);
-  p.chunk = max((static_cast<uint32_t>(fminf(share, 1 << 30)) / a.unit + 1) * a.unit, a.least);
+  p.chunk = (static_cast<uint32_t>(fminf(share, 1 << 30)) / a.unit + 1) * a.unit;
   // pieces of the groups, then of the sequences; one without keys has one, for its zeros
   p.total = 0;
   for (int e0 = 0; e0 < p.groups + n_seq; e0 += threads) {
@@ -491,7 +491,7 @@ struct WavePlan {
     const int mine = max(keys - rows, 0), runs = (members * group + a.cols - 1) / a.cols;
     const float work = static_cast<float>(mine) * parts + (lane == start ? static_cast<float>(rows) * runs : 0.f);
     const float share = group_sum<64>(work) * 1.0001f / static_cast<float>(a.want);  // (no less than its share)
-    const uint32_t chunk = max((static_cast<uint32_t>(fminf(share, 1 << 30)) / a.unit + 1) * a.unit, a.least);
+    const uint32_t chunk = (static_cast<uint32_t>(fminf(share, 1 << 30)) / a.unit + 1) * a.unit;
     shared_n = Plan::count(rows, chunk);
     n = lane < a.n_seq ? max(Plan::count(mine, chunk), rows == 0 ? 1 : 0) : 0;
     shared_before = wave_scan(lane == start ? shared_n * runs : 0);
@@ -586,58 +586,142 @@ __device__ __forceinline__ void paged_piece(const PagedArgs& a, const Piece& p, 
       } else {
         const int64_t at = (static_cast<int64_t>(p.slot + c) * a.kv_heads + kvh) * kCols + col;
         a.part[at * D + d] = o;
-        if (d == 0) {
-          a.ml[2 * at] = m;
-          a.ml[2 * at + 1] = l;
-        }
+        if (d == 0) reinterpret_cast<float2*>(a.ml)[at] = make_float2(m, l);
       }
     }
   }
 }
 
 // A piece of many columns: wave w has columns 16 CT w .. and all of the keys, which arrive in LDS by direct copies, a ring of
-// kStages tiles, so that a row of K and V is read once for 64 CT columns. A tile of a page is contiguous, V's just as the operands
-// are read; K's 16-byte chunks are swapped within a row so that the 16 rows of a read lie in different banks.
-constexpr int kStages = 4, kWaves = 4;
+// kStages steps of two tiles, so that a row of K and V is read once for 64 CT columns. A tile of a page is contiguous, V's just as
+// the operands are read; K's 16-byte chunks are swapped within a row so that the 16 rows of a read lie in different banks.
+constexpr int kStages = 2, kWaves = 4, kStep = 2;
 template <int D>
 __device__ __forceinline__ int wide_swap(int row) {
   return D == 128 ? (row & 3) | ((row >> 3) & 3) << 2 : ((row >> 1) & 1) | ((row >> 3) & 3) << 1;
 }
 
+// A step's keys: K at LDS address k, V at v, a tile kTile bytes on from the other. MASKED: left[t] of the lane's 8 keys of tile t count.
+template <class T, int D, int CT, bool MASKED>
+__device__ __forceinline__ void wide_step(uint32_t k, uint32_t v, const typename Types<T>::v8 (&q)[CT][D / 32], float factor,
+                                          const int (&left)[kStep], PagedState<T, D, CT>& st) {
+  typedef typename Types<T>::v8 v8;
+  typedef typename Types<T>::v2 v2;
+  typedef __attribute__((address_space(3))) v8 lds_v8;
+  constexpr uint32_t kRowBytes = 2 * D, kTile = kTileKeys * kRowBytes;
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  f4v s[CT][kStep][2];
+#pragma unroll
+  for (int c = 0; c < CT; ++c)
+#pragma unroll
+    for (int t = 0; t < kStep; ++t) s[c][t][0] = s[c][t][1] = f4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) {
+    const uint32_t at = k + ((4 * j + g) ^ wide_swap<D>(8 * (i >> 2) + (i & 3))) * 16;
+    v8 x[kStep][2];
+#pragma unroll
+    for (int t = 0; t < kStep; ++t)
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) x[t][kt] = *reinterpret_cast<lds_v8*>(static_cast<uintptr_t>(at + t * kTile + 4 * kt * kRowBytes));
+#pragma unroll
+    for (int t = 0; t < kStep; ++t)
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int c = 0; c < CT; ++c) s[c][t][kt] = mfma16(x[t][kt], q[c][j], s[c][t][kt]);
+  }
+  v8 p[CT][kStep];
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < kStep; ++t)
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (MASKED && 4 * kt + r >= left[t]) s[c][t][kt][r] = -INFINITY;
+          top = __builtin_elementwise_maximum(top, s[c][t][kt][r]);
+        }
+    top = xor_max<32>(xor_max<16>(top)) * factor;
+    if (__builtin_amdgcn_ballot_w64(top > st.m[c] + kSlack)) {
+      const float m_new = fmaxf(st.m[c], top), corr = st.m[c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m[c] - m_new);
+      st.l[c] *= corr;
+#pragma unroll
+      for (int db = 0; db < D / 16; ++db) st.o[c][db] *= corr;
+      st.m[c] = m_new;
+    }
+    const float m = st.m[c] == -INFINITY ? 0.f : st.m[c];
+    float sum[kStep] = {};
+#pragma unroll
+    for (int t = 0; t < kStep; ++t)
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+          v2 x;
+          x[0] = static_cast<T>(__builtin_amdgcn_exp2f(fmaf(s[c][t][kt][r], factor, -m)));
+          x[1] = static_cast<T>(__builtin_amdgcn_exp2f(fmaf(s[c][t][kt][r + 1], factor, -m)));
+          sum[t] = add_pair(x, sum[t]);
+          p[c][t][4 * kt + r] = x[0];
+          p[c][t][4 * kt + r + 1] = x[1];
+        }
+    st.l[c] += sum[0] + sum[1];
+  }
+#pragma unroll
+  for (int t = 0; t < kStep; ++t)
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) {
+      v8 x = *reinterpret_cast<lds_v8*>(static_cast<uintptr_t>(v + t * kTile + (g * D + i) * 16 + db * 256));
+      if constexpr (MASKED) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e >= left[t]) x[e] = static_cast<T>(0.f);
+      }
+#pragma unroll
+      for (int c = 0; c < CT; ++c) st.o[c][db] = mfma16(x, p[c][t], st.o[c][db]);
+    }
+}
+
 template <class T, int D, int CT>
 __device__ __forceinline__ void paged_wide(const PagedArgs& a, const Piece& p, int kvh, const int32_t* table, float* lds) {
   typedef typename Types<T>::v8 v8;
-  typedef __attribute__((address_space(3))) v8 lds_v8;
-  constexpr int kHalf = kTileKeys * D * 2, kStage = 2 * kHalf;  // bytes of a tile of K or V, of both
-  constexpr int kCopies = kHalf / 1024 / kWaves;                // of K, and of V, a wave
+  constexpr int kTile = kTileKeys * D * 2, kStage = 2 * kStep * kTile;  // bytes of a tile of K or V, of a step of both
+  constexpr int kCopies = kTile / 1024 / kWaves;                        // of a tile of K, and of V, a wave
   constexpr int kRowBytes = 2 * D, kCopyRows = 1024 / kRowBytes;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane & 15, g = lane >> 4, group = a.heads / a.kv_heads, col0 = kCols * CT * wave;
   const bool live = col0 < p.cols;
   const uint32_t ring = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
   const int first = p.begin / kTileKeys, tiles = (p.end + kTileKeys - 1) / kTileKeys - first, rows = 1 << a.page_shift;
+  const int steps = (tiles + kStep - 1) / kStep;
   PagedPages pages = paged_pages(a, table, first + lane, p.end);
-  uint32_t ok = 0;  // two bits a stage: the pages of its tile's halves
+  uint32_t ok = 0;  // two bits a tile of the ring: the pages of its halves
   const auto issue = [&](int n) {
-    if (n && (n & 63) == 0) pages = paged_pages(a, table, first + n + lane, p.end);
-    const int lo = __builtin_amdgcn_readlane(pages.lo, n & 63), hi = __builtin_amdgcn_readlane(pages.hi, n & 63), s = n % kStages;
-    ok = (ok & ~(3u << (2 * s))) | static_cast<uint32_t>((lo >= 0) | (hi >= 0) << 1) << (2 * s);
-    const uint32_t to = ring + s * kStage;
-    const int row = ((first + n) * kTileKeys) & (rows - 1);
-    const int64_t at_lo = ((static_cast<int64_t>(max(lo, 0)) * a.kv_heads + kvh) * rows + row) * kRowBytes;
-    // (a page of 16 rows: the second half begins another page's rows)
-    const int64_t at_hi = a.page_shift == 4 ? (static_cast<int64_t>(max(hi, 0)) * a.kv_heads + kvh) * rows * kRowBytes - kHalf / 2 : at_lo;
+    const int s = n % kStages;
 #pragma unroll
-    for (int c = 0; c < kCopies; ++c) {
-      const int blk = kCopies * wave + c, r = blk * kCopyRows + lane / (D / 8), chunk = (lane % (D / 8)) ^ wide_swap<D>(r);
-      const int64_t at = blk * 1024 < kHalf / 2 ? at_lo : at_hi;
-      dma16_s(static_cast<uint32_t>(r * kRowBytes + chunk * 16), static_cast<const uint8_t*>(a.k) + at, to + blk * 1024);
-      dma16_s(static_cast<uint32_t>(blk * 1024 + lane * 16), static_cast<const uint8_t*>(a.v) + at, to + kHalf + blk * 1024);
+    for (int t = 0; t < kStep; ++t) {  // (a tile past the end has no page: page 0 is copied, and none of it counts)
+      const int x = kStep * n + t, place = 2 * (kStep * s + t);
+      if (t == 0 && x && (x & 63) == 0) pages = paged_pages(a, table, first + x + lane, p.end);
+      const int lo = __builtin_amdgcn_readlane(pages.lo, x & 63), hi = __builtin_amdgcn_readlane(pages.hi, x & 63);
+      ok = (ok & ~(3u << place)) | static_cast<uint32_t>((lo >= 0) | (hi >= 0) << 1) << place;
+      const uint32_t to = ring + s * kStage + t * kTile;
+      const int row = ((first + x) * kTileKeys) & (rows - 1);
+      const int64_t at_lo = ((static_cast<int64_t>(max(lo, 0)) * a.kv_heads + kvh) * rows + row) * kRowBytes;
+      // (a page of 16 rows: the second half begins another page's rows)
+      const int64_t at_hi = a.page_shift == 4 ? (static_cast<int64_t>(max(hi, 0)) * a.kv_heads + kvh) * rows * kRowBytes - kTile / 2 : at_lo;
+#pragma unroll
+      for (int c = 0; c < kCopies; ++c) {
+        const int blk = kCopies * wave + c, r = blk * kCopyRows + lane / (D / 8), chunk = (lane % (D / 8)) ^ wide_swap<D>(r);
+        const int64_t at = blk * 1024 < kTile / 2 ? at_lo : at_hi;
+        dma16_s(static_cast<uint32_t>(r * kRowBytes + chunk * 16), static_cast<const uint8_t*>(a.k) + at, to + blk * 1024);
+        dma16_s(static_cast<uint32_t>(blk * 1024 + lane * 16), static_cast<const uint8_t*>(a.v) + at, to + kStep * kTile + blk * 1024);
+      }
     }
   };
 #pragma unroll
   for (int n = 0; n < kStages - 1; ++n)
-    if (n < tiles) issue(n);
+    if (n < steps) issue(n);
   v8 q[CT][D / 32];
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
@@ -658,28 +742,18 @@ __device__ __forceinline__ void paged_wide(const PagedArgs& a, const Piece& p, i
     st.m[c] = -INFINITY;
     st.l[c] = 0.f;
   }
-  const uint32_t k_row = (8 * (i >> 2) + (i & 3)) * kRowBytes, v_at = kHalf + (g * D + i) * 16;
-  for (int n = 0; n < tiles; ++n) {
-    // tile n visible to every wave, every one done with tile n - 1, whose place tile n + kStages - 1 takes
-    wait_stages_ahead<2 * kCopies, kStages - 1>(min(kStages - 2, tiles - 1 - n));
+  for (int n = 0; n < steps; ++n) {
+    // step n visible to every wave, every one done with step n - 1, whose place step n + kStages - 1 takes
+    wait_stages_ahead<2 * kStep * kCopies, kStages - 1>(min(kStages - 2, steps - 1 - n));
     lds_barrier();
-    const uint32_t at = ring + n % kStages * kStage, has = (ok >> (2 * (n % kStages))) & 3;
-    if (n + kStages - 1 < tiles) issue(n + kStages - 1);
+    const uint32_t at = ring + n % kStages * kStage, has = (ok >> (2 * kStep * (n % kStages))) & 15;
+    if (n + kStages - 1 < steps) issue(n + kStages - 1);
     if (!live) continue;
-    PagedTile<T, D> x;
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-      for (int j = 0; j < D / 32; ++j)
-        x.k[kt][j] = *reinterpret_cast<lds_v8*>(
-            static_cast<uintptr_t>(at + k_row + 4 * kt * kRowBytes + ((4 * j + g) ^ wide_swap<D>(8 * (i >> 2) + (i & 3))) * 16));
-#pragma unroll
-    for (int db = 0; db < D / 16; ++db) x.v[db] = *reinterpret_cast<lds_v8*>(static_cast<uintptr_t>(at + v_at + db * 256));
-    f4v s[CT][2];
-    paged_scores<T, D, CT>(x, q, s);
-    const int left = p.end - (first + n) * kTileKeys;
-    if (left >= kTileKeys && has == 3) paged_values<T, D, CT, false>(x, s, factor, 8, st);
-    else paged_values<T, D, CT, true>(x, s, factor, has >> (lane >> 5) & 1 ? left - 8 * g : 0, st);
+    const int end = p.end - (first + kStep * n) * kTileKeys;
+    const uint32_t k = at + (8 * (i >> 2) + (i & 3)) * kRowBytes, v = at + kStep * kTile;
+    const int left[kStep] = {has >> (lane >> 5) & 1 ? end - 8 * g : 0, has >> (2 + (lane >> 5)) & 1 ? end - kTileKeys - 8 * g : 0};
+    if (end >= kStep * kTileKeys && has == 15) wide_step<T, D, CT, false>(k, v, q, factor, left, st);
+    else wide_step<T, D, CT, true>(k, v, q, factor, left, st);
   }
   if (!live) return;
 #pragma unroll
@@ -716,8 +790,8 @@ __global__ void __launch_bounds__(CT < 0 ? 512 : 64 * kWaves, 2) paged_attention
   const int kvh = blockIdx.x % a.kv_heads;
   const unsigned at = blockIdx.x / a.kv_heads;
   if constexpr (CT < 0) {
-    const int group = a.heads / a.kv_heads, parts = (group + kCols - 1) / kCols, col = static_cast<int>(at % parts) * kCols;
-    const int seq = static_cast<int>(at / parts);
+    const int group = a.heads / a.kv_heads, parts = (group + kCols - 1) / kCols;
+    const int col = static_cast<int>(at % parts) * kCols, seq = static_cast<int>(at / parts);
     const Piece p{seq, col, min(kCols, group - col), 0, paged_keys(a, seq), -1, {}};
     paged_piece<T, D, 1>(a, p, kvh, a.table + static_cast<int64_t>(seq) * a.width, lds);
   } else {
@@ -743,63 +817,78 @@ __global__ void __launch_bounds__(CT < 0 ? 512 : 64 * kWaves, 2) paged_attention
   }
 }
 
-// Joins what the pieces of a sequence left: block = (query head, sequence).
-constexpr int kCombine = 256, kMostParts = 2112;
-template <class T, int D>
-__global__ void __launch_bounds__(kCombine) paged_combine_kernel(PagedArgs a) {
-  constexpr int kLanes = kCombine / D, kBatch = 8;
-  __shared__ float weight[kMostParts], red[2][kCombine / 64], sum[kLanes][D];
-  const int seq = blockIdx.y, head = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid / 64, d = tid % D, from = tid / D;
+// Joins what the pieces of a sequence left for a query head: W waves a head, each every W-th piece, a lane a piece's (m, l) and D /
+// 64 dims. What a wave needs is on its way before the weights are known. Bound by latency.
+template <class T, int D, int W>
+__global__ void __launch_bounds__(256) paged_combine_kernel(PagedArgs a) {
+  constexpr int kDims = D / 64, kBatch = 8;
+  typedef float dims __attribute__((ext_vector_type(kDims)));
+  __shared__ float lds[W > 1 ? W : 1][64][kDims + 2];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % W;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * (4 / W) + wave / W;
+  const int seq = static_cast<int>(at / a.heads), head = static_cast<int>(at % a.heads);
+  if (seq >= a.n_seq) return;  // (W = 1)
   const Owner o = owners_of(a)[seq];
-  const int n = min(o.shared_n + o.n, kMostParts);
+  const int n = o.shared_n + o.n, group = a.heads / a.kv_heads, kvh = head / group, col = head % group, step = (group + kCols - 1) / kCols;
   if ((o.shared_n == 0 || o.shared_slot < 0) && (o.n == 0 || o.slot < 0)) return;  // its block finished it
-  const int group = a.heads / a.kv_heads, kvh = head / group, col = head % group;
   const auto slot = [&](int i) {
-    const int c = i < o.shared_n ? o.col + col : col;
-    const int at = i < o.shared_n ? o.shared_slot + i * o.shared_step : o.slot + (i - o.shared_n) * ((group + kCols - 1) / kCols);
-    return (static_cast<int64_t>(at + c / kCols) * a.kv_heads + kvh) * kCols + c % kCols;
+    const int c = i < o.shared_n ? o.col + col : col, first = i < o.shared_n ? o.shared_slot + i * o.shared_step : o.slot + (i - o.shared_n) * step;
+    return (static_cast<int64_t>(first + c / kCols) * a.kv_heads + kvh) * kCols + c % kCols;
   };
-  const auto load = [&](int i, float (&x)[kBatch]) {  // chunks i, i + kLanes, ..; past the end the last one
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j) x[j] = a.part[slot(min(i + j * kLanes, n - 1)) * D + d];
-  };
-  float x[kBatch];
-  load(from, x);
   float m = -INFINITY, l = 0.f;
-  for (int i = tid; i < n; i += kCombine) {
-    weight[i] = a.ml[2 * slot(i)];
-    m = fmaxf(m, weight[i]);
+  dims y = {};
+  for (int i0 = part; i0 < n; i0 += 64 * W) {
+    const int here = min(64, (n - i0 + W - 1) / W);  // pieces of this round: i0, i0 + W, ..
+    dims x[kBatch];
+    const auto load = [&](int j0) {  // past the end the last one
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        x[j] = *reinterpret_cast<const dims*>(a.part + slot(i0 + W * min(j0 + j, here - 1)) * D + kDims * lane);
+    };
+    load(0);
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (lane < here) ml = reinterpret_cast<const float2*>(a.ml)[slot(i0 + W * lane)];
+    const float top = fmaxf(m, group_max<64>(ml.x)), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    const float w = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);
+    l = fmaf(l, f, group_sum<64>(w * ml.y));
+    y *= f;
+    m = top;
+    for (int j0 = 0;;) {
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (j0 + j < here) y += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), j0 + j)) * x[j];
+      j0 += kBatch;
+      if (j0 >= here) break;
+      load(j0);
+    }
   }
-  m = group_max<64>(m);
-  if (lane == 0) red[0][wave] = m;
-  __syncthreads();
+  if constexpr (W > 1) {
+    float* mine = lds[wave][lane];
+    mine[0] = m;
+    mine[1] = l;
 #pragma unroll
-  for (int i = 0; i < kCombine / 64; ++i) m = fmaxf(m, red[0][i]);
-  for (int i = tid; i < n; i += kCombine) {
-    weight[i] = weight[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(weight[i] - m);
-    l = fmaf(weight[i], a.ml[2 * slot(i) + 1], l);
+    for (int d = 0; d < kDims; ++d) mine[2 + d] = y[d];
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int i = 1; i < W; ++i) m = fmaxf(m, lds[i][lane][0]);
+    const float f = mine[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mine[0] - m);
+    l *= f;
+    y *= f;
+#pragma unroll
+    for (int i = 1; i < W; ++i) {
+      const float* other = lds[i][lane];
+      const float w = other[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(other[0] - m);
+      l = fmaf(w, other[1], l);
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) y[d] = fmaf(w, other[2 + d], y[d]);
+    }
   }
-  l = group_sum<64>(l);
-  if (lane == 0) red[1][wave] = l;
-  __syncthreads();
-  float y = 0.f;
-  for (int i = from;;) {
+  typedef T out __attribute__((ext_vector_type(kDims)));
+  out z;
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j)
-      if (i + j * kLanes < n) y = fmaf(weight[i + j * kLanes], x[j], y);
-    i += kBatch * kLanes;
-    if (i >= n) break;
-    load(i, x);
-  }
-  sum[from][d] = y;
-  __syncthreads();
-  if (tid >= D) return;
-  l = 0.f;
-#pragma unroll
-  for (int i = 0; i < kCombine / 64; ++i) l += red[1][i];
-#pragma unroll
-  for (int j = 1; j < kLanes; ++j) y += sum[j][d];
-  static_cast<T*>(a.out)[seq * a.o_row + head * a.o_head + d] = static_cast<T>(l == 0.f || a.lens[seq] <= 0 ? 0.f : y / l);
+  for (int d = 0; d < kDims; ++d) z[d] = static_cast<T>(l == 0.f || a.lens[seq] <= 0 ? 0.f : y[d] / l);
+  *reinterpret_cast<out*>(static_cast<T*>(a.out) + seq * a.o_row + head * a.o_head + kDims * lane) = z;
 }
 
 // What of a call goes by sizes alone (the lengths are on the device).
@@ -807,7 +896,7 @@ struct PagedSizes {
   int cols, want, waves, direct_waves;
   int64_t most, slots, ints, floats;  // pieces, 16-column results, the plan's words, workspace
 };
-constexpr int kDirectRows = 1024, kWantBlocks = 512;
+constexpr int kDirectRows = 1024, kWantBlocks = 512, kManyHeads = 512;
 
 PagedSizes paged_sizes(int n_seq, int heads, int kv_heads, int64_t capacity, int groups, int dim) {
   PagedSizes p = {};
@@ -876,17 +965,19 @@ extern "C" int fw_decode_attention_paged(const void* q, int64_t q_row, int64_t q
   const PagedSizes p = paged_sizes(n_seq, heads, kv_heads, static_cast<int64_t>(width) * page, groups, head_dim);
   if (!ws || ws_floats < p.floats || !aligned(ws, 16))
     return fw_fail(FW_EINVAL, "%s: workspace needs %lld floats, 16-byte aligned", what, static_cast<long long>(p.floats));
+  const int64_t all = static_cast<int64_t>(heads) * n_seq;
+  const bool many = all >= kManyHeads;  // the joining launch has a wave for each, else four
   const int group = heads / kv_heads, parts = (group + kCols - 1) / kCols;
   const int waves = p.most ? p.waves : p.direct_waves, cols = p.cols ? kCols : std::min(kCols, group);
   const int64_t blocks = kv_heads * (p.most ? p.most : static_cast<int64_t>(n_seq) * parts);
-  if (!grid_ok(blocks, 64 * waves) || p.slots > 0x7FFFFFFF / kCols) return fw_fail(FW_EINVAL, "%s: too many sequences", what);
+  if (!grid_ok(blocks, 64 * waves) || !grid_ok((all + 3) / 4, 256) || p.slots > 0x7FFFFFFF / kCols) return fw_fail(FW_EINVAL, "%s: too many sequences", what);
   PagedArgs a{q, k_pages, v_pages, out, q_row, q_head, o_row, o_head, table, lens, cu_groups, shared, n_seq, heads, kv_heads,
               groups, width, n_pages, page_shift_of(page), scale, p.cols, p.want, static_cast<uint32_t>(kTileKeys * p.waves),
-              static_cast<uint32_t>(kTileKeys * p.waves), static_cast<int>(p.most),
-              reinterpret_cast<int*>(ws), ws + p.ints, nullptr};
+              static_cast<int>(p.most), reinterpret_cast<int*>(ws),
+              ws + p.ints, nullptr};
   a.ml = a.part + p.slots * kv_heads * kCols * head_dim;
   int lds = head_dim == 64 ? PagedMerge<64>::bytes(waves, cols) : PagedMerge<128>::bytes(waves, cols);
-  if (p.cols > kCols) lds = std::max(lds, kStages * 2 * kTileKeys * head_dim * 2);
+  if (p.cols > kCols) lds = std::max(lds, kStages * kStep * 2 * kTileKeys * head_dim * 2);
   if (p.most && (n_seq > kWavePlan || groups > kWavePlan)) {
     hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, a);
     if (const int rc = fw_check_launch(what)) return rc;
@@ -894,12 +985,13 @@ extern "C" int fw_decode_attention_paged(const void* q, int64_t q_row, int64_t q
   const auto run = [&](auto t, auto d) {
     typedef decltype(t) T;
     constexpr int D = decltype(d)::value;
-    const auto kernel = !p.most ? paged_attention_kernel<T, D, -1> : p.cols == kCols ? paged_attention_kernel<T, D, 0>
-                        : p.cols == 64 ? paged_attention_kernel<T, D, 1> : paged_attention_kernel<T, D, 2>;
+    const auto kernel = !p.most ? paged_attention_kernel<T, D, -1> : p.cols == kCols ? paged_attention_kernel<T, D, 0> : p.cols == 64 ? paged_attention_kernel<T, D, 1>
+                                                                                     : paged_attention_kernel<T, D, 2>;
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(64 * waves), lds, stream, a);
     if (const int rc = fw_check_launch(what)) return rc;
     if (!p.most) return static_cast<int>(FW_OK);
-    hipLaunchKernelGGL((paged_combine_kernel<T, D>), dim3(heads, n_seq), dim3(kCombine), 0, stream, a);
+    const auto combine = many ? paged_combine_kernel<T, D, 1> : paged_combine_kernel<T, D, 4>;
+    hipLaunchKernelGGL(combine, dim3(static_cast<unsigned>(many ? (all + 3) / 4 : all)), dim3(256), 0, stream, a);
     return fw_check_launch("decode_attention_paged combine");
   };
   const std::integral_constant<int, 64> d64;

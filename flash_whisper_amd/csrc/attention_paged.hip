@@ -896,14 +896,15 @@ struct PagedSizes {
   int cols, want, waves, direct_waves;
   int64_t most, slots, ints, floats;  // pieces, 16-column results, the plan's words, workspace
 };
-constexpr int kDirectRows = 1024, kWantBlocks = 512, kManyHeads = 512;
+constexpr int kDirectRows = 1024, kDirectMany = 2048, kDirectFew = 768, kManyItems = 128, kWantBlocks = 512, kManyHeads = 512;
 
 PagedSizes paged_sizes(int n_seq, int heads, int kv_heads, int64_t capacity, int groups, int dim) {
   PagedSizes p = {};
   const int64_t group = heads / kv_heads, parts = (group + kCols - 1) / kCols;
   p.direct_waves = static_cast<int>(std::min<int64_t>(8, (capacity + kTileKeys - 1) / kTileKeys));
   p.waves = kWaves;
-  if (capacity <= kDirectRows) {
+  const bool many_items = static_cast<int64_t>(n_seq) * kv_heads * parts >= kManyItems;
+  if (capacity <= (many_items ? groups ? kDirectRows : kDirectMany : dim == 64 ? kDirectRows : kDirectFew)) {
     p.floats = 4;
     return p;
   }
@@ -911,7 +912,7 @@ PagedSizes paged_sizes(int n_seq, int heads, int kv_heads, int64_t capacity, int
   p.cols = columns > 64 ? 128 : columns > kCols ? 64 : kCols;
   p.want = std::max(1, kWantBlocks / kv_heads);
   // each run of columns has the pieces that fill its share of `want`, and one more
-  const int64_t runs = groups ? n_seq * group / p.cols + groups : 0;
+  const int64_t runs = groups ? n_seq * group / p.cols + std::min(groups, n_seq / 2) : 0;
   p.most = p.want + runs + n_seq * parts + 1;
   p.slots = p.cols / kCols * (p.want + runs) + n_seq * parts + 1;
   p.ints = 4 + 8 * p.most + 8 * static_cast<int64_t>(n_seq) + (n_seq <= kPlanLds && groups <= kPlanLds ? 0 : plan_words(n_seq, groups));

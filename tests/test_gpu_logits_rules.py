@@ -88,6 +88,33 @@ def test_each_rule(hip_device, dtype, kwargs):
     check(run(hip_device, x, rules), x, rules, dtype)
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+def test_long_lists(hip_device, dtype):
+    """Histories and lists too long for a cell of both: counts of 32767 and more, places past 65535; beside them short ones."""
+    rng = np.random.default_rng(21)
+    vocab, lengths, listed = 9001, [32767, 32768, 90000, 0, 10], [65535, 65536, 3, 70000, 0]
+    x, _ = make(rng, 5, vocab, dtype)
+    tokens = rng.integers(0, vocab, sum(lengths))
+    tokens[:32767] = 17                           # one token alone: the largest count that a cell holds
+    tokens[32767 + 32768:32767 + 32768 + 60000] = 4096
+    rules = dict(tokens=tokens, cu=np.r_[0, np.cumsum(lengths)], prompt=np.array([0, 5, 100, 0, 3]),
+                 repetition=rng.uniform(0.5, 2, 5).astype(np.float32), presence=rng.uniform(-1, 2, 5).astype(np.float32),
+                 frequency=rng.uniform(-1e-3, 1e-3, 5).astype(np.float32), bias_ids=rng.integers(-5, vocab + 5, sum(listed)),
+                 bias=rng.uniform(-9, 9, sum(listed)).astype(np.float32), cu_bias=np.r_[0, np.cumsum(listed)])
+    check(run(hip_device, x, rules), x, rules, dtype)
+    check(run(hip_device, x, {k: v for k, v in rules.items() if 'bias' not in k}), x, {k: v for k, v in rules.items() if 'bias' not in k}, dtype)
+    check(run(hip_device, x, {k: v for k, v in rules.items() if 'bias' in k}), x, {k: v for k, v in rules.items() if 'bias' in k}, dtype)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('rows, vocab, history', [(3, 20001, 300), (3, 20001, 3000), (90, 100001, 2500)])
+def test_slices(hip_device, dtype, rows, vocab, history):
+    """Slices of each size, the last of a row partial."""
+    rng = np.random.default_rng(rows + history)
+    x, rules = make(rng, rows, vocab, dtype, history=history, biased=40, sets=2)
+    check(run(hip_device, x, rules), x, rules, dtype)
+
+
 def test_mask_forms(hip_device):
     """One set for all rows, a set for each row, more sets and words than needed."""
     rng = np.random.default_rng(4)

@@ -250,17 +250,6 @@ struct PagedMerge {
 __device__ __forceinline__ Piece* pieces_of(const PagedArgs& a) { return reinterpret_cast<Piece*>(a.plan + 4); }
 __device__ __forceinline__ Owner* owners_of(const PagedArgs& a) { return reinterpret_cast<Owner*>(pieces_of(a) + a.most); }
 
-// Inclusive sum over the wave by DPP: within rows of 16 lanes, then row 0 to 1 and 2 to 3, then the lower half to the upper.
-__device__ __forceinline__ int wave_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);   // row_shr:1
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);   // row_shr:2
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);   // row_shr:4
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);   // row_shr:8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 to rows 1 and 3
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 to rows 2 and 3
-  return v;
-}
-
 // ------------------------------------------------------------------------------------------
 // The plan turns the lengths into pieces. A group's shared rows are those that all its live sequences have, cut to whole
 // tiles unless they are all that any of them has. All keys, times the runs of columns that see them, make about `want` pieces, a

@@ -53,11 +53,7 @@ __device__ __forceinline__ int64_t map_slot(const MapArgs& a, int s, int64_t row
 // Inclusive sum over the block's threads of v; `part` holds a sum for each wave.
 __device__ __forceinline__ int block_scan(int v, int* part, int& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int x = __shfl_up(v, o);
-    if (lane >= o) v += x;
-  }
+  v = wave_scan(v);
   __syncthreads();  // `part` of the call before is read
   if (lane == 63) part[wave] = v;
   __syncthreads();
@@ -137,6 +133,19 @@ __global__ void __launch_bounds__(kTile) kv_page_map_kernel(MapArgs a) {
       if (rank + i < top)
         a.table[static_cast<int64_t>(t * kTile + l) * a.width + from[l] + (i - before[l])] = a.stack[top - 1 - rank - i];
     }
+    if (SLOTS) {  // (of pages taken now from the stack itself: the table's entries may not be there yet)
+      const int end = static_cast<int>(within(a.cu[a.n_seq], 0, a.rows));
+      for (int r = begin[0] + tid; r < end; r += kTile) {
+        const int l = last_up_to(begin, a.n_seq, r);
+        const int64_t at = first[l] + (r - begin[l]), entry = at >> a.page_shift;
+        int64_t slot = -1;
+        if (first[l] >= 0 && at >= 0 && entry < holds[l]) {
+          const int64_t page = entry < from[l] ? a.table[static_cast<int64_t>(l) * a.width + entry] : a.stack[top - 1 - before[l] - (entry - from[l])];
+          slot = (page << a.page_shift) + (at & ((int64_t{1} << a.page_shift) - 1));
+        }
+        a.slots[r] = slot;
+      }
+    }
     rank += total;
     __syncthreads();
   }
@@ -149,12 +158,6 @@ __global__ void __launch_bounds__(kTile) kv_page_map_kernel(MapArgs a) {
     for (int w = 1; w < kTile / 64; ++w) missing += lost[w];
     a.count_out[0] = max(top - rank, int64_t{0});
     a.count_out[1] = missing;
-  }
-  if (!SLOTS) return;
-  const int end = static_cast<int>(within(a.cu[a.n_seq], 0, a.rows));
-  for (int r = begin[0] + tid; r < end; r += kTile) {
-    const int l = last_up_to(begin, a.n_seq, r);
-    a.slots[r] = first[l] < 0 ? -1 : map_slot(a, l, first[l] + (r - begin[l]), holds[l]);
   }
 }
 

@@ -892,14 +892,15 @@ PagedSizes paged_sizes(int n_seq, int heads, int kv_heads, int64_t capacity, int
   const int64_t group = heads / kv_heads, parts = (group + kCols - 1) / kCols;
   p.direct_waves = static_cast<int>(std::min<int64_t>(8, (capacity + kTileKeys - 1) / kTileKeys));
   p.waves = kWaves;
+  if (groups >= n_seq) groups = 0;  // a sequence each: nothing is shared
   const bool many_items = static_cast<int64_t>(n_seq) * kv_heads * parts >= kManyItems;
   if (capacity <= (many_items ? groups ? kDirectRows : kDirectMany : dim == 64 ? kDirectRows : kDirectFew)) {
     p.floats = 4;
     return p;
   }
   const int64_t columns = groups ? (n_seq + groups - 1) / groups * group : 0;  // of an average group
-  p.cols = columns > 64 ? 128 : columns > kCols ? 64 : kCols;
-  p.want = std::max(1, kWantBlocks / kv_heads);
+  p.cols = columns > 256 ? 128 : columns > kCols ? 64 : kCols;
+  p.want = std::max(1, (columns > 64 && columns <= 256 ? kWantBlocks / 2 : kWantBlocks) / kv_heads);
   // each run of columns has the pieces that fill its share of `want`, and one more
   const int64_t runs = groups ? n_seq * group / p.cols + std::min(groups, n_seq / 2) : 0;
   p.most = p.want + runs + n_seq * parts + 1;
@@ -953,6 +954,7 @@ extern "C" int fw_decode_attention_paged(const void* q, int64_t q_row, int64_t q
   if (!rows_ok(q, q_row, q_head) || !rows_ok(out, o_row, o_head) || !aligned(k_pages, 16) || !aligned(v_pages, 16))
     return fw_fail(FW_EINVAL, "%s: q, out and the pages must be 16-byte aligned with strides in multiples of 8", what);
   const PagedSizes p = paged_sizes(n_seq, heads, kv_heads, static_cast<int64_t>(width) * page, groups, head_dim);
+  if (groups >= n_seq) groups = 0;
   if (!ws || ws_floats < p.floats || !aligned(ws, 16))
     return fw_fail(FW_EINVAL, "%s: workspace needs %lld floats, 16-byte aligned", what, static_cast<long long>(p.floats));
   const int64_t all = static_cast<int64_t>(heads) * n_seq;

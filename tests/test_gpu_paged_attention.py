@@ -124,7 +124,10 @@ def test_alone_long(hip_device, dtype, dim, page, kv_heads, group, lens):
     ([20], [1216], 60, 1, 4),                      # 80 columns in several runs
     ([7, 9], [2000, 31], 500, 1, 20),              # 20 heads a key/value head; less than a tile shared
     ([40], [1100], 3, 1, 1),                       # more than 32 sequences
-    ([1, 1, 3], [1200, 0, 33], 1200, 2, 2)])
+    ([1, 1, 3], [1200, 0, 33], 1200, 2, 2),
+    ([20], [1500], 0, 1, 16),                      # 320 columns: 128 in a run, the last one partial
+    ([3, 30], [1300, 1411], 70, 1, 20),
+    ([2, 2, 2], [1290, 1300, 1400], 200, 2, 32)])  # 64 columns: all of a run
 def test_groups(hip_device, dtype, dim, page, groups, shared, rest, kv_heads, group):
     """Groups of every make, and the same sequences without them: both within the bound."""
     n = sum(groups)
@@ -178,6 +181,30 @@ def test_bad_pages(hip_device, page, spare):
     out = scene.run(hip_device)
     scene.check(out)
     assert not out[3].any()
+
+
+@pytest.mark.parametrize('page, dim', [(16, 64), (16, 128), (64, 64), (64, 128)])
+@pytest.mark.parametrize('group', [5, 70])
+def test_bad_pages_of_many_columns(hip_device, page, dim, group):
+    """Entries that are no page among shared rows that many columns see, at halves and ends of steps, and in the last one."""
+    scene = Scene(20, [5, 1], [1500, 0], [0, 0, 0, 0, 0, 700], page, 1, group, dim, 'bf16')
+    t = scene.table
+    for j in (0, 1, 2, 3, 5, 8, 13, 1499 // page):
+        if j <= 1499 // page:
+            t[:5, j] = (-1, len(scene.k), 2 ** 31 - 1)[j % 3]
+    scene.check(scene.run(hip_device))
+    t[:5] = -1
+    out = scene.run(hip_device)
+    scene.check(out)
+    assert not out[:5].any()
+
+
+def test_groups_of_one(hip_device):
+    """As many groups as sequences: taken as none, whatever they say."""
+    scene = Scene(21, [1] * 6, [0] * 6, [1300, 5, 0, 900, 33, 64], 32, 2, 2, 64, 'fp16', spare_width=20)
+    for cu, shared in ((np.arange(7), [900] * 6), ([0, 6, 6, 6, 6, 6, 6], [0] * 6)):
+        scene.cu, scene.shared = np.array(cu), np.array(shared)
+        scene.check(scene.run(hip_device))
 
 
 def test_seen_with_hidden_nan(hip_device):

@@ -369,7 +369,10 @@ __device__ __forceinline__ Plan make_plan(const PagedArgs& a, int* mem) {
   __syncthreads();
   int64_t work = 0;
   for (int g = tid; g < p.groups; g += threads) {
-    const int most = p.starts[g + 1] - p.starts[g] > 1 && p.high[g] > 0 ? min(p.rows[g], p.low[g]) : 0, whole = most == p.high[g];
+    // (read where the atomics left them, which may be memory)
+    const int low = __hip_atomic_load(&p.low[g], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const int high = __hip_atomic_load(&p.high[g], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const int most = p.starts[g + 1] - p.starts[g] > 1 && high > 0 ? min(p.rows[g], low) : 0, whole = most == high;
     p.rows[g] = whole ? most : most & ~(kTileKeys - 1);
     p.low[g] = whole;
     work += static_cast<int64_t>(p.rows[g]) * p.runs_of(g);
@@ -887,10 +890,13 @@ struct PagedSizes {
 };
 constexpr int kDirectRows = 1024, kDirectMany = 2048, kDirectFew = 768, kManyItems = 128, kWantBlocks = 512, kManyHeads = 512;
 
+int merge_bytes(int dim, int waves, int cols) { return dim == 64 ? PagedMerge<64>::bytes(waves, cols) : PagedMerge<128>::bytes(waves, cols); }
+
 PagedSizes paged_sizes(int n_seq, int heads, int kv_heads, int64_t capacity, int groups, int dim) {
   PagedSizes p = {};
   const int64_t group = heads / kv_heads, parts = (group + kCols - 1) / kCols;
   p.direct_waves = static_cast<int>(std::min<int64_t>(8, (capacity + kTileKeys - 1) / kTileKeys));
+  while (merge_bytes(dim, p.direct_waves, static_cast<int>(std::min<int64_t>(kCols, group))) > 65536) --p.direct_waves;
   p.waves = kWaves;
   if (groups >= n_seq) groups = 0;  // a sequence each: nothing is shared
   const bool many_items = static_cast<int64_t>(n_seq) * kv_heads * parts >= kManyItems;
@@ -968,7 +974,7 @@ extern "C" int fw_decode_attention_paged(const void* q, int64_t q_row, int64_t q
               static_cast<int>(p.most), reinterpret_cast<int*>(ws),
               ws + p.ints, nullptr};
   a.ml = a.part + p.slots * kv_heads * kCols * head_dim;
-  int lds = head_dim == 64 ? PagedMerge<64>::bytes(waves, cols) : PagedMerge<128>::bytes(waves, cols);
+  int lds = merge_bytes(head_dim, waves, cols);
   if (p.cols > kCols) lds = std::max(lds, kStages * kStep * 2 * kTileKeys * head_dim * 2);
   if (p.most && (n_seq > kWavePlan || groups > kWavePlan)) {
     hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, a);

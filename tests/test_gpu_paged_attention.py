@@ -255,6 +255,26 @@ def test_many_sequences(hip_device):
     scene.check(scene.run(hip_device, groups=False))
 
 
+@pytest.mark.parametrize('groups, shared', [([1500], [65]), ([2, 1400], [40, 70]), ([1] * 100 + [1300] + [1] * 50, [0] * 100 + [33] + [0] * 50)])
+def test_many_sequences_few_groups(hip_device, groups, shared):
+    n = sum(groups)
+    scene = Scene(22, groups, shared, _rest(22, n, 0, 40), 16, 1, 1, 64, 'bf16', spare_width=70, idle=[3, 1000])
+    scene.check(scene.run(hip_device))
+
+
+@pytest.mark.parametrize('spare', [0, 70])
+def test_lengths_past_the_table(hip_device, spare):
+    """A sequence longer than its table has the table's rows; the smallest length is idle."""
+    scene = Scene(23, [3], [128], [64, 128, 32], 32, 2, 2, 64, 'fp16', spare_width=spare)
+    scene.table[scene.table < 0] = 0
+    scene.k, scene.v = torch.nan_to_num(scene.k), torch.nan_to_num(scene.v)
+    scene.lens = np.array([2 ** 63 - 1, 2 ** 31 + 5, -2 ** 63])
+    scene.shared = np.array([128])
+    out = scene.run(hip_device)
+    scene.check(out)
+    assert not out[2].any()
+
+
 def test_far_pages(hip_device):
     """Pages past 2^31 elements of an array."""
     from flash_whisper_amd.ext import KvPages

@@ -77,12 +77,11 @@ def test_workspace_sizes(built_lib):
     for bad in ((0, 20, 20, 28, 16, 1, 64), (5, 20, 8, 28, 16, 1, 64), (5, 20, 20, 28, 24, 1, 64), (5, 20, 20, 0, 16, 1, 64),
                 (5, 20, 20, 28, 16, -1, 64), (5, 20, 20, 28, 16, 1, 96), (1 << 20, 20, 20, 28, 16, 1, 64)):
         assert need(*bad) == 0
-    # results of every piece there may be: some 1024 blocks, two more a group's run of columns, one more a sequence
-    for n, heads, kv, groups, dim in ((1, 1, 1, 0, 64), (65535, 64, 8, 65535, 128), (4096, 16384, 1, 3, 64), (64, 16384, 16384, 64, 64)):
-        group = heads // kv
-        runs = n * group // 16 + groups if groups else 0
-        slots = 2 * (max(1, 1024 // kv) + runs) + n * -(-group // 16) + 1
-        assert 0 < need(n, heads, kv, 1 << 20, 256, groups, dim) <= slots * (kv * 16 * (dim + 2) + 8) + 17 * (n + groups) + 16
+    # results of every piece there may be: 512 blocks' worth, one more for a run of a group's columns, one more a sequence; and the plan
+    for n, heads, kv, groups, dim in ((1, 1, 1, 0, 64), (65535, 64, 8, 60000, 128), (4096, 16384, 1, 3, 64), (64, 16384, 16384, 60, 64), (64, 32, 8, 1, 128)):
+        group, want = heads // kv, max(1, 512 // kv)
+        slots = max(c // 16 * (want + n * group // c + groups) for c in (16, 64, 128)) + n * -(-group // 16) + 1
+        assert 0 < need(n, heads, kv, 1 << 20, 256, groups, dim) <= slots * (kv * 16 * (dim + 2) + 8) + 11 * n + 5 * groups + 16
 
 
 def _cpu_cache(ext, dtype=torch.float16):

@@ -524,62 +524,79 @@ struct WavePlan {
   }
 };
 
-template <class T, int D, int CT>
-__device__ __forceinline__ void paged_piece(const PagedArgs& a, const Piece& p, int kvh, const int32_t* table, float* lds) {
+// The queries of 16 columns from `col` on of the sequences from `seq` on; columns past the last of `cols` repeat it.
+template <class T, int D>
+__device__ __forceinline__ void paged_queries(const PagedArgs& a, int seq, int col, int cols, int kvh, int lane, typename Types<T>::v8 (&q)[D / 32]) {
   typedef typename Types<T>::v8 v8;
-  const int waves = blockDim.x / 64, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int i = lane & 15, g = lane >> 4, group = a.heads / a.kv_heads;
-  v8 q[CT][D / 32];
+  const int group = a.heads / a.kv_heads, x = col + min(lane & 15, cols - 1);
+  const T* at = static_cast<const T*>(a.q) + (seq + x / group) * a.q_row + (kvh * group + x % group) * a.q_head + 8 * (lane >> 4);
 #pragma unroll
-  for (int c = 0; c < CT; ++c) {
-    const int col = p.col + min(16 * c + i, p.cols - 1);  // columns past the end repeat the last one
-    const T* at = static_cast<const T*>(a.q) + (p.seq + col / group) * a.q_row + (kvh * group + col % group) * a.q_head + 8 * g;
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) {
-      q[c][j] = *reinterpret_cast<const v8*>(at + 32 * j);
-      if (a.scale < 0.f) q[c][j] = -q[c][j];  // scores are scaled by a positive factor after the product
-    }
+  for (int j = 0; j < D / 32; ++j) {
+    q[j] = *reinterpret_cast<const v8*>(at + 32 * j);
+    if (a.scale < 0.f) q[j] = -q[j];  // scores are scaled by a positive factor after the product
   }
-  // 0: the smallest number instead; a hidden score (-infinity) times zero would be NaN
-  const float factor = fmaxf(__builtin_fabsf(a.scale) * kLog2e, __FLT_DENORM_MIN__);
-  PagedState<T, D, CT> st;
-  paged_tiles<T, D, CT>(a, table, kvh, p.begin / kTileKeys + wave, waves, p.end, q, factor, lane, st);
+}
+// 0: the smallest number instead; a hidden score (-infinity) times zero would be NaN.
+__device__ __forceinline__ float paged_factor(const PagedArgs& a) { return fmaxf(__builtin_fabsf(a.scale) * kLog2e, __FLT_DENORM_MIN__); }
+
+// A wave's results of columns [first, last) to part `part`.
+template <class T, int D>
+__device__ __forceinline__ void paged_hand_in(const PagedMerge<D>& x, const PagedState<T, D, 1>& st, int part, int first, int last, int lane) {
+  const int i = lane & 15, g = lane >> 4;
+  const float l = xor_add<32>(xor_add<16>(st.l[0]));
+  if (i < first || i >= last) return;
+  if (g == 0) {
+    x.m[part * kCols + i] = st.m[0];
+    x.l[part * kCols + i] = l;
+  }
+  float* to = x.acc + (part * x.cols + i) * PagedMerge<D>::kPitch + 4 * g;
 #pragma unroll
-  for (int c = 0; c < CT; ++c) {
-    const int cols = min(kCols, p.cols - kCols * c);
-    if (cols <= 0) break;
-    const PagedMerge<D> x(lds, waves, cols);
-    const float own_l = xor_add<32>(xor_add<16>(st.l[c]));
-    if (c > 0) __syncthreads();
-    if (i < cols) {
-      if (g == 0) {
-        x.m[wave * kCols + i] = st.m[c];
-        x.l[wave * kCols + i] = own_l;
-      }
-      float* to = x.acc + (wave * cols + i) * PagedMerge<D>::kPitch + 4 * g;
-#pragma unroll
-      for (int db = 0; db < D / 16; ++db) *reinterpret_cast<f4v*>(to + 16 * db) = st.o[c][db];
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < cols * D; e += blockDim.x) {
-      const int col = e / D, d = e % D;
-      float m = -INFINITY, l = 0.f, o = 0.f;
-      for (int w = 0; w < waves; ++w) m = fmaxf(m, x.m[w * kCols + col]);
-      for (int w = 0; w < waves; ++w) {
-        const float mw = x.m[w * kCols + col], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - m);
-        l = fmaf(f, x.l[w * kCols + col], l);
-        o = fmaf(f, x.acc[(w * cols + col) * PagedMerge<D>::kPitch + d], o);
-      }
-      if (p.slot < 0) {
-        const int at = p.col + kCols * c + col, seq = p.seq + at / group, head = kvh * group + at % group;
-        // (an idle sequence of a group sees nothing, whatever its group sees)
-        const float y = l == 0.f || a.lens[seq] <= 0 ? 0.f : o / l;
-        static_cast<T*>(a.out)[seq * a.o_row + head * a.o_head + d] = static_cast<T>(y);
-      } else {
-        const int64_t at = (static_cast<int64_t>(p.slot + c) * a.kv_heads + kvh) * kCols + col;
-        a.part[at * D + d] = o;
-        if (d == 0) reinterpret_cast<float2*>(a.ml)[at] = make_float2(m, l);
-      }
+  for (int db = 0; db < D / 16; ++db) *reinterpret_cast<f4v*>(to + 16 * db) = st.o[0][db];
+}
+
+// The sum over the parts for column col and dim d: o and l relative to exp2(m).
+template <int D>
+__device__ __forceinline__ float paged_sum(const PagedMerge<D>& x, int parts, int col, int d, float& m, float& l) {
+  m = -INFINITY;
+  l = 0.f;
+  float o = 0.f;
+  for (int w = 0; w < parts; ++w) m = fmaxf(m, x.m[w * kCols + col]);
+  for (int w = 0; w < parts; ++w) {
+    const float mw = x.m[w * kCols + col], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - m);
+    l = fmaf(f, x.l[w * kCols + col], l);
+    o = fmaf(f, x.acc[(w * x.cols + col) * PagedMerge<D>::kPitch + d], o);
+  }
+  return o;
+}
+
+// (An idle sequence of a group sees nothing, whatever its group sees.)
+template <class T>
+__device__ __forceinline__ void paged_store(const PagedArgs& a, int seq, int head, int d, float o, float l) {
+  static_cast<T*>(a.out)[seq * a.o_row + head * a.o_head + d] = static_cast<T>(l == 0.f || a.lens[seq] <= 0 ? 0.f : o / l);
+}
+
+// A piece of at most 16 columns: its tiles in turn to the block's waves.
+template <class T, int D>
+__device__ __forceinline__ void paged_piece(const PagedArgs& a, const Piece& p, int kvh, const int32_t* table, float* lds) {
+  const int waves = blockDim.x / 64, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = a.heads / a.kv_heads;
+  typename Types<T>::v8 q[1][D / 32];
+  paged_queries<T, D>(a, p.seq, p.col, p.cols, kvh, lane, q[0]);
+  PagedState<T, D, 1> st;
+  paged_tiles<T, D, 1>(a, table, kvh, p.begin / kTileKeys + wave, waves, p.end, q, paged_factor(a), lane, st);
+  const PagedMerge<D> x(lds, waves, p.cols);
+  paged_hand_in<T, D>(x, st, wave, 0, p.cols, lane);
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.cols * D; e += blockDim.x) {
+    const int col = e / D, d = e % D;
+    float m, l;
+    const float o = paged_sum<D>(x, waves, col, d, m, l);
+    if (p.slot < 0) {
+      paged_store<T>(a, p.seq + (p.col + col) / group, kvh * group + (p.col + col) % group, d, o, l);
+    } else {
+      const int64_t at = (static_cast<int64_t>(p.slot) * a.kv_heads + kvh) * kCols + col;
+      a.part[at * D + d] = o;
+      if (d == 0) reinterpret_cast<float2*>(a.ml)[at] = make_float2(m, l);
     }
   }
 }
@@ -717,15 +734,10 @@ __device__ __forceinline__ void paged_wide(const PagedArgs& a, const Piece& p, i
   v8 q[CT][D / 32];
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
-    const int col = p.col + min(col0 + kCols * c + i, p.cols - 1);  // columns past the end repeat the last one
-    const T* at = static_cast<const T*>(a.q) + (p.seq + col / group) * a.q_row + (kvh * group + col % group) * a.q_head + 8 * g;
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) {
-      q[c][j] = *reinterpret_cast<const v8*>(at + 32 * j);
-      if (a.scale < 0.f) q[c][j] = -q[c][j];
-    }
+    const int col = min(col0 + kCols * c, p.cols - 1);  // (a wave without columns has the last one's)
+    paged_queries<T, D>(a, p.seq, p.col + col, p.cols - col, kvh, lane, q[c]);
   }
-  const float factor = fmaxf(__builtin_fabsf(a.scale) * kLog2e, __FLT_DENORM_MIN__);
+  const float factor = paged_factor(a);
   PagedState<T, D, CT> st;
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
@@ -785,7 +797,7 @@ __global__ void __launch_bounds__(CT < 0 ? 512 : 64 * kWaves, 2) paged_attention
     const int group = a.heads / a.kv_heads, parts = (group + kCols - 1) / kCols;
     const int col = static_cast<int>(at % parts) * kCols, seq = static_cast<int>(at / parts);
     const Piece p{seq, col, min(kCols, group - col), 0, paged_keys(a, seq), -1, {}};
-    paged_piece<T, D, 1>(a, p, kvh, a.table + static_cast<int64_t>(seq) * a.width, lds);
+    paged_piece<T, D>(a, p, kvh, a.table + static_cast<int64_t>(seq) * a.width, lds);
   } else {
     Piece p;
     if (a.n_seq <= kWavePlan && a.groups <= kWavePlan) {
@@ -805,7 +817,7 @@ __global__ void __launch_bounds__(CT < 0 ? 512 : 64 * kWaves, 2) paged_attention
         return;
       }
     }
-    paged_piece<T, D, 1>(a, p, kvh, table, lds);
+    paged_piece<T, D>(a, p, kvh, table, lds);
   }
 }
 

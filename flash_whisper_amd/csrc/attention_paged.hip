@@ -539,12 +539,12 @@ __device__ __forceinline__ void paged_queries(const PagedArgs& a, int seq, int c
 // 0: the smallest number instead; a hidden score (-infinity) times zero would be NaN.
 __device__ __forceinline__ float paged_factor(const PagedArgs& a) { return fmaxf(__builtin_fabsf(a.scale) * kLog2e, __FLT_DENORM_MIN__); }
 
-// A wave's results of columns [first, last) to part `part`.
+// A wave's results of its first `cols` columns to part `part`.
 template <class T, int D>
-__device__ __forceinline__ void paged_hand_in(const PagedMerge<D>& x, const PagedState<T, D, 1>& st, int part, int first, int last, int lane) {
+__device__ __forceinline__ void paged_hand_in(const PagedMerge<D>& x, const PagedState<T, D, 1>& st, int part, int cols, int lane) {
   const int i = lane & 15, g = lane >> 4;
   const float l = xor_add<32>(xor_add<16>(st.l[0]));
-  if (i < first || i >= last) return;
+  if (i >= cols) return;
   if (g == 0) {
     x.m[part * kCols + i] = st.m[0];
     x.l[part * kCols + i] = l;
@@ -554,48 +554,55 @@ __device__ __forceinline__ void paged_hand_in(const PagedMerge<D>& x, const Page
   for (int db = 0; db < D / 16; ++db) *reinterpret_cast<f4v*>(to + 16 * db) = st.o[0][db];
 }
 
-// The sum over the parts for column col and dim d: o and l relative to exp2(m).
+// The sum over the parts for column col and dims d .. d + 3: o and l relative to exp2(m).
 template <int D>
-__device__ __forceinline__ float paged_sum(const PagedMerge<D>& x, int parts, int col, int d, float& m, float& l) {
+__device__ __forceinline__ f4v paged_sum(const PagedMerge<D>& x, int parts, int col, int d, float& m, float& l) {
   m = -INFINITY;
   l = 0.f;
-  float o = 0.f;
+  f4v o = {};
   for (int w = 0; w < parts; ++w) m = fmaxf(m, x.m[w * kCols + col]);
   for (int w = 0; w < parts; ++w) {
     const float mw = x.m[w * kCols + col], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - m);
     l = fmaf(f, x.l[w * kCols + col], l);
-    o = fmaf(f, x.acc[(w * x.cols + col) * PagedMerge<D>::kPitch + d], o);
+    o += f * *reinterpret_cast<const f4v*>(x.acc + (w * x.cols + col) * PagedMerge<D>::kPitch + d);
   }
   return o;
 }
 
-// (An idle sequence of a group sees nothing, whatever its group sees.)
+// Four dims of a column, or zeros: nothing was seen. (An idle sequence of a group sees nothing, whatever its group sees.)
 template <class T>
-__device__ __forceinline__ void paged_store(const PagedArgs& a, int seq, int head, int d, float o, float l) {
-  static_cast<T*>(a.out)[seq * a.o_row + head * a.o_head + d] = static_cast<T>(l == 0.f || a.lens[seq] <= 0 ? 0.f : o / l);
+__device__ __forceinline__ void paged_store(const PagedArgs& a, int seq, int head, int d, const f4v& o, float l) {
+  typedef T v4 __attribute__((ext_vector_type(4)));
+  const bool none = l == 0.f || a.lens[seq] <= 0;
+  v4 y;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) y[r] = static_cast<T>(none ? 0.f : o[r] / l);
+  *reinterpret_cast<v4*>(static_cast<T*>(a.out) + seq * a.o_row + head * a.o_head + d) = y;
 }
 
-// A piece of at most 16 columns: its tiles in turn to the block's waves.
+// A piece of at most 16 columns: its tiles in turn to the block's waves, as many as there are tiles.
 template <class T, int D>
 __device__ __forceinline__ void paged_piece(const PagedArgs& a, const Piece& p, int kvh, const int32_t* table, float* lds) {
   const int waves = blockDim.x / 64, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int group = a.heads / a.kv_heads;
-  typename Types<T>::v8 q[1][D / 32];
-  paged_queries<T, D>(a, p.seq, p.col, p.cols, kvh, lane, q[0]);
-  PagedState<T, D, 1> st;
-  paged_tiles<T, D, 1>(a, table, kvh, p.begin / kTileKeys + wave, waves, p.end, q, paged_factor(a), lane, st);
+  const int group = a.heads / a.kv_heads, parts = min(waves, (p.end - p.begin + kTileKeys - 1) / kTileKeys);
   const PagedMerge<D> x(lds, waves, p.cols);
-  paged_hand_in<T, D>(x, st, wave, 0, p.cols, lane);
+  if (wave < parts) {
+    typename Types<T>::v8 q[1][D / 32];
+    paged_queries<T, D>(a, p.seq, p.col, p.cols, kvh, lane, q[0]);
+    PagedState<T, D, 1> st;
+    paged_tiles<T, D, 1>(a, table, kvh, p.begin / kTileKeys + wave, waves, p.end, q, paged_factor(a), lane, st);
+    paged_hand_in<T, D>(x, st, wave, p.cols, lane);
+  }
   __syncthreads();
-  for (int e = threadIdx.x; e < p.cols * D; e += blockDim.x) {
-    const int col = e / D, d = e % D;
+  for (int e = threadIdx.x; e < p.cols * (D / 4); e += blockDim.x) {
+    const int col = e / (D / 4), d = e % (D / 4) * 4;
     float m, l;
-    const float o = paged_sum<D>(x, waves, col, d, m, l);
+    const f4v o = paged_sum<D>(x, parts, col, d, m, l);
     if (p.slot < 0) {
       paged_store<T>(a, p.seq + (p.col + col) / group, kvh * group + (p.col + col) % group, d, o, l);
     } else {
       const int64_t at = (static_cast<int64_t>(p.slot) * a.kv_heads + kvh) * kCols + col;
-      a.part[at * D + d] = o;
+      *reinterpret_cast<f4v*>(a.part + at * D + d) = o;
       if (d == 0) reinterpret_cast<float2*>(a.ml)[at] = make_float2(m, l);
     }
   }
@@ -766,17 +773,9 @@ __device__ __forceinline__ void paged_wide(const PagedArgs& a, const Piece& p, i
     const int col = col0 + kCols * c + i;
     if (col >= p.cols) continue;
     if (p.slot < 0) {
-      typedef T v4 __attribute__((ext_vector_type(4)));
       const int seq = p.seq + (p.col + col) / group, head = kvh * group + (p.col + col) % group;
-      const float inv = l == 0.f || a.lens[seq] <= 0 ? 0.f : 1.0f / l;
-      T* to = static_cast<T*>(a.out) + seq * a.o_row + head * a.o_head + 4 * g;
 #pragma unroll
-      for (int db = 0; db < D / 16; ++db) {
-        v4 y;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) y[r] = static_cast<T>(inv == 0.f ? 0.f : st.o[c][db][r] * inv);
-        *reinterpret_cast<v4*>(to + 16 * db) = y;
-      }
+      for (int db = 0; db < D / 16; ++db) paged_store<T>(a, seq, head, 16 * db + 4 * g, st.o[c][db], l);
     } else {
       const int64_t to = (static_cast<int64_t>(p.slot + col / kCols) * a.kv_heads + kvh) * kCols + i;
       if (g == 0) *reinterpret_cast<float2*>(a.ml + 2 * to) = make_float2(st.m[c], l);

@@ -49,6 +49,9 @@ __device__ __forceinline__ float add_pair(b2v x, float s) {
 //  - V: a lane's 8 keys of a dim are 16 bytes of a page.
 //  - The running maximum only moves when a score passes it by kSlack (log2 units), so weights are at most 2^8; they are
 //    rounded to the type, which the matrix instructions take, and their sum, in fp32, is over the rounded ones.
+// Bound by memory where there is much to read (17 sequences of up to 48000 rows in groups of 1 to 7, 64 query heads over 8 of 128:
+// 409 MB in 88 us, 4.6 TB/s, with the joining; 16 of 1500 rows x 20 heads of 64 28 us, 4.4 TB/s), else by the chain of dependent
+// loads (lengths, table, keys, results of the pieces), about 10 us in two launches, 5 in one.
 // ------------------------------------------------------------------------------------------
 struct PagedArgs {
   const void *q, *k, *v;
@@ -254,7 +257,7 @@ __device__ __forceinline__ Owner* owners_of(const PagedArgs& a) { return reinter
 // The plan turns the lengths into pieces. A group's shared rows are those that all its live sequences have, cut to whole
 // tiles unless they are all that any of them has. All keys, times the runs of columns that see them, make about `want` pieces, a
 // multiple of a tile for each wave; the pieces of one run of keys are alike, those of groups come first. Bound by latency, and a
-// launch of its own costs as much as a small call's attention: up to 64 sequences and groups every wave of the attention makes
+// launch of its own costs as much as a small call's attention (6 to 8 us; a wave's own plan 2): up to 64 sequences and groups every wave of the attention makes
 // the plan for itself, a sequence a lane, without barriers, and finds its block's piece in it (WavePlan); more of them are planned by
 // one block, which leaves it in the workspace.
 // ------------------------------------------------------------------------------------------
@@ -611,6 +614,9 @@ __device__ __forceinline__ void paged_piece(const PagedArgs& a, const Piece& p, 
 // A piece of many columns: wave w has columns 16 CT w .. and all of the keys, which arrive in LDS by direct copies, a ring of
 // kStages steps of two tiles, so that a row of K and V is read once for 64 CT columns. A tile of a page is contiguous, V's just as
 // the operands are read; K's 16-byte chunks are swapped within a row so that the 16 rows of a read lie in different banks.
+// Bound by what every block pays once (plan, first tiles, results: about 12 us) and then by the LDS reads, 32 KB a wave and step:
+// 64 answers x 4 heads over 8000 shared rows of 8 heads of 128 take 20 us with the plan, each further 8000 rows 10 (0.84 PFLOP/s); waves
+// that share out the keys instead, 32 columns each, took 62. Steps of one tile, four stages: 2% more.
 constexpr int kStages = 2, kWaves = 4, kStep = 2;
 template <int D>
 __device__ __forceinline__ int wide_swap(int row) {
@@ -899,6 +905,16 @@ struct PagedSizes {
   int cols, want, waves, direct_waves;
   int64_t most, slots, ints, floats;  // pieces, 16-column results, the plan's words, workspace
 };
+// Short tables are not cut up: a block takes a sequence whole, and reads rows that it shares as the others do, which the last-level
+// caches bear. Up to 1024 rows, 768 for few sequences with heads of 128, and 2048 for many of which none shares (us whole / cut:
+// 1 x 20 heads of 64 over 600 rows 5.9 / 9.1, 1000 7.7 / 9.1, 1500 9.7 / 9.2; 1 x 8 heads of 128 over 600 8.7 / 10.5, 1000 12.3 / 10.7;
+// 16 x 20 over 1500 27.8 / 31.2; 64 x 8 of 128 over 2000 91 / 95; 8 groups of 5 x 20 over 400 shared and 100 own rows 11.3 / 13.9,
+// 1000 shared 14.4 / 12.9).
+// Else the keys make about 512 blocks' pieces, one or two a CU at a time (the 17 long sequences above with 256 / 512 / 768 / 1024: 96 / 87 /
+// 93 / 90 us), half as many where a group's columns are 65 to 256, whose results cost as much as keys (64 answers above 34.0 and
+// 36.3 us). Groups of more than 16 columns go by 64 at a time, of more than 256 by 128 (us by 64 / 128: 256 columns over 8000 rows 34.0 /
+// 35.6, 512 over 30000 109 / 99). The joining launch has a wave a query head where there are 512 of them and more (800: 15.6 us a call,
+// with four 16.4; 20: 9.9 and 9.1).
 constexpr int kDirectRows = 1024, kDirectMany = 2048, kDirectFew = 768, kManyItems = 128, kWantBlocks = 512, kManyHeads = 512;
 
 int merge_bytes(int dim, int waves, int cols) { return dim == 64 ? PagedMerge<64>::bytes(waves, cols) : PagedMerge<128>::bytes(waves, cols); }

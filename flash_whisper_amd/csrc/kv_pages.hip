@@ -11,7 +11,7 @@ namespace {
 // back onto the stack of free pages, in the order of sequences and entries, then the missing ones are taken off its top in the
 // same order: an exclusive sum over the sequences gives each its places, so the result depends on nothing else.
 // Bound by latency: one block does all of it in LDS, kTile sequences at a time, and the slots too where the rows are few;
-// else a second launch has a thread for each row.
+// else a second launch has a thread for each row (64 sequences of a token 5.4 us; 600 of which some bring prompts, 83000 rows, 12.1).
 // ------------------------------------------------------------------------------------------
 constexpr int kTile = 1024;
 
@@ -182,6 +182,7 @@ __global__ void __launch_bounds__(256) kv_page_slots_kernel(MapArgs a) {
 // Append: a wave = 8 packed rows x 64 dims of a head (lane = row lane / 8, dims 8 (lane % 8)). K leaves as it came. Of V, 8 rows
 // that fill one unit of 8 are turned in LDS and leave as 16 bytes a lane: they begin anywhere in the wave's 8 rows and end in the
 // next wave's, so each wave looks at the slots of 8 rows before and after its own; other rows leave in pieces of 2 bytes.
+// Bound by memory: 14300 rows of 8 heads of 128 (118 MB) 26.3 us, 4.5 TB/s; a token of each of 40 sequences 4.2 us, a launch.
 // ------------------------------------------------------------------------------------------
 struct AppendArgs {
   const uint16_t *k, *v;

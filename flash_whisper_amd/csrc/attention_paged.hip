@@ -65,7 +65,7 @@ struct PagedArgs {
   int want;           // pieces that all keys are to make, about
   uint32_t unit;      // what a chunk of keys is a multiple of: a tile for each wave
   int most;           // pieces there may be; 0: each sequence is a piece, and nothing is shared
-  int* plan;          // Header, Pieces, Owners, and the plan's arrays where LDS does not hold them
+  int* plan;          // the number of Pieces, they from word 4 on, Owners, and the plan's arrays where LDS does not hold them
   float *part, *ml;   // O [slot][kv head][16][D], (m, l) [slot][kv head][16][2]
 };
 
@@ -86,6 +86,8 @@ struct __align__(16) Owner {
   int slot, n;
   int pad[2];
 };
+
+// The keys that a sequence sees, 0 for an idle one.
 __device__ __forceinline__ int paged_keys(const PagedArgs& a, int seq) {
   return static_cast<int>(within(a.lens[seq], 0, static_cast<int64_t>(a.width) << a.page_shift));
 }
@@ -116,7 +118,7 @@ __device__ __forceinline__ PagedPages paged_pages(const PagedArgs& a, const int3
   return p;
 }
 
-// A lane's addresses in a tile whose rows lie in pages lo and hi: of its two K rows and of its V unit.
+// A tile whose rows lie in pages lo and hi (no page: page 0 is read, and none of it counts): the lane's two rows of K, its unit of V.
 template <class T, int D>
 __device__ __forceinline__ void paged_load_k(const PagedArgs& a, int kvh, int tile, int lo, int hi, int lane, PagedTile<T, D>& t) {
   typedef typename Types<T>::v8 v8;
@@ -138,7 +140,7 @@ __device__ __forceinline__ void paged_load_v(const PagedArgs& a, int kvh, int ti
   for (int db = 0; db < D / 16; ++db) t.v[db] = *reinterpret_cast<const v8*>(at + 128 * db);
 }
 
-// A tile's scores for the columns; masked: only the first `left` of the lane's 8 keys count.
+// A tile's scores for the columns.
 template <class T, int D, int CT>
 __device__ __forceinline__ void paged_scores(const PagedTile<T, D>& t, const typename Types<T>::v8 (&q)[CT][D / 32], f4v (&s)[CT][2]) {
 #pragma unroll
@@ -153,6 +155,7 @@ __device__ __forceinline__ void paged_scores(const PagedTile<T, D>& t, const typ
       for (int kt = 0; kt < 2; ++kt) s[c][kt] = mfma16(t.k[kt][j], q[c][j], s[c][kt]);
 }
 
+// Their weights and the sum over the values; MASKED: only the first `left` of the lane's 8 keys count.
 template <class T, int D, int CT, bool MASKED>
 __device__ __forceinline__ void paged_values(PagedTile<T, D>& t, f4v (&s)[CT][2], float factor, int left, PagedState<T, D, CT>& st) {
   typedef typename Types<T>::v8 v8;
@@ -257,9 +260,9 @@ __device__ __forceinline__ Owner* owners_of(const PagedArgs& a) { return reinter
 // The plan turns the lengths into pieces. A group's shared rows are those that all its live sequences have, cut to whole
 // tiles unless they are all that any of them has. All keys, times the runs of columns that see them, make about `want` pieces, a
 // multiple of a tile for each wave; the pieces of one run of keys are alike, those of groups come first. Bound by latency, and a
-// launch of its own costs as much as a small call's attention (6 to 8 us; a wave's own plan 2): up to 64 sequences and groups every wave of the attention makes
-// the plan for itself, a sequence a lane, without barriers, and finds its block's piece in it (WavePlan); more of them are planned by
-// one block, which leaves it in the workspace.
+// launch of its own costs as much as a small call's attention (6 to 8 us; a wave's own plan 2): up to 64 sequences and groups every
+// wave of the attention makes the plan for itself, a sequence a lane, without barriers, and finds its block's piece in it
+// (WavePlan); more of them are planned by one block, which leaves it in the workspace.
 // ------------------------------------------------------------------------------------------
 constexpr int kPlanThreads = 1024, kPlanLds = 1024;
 
@@ -460,7 +463,7 @@ struct WavePlan {
       // (lane 63 begins no group of several, so what the others tell it is nothing)
       const uint64_t firsts = __builtin_amdgcn_ballot_w64(told > 0 && lane < 63) & (~uint64_t{0} >> (63 - lane));
       const int first = firsts ? 63 - __builtin_clzll(firsts) : lane, g = __shfl(told, first) - 1;
-      const int last = __shfl(e, max(g, 0)), most = static_cast<int>(within(__shfl(static_cast<int>(within(want, 0, 1 << 30)), max(g, 0)), 0, 1 << 30));
+      const int last = __shfl(e, max(g, 0)), most = __shfl(static_cast<int>(within(want, 0, 1 << 30)), max(g, 0));
       const bool in = firsts && lane < last;
       if (in) {
         start = first;
@@ -499,7 +502,8 @@ struct WavePlan {
     const int group = a.heads / a.kv_heads, parts = (group + kCols - 1) / kCols, tiles = a.cols / kCols;
     if (at < of_groups) {
       const int s = __builtin_ctzll(__builtin_amdgcn_ballot_w64(shared_before > at));
-      const int columns = lane_of(members, s) * group, runs = (columns + a.cols - 1) / a.cols, k = lane_of(rows, s), pieces = lane_of(shared_n, s);
+      const int columns = lane_of(members, s) * group, runs = (columns + a.cols - 1) / a.cols;
+      const int k = lane_of(rows, s), pieces = lane_of(shared_n, s);
       const int x = at - (lane_of(shared_before, s) - pieces * runs), i = x / runs, r = x % runs, size = Plan::size_of(k, pieces);
       return Piece{s, r * a.cols, min(a.cols, columns - r * a.cols), i * size, min((i + 1) * size, k),
                    lane_of(whole, s) && pieces == 1 ? -1 : at * tiles, {}};
@@ -529,7 +533,8 @@ struct WavePlan {
 
 // The queries of 16 columns from `col` on of the sequences from `seq` on; columns past the last of `cols` repeat it.
 template <class T, int D>
-__device__ __forceinline__ void paged_queries(const PagedArgs& a, int seq, int col, int cols, int kvh, int lane, typename Types<T>::v8 (&q)[D / 32]) {
+__device__ __forceinline__ void paged_queries(const PagedArgs& a, int seq, int col, int cols, int kvh, int lane,
+                                              typename Types<T>::v8 (&q)[D / 32]) {
   typedef typename Types<T>::v8 v8;
   const int group = a.heads / a.kv_heads, x = col + min(lane & 15, cols - 1);
   const T* at = static_cast<const T*>(a.q) + (seq + x / group) * a.q_row + (kvh * group + x % group) * a.q_head + 8 * (lane >> 4);
@@ -731,7 +736,8 @@ __device__ __forceinline__ void paged_wide(const PagedArgs& a, const Piece& p, i
       const int row = ((first + x) * kTileKeys) & (rows - 1);
       const int64_t at_lo = ((static_cast<int64_t>(max(lo, 0)) * a.kv_heads + kvh) * rows + row) * kRowBytes;
       // (a page of 16 rows: the second half begins another page's rows)
-      const int64_t at_hi = a.page_shift == 4 ? (static_cast<int64_t>(max(hi, 0)) * a.kv_heads + kvh) * rows * kRowBytes - kTile / 2 : at_lo;
+      const int64_t other = (static_cast<int64_t>(max(hi, 0)) * a.kv_heads + kvh) * rows * kRowBytes - kTile / 2;
+      const int64_t at_hi = a.page_shift == 4 ? other : at_lo;
 #pragma unroll
       for (int c = 0; c < kCopies; ++c) {
         const int blk = kCopies * wave + c, r = blk * kCopyRows + lane / (D / 8), chunk = (lane % (D / 8)) ^ wide_swap<D>(r);
@@ -841,7 +847,8 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(PagedArgs a) {
   const int n = o.shared_n + o.n, group = a.heads / a.kv_heads, kvh = head / group, col = head % group, step = (group + kCols - 1) / kCols;
   if ((o.shared_n == 0 || o.shared_slot < 0) && (o.n == 0 || o.slot < 0)) return;  // its block finished it
   const auto slot = [&](int i) {
-    const int c = i < o.shared_n ? o.col + col : col, first = i < o.shared_n ? o.shared_slot + i * o.shared_step : o.slot + (i - o.shared_n) * step;
+    const bool shared = i < o.shared_n;
+    const int c = shared ? o.col + col : col, first = shared ? o.shared_slot + i * o.shared_step : o.slot + (i - o.shared_n) * step;
     return (static_cast<int64_t>(first + c / kCols) * a.kv_heads + kvh) * kCols + c % kCols;
   };
   float m = -INFINITY, l = 0.f;
@@ -910,14 +917,16 @@ struct PagedSizes {
 // 1 x 20 heads of 64 over 600 rows 5.9 / 9.1, 1000 7.7 / 9.1, 1500 9.7 / 9.2; 1 x 8 heads of 128 over 600 8.7 / 10.5, 1000 12.3 / 10.7;
 // 16 x 20 over 1500 27.8 / 31.2; 64 x 8 of 128 over 2000 91 / 95; 8 groups of 5 x 20 over 400 shared and 100 own rows 11.3 / 13.9,
 // 1000 shared 14.4 / 12.9).
-// Else the keys make about 512 blocks' pieces, one or two a CU at a time (the 17 long sequences above with 256 / 512 / 768 / 1024: 96 / 87 /
-// 93 / 90 us), half as many where a group's columns are 65 to 256, whose results cost as much as keys (64 answers above 34.0 and
+// Else the keys make about 512 blocks' pieces, one or two a CU at a time (the 17 long sequences above with 256 / 512 / 768 / 1024:
+// 96 / 87 / 93 / 90 us), half as many where a group's columns are 65 to 256, whose results cost as much as keys (64 answers above 34.0 and
 // 36.3 us). Groups of more than 16 columns go by 64 at a time, of more than 256 by 128 (us by 64 / 128: 256 columns over 8000 rows 34.0 /
 // 35.6, 512 over 30000 109 / 99). The joining launch has a wave a query head where there are 512 of them and more (800: 15.6 us a call,
 // with four 16.4; 20: 9.9 and 9.1).
 constexpr int kDirectRows = 1024, kDirectMany = 2048, kDirectFew = 768, kManyItems = 128, kWantBlocks = 512, kManyHeads = 512;
 
-int merge_bytes(int dim, int waves, int cols) { return dim == 64 ? PagedMerge<64>::bytes(waves, cols) : PagedMerge<128>::bytes(waves, cols); }
+int merge_bytes(int dim, int waves, int cols) {
+  return dim == 64 ? PagedMerge<64>::bytes(waves, cols) : PagedMerge<128>::bytes(waves, cols);
+}
 
 PagedSizes paged_sizes(int n_seq, int heads, int kv_heads, int64_t capacity, int groups, int dim) {
   PagedSizes p = {};
@@ -995,7 +1004,8 @@ extern "C" int fw_decode_attention_paged(const void* q, int64_t q_row, int64_t q
   const int group = heads / kv_heads, parts = (group + kCols - 1) / kCols;
   const int waves = p.most ? p.waves : p.direct_waves, cols = p.cols ? kCols : std::min(kCols, group);
   const int64_t blocks = kv_heads * (p.most ? p.most : static_cast<int64_t>(n_seq) * parts);
-  if (!grid_ok(blocks, 64 * waves) || !grid_ok((all + 3) / 4, 256) || p.slots > 0x7FFFFFFF / kCols) return fw_fail(FW_EINVAL, "%s: too many sequences", what);
+  if (!grid_ok(blocks, 64 * waves) || !grid_ok((all + 3) / 4, 256) || p.slots > 0x7FFFFFFF / kCols)
+    return fw_fail(FW_EINVAL, "%s: too many sequences", what);
   PagedArgs a{q, k_pages, v_pages, out, q_row, q_head, o_row, o_head, table, lens, cu_groups, shared, n_seq, heads, kv_heads,
               groups, width, n_pages, page_shift_of(page), scale, p.cols, p.want, static_cast<uint32_t>(kTileKeys * p.waves),
               static_cast<int>(p.most), reinterpret_cast<int*>(ws),
@@ -1010,8 +1020,10 @@ extern "C" int fw_decode_attention_paged(const void* q, int64_t q_row, int64_t q
   const auto run = [&](auto t, auto d) {
     typedef decltype(t) T;
     constexpr int D = decltype(d)::value;
-    const auto kernel = !p.most ? paged_attention_kernel<T, D, -1> : p.cols == kCols ? paged_attention_kernel<T, D, 0> : p.cols == 64 ? paged_attention_kernel<T, D, 1>
-                                                                                     : paged_attention_kernel<T, D, 2>;
+    const auto kernel = !p.most            ? paged_attention_kernel<T, D, -1>
+                        : p.cols == kCols ? paged_attention_kernel<T, D, 0>
+                        : p.cols == 64    ? paged_attention_kernel<T, D, 1>
+                                          : paged_attention_kernel<T, D, 2>;
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(64 * waves), lds, stream, a);
     if (const int rc = fw_check_launch(what)) return rc;
     if (!p.most) return static_cast<int>(FW_OK);

@@ -140,7 +140,8 @@ __global__ void __launch_bounds__(kTile) kv_page_map_kernel(MapArgs a) {
         const int64_t at = first[l] + (r - begin[l]), entry = at >> a.page_shift;
         int64_t slot = -1;
         if (first[l] >= 0 && at >= 0 && entry < holds[l]) {
-          const int64_t page = entry < from[l] ? a.table[static_cast<int64_t>(l) * a.width + entry] : a.stack[top - 1 - before[l] - (entry - from[l])];
+          const int64_t page = entry < from[l] ? a.table[static_cast<int64_t>(l) * a.width + entry]
+                                               : a.stack[top - 1 - before[l] - (entry - from[l])];
           slot = (page << a.page_shift) + (at & ((int64_t{1} << a.page_shift) - 1));
         }
         a.slots[r] = slot;
@@ -257,7 +258,8 @@ __global__ void __launch_bounds__(256) kv_page_append_kernel(AppendArgs a) {
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 bool rows_ok(const void* p, int64_t row, int64_t head) { return aligned(p, 16) && row % 8 == 0 && head % 8 == 0; }
 
-// Slots that one block finds beside the map (us in one launch / two: 64 sequences of 1500 rows 6.2 / 8.1, 3400 7.5 / 8.1, 8 of 6300 8.1 / 7.2).
+// Slots that one block finds beside the map (us in one launch / two: 64 sequences with 1500 rows 6.2 / 8.1, with 3400 7.5 / 8.1,
+// 8 with 6300 8.1 / 7.2).
 constexpr int64_t kOneBlockRows = 4 * kTile;
 
 }  // namespace

@@ -118,6 +118,21 @@ def test_torch_level_checks(built_lib):
             ext.logits_rules(*args)
 
 
+def test_binding_refuses_without_a_call(built_lib):
+    """The compiled binding answers False, and makes no call, for anything that is not a valid call on the GPU named."""
+    from flash_whisper_amd import _bind
+    from flash_whisper_amd.ext import load_ext
+
+    cache = _cpu_cache(load_ext())
+    q, i64, i32, f32 = torch.zeros(3, 2, 64, dtype=torch.float16), torch.zeros(4, dtype=torch.int64), torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3)
+    none = (None,) * 3
+    for call, args in ((_bind.kv_page_map, (i64[:3], i64, i32, i64[:3], i32[0], i64[:2], i64, 16, *none, 0, 0)), (_bind.kv_page_append, (q, q, i64[:3], cache, 0, 0)),
+                       (_bind.decode_attention_paged, (q, cache, i32, i64[:3], q, f32, 0.1, None, None, 0, 0)),
+                       (_bind.logits_rules, (f32[None], f32[None], *none, *none, *none, None, None, 0, 0))):
+        assert call(*args) is False and call() is False and call(*args[:-1]) is False and call(*(None,) * len(args)) is False
+        assert call(*args[:-2], 1 << 70, 0) is False
+
+
 def test_oracle_map():
     """A sequence that ends gives its pages to one that grows; shared entries are only dropped; what is missing is counted."""
     table = [[5, 6, 7], [1, 0, 0], [2, 3, 0]]

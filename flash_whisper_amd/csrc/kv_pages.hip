@@ -1,5 +1,7 @@
 // A key/value cache in pages for gfx950: the pages that sequences hold brought up to their lengths, the slots of new rows,
 // and rows written to their slots (layout: pages.h).
+#include <algorithm>
+
 #include "packed_rows.h"
 #include "pages.h"
 
@@ -10,8 +12,9 @@ namespace {
 // Page map. Sequence s wants the pages of rows 0 .. pos[s] + new - 1 (at most `width`). What it holds beyond them and owns goes
 // back onto the stack of free pages, in the order of sequences and entries, then the missing ones are taken off its top in the
 // same order: an exclusive sum over the sequences gives each its places, so the result depends on nothing else.
-// Bound by latency: one block does all of it in LDS, kTile sequences at a time, and the slots too where the rows are few;
-// else a second launch has a thread for each row (64 sequences of a token 5.4 us; 600 of which some bring prompts, 83000 rows, 12.1).
+// Bound by latency: one block does all of it in LDS, kTile sequences at a time. The slots are found in the same launch where
+// the rows are few, or by further blocks where nothing that the sums are made from is written; else a second launch has a thread for
+// each row (64 sequences of a token 5.4 us; 600 of which some bring prompts, 84000 rows, 9.7, in two launches 12.1).
 // ------------------------------------------------------------------------------------------
 constexpr int kTile = 1024;
 
@@ -77,11 +80,19 @@ __device__ __forceinline__ int last_up_to(const int* at, int n, int x) {
   return lo;
 }
 
-template <bool SLOTS>
+// Who finds the rows' slots: another launch; this block; this and further blocks, kTile rows each, which make the same sums for
+// themselves and take what they need from what the first block leaves as it is: entries that are held, and the stack as it was.
+enum { kSlotsLater, kSlotsHere, kSlotsByAll };
+
+template <int SLOTS>
 __global__ void __launch_bounds__(kTile) kv_page_map_kernel(MapArgs a) {
-  __shared__ int before[kTile], from[kTile], begin[kTile], holds[kTile], part[kTile / 64];
-  __shared__ int64_t first[kTile];
+  constexpr int kRows = SLOTS == kSlotsLater ? 1 : kTile;
+  __shared__ int before[kTile], from[kTile], part[kTile / 64];     // pages taken before a sequence's, the entries they begin at
+  __shared__ int backs[kTile], lows[kTile];                        // the same of pages that go back
+  __shared__ int begin[kRows], holds[kRows];
+  __shared__ int64_t first[kRows];
   const int tid = threadIdx.x;
+  const bool moves = SLOTS != kSlotsByAll || blockIdx.x == 0;
   const int64_t there = within(a.count[0], 0, a.stack_size);
   const int tiles = (a.n_seq + kTile - 1) / kTile;
   MapSeq x = {};
@@ -94,13 +105,13 @@ __global__ void __launch_bounds__(kTile) kv_page_map_kernel(MapArgs a) {
     int total;
     const int back = live ? max(0, x.held - x.low) : 0, sum = block_scan(back, part, total);
     if (total == 0) continue;
-    before[tid] = sum - back;
-    from[tid] = x.low;
+    backs[tid] = sum - back;
+    lows[tid] = x.low;
     __syncthreads();
-    for (int i = tid; i < total; i += kTile) {
-      const int l = last_up_to(before, min(kTile, a.n_seq - t * kTile), i);
+    for (int i = tid; moves && i < total; i += kTile) {
+      const int l = last_up_to(backs, min(kTile, a.n_seq - t * kTile), i);
       if (top + i < a.stack_size)
-        a.stack[top + i] = a.table[static_cast<int64_t>(t * kTile + l) * a.width + from[l] + (i - before[l])];
+        a.stack[top + i] = a.table[static_cast<int64_t>(t * kTile + l) * a.width + lows[l] + (i - backs[l])];
     }
     top = min(top + total, a.stack_size);
     __syncthreads();
@@ -118,30 +129,36 @@ __global__ void __launch_bounds__(kTile) kv_page_map_kernel(MapArgs a) {
     const int now = take ? x.held + got : x.want;
     if (live) {
       missing += max(x.need - x.want, int64_t{0}) + (take - got);
-      a.held_out[s] = now;
+      if (moves) a.held_out[s] = now;
     }
     before[tid] = sum - take;
     from[tid] = x.held;
-    if (SLOTS) {
+    if constexpr (SLOTS != kSlotsLater) {
       begin[tid] = live ? static_cast<int>(x.begin) : 0x7FFFFFFF;
       first[tid] = x.pos;
       holds[tid] = now;
     }
     __syncthreads();
-    for (int i = tid; i < total; i += kTile) {
+    for (int i = tid; moves && i < total; i += kTile) {
       const int l = last_up_to(before, min(kTile, a.n_seq - t * kTile), i);
       if (rank + i < top)
         a.table[static_cast<int64_t>(t * kTile + l) * a.width + from[l] + (i - before[l])] = a.stack[top - 1 - rank - i];
     }
-    if (SLOTS) {  // (of pages taken now from the stack itself: the table's entries may not be there yet)
+    if constexpr (SLOTS != kSlotsLater) {  // (one tile; of pages taken now not by the table: its entries may not be there yet)
       const int end = static_cast<int>(within(a.cu[a.n_seq], 0, a.rows));
-      for (int r = begin[0] + tid; r < end; r += kTile) {
+      const auto taken = [&](int64_t place) -> int64_t {
+        if (SLOTS == kSlotsHere || place < there) return a.stack[place];
+        const int i = static_cast<int>(place - there), l = last_up_to(backs, a.n_seq, i);  // one that came back in this call
+        return a.table[static_cast<int64_t>(l) * a.width + lows[l] + (i - backs[l])];
+      };
+      const int step = SLOTS == kSlotsHere ? kTile : kTile * gridDim.x;
+      for (int r = begin[0] + static_cast<int>(blockIdx.x) * kTile + tid; r < end; r += step) {
         const int l = last_up_to(begin, a.n_seq, r);
         const int64_t at = first[l] + (r - begin[l]), entry = at >> a.page_shift;
         int64_t slot = -1;
         if (first[l] >= 0 && at >= 0 && entry < holds[l]) {
           const int64_t page = entry < from[l] ? a.table[static_cast<int64_t>(l) * a.width + entry]
-                                               : a.stack[top - 1 - before[l] - (entry - from[l])];
+                                               : taken(top - 1 - before[l] - (entry - from[l]));
           slot = (page << a.page_shift) + (at & ((int64_t{1} << a.page_shift) - 1));
         }
         a.slots[r] = slot;
@@ -150,6 +167,7 @@ __global__ void __launch_bounds__(kTile) kv_page_map_kernel(MapArgs a) {
     rank += total;
     __syncthreads();
   }
+  if (!moves) return;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) missing += __shfl_xor(missing, o);
   __shared__ int64_t lost[kTile / 64];
@@ -260,7 +278,7 @@ bool rows_ok(const void* p, int64_t row, int64_t head) { return aligned(p, 16) &
 
 // Slots that one block finds beside the map (us in one launch / two: 64 sequences with 1500 rows 6.2 / 8.1, with 3400 7.5 / 8.1,
 // 8 with 6300 8.1 / 7.2).
-constexpr int64_t kOneBlockRows = 4 * kTile;
+constexpr int64_t kOneBlockRows = 4 * kTile, kMostBlocks = 512;
 
 }  // namespace
 }  // namespace fw
@@ -279,11 +297,19 @@ extern "C" int fw_kv_page_map(const int64_t* pos, const int64_t* cu, int32_t* ta
   if (!pos || !cu || !table || !held || !count || !held_out || !count_out || (stack_size > 0 && !stack) || (rows > 0 && !slots))
     return fw_fail(FW_EINVAL, "kv_page_map: null pointer");
   const MapArgs a{pos, cu, held, own, count, table, stack, held_out, count_out, slots, rows, stack_size, n_seq, width, shift};
+  // what the first block writes while others read: only with outputs of their own there is nothing of the inputs among it
+  const auto apart = [&](const int64_t* out, int64_t n) {
+    const auto from = [&](const int64_t* in, int64_t m) { return !in || out + n <= in || in + m <= out; };
+    return from(pos, n_seq) && from(cu, n_seq + 1) && from(held, n_seq) && from(own, n_seq) && from(count, 2);
+  };
+  const bool by_all = n_seq <= kTile && rows > kTile && apart(held_out, n_seq) && apart(count_out, 2);
   const bool one = n_seq <= kTile && rows <= kOneBlockRows;
-  if (one) hipLaunchKernelGGL(kv_page_map_kernel<true>, dim3(1), dim3(kTile), 0, stream, a);
-  else hipLaunchKernelGGL(kv_page_map_kernel<false>, dim3(1), dim3(kTile), 0, stream, a);
+  const int64_t blocks = std::min<int64_t>((rows + kTile - 1) / kTile, kMostBlocks);
+  if (by_all) hipLaunchKernelGGL(kv_page_map_kernel<kSlotsByAll>, dim3(static_cast<unsigned>(blocks)), dim3(kTile), 0, stream, a);
+  else if (one) hipLaunchKernelGGL(kv_page_map_kernel<kSlotsHere>, dim3(1), dim3(kTile), 0, stream, a);
+  else hipLaunchKernelGGL(kv_page_map_kernel<kSlotsLater>, dim3(1), dim3(kTile), 0, stream, a);
   if (const int rc = fw_check_launch("kv_page_map")) return rc;
-  if (one || rows == 0) return FW_OK;
+  if (by_all || one || rows == 0) return FW_OK;
   hipLaunchKernelGGL(kv_page_slots_kernel, dim3(static_cast<unsigned>((rows + 255) / 256)), dim3(256), 0, stream, a);
   return fw_check_launch("kv_page_map slots");
 }

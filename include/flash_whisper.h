@@ -513,8 +513,8 @@ int64_t fw_decode_attention_q4_ws_floats(int n_seq, int heads, int kv_heads, int
  * stack, count_out[1] <- the pages that were wanted and not there (the stack was empty, or the table is too narrow).
  * slots[r] <- the slot of packed row r, -1 where it has no page. pos[s] < 0: an idle sequence, which keeps its pages and whose
  * rows get -1. Rows of slots outside the sequences are left as they are. held_out may be held, and count_out count; a call with
- * others can be repeated and does the same again. cu ascends; entries outside the rows are clamped to them. width is at most
- * 2^20. Up to 1024 sequences and 4096 rows take one launch, else two. */
+ * others can be repeated and does the same again. No other argument overlaps what is written. cu ascends; entries outside the rows
+ * are clamped to them. width is at most 2^20. Up to 1024 sequences take one launch, in place up to 4096 rows; else it is two. */
 int fw_kv_page_map(const int64_t* pos, const int64_t* cu, int32_t* table, const int64_t* held, const int64_t* own,
                    int32_t* stack, const int64_t* count, int64_t* held_out, int64_t* count_out, int64_t* slots, int n_seq,
                    int width, int64_t stack_size, int64_t rows, int page, hipStream_t stream);

@@ -57,13 +57,23 @@ def _run_map(dev, scene, page, rows=None, with_own=True, in_place=False, calls=1
 
 
 @pytest.mark.parametrize('page', [16, 32, 64, 128, 256])
+@pytest.mark.parametrize('in_place', [False, True])
 @pytest.mark.parametrize('n, most, new, gone, spare', [
     (1, 0, 1, 0.0, 3), (1, 500, 3000, 0.0, 400), (7, 40, 1, 0.0, 0), (64, 400, 1, 0.1, 70), (64, 400, 50, 0.5, 10), (300, 900, 40, 0.3, 900),
     (1023, 200, 3, 0.2, 500), (1024, 200, 3, 0.2, 500), (1025, 200, 3, 0.2, 500), (2500, 100, 60, 0.4, 20000), (5, 30000, 9000, 0.4, 3000)])
-def test_map(hip_device, page, n, most, new, gone, spare):
+def test_map(hip_device, page, n, most, new, gone, spare, in_place):
     """Requests that come, go on, are cut back, end and idle; stacks with pages for all, some and none; one launch and two."""
     rng = np.random.default_rng(page * 1000 + n)
-    _run_map(hip_device, _scene(rng, n, page, most, new, gone, spare), page)
+    _run_map(hip_device, _scene(rng, n, page, most, new, gone, spare), page, in_place=in_place)
+
+
+@pytest.mark.parametrize('n, calls', [(40, 3), (1024, 1)])
+def test_map_many_rows_take_what_came_back(hip_device, n, calls):
+    """Few free pages but many that come back in the same call, and go to rows of many blocks."""
+    rng = np.random.default_rng(n)
+    pos, cu, table, held, own, stack, spare = _scene(rng, n, 16, 3000, 400, 0.6, 5, idle=0.0)
+    own[:] = 0
+    _run_map(hip_device, (pos, cu, table, held, own, stack, spare), 16, calls=calls)
 
 
 @pytest.mark.parametrize('n', [3, 1500])

@@ -14,7 +14,7 @@ namespace {
 // same order: an exclusive sum over the sequences gives each its places, so the result depends on nothing else.
 // Bound by latency: one block does all of it in LDS, kTile sequences at a time. The slots are found in the same launch where
 // the rows are few, or by further blocks where nothing that the sums are made from is written; else a second launch has a thread for
-// each row (64 sequences of a token 5.4 us; 600 of which some bring prompts, 84000 rows, 9.7, in two launches 12.1).
+// each row (64 sequences of a token 4.5 us; 600 of which some bring prompts, 84000 rows, 8.1, in place with two launches 12).
 // ------------------------------------------------------------------------------------------
 constexpr int kTile = 1024;
 
@@ -53,20 +53,27 @@ __device__ __forceinline__ int64_t map_slot(const MapArgs& a, int s, int64_t row
   return (page << a.page_shift) + (row & ((int64_t{1} << a.page_shift) - 1));
 }
 
-// Inclusive sum over the block's threads of v; `part` holds a sum for each wave.
-__device__ __forceinline__ int block_scan(int v, int* part, int& total) {
+// Inclusive sums over the block's threads of u and v, their totals behind; `part` holds sums for each wave.
+__device__ __forceinline__ void block_scan(int& u, int& v, int (*part)[kTile / 64], int& u_all, int& v_all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  u = wave_scan(u);
   v = wave_scan(v);
   __syncthreads();  // `part` of the call before is read
-  if (lane == 63) part[wave] = v;
+  if (lane == 63) {
+    part[0][wave] = u;
+    part[1][wave] = v;
+  }
   __syncthreads();
-  total = 0;
+  u_all = v_all = 0;
 #pragma unroll
   for (int w = 0; w < kTile / 64; ++w) {
-    if (w < wave) v += part[w];
-    total += part[w];
+    if (w < wave) {
+      u += part[0][w];
+      v += part[1][w];
+    }
+    u_all += part[0][w];
+    v_all += part[1][w];
   }
-  return v;
 }
 
 // The last of n ascending values that is <= x, the first being 0 or less.
@@ -80,14 +87,15 @@ __device__ __forceinline__ int last_up_to(const int* at, int n, int x) {
   return lo;
 }
 
-// Who finds the rows' slots: another launch; this block; this and further blocks, kTile rows each, which make the same sums for
+// Who finds the rows' slots: another launch; this block; further blocks, kTile rows at a time, which make the same sums for
 // themselves and take what they need from what the first block leaves as it is: entries that are held, and the stack as it was.
 enum { kSlotsLater, kSlotsHere, kSlotsByAll };
 
 template <int SLOTS>
 __global__ void __launch_bounds__(kTile) kv_page_map_kernel(MapArgs a) {
   constexpr int kRows = SLOTS == kSlotsLater ? 1 : kTile;
-  __shared__ int before[kTile], from[kTile], part[kTile / 64];     // pages taken before a sequence's, the entries they begin at
+  __shared__ int part[2][kTile / 64];
+  __shared__ int before[kTile], from[kTile];                       // pages taken before a sequence's, the entries they begin at
   __shared__ int backs[kTile], lows[kTile];                        // the same of pages that go back
   __shared__ int begin[kRows], holds[kRows];
   __shared__ int64_t first[kRows];
@@ -98,12 +106,15 @@ __global__ void __launch_bounds__(kTile) kv_page_map_kernel(MapArgs a) {
   MapSeq x = {};
   // back onto the stack
   int64_t top = there;
+  int take = 0, taken_to = 0, takes = 0;  // of the tile: the sequence's pages to take, up to it, in all
   for (int t = 0; t < tiles; ++t) {
     const int s = t * kTile + tid;
     const bool live = s < a.n_seq;
     if (live) x = map_seq(a, s);
-    int total;
-    const int back = live ? max(0, x.held - x.low) : 0, sum = block_scan(back, part, total);
+    const int back = live ? max(0, x.held - x.low) : 0;
+    int total, sum = back;
+    taken_to = take = live ? max(0, x.want - x.held) : 0;
+    block_scan(sum, taken_to, part, total, takes);
     if (total == 0) continue;
     backs[tid] = sum - back;
     lows[tid] = x.low;
@@ -121,17 +132,20 @@ __global__ void __launch_bounds__(kTile) kv_page_map_kernel(MapArgs a) {
   for (int t = 0; t < tiles; ++t) {
     const int s = t * kTile + tid;
     const bool live = s < a.n_seq;
-    if (live && tiles > 1) x = map_seq(a, s);
-    int total;
-    const int take = live ? max(0, x.want - x.held) : 0, sum = block_scan(take, part, total);
-    const int64_t mine = rank + sum - take;
+    if (tiles > 1) {  // (else it is all there)
+      if (live) x = map_seq(a, s);
+      int none = 0, nothing;
+      taken_to = take = live ? max(0, x.want - x.held) : 0;
+      block_scan(none, taken_to, part, nothing, takes);
+    }
+    const int64_t mine = rank + taken_to - take;
     const int got = static_cast<int>(min(max(top - mine, int64_t{0}), static_cast<int64_t>(take)));
     const int now = take ? x.held + got : x.want;
     if (live) {
       missing += max(x.need - x.want, int64_t{0}) + (take - got);
       if (moves) a.held_out[s] = now;
     }
-    before[tid] = sum - take;
+    before[tid] = taken_to - take;
     from[tid] = x.held;
     if constexpr (SLOTS != kSlotsLater) {
       begin[tid] = live ? static_cast<int>(x.begin) : 0x7FFFFFFF;
@@ -139,7 +153,7 @@ __global__ void __launch_bounds__(kTile) kv_page_map_kernel(MapArgs a) {
       holds[tid] = now;
     }
     __syncthreads();
-    for (int i = tid; moves && i < total; i += kTile) {
+    for (int i = tid; moves && i < takes; i += kTile) {
       const int l = last_up_to(before, min(kTile, a.n_seq - t * kTile), i);
       if (rank + i < top)
         a.table[static_cast<int64_t>(t * kTile + l) * a.width + from[l] + (i - before[l])] = a.stack[top - 1 - rank - i];
@@ -151,8 +165,9 @@ __global__ void __launch_bounds__(kTile) kv_page_map_kernel(MapArgs a) {
         const int i = static_cast<int>(place - there), l = last_up_to(backs, a.n_seq, i);  // one that came back in this call
         return a.table[static_cast<int64_t>(l) * a.width + lows[l] + (i - backs[l])];
       };
-      const int step = SLOTS == kSlotsHere ? kTile : kTile * gridDim.x;
-      for (int r = begin[0] + static_cast<int>(blockIdx.x) * kTile + tid; r < end; r += step) {
+      const int step = SLOTS == kSlotsHere ? kTile : kTile * (gridDim.x - 1);
+      for (int r = begin[0] + (SLOTS == kSlotsHere ? 0 : static_cast<int>(blockIdx.x) - 1) * kTile + tid; r < end; r += step) {
+        if (SLOTS == kSlotsByAll && moves) break;  // (it has enough to do)
         const int l = last_up_to(begin, a.n_seq, r);
         const int64_t at = first[l] + (r - begin[l]), entry = at >> a.page_shift;
         int64_t slot = -1;
@@ -164,7 +179,7 @@ __global__ void __launch_bounds__(kTile) kv_page_map_kernel(MapArgs a) {
         a.slots[r] = slot;
       }
     }
-    rank += total;
+    rank += takes;
     __syncthreads();
   }
   if (!moves) return;
@@ -302,10 +317,10 @@ extern "C" int fw_kv_page_map(const int64_t* pos, const int64_t* cu, int32_t* ta
     const auto from = [&](const int64_t* in, int64_t m) { return !in || out + n <= in || in + m <= out; };
     return from(pos, n_seq) && from(cu, n_seq + 1) && from(held, n_seq) && from(own, n_seq) && from(count, 2);
   };
-  const bool by_all = n_seq <= kTile && rows > kTile && apart(held_out, n_seq) && apart(count_out, 2);
+  const bool by_all = n_seq <= kTile && rows > 0 && apart(held_out, n_seq) && apart(count_out, 2);
   const bool one = n_seq <= kTile && rows <= kOneBlockRows;
   const int64_t blocks = std::min<int64_t>((rows + kTile - 1) / kTile, kMostBlocks);
-  if (by_all) hipLaunchKernelGGL(kv_page_map_kernel<kSlotsByAll>, dim3(static_cast<unsigned>(blocks)), dim3(kTile), 0, stream, a);
+  if (by_all) hipLaunchKernelGGL(kv_page_map_kernel<kSlotsByAll>, dim3(static_cast<unsigned>(blocks) + 1), dim3(kTile), 0, stream, a);
   else if (one) hipLaunchKernelGGL(kv_page_map_kernel<kSlotsHere>, dim3(1), dim3(kTile), 0, stream, a);
   else hipLaunchKernelGGL(kv_page_map_kernel<kSlotsLater>, dim3(1), dim3(kTile), 0, stream, a);
   if (const int rc = fw_check_launch("kv_page_map")) return rc;

@@ -17,6 +17,10 @@ def _ext():
     return load_ext()
 
 
+def _rest(seed, n, low, high):
+    return [int(x) for x in np.random.default_rng(seed).integers(low, high + 1, n)]
+
+
 class Scene:
     """Groups of sequences whose first rows are the same pages; the rest of each is its own, the page in which the shared
     rows end copied. Rows behind a sequence's length and spare pages hold NaN."""
@@ -88,10 +92,6 @@ class Scene:
                 assert not got[s].any()
 
 
-def _rest(seed, n, low, high):
-    return [int(x) for x in np.random.default_rng(seed).integers(low, high + 1, n)]
-
-
 @pytest.mark.parametrize('dtype', ['fp16', 'bf16'])
 @pytest.mark.parametrize('dim', [64, 128])
 @pytest.mark.parametrize('page', [16, 32, 128])
@@ -111,6 +111,16 @@ def test_alone(hip_device, dtype, dim, page, kv_heads, group, lens):
 def test_alone_long(hip_device, dtype, dim, page, kv_heads, group, lens):
     """Long tables, cut into pieces by the lengths there are."""
     scene = Scene(8, [1] * len(lens), [0] * len(lens), lens, page, kv_heads, group, dim, dtype, spare_width=1100 // page + 1)
+    scene.check(scene.run(hip_device, groups=False))
+
+
+@pytest.mark.parametrize('dtype, dim', [('fp16', 128), ('bf16', 64)])
+@pytest.mark.parametrize('n, most, width', [(70, 1900, 2048), (70, 1900, 2064), (40, 900, 1024), (6, 700, 768), (6, 740, 784), (6, 1000, 1024)])
+def test_alone_sides_of_the_rules(hip_device, dtype, dim, n, most, width):
+    """Tables on either side of what is taken whole: of many sequences, of few, of heads of both sizes."""
+    lens = [most, *_rest(n, n - 1, 0, most)]
+    scene = Scene(24, [1] * n, [0] * n, lens, 16, 2, 2, dim, dtype, spare_width=width // 16 - -(-most // 16))
+    assert scene.table.shape[1] * 16 == width
     scene.check(scene.run(hip_device, groups=False))
 
 

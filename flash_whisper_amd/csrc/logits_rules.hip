@@ -14,7 +14,7 @@ typedef __bf16 bf16;
 //   x <- -infinity where the token's bit in the row's mask is 0
 // A block has a slice of a row. It counts the history's and the list's tokens that fall into the slice in LDS (whole numbers, so
 // their order does not matter), then takes the slice. Bound by memory, each logit once in and once out, where histories are short
-// (256 x 100003 fp32 with a mask each, 41 us: 5.0 TB/s); long ones add their latency (65 us with up to 9000 tokens a row).
+// (256 x 100003 fp32 with a mask each, 41 us: 5.0 TB/s); long ones add their latency (61 us with up to 9000 tokens a row).
 // ------------------------------------------------------------------------------------------
 struct RulesArgs {
   const void* x;
@@ -35,8 +35,8 @@ struct RulesArgs {
 
 // Slices: every block of a row reads its history, so long ones are read for larger slices, of 4096 tokens, or 8192 where there are
 // blocks enough; else they are the smallest, of 16 bytes a thread (us with slices of 1024 or 2048 / 4096 / 8192: 1 x 51866 fp16, 224
-// tokens 4.6 / 4.6 / 5.5; 40 x 51866, 448 tokens 6.7 / 6.7 / 7.2; 8 x 128000 bf16, up to 30000 tokens 15.7 / 11.3 / 13.4; 256 x 100003
-// fp32, no history 41 / 42 / 45, up to 9000 tokens 125 / 81 / 65).
+// tokens 4.8 / 4.3 / 5.2; 40 x 51866, 448 tokens 6.1 / 6.4 / 6.9; 8 x 128000 bf16, up to 30000 tokens 17.3 / 11.3 / 12.9; 256 x 100003
+// fp32, no history 41 / 42 / 43, up to 9000 tokens 127 / 73 / 61).
 constexpr int64_t kFewMarks = 1024, kFewLogits = int64_t{1} << 23;
 
 // 16 bytes at any element's address.
@@ -45,10 +45,12 @@ struct __attribute__((packed, aligned(sizeof(T)))) Loose {
   T e[16 / sizeof(T)];
 };
 
-// f(place, token) for the list's places b .. e - 1, a thread's every THREADS-th, kBatch of them requested at once.
+// f(place, token) for the list's places b .. e - 1, a thread's every THREADS-th, kBatch of them requested at once (8 take
+// registers that cost blocks a CU: 256 x 100003 fp32 with up to 9000 tokens a row 65 us against 61; with 2 or 3 8 x 128000 bf16 with up
+// to 30000 12 to 13 against 11.3).
 template <int THREADS, class F>
 __device__ __forceinline__ void each_token(const int64_t* tokens, int64_t b, int64_t e, F f) {
-  constexpr int kBatch = 8;
+  constexpr int kBatch = 4;
   for (int64_t i = b + threadIdx.x; i < e; i += kBatch * THREADS) {
     int64_t t[kBatch];
 #pragma unroll

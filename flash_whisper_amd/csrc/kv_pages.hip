@@ -159,16 +159,16 @@ __global__ void __launch_bounds__(kTile) kv_page_map_kernel(MapArgs a) {
         a.table[static_cast<int64_t>(t * kTile + l) * a.width + from[l] + (i - before[l])] = a.stack[top - 1 - rank - i];
     }
     if constexpr (SLOTS != kSlotsLater) {  // (one tile; of pages taken now not by the table: its entries may not be there yet)
-      const int end = static_cast<int>(within(a.cu[a.n_seq], 0, a.rows));
+      const unsigned end = static_cast<unsigned>(within(a.cu[a.n_seq], 0, a.rows));
       const auto taken = [&](int64_t place) -> int64_t {
         if (SLOTS == kSlotsHere || place < there) return a.stack[place];
         const int i = static_cast<int>(place - there), l = last_up_to(backs, a.n_seq, i);  // one that came back in this call
         return a.table[static_cast<int64_t>(l) * a.width + lows[l] + (i - backs[l])];
       };
-      const int step = SLOTS == kSlotsHere ? kTile : kTile * (gridDim.x - 1);
-      for (int r = begin[0] + (SLOTS == kSlotsHere ? 0 : static_cast<int>(blockIdx.x) - 1) * kTile + tid; r < end; r += step) {
+      const unsigned step = SLOTS == kSlotsHere ? kTile : kTile * (gridDim.x - 1);  // (unsigned: past the end may be past 2^31)
+      for (unsigned at_row = begin[0] + (SLOTS == kSlotsHere ? 0 : blockIdx.x - 1) * kTile + tid; at_row < end; at_row += step) {
         if (SLOTS == kSlotsByAll && moves) break;  // (it has enough to do)
-        const int l = last_up_to(begin, a.n_seq, r);
+        const int r = static_cast<int>(at_row), l = last_up_to(begin, a.n_seq, r);
         const int64_t at = first[l] + (r - begin[l]), entry = at >> a.page_shift;
         int64_t slot = -1;
         if (first[l] >= 0 && at >= 0 && entry < holds[l]) {

@@ -101,6 +101,25 @@ def test_map_empty(hip_device):
     assert held.tolist() == [4, 1] and slots.tolist() == [-1, -1, 4 * 16 + 5] and count.tolist() == [0, 2 ** 36 + 1 - 4]
 
 
+@pytest.mark.parametrize('in_place', [False, True])
+def test_map_most_rows(hip_device, in_place):
+    """As many packed rows as a call may have, 2^31 - 256: what the launch has threads for passes 2^31."""
+    i64 = lambda *x: torch.tensor(x, dtype=torch.int64, device=hip_device)
+    rows, last = 2 ** 31 - 256, 300
+    table = torch.zeros((2, 24), dtype=torch.int32, device=hip_device)
+    stack = torch.arange(44, dtype=torch.int32, device=hip_device)
+    held, count, slots = i64(0, 0), i64(44, 0), torch.full((rows,), -77, dtype=torch.int64, device=hip_device)
+    outs = () if in_place else (torch.zeros_like(held), torch.zeros_like(count))
+    _ext().kv_page_map(i64(0, 5), i64(0, rows - last, rows), table, held, stack, count, slots, 16, None, *outs)
+    held, count = outs or (held, count)
+    assert held.tolist() == [24, 20] and count.tolist() == [0, (rows - last + 15) // 16 - 24]
+    assert table[0].tolist() == list(range(43, 19, -1)) and table[1, :20].tolist() == list(range(19, -1, -1))
+    assert slots[:384].tolist() == [16 * (43 - r // 16) + r % 16 for r in range(384)]
+    assert slots[-last:].tolist() == [16 * (19 - r // 16) + r % 16 for r in range(5, 5 + last)]
+    low, high = torch.aminmax(slots[384:-last])
+    assert low.item() == high.item() == -1
+
+
 def test_map_takes_what_came_back(hip_device):
     """Pages that one sequence gives back go to another in the same call."""
     i64 = lambda *x: torch.tensor(x, dtype=torch.int64, device=hip_device)

@@ -1,7 +1,9 @@
 // The calls of the small ops straight from torch tensors: what a Python layer spends on attributes and argument
 // conversion (10 us a call) is more than their kernels take. Each function checks its arguments and calls the C entry
-// point, whose address ext.py hands over with set_entry; it returns True if the call was made and succeeded. False
-// leaves everything to ext.py: its checks name what is wrong, and its call reports the library's error.
+// point, whose address ext.py hands over with set_entry; it returns True if the call was made and succeeded. False: the
+// arguments are no call or the entry refused them, and nothing was launched; ext.py's checks then name what is wrong, and its
+// call reports the library's error. A launch's error is raised here: the kernel may be queued all the same (the error can be
+// one that was left before it), and a second call would do its work twice.
 #include <Python.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -90,7 +92,17 @@ bool number(PyObject* o, float& v) {
   return true;
 }
 hipStream_t stream_of(PyObject* o) { return reinterpret_cast<hipStream_t>(PyLong_AsVoidPtr(o)); }
-PyObject* made(int status) { return PyBool_FromLong(status == FW_OK); }
+// What the entry point `name` returned.
+PyObject* made(const char* name, int status) {
+  if (status == FW_OK) Py_RETURN_TRUE;
+  if (status == FW_EINVAL) Py_RETURN_FALSE;
+  PyObject* lib = PyImport_ImportModule("flash_whisper_amd._lib");
+  PyObject* raised = lib ? PyObject_CallMethod(lib, "check", "is", status, name) : nullptr;
+  Py_XDECREF(lib);
+  Py_XDECREF(raised);
+  if (!PyErr_Occurred()) PyErr_Format(PyExc_RuntimeError, "%s: status %d", name, status);
+  return nullptr;
+}
 bool fits(int64_t n) { return n >= 0 && n <= 0x7FFFFFFF; }
 
 // prompt_attention(q, k, v, out, cu_q, cu_k, scale, causal, device, stream)
@@ -110,8 +122,9 @@ PyObject* prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_FALSE;
   const int64_t *q0 = index(cu_q, seqs), *k0 = index(tensor(a[5], dev), seqs);
   if (!q0 || !k0 || !fits(seqs) || !fits(q.heads)) Py_RETURN_FALSE;
-  return made(prompt_attention_entry(q.p, q.row, q.head, k.p, k.row, k.head, v.p, v.row, v.head, out.p, out.row, out.head, q0, k0,
-                                     static_cast<int>(seqs) - 1, q.rows, k.rows, static_cast<int>(q.heads),
+  return made("fw_prompt_attention",
+              prompt_attention_entry(q.p, q.row, q.head, k.p, k.row, k.head, v.p, v.row, v.head, out.p, out.row, out.head,
+                                     q0, k0, static_cast<int>(seqs) - 1, q.rows, k.rows, static_cast<int>(q.heads),
                                      static_cast<int>(k.heads), static_cast<int>(dim), dtype, scale, a[7] == Py_True,
                                      stream_of(a[9])));
 }
@@ -141,8 +154,9 @@ bool packed(PyObject* ok, PyObject* ov, PyObject* ocu, PyObject* opos, PyObject*
 PyObject* kv_q4_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Packed r;
   if (n != 7 || !kv_q4_append_entry || !packed(a[0], a[1], a[2], a[3], a[4], a[5], r)) Py_RETURN_FALSE;
-  return made(kv_q4_append_entry(r.k.p, r.k.row, r.k.head, r.v.p, r.v.row, r.v.head, r.k.rows, r.cu, r.pos, r.c.p[0], r.c.p[1],
-                                 r.c.p[2], r.c.p[3], static_cast<int>(r.c.n), static_cast<int>(r.c.heads),
+  return made("fw_kv_q4_append",
+              kv_q4_append_entry(r.k.p, r.k.row, r.k.head, r.v.p, r.v.row, r.v.head, r.k.rows, r.cu, r.pos, r.c.p[0],
+                                 r.c.p[1], r.c.p[2], r.c.p[3], static_cast<int>(r.c.n), static_cast<int>(r.c.heads),
                                  static_cast<int>(r.c.max_len), static_cast<int>(r.c.dim), r.dtype, stream_of(a[6])));
 }
 
@@ -152,9 +166,10 @@ PyObject* kv_q4_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 7 || !kv_q4_read_entry || !packed(a[3], a[4], a[1], a[2], a[0], a[5], r) || !apart(r.k, r.c.dim) ||
       !apart(r.v, r.c.dim))
     Py_RETURN_FALSE;
-  return made(kv_q4_read_entry(r.c.p[0], r.c.p[1], r.c.p[2], r.c.p[3], static_cast<int>(r.c.n), static_cast<int>(r.c.heads),
-                               static_cast<int>(r.c.max_len), static_cast<int>(r.c.dim), r.cu, r.pos, r.k.rows, r.k.p, r.k.row,
-                               r.k.head, r.v.p, r.v.row, r.v.head, r.dtype, stream_of(a[6])));
+  return made("fw_kv_q4_read",
+              kv_q4_read_entry(r.c.p[0], r.c.p[1], r.c.p[2], r.c.p[3], static_cast<int>(r.c.n), static_cast<int>(r.c.heads),
+                               static_cast<int>(r.c.max_len), static_cast<int>(r.c.dim), r.cu, r.pos, r.k.rows, r.k.p,
+                               r.k.row, r.k.head, r.v.p, r.v.row, r.v.head, r.dtype, stream_of(a[6])));
 }
 
 // decode_attention_q4(q, cache, lens, out, ws, scale, k_new, v_new, device, stream)
@@ -177,10 +192,12 @@ PyObject* decode_attention_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_FALSE;
   const int64_t* lens = index(tensor(a[2], dev), c.n);
   if (!lens || !fits(c.n) || !fits(q.heads) || !fits(c.max_len)) Py_RETURN_FALSE;
-  return made(decode_attention_q4_entry(
-      q.p, q.row, q.head, c.p[0], c.p[1], c.p[2], c.p[3], lens, out.p, out.row, out.head, k.p, k.row, k.head, v.p, v.row, v.head,
-      static_cast<int>(c.n), static_cast<int>(q.heads), static_cast<int>(c.heads), static_cast<int>(c.max_len),
-      static_cast<int>(c.dim), dtype, scale, static_cast<float*>(ws->data_ptr()), ws->numel(), stream_of(a[9])));
+  return made("fw_decode_attention_q4",
+              decode_attention_q4_entry(
+                  q.p, q.row, q.head, c.p[0], c.p[1], c.p[2], c.p[3], lens, out.p, out.row, out.head, k.p, k.row, k.head,
+                  v.p, v.row, v.head, static_cast<int>(c.n), static_cast<int>(q.heads), static_cast<int>(c.heads),
+                  static_cast<int>(c.max_len), static_cast<int>(c.dim), dtype, scale, static_cast<float*>(ws->data_ptr()),
+                  ws->numel(), stream_of(a[9])));
 }
 
 // The contiguous tensor of a type and dimension, or null.
@@ -213,8 +230,10 @@ PyObject* kv_page_map(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!pos || !cu || !held || !count || !held_out || !count_out || !optional(a[8], dev, at::kLong, seqs, own) || !fits(seqs) ||
       !fits(table->size(1)))
     Py_RETURN_FALSE;
-  return made(kv_page_map_entry(pos, cu, static_cast<int32_t*>(table->data_ptr()), held, own, static_cast<int32_t*>(stack->data_ptr()),
-                                count, held_out, count_out, static_cast<int64_t*>(slots->data_ptr()), static_cast<int>(seqs),
+  return made("fw_kv_page_map",
+              kv_page_map_entry(pos, cu, static_cast<int32_t*>(table->data_ptr()), held, own,
+                                static_cast<int32_t*>(stack->data_ptr()), count, held_out, count_out,
+                                static_cast<int64_t*>(slots->data_ptr()), static_cast<int>(seqs),
                                 static_cast<int>(table->size(1)), stack->size(0), slots->size(0), static_cast<int>(page),
                                 stream_of(a[12])));
 }
@@ -251,8 +270,10 @@ PyObject* kv_page_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_FALSE;
   const int64_t* slots = index(tensor(a[2], dev), k.rows);
   if (!slots) Py_RETURN_FALSE;
-  return made(kv_page_append_entry(k.p, k.row, k.head, v.p, v.row, v.head, slots, k.rows, c.k, c.v, static_cast<int>(c.n),
-                                   static_cast<int>(c.heads), static_cast<int>(c.page), static_cast<int>(c.dim), stream_of(a[5])));
+  return made("fw_kv_page_append",
+              kv_page_append_entry(k.p, k.row, k.head, v.p, v.row, v.head, slots, k.rows, c.k, c.v, static_cast<int>(c.n),
+                                   static_cast<int>(c.heads), static_cast<int>(c.page), static_cast<int>(c.dim),
+                                   stream_of(a[5])));
 }
 
 // decode_attention_paged(q, cache, table, lens, out, ws, scale, cu_groups, shared, device, stream)
@@ -278,11 +299,13 @@ PyObject* decode_attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!cu) Py_RETURN_FALSE;
   }
   if (!lens || !fits(q.rows) || !fits(q.heads) || !fits(table->size(1)) || !fits(groups)) Py_RETURN_FALSE;
-  return made(decode_attention_paged_entry(
-      q.p, q.row, q.head, c.k, c.v, static_cast<const int32_t*>(table->data_ptr()), lens, cu, shared, out.p, out.row, out.head,
-      static_cast<int>(q.rows), static_cast<int>(q.heads), static_cast<int>(c.heads), static_cast<int>(c.n), static_cast<int>(c.page),
-      static_cast<int>(table->size(1)), static_cast<int>(groups), static_cast<int>(c.dim), c.type == at::kHalf ? FW_F16 : FW_BF16, scale,
-      static_cast<float*>(ws->data_ptr()), ws->numel(), stream_of(a[10])));
+  return made("fw_decode_attention_paged",
+              decode_attention_paged_entry(
+                  q.p, q.row, q.head, c.k, c.v, static_cast<const int32_t*>(table->data_ptr()), lens, cu, shared, out.p,
+                  out.row, out.head, static_cast<int>(q.rows), static_cast<int>(q.heads), static_cast<int>(c.heads),
+                  static_cast<int>(c.n), static_cast<int>(c.page), static_cast<int>(table->size(1)),
+                  static_cast<int>(groups), static_cast<int>(c.dim), c.type == at::kHalf ? FW_F16 : FW_BF16, scale,
+                  static_cast<float*>(ws->data_ptr()), ws->numel(), stream_of(a[10])));
 }
 
 // logits_rules(logits, out, tokens, cu, prompt, repetition, presence, frequency, bias_ids, bias, cu_bias, masks, mask_of,
@@ -327,10 +350,11 @@ PyObject* logits_rules(PyObject*, PyObject* const* a, Py_ssize_t n) {
     masks = static_cast<const int32_t*>(t->data_ptr());
   }
   if (!optional(a[12], dev, at::kLong, rows, of)) Py_RETURN_FALSE;
-  return made(logits_rules_entry(x->data_ptr(), rows > 1 ? x->stride(0) : 0, out->data_ptr(), rows > 1 ? out->stride(0) : 0,
-                                 static_cast<int>(rows), static_cast<int>(vocab), dtype, tokens, n_tokens, cu, prompt, repetition,
-                                 presence, frequency, ids, bias, n_bias, cu_bias, masks, words, static_cast<int>(sets), of,
-                                 stream_of(a[14])));
+  return made("fw_logits_rules",
+              logits_rules_entry(x->data_ptr(), rows > 1 ? x->stride(0) : 0, out->data_ptr(), rows > 1 ? out->stride(0) : 0,
+                                 static_cast<int>(rows), static_cast<int>(vocab), dtype, tokens, n_tokens, cu, prompt,
+                                 repetition, presence, frequency, ids, bias, n_bias, cu_bias, masks, words,
+                                 static_cast<int>(sets), of, stream_of(a[14])));
 }
 
 // set_entry(name, address)

@@ -19,11 +19,13 @@ template <>
 struct Types<_Float16> {
   typedef h8v v8;
   typedef h2v v2;
+  static constexpr float kLift = 7.f;  // log2 of what all weights are multiplied by, below
 };
 template <>
 struct Types<__bf16> {
   typedef b8v v8;
   typedef b2v v2;
+  static constexpr float kLift = 0.f;
 };
 
 __device__ __forceinline__ f4v mfma16(const h8v& a, const h8v& b, const f4v& c) {
@@ -48,7 +50,9 @@ __device__ __forceinline__ float add_pair(b2v x, float s) {
 //    scores of keys 8 g .. 8 g + 7 for column lane % 16: what the P V products take from it, without crossing lanes.
 //  - V: a lane's 8 keys of a dim are 16 bytes of a page.
 //  - The running maximum only moves when a score passes it by kSlack (log2 units), so weights are at most 2^8; they are
-//    rounded to the type, which the matrix instructions take, and their sum, in fp32, is over the rounded ones.
+//    rounded to the type, which the matrix instructions take, and their sum, in fp32, is over the rounded ones. fp16 ones are
+//    2^kLift times as large, at most 2^15: those from 2^-21 of the maximum's on keep all bits of the type, smaller ones are
+//    multiples of 2^-31 of it. (As they are, that would begin at 2^-14, and many keys far below one lose or gain half their sum.)
 // Bound by memory where there is much to read (17 sequences of up to 48000 rows in groups of 1 to 7, 64 query heads over 8 of 128:
 // 409 MB in 88 us, 4.6 TB/s, with the joining; 16 of 1500 rows x 20 heads of 64 28 us, 4.4 TB/s), else by the chain of dependent
 // loads (lengths, table, keys, results of the pieces), about 10 us in two launches, 5 in one.
@@ -179,7 +183,7 @@ __device__ __forceinline__ void paged_values(PagedTile<T, D>& t, f4v (&s)[CT][2]
       for (int db = 0; db < D / 16; ++db) st.o[c][db] *= corr;
       st.m[c] = m_new;
     }
-    const float m = st.m[c] == -INFINITY ? 0.f : st.m[c];  // no key seen yet: the weights are 0
+    const float m = (st.m[c] == -INFINITY ? 0.f : st.m[c]) - Types<T>::kLift;  // no key seen yet: the weights are 0
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -577,7 +581,7 @@ __device__ __forceinline__ f4v paged_sum(const PagedMerge<D>& x, int parts, int 
   return o;
 }
 
-// Four dims of a column, or zeros: nothing was seen. (An idle sequence of a group sees nothing, whatever its group sees.)
+// Four dims of a column, or zeros: nothing was seen (kLift is in o and l alike). (An idle sequence of a group sees nothing, whatever its group sees.)
 template <class T>
 __device__ __forceinline__ void paged_store(const PagedArgs& a, int seq, int head, int d, const f4v& o, float l) {
   typedef T v4 __attribute__((ext_vector_type(4)));
@@ -678,7 +682,7 @@ __device__ __forceinline__ void wide_step(uint32_t k, uint32_t v, const typename
       for (int db = 0; db < D / 16; ++db) st.o[c][db] *= corr;
       st.m[c] = m_new;
     }
-    const float m = st.m[c] == -INFINITY ? 0.f : st.m[c];
+    const float m = (st.m[c] == -INFINITY ? 0.f : st.m[c]) - Types<T>::kLift;
     float sum[kStep] = {};
 #pragma unroll
     for (int t = 0; t < kStep; ++t)

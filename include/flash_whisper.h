@@ -535,7 +535,7 @@ int fw_kv_page_append(const void* k, int64_t k_row, int64_t k_head, const void* 
  * shortest sequence has them. The first sequence may be idle; its table then lists them all the same. groups 0: cu_groups and
  * shared may be null. Sequences outside the groups share nothing; starts that do not ascend make no groups.
  * Scores, softmax and sums are fp32; the weights are rounded to the type for their sum and the product with v, of which fp16
- * ones below 2^-25 of the largest are lost. Rows that are not seen do not reach the output, whatever they hold; those that are
+ * ones below 2^-21 of the largest are multiples of at most 2^-31 of it. Rows that are not seen do not reach the output, whatever they hold; those that are
  * seen are finite. scale and scores are within the limits of fw_prompt_attention. out overlaps no input. At most 65535 sequences,
  * 65535 groups, 16384 heads and 2^30 rows a sequence. ws: fw_decode_attention_paged_ws_floats floats, 16-byte aligned,
  * uninitialised; calls that may overlap need one each. */

@@ -1,0 +1,76 @@
+"""Single-token attention over a cache in pages at the limits of its types, of its plan and of what a group may hold."""
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+TYPES = {'fp16': torch.float16, 'bf16': torch.bfloat16}
+
+
+def _ext():
+    from flash_whisper_amd.ext import load_ext
+
+    return load_ext()
+
+
+def _i64(x, dev):
+    return torch.tensor(np.asarray(x), dtype=torch.int64, device=dev)
+
+
+@pytest.mark.parametrize('dtype', ['fp16', 'bf16'])
+@pytest.mark.parametrize('dim', [64, 128])
+@pytest.mark.parametrize('below', [9, 15, 20.9, 23.4, 24.6, 27.4])
+@pytest.mark.parametrize('rows, members, group', [(32, 1, 1), (1000, 1, 3), (5000, 1, 2), (1504, 3, 4), (1504, 9, 8), (4096, 10, 30)])
+def test_small_weights(hip_device, dtype, dim, below, rows, members, group):
+    """A key of large weight and value 0 among 31 that weigh 2^-below of it, tile by tile: the output is what the small ones
+    sum up to. A block a sequence, pieces, groups of up to 16, 64 and 128 columns a run."""
+    dtype, page, large, value = TYPES[dtype], 32, 16.0, 4096.0
+    pages, scale = -(-rows // page), below * np.log(2) / large
+    k = torch.zeros(pages, 1, page, dim, dtype=dtype, device=hip_device)
+    v = torch.full((pages, 1, page // 8, dim, 8), value, dtype=dtype, device=hip_device)
+    k[:, :, 5, 0], v[:, :, 0, :, 5] = large, 0.0
+    q = torch.zeros(members, group, dim, dtype=dtype, device=hip_device)
+    q[..., 0] = 1.0
+    from flash_whisper_amd.ext import KvPages
+
+    ext, cache, out = _ext(), KvPages(k, v), torch.full_like(q, 9.0)
+    table = torch.arange(pages, dtype=torch.int32, device=hip_device).expand(members, pages).contiguous()
+    ws = ext.decode_attention_paged_workspace(members, group, cache, pages, 1)
+    ext.decode_attention_paged(q, cache, table, _i64([rows] * members, hip_device), out, ws, scale,
+                               _i64([0, members], hip_device), _i64([rows], hip_device))
+    # sinks and small keys of a sequence (rows may end inside a tile, behind its sink)
+    sinks = -(-rows // page)
+    w = np.exp2(-below) * (rows - sinks)
+    want = w * value / (sinks + w)
+    # The output rounded; each weight rounded for the product and for the sum (u each, of what it adds to the output: the small
+    # ones' sum is the output itself); scores of size below x ln 2 and their exponentials in fp32; fp32 sums; fp16 weights
+    # below 2^-21 of the maximum are off by at most 2^-32 of it (the type's smallest step, halved, 2^kLift times as large), and
+    # outputs there by 2^-25.
+    u = torch.finfo(dtype).eps / 2
+    tol = want * (3 * u + 2.0 ** -15 * below * np.log(2) + 2.0 ** -19 + rows * 2.0 ** -24) + 2.0 ** -25
+    if dtype == torch.float16:
+        tol += rows * 2.0 ** -32 * value / sinks
+    err = np.abs(out.double().cpu().numpy() - want).max()
+    assert err <= tol, f'{err:.3e} of {want:.3e}, {err / tol:.2f}'
+
+
+def test_sum_of_subnormal_weights(hip_device):
+    """Values of 1 and weights that fp16 holds without a leading one (2^-22 of each wave's first key): what they add to the sum of
+    the weights (one instruction) and to the values (another) is the same, so the output is 1. 8 sequences, a piece each of
+    2^21 rows of one page; its four waves have 2^19 keys each, which sum up to an eighth of the largest."""
+    from flash_whisper_amd.ext import KvPages
+
+    ext, n, heads, page, rows = _ext(), 8, 64, 256, 1 << 21
+    k = torch.zeros(2, heads, page, 64, dtype=torch.float16, device=hip_device)
+    k[1, :, :128:32, 0] = 16.0  # a key of each wave's first tile
+    table = torch.zeros(n, rows // page, dtype=torch.int32, device=hip_device)
+    table[:, 0] = 1
+    q = torch.zeros(n, heads, 64, dtype=torch.float16, device=hip_device)
+    q[..., 0] = 1.0
+    cache, out = KvPages(k, torch.ones(2, heads, page // 8, 64, 8, dtype=torch.float16, device=hip_device)), torch.full_like(q, 9.0)
+    ws = ext.decode_attention_paged_workspace(n, heads, cache, rows // page)
+    ext.decode_attention_paged(q, cache, table, _i64([rows] * n, hip_device), out, ws, 22 * np.log(2) / 16)
+    # per wave and lane 2^14 tiles of 4 additions each to a sum between 2^7 and 2^8, half a step of it (2^-17) each; the
+    # values' sums the same; the output rounded
+    assert (out.float() - 1).abs().max().item() <= 2 * 2 ** 16 * 2.0 ** -17 / 2 ** 7 + 2.0 ** -11

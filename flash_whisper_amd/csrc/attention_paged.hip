@@ -78,11 +78,12 @@ constexpr int kCols = 16;
 constexpr float kSlack = 8.f;
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Columns [col, col + cols) of the sequences from `seq` on see keys [begin, end) of seq's table.
+// Columns [col, col + cols) of the sequences from `seq` on see keys [begin, end) of the table of sequence `table`, the first of them
+// that is not idle.
 struct __align__(16) Piece {
   int seq, col, cols, begin;
   int end, slot;  // where 16 columns' results go, cols / 16 slots; -1: they are the whole, and go to `out`
-  int pad[2];
+  int table, pad;
 };
 // What the pieces of a sequence left: of its group's shared keys, its columns from `col` on in runs of `step` slots, and its own.
 struct __align__(16) Owner {
@@ -270,12 +271,12 @@ __device__ __forceinline__ Owner* owners_of(const PagedArgs& a) { return reinter
 // ------------------------------------------------------------------------------------------
 constexpr int kPlanThreads = 1024, kPlanLds = 1024;
 
-// Words of its arrays: keys, groups of n sequences; starts, rows, low, high of the groups; the first piece of each.
-__host__ __device__ constexpr int64_t plan_words(int64_t n, int64_t groups) { return 2 * n + 4 * groups + 1 + (n + groups + 1); }
+// Words of its arrays: keys, groups of n sequences; starts, rows, low, high, live of the groups; the first piece of each.
+__host__ __device__ constexpr int64_t plan_words(int64_t n, int64_t groups) { return 2 * n + 5 * groups + 1 + (n + groups + 1); }
 
 struct Plan {
   const PagedArgs& a;
-  int *keys, *of, *starts, *rows, *low, *high, *before;  // low: the fewest keys, in the end whether no sequence sees more
+  int *keys, *of, *starts, *rows, *low, *high, *live, *before;  // low: the fewest keys, in the end whether no sequence sees more
   int groups, group, parts, total;
   uint32_t chunk;
 
@@ -288,17 +289,19 @@ struct Plan {
     return at < shared ? at * (a.cols / kCols) : shared * (a.cols / kCols) + (at - shared);
   }
   __device__ static int size_of(int keys, int n) { return ((keys + n - 1) / n + kTileKeys - 1) / kTileKeys * kTileKeys; }
+  // What atomics made, read where they left it, which may be memory.
+  __device__ static int made(const int* at) { return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
   __device__ Piece piece(int at) const {
     const int e = find(before, groups + a.n_seq, at), s = e - groups, x = at - before[e];
     if (s < 0) {
       const int n = count(rows[e], chunk), runs = runs_of(e), i = x / runs, r = x % runs, size = size_of(rows[e], n);
       return Piece{starts[e], r * a.cols, min(a.cols, (starts[e + 1] - starts[e]) * group - r * a.cols), i * size,
-                   min((i + 1) * size, rows[e]), low[e] && n == 1 ? -1 : slot_of(at), {}};
+                   min((i + 1) * size, rows[e]), low[e] && n == 1 ? -1 : slot_of(at), made(live + e), 0};
     }
     const int n = (before[e + 1] - before[e]) / parts, begin = begin_of(s), mine = max(keys[s] - begin, 0), i = x / parts, r = x % parts;
     const int size = size_of(mine, n);
     return Piece{s, r * kCols, min(kCols, group - r * kCols), begin + i * size, begin + min((i + 1) * size, mine),
-                 begin == 0 && n == 1 ? -1 : slot_of(at), {}};
+                 begin == 0 && n == 1 ? -1 : slot_of(at), s, 0};
   }
   __device__ Owner owner(int s) const {
     Owner o{};
@@ -337,7 +340,8 @@ __device__ __forceinline__ Plan make_plan(const PagedArgs& a, int* mem) {
   p.rows = p.starts + a.groups + 1;
   p.low = p.rows + a.groups;
   p.high = p.low + a.groups;
-  p.before = p.high + a.groups;
+  p.live = p.high + a.groups;
+  p.before = p.live + a.groups;
   p.group = a.heads / a.kv_heads;
   p.parts = (p.group + kCols - 1) / kCols;
   for (int s = tid; s < n_seq; s += threads) p.keys[s] = a.lens[s] < 0 ? -1 : paged_keys(a, s);  // -1: idle
@@ -350,17 +354,21 @@ __device__ __forceinline__ Plan make_plan(const PagedArgs& a, int* mem) {
     p.rows[g] = static_cast<int>(within(a.shared[g], 0, 1 << 30));
     p.low[g] = 0x7FFFFFFF;
     p.high[g] = 0;
+    p.live[g] = 0x7FFFFFFF;
   }
   p.groups = __syncthreads_or(descends) ? 0 : a.groups;
-  // the fewest and most keys of a group's live sequences; a wave of one group asks once
+  // the first of a group's live sequences, the fewest and most keys of them; a wave of one group asks once
   for (int s0 = tid & ~63; s0 < n_seq; s0 += threads) {
     const int s = s0 + lane;
-    int g = -1, lo = 0x7FFFFFFF, hi = 0;
+    int g = -1, lo = 0x7FFFFFFF, hi = 0, first = 0x7FFFFFFF;
     if (s < n_seq) {
       g = Plan::find(p.starts, p.groups, s);
       if (g >= 0 && s >= p.starts[g + 1]) g = -1;
       p.of[s] = g;
-      if (p.keys[s] >= 0) lo = hi = p.keys[s];
+      if (p.keys[s] >= 0) {
+        lo = hi = p.keys[s];
+        first = s;
+      }
     }
     const int one = __builtin_amdgcn_readfirstlane(g);
     if (__builtin_amdgcn_ballot_w64(g == one) == __builtin_amdgcn_ballot_w64(true)) {
@@ -368,20 +376,20 @@ __device__ __forceinline__ Plan make_plan(const PagedArgs& a, int* mem) {
       for (int o = 1; o < 64; o <<= 1) {
         lo = min(lo, __shfl_xor(lo, o));
         hi = max(hi, __shfl_xor(hi, o));
+        first = min(first, __shfl_xor(first, o));
       }
       if (lane != 0) g = -1;
     }
     if (g >= 0) {
       atomicMin(&p.low[g], lo);
       atomicMax(&p.high[g], hi);
+      atomicMin(&p.live[g], first);
     }
   }
   __syncthreads();
   int64_t work = 0;
   for (int g = tid; g < p.groups; g += threads) {
-    // (read where the atomics left them, which may be memory)
-    const int low = __hip_atomic_load(&p.low[g], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const int high = __hip_atomic_load(&p.high[g], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const int low = Plan::made(&p.low[g]), high = Plan::made(&p.high[g]);
     const int most = p.starts[g + 1] - p.starts[g] > 1 && high > 0 ? min(p.rows[g], low) : 0, whole = most == high;
     p.rows[g] = whole ? most : most & ~(kTileKeys - 1);
     p.low[g] = whole;
@@ -509,14 +517,15 @@ struct WavePlan {
       const int columns = lane_of(members, s) * group, runs = (columns + a.cols - 1) / a.cols;
       const int k = lane_of(rows, s), pieces = lane_of(shared_n, s);
       const int x = at - (lane_of(shared_before, s) - pieces * runs), i = x / runs, r = x % runs, size = Plan::size_of(k, pieces);
+      const int live = s + __builtin_ctzll(__builtin_amdgcn_ballot_w64(keys >= 0) >> s);  // (shared rows are those of live ones)
       return Piece{s, r * a.cols, min(a.cols, columns - r * a.cols), i * size, min((i + 1) * size, k),
-                   lane_of(whole, s) && pieces == 1 ? -1 : at * tiles, {}};
+                   lane_of(whole, s) && pieces == 1 ? -1 : at * tiles, live, 0};
     }
     const int s = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before > at)), pieces = lane_of(n, s), begin = lane_of(rows, s);
     const int mine = max(lane_of(keys, s) - begin, 0), x = at - (lane_of(before, s) - pieces * parts), i = x / parts, r = x % parts;
     const int size = Plan::size_of(mine, pieces);
     return Piece{s, r * kCols, min(kCols, group - r * kCols), begin + i * size, begin + min((i + 1) * size, mine),
-                 begin == 0 && pieces == 1 ? -1 : of_groups * tiles + (at - of_groups), {}};
+                 begin == 0 && pieces == 1 ? -1 : of_groups * tiles + (at - of_groups), s, 0};
   }
   // Of the lane's own sequence.
   __device__ __forceinline__ Owner owner(const PagedArgs& a, int lane) const {
@@ -811,7 +820,7 @@ __global__ void __launch_bounds__(CT < 0 ? 512 : 64 * kWaves, 2) paged_attention
   if constexpr (CT < 0) {
     const int group = a.heads / a.kv_heads, parts = (group + kCols - 1) / kCols;
     const int col = static_cast<int>(at % parts) * kCols, seq = static_cast<int>(at / parts);
-    const Piece p{seq, col, min(kCols, group - col), 0, paged_keys(a, seq), -1, {}};
+    const Piece p{seq, col, min(kCols, group - col), 0, paged_keys(a, seq), -1, seq, 0};
     paged_piece<T, D>(a, p, kvh, a.table + static_cast<int64_t>(seq) * a.width, lds);
   } else {
     Piece p;
@@ -825,7 +834,7 @@ __global__ void __launch_bounds__(CT < 0 ? 512 : 64 * kWaves, 2) paged_attention
       if (static_cast<int>(at) >= a.plan[0]) return;
       p = pieces_of(a)[at];
     }
-    const int32_t* table = a.table + static_cast<int64_t>(p.seq) * a.width;
+    const int32_t* table = a.table + static_cast<int64_t>(p.table) * a.width;
     if constexpr (CT > 0) {
       if (p.cols > kCols) {
         paged_wide<T, D, CT>(a, p, kvh, table, lds);

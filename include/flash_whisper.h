@@ -531,14 +531,14 @@ int fw_kv_page_append(const void* k, int64_t k_row, int64_t k_head, const void* 
  * an idle one (lens[s] < 0) get zeros. A table entry outside the pages hides its rows, as if they were not there.
  * The sequences cu_groups[g] .. cu_groups[g + 1] - 1 (int64, device, groups + 1 entries, ascending) form a group, whose first
  * shared[g] rows (int64, device) are the same, keys and values, in the tables of all its sequences that are not idle: the result
- * is that of each sequence alone, but those rows are read from the first sequence's table, once for all, as far as the
- * shortest sequence has them. The first sequence may be idle; its table then lists them all the same. groups 0: cu_groups and
- * shared may be null. Sequences outside the groups share nothing; starts that do not ascend make no groups.
+ * is that of each sequence alone, but those rows are read from the table of the first that is not idle, once for all, as far as
+ * the shortest of them has them. What an idle one's table holds is not looked at. groups 0: cu_groups and shared may be null.
+ * Sequences outside the groups share nothing; starts that do not ascend make no groups.
  * Scores, softmax and sums are fp32; the weights are rounded to the type for their sum and the product with v, of which fp16
- * ones below 2^-21 of the largest are multiples of at most 2^-31 of it. Rows that are not seen do not reach the output, whatever they hold; those that are
- * seen are finite. scale and scores are within the limits of fw_prompt_attention. out overlaps no input. At most 65535 sequences,
- * 65535 groups, 16384 heads and 2^30 rows a sequence. ws: fw_decode_attention_paged_ws_floats floats, 16-byte aligned,
- * uninitialised; calls that may overlap need one each. */
+ * ones below 2^-21 of the largest are multiples of at most 2^-31 of it. Rows that are not seen do not reach the output,
+ * whatever they hold; those that are seen are finite. scale and scores are within the limits of fw_prompt_attention. out
+ * overlaps no input. At most 65535 sequences, 65535 groups, 16384 heads and 2^30 rows a sequence. ws:
+ * fw_decode_attention_paged_ws_floats floats, 16-byte aligned, uninitialised; calls that may overlap need one each. */
 int fw_decode_attention_paged(const void* q, int64_t q_row, int64_t q_head, const void* k_pages, const void* v_pages,
                               const int32_t* table, const int64_t* lens, const int64_t* cu_groups, const int64_t* shared,
                               void* out, int64_t o_row, int64_t o_head, int n_seq, int heads, int kv_heads, int n_pages,

@@ -74,3 +74,23 @@ def test_sum_of_subnormal_weights(hip_device):
     # per wave and lane 2^14 tiles of 4 additions each to a sum between 2^7 and 2^8, half a step of it (2^-17) each; the
     # values' sums the same; the output rounded
     assert (out.float() - 1).abs().max().item() <= 2 * 2 ** 16 * 2.0 ** -17 / 2 ** 7 + 2.0 ** -11
+
+
+@pytest.mark.parametrize('groups, shared, rest, idle', [
+    ([5], [1500], 0, [0]), ([5], [1500], 40, [0, 1, 3]), ([3, 40], [1300, 1411], 70, [0, 3, 4, 5]), ([2, 62], [1200, 1333], 9, [0, *range(2, 63)]),
+    ([30, 40], [1300, 1280], 90, [0, 30, 31]),                                 # the plan of a launch
+    ([1100, 3], [70, 64], 20, [*range(700), 1100]), ([1] * 300 + [800], [0] * 300 + [50], 20, [*range(300, 500)])])  # its arrays in memory
+@pytest.mark.parametrize('group', [1, 20])
+def test_idle_first(hip_device, groups, shared, rest, idle, group):
+    """Idle sequences in front of a group whose tables list nothing, or pages of others: the live ones share their own."""
+    from test_gpu_paged_attention import Scene, _rest
+
+    n = sum(groups)
+    if n > 100:
+        group = 1 + group // 8  # (the oracle's time)
+    scene = Scene(41, groups, shared, _rest(41, n, 0, rest), 16, 1, group, 64, 'bf16', spare_width=70, idle=idle)
+    for entry in (-1, 2 ** 31 - 1, 0):
+        scene.table[idle] = entry
+        out = scene.run(hip_device)
+        scene.check(out)
+        assert not out[idle].any()

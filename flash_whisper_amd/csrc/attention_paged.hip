@@ -929,11 +929,15 @@ struct PagedSizes {
 // caches bear. Up to 1024 rows, 768 for few sequences with heads of 128, and 2048 for many of which none shares (us whole / cut:
 // 1 x 20 heads of 64 over 600 rows 5.9 / 9.1, 1000 7.7 / 9.1, 1500 9.7 / 9.2; 1 x 8 heads of 128 over 600 8.7 / 10.5, 1000 12.3 / 10.7;
 // 16 x 20 over 1500 27.8 / 31.2; 64 x 8 of 128 over 2000 91 / 95; 8 groups of 5 x 20 over 400 shared and 100 own rows 11.3 / 13.9,
-// 1000 shared 14.4 / 12.9).
+// 1000 shared 14.4 / 12.9). How many sequences a group has is on the device: a call captured once lists as many groups as it may
+// ever have, most of them empty, so as many groups as sequences are groups too (8 x 5 beams over 1500 rows, as 40 groups: 14.7 us,
+// taken as none 22.8; 64 answers to 8000 rows, as 64: 36.6 and 217; but 17 x 20 heads over 1500 rows that share nothing 32.5 and 28.9
+// when they are called 17 groups, 64 x 8 of 128 over 2000 94 and 91).
 // Else the keys make about 512 blocks' pieces, one or two a CU at a time (the 17 long sequences above with 256 / 512 / 768 / 1024:
 // 96 / 87 / 93 / 90 us), half as many where a group's columns are 65 to 256, whose results cost as much as keys (64 answers above 34.0 and
 // 36.3 us). Groups of more than 16 columns go by 64 at a time, of more than 256 by 128 (us by 64 / 128: 256 columns over 8000 rows 34.0 /
-// 35.6, 512 over 30000 109 / 99). The joining launch has a wave a query head where there are 512 of them and more (800: 15.6 us a call,
+// 35.6, 512 over 30000 109 / 99). Where any group could have more than 16 columns the launch is ready for 64, which costs smaller
+// ones nothing (8 x 5 beams 14.7 us by either); 128, and half the pieces, go by the average of as many groups as the call names. The joining launch has a wave a query head where there are 512 of them and more (800: 15.6 us a call,
 // with four 16.4; 20: 9.9 and 9.1).
 constexpr int kDirectRows = 1024, kDirectMany = 2048, kDirectFew = 768, kManyItems = 128, kWantBlocks = 512, kManyHeads = 512;
 
@@ -947,14 +951,14 @@ PagedSizes paged_sizes(int n_seq, int heads, int kv_heads, int64_t capacity, int
   p.direct_waves = static_cast<int>(std::min<int64_t>(8, (capacity + kTileKeys - 1) / kTileKeys));
   while (merge_bytes(dim, p.direct_waves, static_cast<int>(std::min<int64_t>(kCols, group))) > 65536) --p.direct_waves;
   p.waves = kWaves;
-  if (groups >= n_seq) groups = 0;  // a sequence each: nothing is shared
+  if (n_seq == 1) groups = 0;
   const bool many_items = static_cast<int64_t>(n_seq) * kv_heads * parts >= kManyItems;
   if (capacity <= (many_items ? groups ? kDirectRows : kDirectMany : dim == 64 ? kDirectRows : kDirectFew)) {
     p.floats = 4;
     return p;
   }
   const int64_t columns = groups ? (n_seq + groups - 1) / groups * group : 0;  // of an average group
-  p.cols = columns > 256 ? 128 : columns > kCols ? 64 : kCols;
+  p.cols = columns > 256 ? 128 : groups && n_seq * group > kCols ? 64 : kCols;
   p.want = std::max(1, (columns > 64 && columns <= 256 ? kWantBlocks / 2 : kWantBlocks) / kv_heads);
   // each run of columns has the pieces that fill its share of `want`, and one more
   const int64_t runs = groups ? n_seq * group / p.cols + std::min(groups, n_seq / 2) : 0;
@@ -1009,7 +1013,7 @@ extern "C" int fw_decode_attention_paged(const void* q, int64_t q_row, int64_t q
   if (!rows_ok(q, q_row, q_head) || !rows_ok(out, o_row, o_head) || !aligned(k_pages, 16) || !aligned(v_pages, 16))
     return fw_fail(FW_EINVAL, "%s: q, out and the pages must be 16-byte aligned with strides in multiples of 8", what);
   const PagedSizes p = paged_sizes(n_seq, heads, kv_heads, static_cast<int64_t>(width) * page, groups, head_dim);
-  if (groups >= n_seq) groups = 0;
+  if (n_seq == 1) groups = 0;
   if (!ws || ws_floats < p.floats || !aligned(ws, 16))
     return fw_fail(FW_EINVAL, "%s: workspace needs %lld floats, 16-byte aligned", what, static_cast<long long>(p.floats));
   const int64_t all = static_cast<int64_t>(heads) * n_seq;

@@ -623,7 +623,7 @@ class WhisperExt:
         """One query a sequence, q and out [n_seq, heads, head_dim], over the first lens[s] rows (int64) of the pages
         table[s] (int32 [n_seq, width]) (fw_decode_attention_paged); a sequence without rows, or idle (lens[s] < 0), gets
         zeros. The sequences cu_groups[g] .. cu_groups[g + 1] - 1 have their first shared[g] rows in common (int64): these are
-        read once for all of them, from the table of the first that is not idle."""
+        read once for all of them, from the table of the first that is not idle. Groups may be empty."""
         dev = _current_device()
         if self._bind and dev is not None and self._bind.decode_attention_paged(q, cache, table, lens, out, ws, scale, cu_groups,
                                                                                shared, dev, _raw_stream(dev)):

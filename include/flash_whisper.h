@@ -533,7 +533,9 @@ int fw_kv_page_append(const void* k, int64_t k_row, int64_t k_head, const void* 
  * shared[g] rows (int64, device) are the same, keys and values, in the tables of all its sequences that are not idle: the result
  * is that of each sequence alone, but those rows are read from the table of the first that is not idle, once for all, as far as
  * the shortest of them has them. What an idle one's table holds is not looked at. groups 0: cu_groups and shared may be null.
- * Sequences outside the groups share nothing; starts that do not ascend make no groups.
+ * Sequences outside the groups share nothing; starts that do not ascend make no groups. Groups may be empty or of one sequence, so
+ * that a captured call can have a fixed number of them (columns are best taken together where n_seq / groups is the usual
+ * size of a group). Tables of at most 1024 rows (width x page; without groups 2048) may be read by each sequence for itself.
  * Scores, softmax and sums are fp32; the weights are rounded to the type for their sum and the product with v, of which fp16
  * ones below 2^-21 of the largest are multiples of at most 2^-31 of it. Rows that are not seen do not reach the output,
  * whatever they hold; those that are seen are finite. scale and scores are within the limits of fw_prompt_attention. out

@@ -94,3 +94,30 @@ def test_idle_first(hip_device, groups, shared, rest, idle, group):
         out = scene.run(hip_device)
         scene.check(out)
         assert not out[idle].any()
+
+
+@pytest.mark.parametrize('where', ['behind', 'before', 'between'])
+@pytest.mark.parametrize('groups, shared, rest, count', [
+    ([5], [1500], 40, 5), ([5, 5], [1500, 1460], 0, 10), ([3, 20], [1280, 1411], 70, 23), ([3, 20], [1280, 1411], 70, 64),
+    ([3, 20], [1280, 1411], 70, 65), ([30, 40], [1300, 1280], 90, 70), ([2, 64], [1200, 1333], 9, 3000)])
+@pytest.mark.parametrize('group', [1, 9])
+def test_empty_groups(hip_device, groups, shared, rest, count, where, group):
+    """As many groups as sequences and more, all but a few empty: the rows of those are still read once, from the first
+    sequence's table (whole pages of them are in no other table here), and the results are those without groups."""
+    from test_gpu_paged_attention import Scene, _rest
+
+    n, page = sum(groups), 16
+    scene = Scene(42, groups, shared, _rest(42, n, 0, rest), page, 1, group, 64, 'fp16', spare_width=90)
+    scene.check(scene.run(hip_device, groups=False))
+    spare, cu, to = count - len(groups), scene.cu.tolist(), scene.shared.tolist()
+    at = {'behind': len(groups), 'before': 0, 'between': 1}[where]
+    scene.cu = np.array(cu[:at + 1] + [cu[at]] * spare + cu[at + 1:])
+    scene.shared = np.array(to[:at] + [999] * spare + to[at:])
+    scene.check(scene.run(hip_device))
+    table = scene.table.copy()
+    for a, b, rows in zip(cu, cu[1:], to):
+        least = min(rows, *scene.lens[a:b])
+        all_alike = (scene.lens[a:b] == least).all()
+        scene.table[a + 1:b, :(least if all_alike else least // 32 * 32) // page] = -1
+    out, scene.table = scene.run(hip_device), table
+    scene.check(out)

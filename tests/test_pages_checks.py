@@ -159,3 +159,11 @@ def test_oracle_rows():
     assert np.array_equal(got[0], k) and np.array_equal(got[1], v)
     table[1] = -1
     assert np.array_equal(oracle.rows_of(*cache, table, 40)[0], np.concatenate([k[:16], k[32:]]))
+
+
+def test_workspace_of_padded_groups(built_lib):
+    """As many groups as sequences, or more, may be a few large ones among empty ones: there is room for what these leave."""
+    need = built_lib.fw_decode_attention_paged_ws_floats
+    for n in (2, 5, 64, 300):
+        assert need(n, 32, 8, 288, 32, n, 128) > need(n, 32, 8, 288, 32, 0, 128) < need(n, 32, 8, 288, 32, 4 * n, 128)
+    assert need(1, 32, 8, 288, 32, 1, 128) == need(1, 32, 8, 288, 32, 0, 128)  # nobody to share with

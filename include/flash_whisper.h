@@ -513,8 +513,9 @@ int64_t fw_decode_attention_q4_ws_floats(int n_seq, int heads, int kv_heads, int
  * stack, count_out[1] <- the pages that were wanted and not there (the stack was empty, or the table is too narrow).
  * slots[r] <- the slot of packed row r, -1 where it has no page. pos[s] < 0: an idle sequence, which keeps its pages and whose
  * rows get -1. Rows of slots outside the sequences are left as they are. held_out may be held, and count_out count; a call with
- * others can be repeated and does the same again. No other argument overlaps what is written. cu ascends; entries outside the rows
- * are clamped to them. width is at most 2^20. Up to 1024 sequences take one launch, in place up to 4096 rows; else it is two. */
+ * others leaves held and count, and repeated (table and stack as it left them) it does the same again. No other argument overlaps
+ * what is written. cu ascends; entries outside the rows are clamped to them. own is only read: what a sequence takes after it was
+ * cut below own[s] is its own only once own[s] is lowered to what it held then. n_seq and width are positive, width at most 2^20. Up to 1024 sequences take one launch, in place up to 4096 rows; else it is two. */
 int fw_kv_page_map(const int64_t* pos, const int64_t* cu, int32_t* table, const int64_t* held, const int64_t* own,
                    int32_t* stack, const int64_t* count, int64_t* held_out, int64_t* count_out, int64_t* slots, int n_seq,
                    int width, int64_t stack_size, int64_t rows, int page, hipStream_t stream);
@@ -539,7 +540,7 @@ int fw_kv_page_append(const void* k, int64_t k_row, int64_t k_head, const void* 
  * Scores, softmax and sums are fp32; the weights are rounded to the type for their sum and the product with v, of which fp16
  * ones below 2^-21 of the largest are multiples of at most 2^-31 of it. Rows that are not seen do not reach the output,
  * whatever they hold; those that are seen are finite. scale and scores are within the limits of fw_prompt_attention. out
- * overlaps no input. At most 65535 sequences, 65535 groups, 16384 heads and 2^30 rows a sequence. ws:
+ * overlaps no input. At least one sequence, at most 65535, 65535 groups, 16384 heads and 2^30 rows a sequence. ws:
  * fw_decode_attention_paged_ws_floats floats, 16-byte aligned, uninitialised; calls that may overlap need one each. */
 int fw_decode_attention_paged(const void* q, int64_t q_row, int64_t q_head, const void* k_pages, const void* v_pages,
                               const int32_t* table, const int64_t* lens, const int64_t* cu_groups, const int64_t* shared,

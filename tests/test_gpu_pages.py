@@ -192,3 +192,27 @@ def test_append_far_rows(hip_device):
     got = cache.v[-1].permute(0, 1, 3, 2).reshape(heads, page, dim)
     assert torch.equal(got[:, 3:], v[:page - 3].transpose(0, 1)) and torch.equal(cache.v[0, :, 0, :, 0], v[-2])
     assert not cache.k[1:-1].any() and not cache.v[1:-1].any()
+
+
+def test_map_below_own(hip_device):
+    """A sequence that is cut back into pages of others, and whose `own` is lowered to what it then held, owns what it takes
+    from there on: when it ends, every page but those of others is on the stack again."""
+    i64 = lambda *x: torch.tensor(x, dtype=torch.int64, device=hip_device)
+    table = torch.zeros(2, 8, dtype=torch.int32, device=hip_device)
+    stack, count, held, own = torch.arange(12, dtype=torch.int32, device=hip_device), i64(12, 0), i64(0, 0), i64(0, 0)
+    step = lambda pos, new: _ext().kv_page_map(i64(*pos), i64(0, new[0], sum(new)), table, held, stack, count,
+                                               torch.empty(sum(new), dtype=torch.int64, device=hip_device), 16, own)
+    step((0, -1), (80, 0))                                  # five pages of the first
+    table[1, :5] = table[0, :5]                             # a fork that lists them, and goes on
+    held[1] = own[1] = 5
+    step((80, 80), (0, 30))
+    assert held.tolist() == [5, 7] and count.tolist() == [5, 0]
+    step((80, 40), (0, 0))                                  # cut back to 40 rows: three pages, all of the first's
+    assert held.tolist() == [5, 3] and count.tolist() == [7, 0]
+    torch.minimum(own, held, out=own)
+    step((80, 48), (0, 20))                                 # two pages of its own
+    assert held.tolist() == [5, 5] and count.tolist() == [5, 0] and not set(table[1, 3:5].tolist()) & set(table[0, :5].tolist())
+    step((80, 0), (0, 0))
+    assert held.tolist() == [5, 0] and count.tolist() == [7, 0]
+    step((0, 0), (0, 0))
+    assert held.tolist() == [0, 0] and count.tolist() == [12, 0] and sorted(stack.tolist()) == list(range(12))

@@ -590,7 +590,8 @@ __device__ __forceinline__ f4v paged_sum(const PagedMerge<D>& x, int parts, int 
   return o;
 }
 
-// Four dims of a column, or zeros: nothing was seen (kLift is in o and l alike). (An idle sequence of a group sees nothing, whatever its group sees.)
+// Four dims of a column, or zeros: nothing was seen. (kLift is in o and l alike; an idle sequence of a group sees nothing, whatever
+// its group sees.)
 template <class T>
 __device__ __forceinline__ void paged_store(const PagedArgs& a, int seq, int head, int d, const f4v& o, float l) {
   typedef T v4 __attribute__((ext_vector_type(4)));
@@ -926,19 +927,21 @@ struct PagedSizes {
   int64_t most, slots, ints, floats;  // pieces, 16-column results, the plan's words, workspace
 };
 // Short tables are not cut up: a block takes a sequence whole, and reads rows that it shares as the others do, which the last-level
-// caches bear. Up to 1024 rows, 768 for few sequences with heads of 128, and 2048 for many of which none shares (us whole / cut:
-// 1 x 20 heads of 64 over 600 rows 5.9 / 9.1, 1000 7.7 / 9.1, 1500 9.7 / 9.2; 1 x 8 heads of 128 over 600 8.7 / 10.5, 1000 12.3 / 10.7;
-// 16 x 20 over 1500 27.8 / 31.2; 64 x 8 of 128 over 2000 91 / 95; 8 groups of 5 x 20 over 400 shared and 100 own rows 11.3 / 13.9,
-// 1000 shared 14.4 / 12.9). How many sequences a group has is on the device: a call captured once lists as many groups as it may
-// ever have, most of them empty, so as many groups as sequences are groups too (8 x 5 beams over 1500 rows, as 40 groups: 14.7 us,
-// taken as none 22.8; 64 answers to 8000 rows, as 64: 36.6 and 217; but 17 x 20 heads over 1500 rows that share nothing 32.5 and 28.9
-// when they are called 17 groups, 64 x 8 of 128 over 2000 94 and 91).
-// Else the keys make about 512 blocks' pieces, one or two a CU at a time (the 17 long sequences above with 256 / 512 / 768 / 1024:
-// 96 / 87 / 93 / 90 us), half as many where a group's columns are 65 to 256, whose results cost as much as keys (64 answers above 34.0 and
-// 36.3 us). Groups of more than 16 columns go by 64 at a time, of more than 256 by 128 (us by 64 / 128: 256 columns over 8000 rows 34.0 /
-// 35.6, 512 over 30000 109 / 99). Where any group could have more than 16 columns the launch is ready for 64, which costs smaller
-// ones nothing (8 x 5 beams 14.7 us by either); 128, and half the pieces, go by the average of as many groups as the call names. The joining launch has a wave a query head where there are 512 of them and more (800: 15.6 us a call,
-// with four 16.4; 20: 9.9 and 9.1).
+// caches bear. Up to 1024 rows, 768 for few sequences with heads of 128, and 2048 for many of which none shares (us whole / cut: 1 x 20
+// heads of 64 over 600 rows 5.9 / 9.1, 1000 7.7 / 9.1, 1500 9.7 / 9.2; 1 x 8 heads of 128 over 600 8.7 / 10.5, 1000 12.3 / 10.7; 16 x
+// 20 over 1500 27.8 / 31.2; 64 x 8 of 128 over 2000 91 / 95; 8 groups of 5 x 20 over 400 shared and 100 own rows 11.3 / 13.9, 1000
+// shared 14.4 / 12.9). How many sequences a group has is on the device: a call captured once lists as many groups as it may ever have,
+// most of them empty, so as many groups as sequences are groups too (8 x 5 beams over 1500 rows, as 40 groups: 14.7 us, taken as none
+// 22.8; 64 answers to 8000 rows, as 64: 36.6 and 217; but 17 x 20 heads over 1500 rows that share nothing 32.5 and 28.9 when they are
+// called 17 groups, 64 x 8 of 128 over 2000 94 and 91).
+// Else the keys make about 512 blocks' pieces, one or two a CU at a time (the 17 long sequences above with 256 / 512 / 768 / 1024: 96 /
+// 87 / 93 / 90 us), half as many where a group's columns are 65 to 256, whose results cost as much as keys (us with half / all, 8 heads
+// of 128: 80 columns over 8000 rows 21.7 / 25.2, 128 22.6 / 26.3, 192 28.7 / 29.6, 256 31.5 / 32.7, and 64 answers above 34.0 / 36.3;
+// over 2000 15.7 / 15.2, 16.3 / 17.6, 17.5 / 22.2, 19.7 / 21.1; but over 40000 62 / 59, 63 / 57, 84 / 69, 101 / 85). Groups of more
+// than 16 columns go by 64 at a time, of more than 256 by 128 (us by 64 / 128: 256 columns over 8000 rows 34.0 / 35.6, 512 over 30000
+// 109 / 99). Where any group could have more than 16 columns the launch is ready for 64, which costs smaller ones nothing (8 x 5 beams
+// 14.7 us by either); 128, and half the pieces, go by the average of as many groups as the call names. The joining launch has a wave a
+// query head where there are 512 of them and more (800: 15.6 us a call, with four 16.4; 20: 9.9 and 9.1).
 constexpr int kDirectRows = 1024, kDirectMany = 2048, kDirectFew = 768, kManyItems = 128, kWantBlocks = 512, kManyHeads = 512;
 
 int merge_bytes(int dim, int waves, int cols) {

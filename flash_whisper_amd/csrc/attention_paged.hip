@@ -19,13 +19,13 @@ template <>
 struct Types<_Float16> {
   typedef h8v v8;
   typedef h2v v2;
-  static constexpr float kLift = 7.f;  // log2 of what all weights are multiplied by, below
+  static constexpr float kSlack = 3.f, kLift = 8.f;
 };
 template <>
 struct Types<__bf16> {
   typedef b8v v8;
   typedef b2v v2;
-  static constexpr float kLift = 0.f;
+  static constexpr float kSlack = 8.f, kLift = 0.f;
 };
 
 __device__ __forceinline__ f4v mfma16(const h8v& a, const h8v& b, const f4v& c) {
@@ -49,10 +49,13 @@ __device__ __forceinline__ float add_pair(b2v x, float s) {
 //  - K: row i of the first 16 is key 8 (i / 4) + i % 4, of the second 4 more, so that lane group g = lane / 16 ends with the
 //    scores of keys 8 g .. 8 g + 7 for column lane % 16: what the P V products take from it, without crossing lanes.
 //  - V: a lane's 8 keys of a dim are 16 bytes of a page.
-//  - The running maximum only moves when a score passes it by kSlack (log2 units), so weights are at most 2^8; they are
-//    rounded to the type, which the matrix instructions take, and their sum, in fp32, is over the rounded ones. fp16 ones are
-//    2^kLift times as large, at most 2^15: those from 2^-21 of the maximum's on keep all bits of the type, smaller ones are
-//    multiples of 2^-31 of it. (As they are, that would begin at 2^-14, and many keys far below one lose or gain half their sum.)
+//  - The running maximum only moves when a score passes it by kSlack (log2 units); weights are 2^kLift exp2(score - maximum),
+//    rounded to the type, which the matrix instructions take, and their sum, in fp32, is over the rounded ones. fp16 ones, lifted
+//    by 2^8, keep all bits of the type from 2^-22 of the maximum on, and smaller ones are multiples of 2^-32 of it (without it that
+//    begins at 2^-14, and many keys far below one lose or gain half their sum). 8 can be taken off any maximum below 2^27 in size
+//    without rounding, so o and l of waves and pieces carry the same factor. And weights stay in the type as long as scores
+//    are defined: below 2^27 a product rounded to fp32 is off by at most 4, and the maximum moves once a score passes it by 4 (3 as
+//    it is rounded there; above 2^26 at once), so the largest exponent is 14 (with a slack of 8 it is 20, past the type).
 // Bound by memory where there is much to read (17 sequences of up to 48000 rows in groups of 1 to 7, 64 query heads over 8 of 128:
 // 409 MB in 88 us, 4.6 TB/s, with the joining; 16 of 1500 rows x 20 heads of 64 28 us, 4.4 TB/s), else by the chain of dependent
 // loads (lengths, table, keys, results of the pieces), about 10 us in two launches, 5 in one.
@@ -75,7 +78,6 @@ struct PagedArgs {
 
 constexpr int kTileKeys = 32;
 constexpr int kCols = 16;
-constexpr float kSlack = 8.f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Columns [col, col + cols) of the sequences from `seq` on see keys [begin, end) of the table of sequence `table`, the first of them
@@ -177,7 +179,7 @@ __device__ __forceinline__ void paged_values(PagedTile<T, D>& t, f4v (&s)[CT][2]
         top = __builtin_elementwise_maximum(top, s[c][kt][r]);  // a NaN stays: its column is NaN anyway
       }
     top = xor_max<32>(xor_max<16>(top)) * factor;
-    if (__builtin_amdgcn_ballot_w64(top > st.m[c] + kSlack)) {
+    if (__builtin_amdgcn_ballot_w64(top > st.m[c] + Types<T>::kSlack)) {
       const float m_new = fmaxf(st.m[c], top), corr = st.m[c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m[c] - m_new);
       st.l[c] *= corr;
 #pragma unroll
@@ -685,7 +687,7 @@ __device__ __forceinline__ void wide_step(uint32_t k, uint32_t v, const typename
           top = __builtin_elementwise_maximum(top, s[c][t][kt][r]);
         }
     top = xor_max<32>(xor_max<16>(top)) * factor;
-    if (__builtin_amdgcn_ballot_w64(top > st.m[c] + kSlack)) {
+    if (__builtin_amdgcn_ballot_w64(top > st.m[c] + Types<T>::kSlack)) {
       const float m_new = fmaxf(st.m[c], top), corr = st.m[c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m[c] - m_new);
       st.l[c] *= corr;
 #pragma unroll

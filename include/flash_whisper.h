@@ -538,7 +538,7 @@ int fw_kv_page_append(const void* k, int64_t k_row, int64_t k_head, const void* 
  * that a captured call can have a fixed number of them (columns are best taken together where n_seq / groups is the usual
  * size of a group). Tables of at most 1024 rows (width x page; without groups 2048) may be read by each sequence for itself.
  * Scores, softmax and sums are fp32; the weights are rounded to the type for their sum and the product with v, of which fp16
- * ones below 2^-21 of the largest are multiples of at most 2^-31 of it. Rows that are not seen do not reach the output,
+ * ones below 2^-22 of the largest are multiples of at most 2^-32 of it. Rows that are not seen do not reach the output,
  * whatever they hold; those that are seen are finite. scale and scores are within the limits of fw_prompt_attention. out
  * overlaps no input. At least one sequence, at most 65535, 65535 groups, 16384 heads and 2^30 rows a sequence. ws:
  * fw_decode_attention_paged_ws_floats floats, 16-byte aligned, uninitialised; calls that may overlap need one each. */

@@ -49,13 +49,12 @@ __device__ __forceinline__ float add_pair(b2v x, float s) {
 //  - K: row i of the first 16 is key 8 (i / 4) + i % 4, of the second 4 more, so that lane group g = lane / 16 ends with the
 //    scores of keys 8 g .. 8 g + 7 for column lane % 16: what the P V products take from it, without crossing lanes.
 //  - V: a lane's 8 keys of a dim are 16 bytes of a page.
-//  - The running maximum only moves when a score passes it by kSlack (log2 units); weights are 2^kLift exp2(score - maximum),
-//    rounded to the type, which the matrix instructions take, and their sum, in fp32, is over the rounded ones. fp16 ones, lifted
-//    by 2^8, keep all bits of the type from 2^-22 of the maximum on, and smaller ones are multiples of 2^-32 of it (without it that
-//    begins at 2^-14, and many keys far below one lose or gain half their sum). 8 can be taken off any maximum below 2^27 in size
-//    without rounding, so o and l of waves and pieces carry the same factor. And weights stay in the type as long as scores
-//    are defined: below 2^27 a product rounded to fp32 is off by at most 4, and the maximum moves once a score passes it by 4 (3 as
-//    it is rounded there; above 2^26 at once), so the largest exponent is 14 (with a slack of 8 it is 20, past the type).
+//  - Weights are exp2(score - m), m the running maximum less kLift (log2 units), which only moves when a score passes the maximum
+//    by kSlack; they are rounded to the type, which the matrix instructions take, and their sum, in fp32, is over the rounded
+//    ones. fp16 ones, lifted by 2^8, keep all bits of the type from 2^-22 of the maximum on, and smaller ones are multiples of 2^-32
+//    of it (without it that begins at 2^-14, and many keys far below one lose or gain half their sum). They stay in the type as
+//    long as scores are defined: below 2^27 in size m, rounded to fp32, is off by at most 4, and moves once a score passes it by 4
+//    (3 as it is rounded there; above 2^26 at once), so the largest exponent is 14 (with a slack of 8 20, past the type).
 // Bound by memory where there is much to read (17 sequences of up to 48000 rows in groups of 1 to 7, 64 query heads over 8 of 128:
 // 409 MB in 88 us, 4.6 TB/s, with the joining; 16 of 1500 rows x 20 heads of 64 28 us, 4.4 TB/s), else by the chain of dependent
 // loads (lengths, table, keys, results of the pieces), about 10 us in two launches, 5 in one.
@@ -178,7 +177,7 @@ __device__ __forceinline__ void paged_values(PagedTile<T, D>& t, f4v (&s)[CT][2]
         if (MASKED && 4 * kt + r >= left) s[c][kt][r] = -INFINITY;
         top = __builtin_elementwise_maximum(top, s[c][kt][r]);  // a NaN stays: its column is NaN anyway
       }
-    top = xor_max<32>(xor_max<16>(top)) * factor;
+    top = fmaf(xor_max<32>(xor_max<16>(top)), factor, -Types<T>::kLift);
     if (__builtin_amdgcn_ballot_w64(top > st.m[c] + Types<T>::kSlack)) {
       const float m_new = fmaxf(st.m[c], top), corr = st.m[c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m[c] - m_new);
       st.l[c] *= corr;
@@ -186,7 +185,7 @@ __device__ __forceinline__ void paged_values(PagedTile<T, D>& t, f4v (&s)[CT][2]
       for (int db = 0; db < D / 16; ++db) st.o[c][db] *= corr;
       st.m[c] = m_new;
     }
-    const float m = (st.m[c] == -INFINITY ? 0.f : st.m[c]) - Types<T>::kLift;  // no key seen yet: the weights are 0
+    const float m = st.m[c] == -INFINITY ? 0.f : st.m[c];  // no key seen yet: the weights are 0
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -592,8 +591,7 @@ __device__ __forceinline__ f4v paged_sum(const PagedMerge<D>& x, int parts, int 
   return o;
 }
 
-// Four dims of a column, or zeros: nothing was seen. (kLift is in o and l alike; an idle sequence of a group sees nothing, whatever
-// its group sees.)
+// Four dims of a column, or zeros: nothing was seen. (An idle sequence of a group sees nothing, whatever its group sees.)
 template <class T>
 __device__ __forceinline__ void paged_store(const PagedArgs& a, int seq, int head, int d, const f4v& o, float l) {
   typedef T v4 __attribute__((ext_vector_type(4)));
@@ -686,7 +684,7 @@ __device__ __forceinline__ void wide_step(uint32_t k, uint32_t v, const typename
           if (MASKED && 4 * kt + r >= left[t]) s[c][t][kt][r] = -INFINITY;
           top = __builtin_elementwise_maximum(top, s[c][t][kt][r]);
         }
-    top = xor_max<32>(xor_max<16>(top)) * factor;
+    top = fmaf(xor_max<32>(xor_max<16>(top)), factor, -Types<T>::kLift);
     if (__builtin_amdgcn_ballot_w64(top > st.m[c] + Types<T>::kSlack)) {
       const float m_new = fmaxf(st.m[c], top), corr = st.m[c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m[c] - m_new);
       st.l[c] *= corr;
@@ -694,7 +692,7 @@ __device__ __forceinline__ void wide_step(uint32_t k, uint32_t v, const typename
       for (int db = 0; db < D / 16; ++db) st.o[c][db] *= corr;
       st.m[c] = m_new;
     }
-    const float m = (st.m[c] == -INFINITY ? 0.f : st.m[c]) - Types<T>::kLift;
+    const float m = st.m[c] == -INFINITY ? 0.f : st.m[c];
     float sum[kStep] = {};
 #pragma unroll
     for (int t = 0; t < kStep; ++t)

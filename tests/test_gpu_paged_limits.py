@@ -124,36 +124,39 @@ def test_empty_groups(hip_device, groups, shared, rest, count, where, group):
 
 
 @pytest.mark.parametrize('dtype', ['fp16', 'bf16'])
-@pytest.mark.parametrize('size', [20, 23, 24, 24.5, 25, 25.7, 26, 26.2, 26.5, 26.8, 26.95])
+@pytest.mark.parametrize('size', [10, 14, 18, 20, 23, 24, 24.5, 25, 25.7, 26, 26.2, 26.5, 26.8, 26.95])
 @pytest.mark.parametrize('rows, members, group', [(1000, 1, 3), (5000, 1, 2), (1504, 9, 8), (4096, 10, 30)])
 def test_scores_up_to_their_limit(hip_device, dtype, size, rows, members, group):
-    """Scores near 2^size, up to 2^27, that grow by one step of fp32 from tile to tile, by fewer log2 units than they can be off
-    when they are rounded: the weights of keys that do not yet move the maximum stay in the type."""
+    """Scores near 2^size in size, up to 2^27, of either sign, that grow or fall by one step of fp32 from tile to tile, by fewer
+    log2 units than they can be off when they are rounded: the weights of keys that do not yet move the maximum stay in the type,
+    and the waves' and pieces' results are relative to what they say."""
     from flash_whisper_amd.ext import KvPages
 
     ext, dtype, page, dim, rng = _ext(), TYPES[dtype], 32, 64, np.random.default_rng(rows)
     tiles = -(-rows // page)
-    up = np.arange(tiles) * 60 // tiles if size < 24 else np.arange(tiles) * 7 // tiles
-    k = torch.zeros(tiles, 1, page, dim, dtype=dtype, device=hip_device)
-    k[..., 0], k[..., 1] = 2.0 ** 15, torch.from_numpy(up).to(hip_device)[:, None, None]
+    up = np.arange(tiles) * (120 if size < 24 else 7) // tiles
     v = torch.from_numpy(rng.standard_normal((tiles, 1, page // 8, dim, 8))).to(dtype)
+    v64 = v.double().numpy().transpose(0, 2, 4, 1, 3).reshape(-1, dim)[:rows]
     q = torch.zeros(members, group, dim, dtype=dtype, device=hip_device)
     q[..., 0], q[..., 1] = 1.0, 2.0 ** -8
-    scale = float(np.float32(2.0 ** (size - 15) * np.log(2)))
-    cache, out = KvPages(k, v.to(hip_device)), torch.full_like(q, 9.0)
     table = torch.arange(tiles, dtype=torch.int32, device=hip_device).expand(members, tiles).contiguous()
-    ws = ext.decode_attention_paged_workspace(members, group, cache, tiles, 1)
-    ext.decode_attention_paged(q, cache, table, _i64([rows] * members, hip_device), out, ws, scale, _i64([0, members], hip_device),
-                               _i64([rows], hip_device))
-    v64 = v.double().numpy().transpose(0, 2, 4, 1, 3).reshape(-1, dim)[:rows]
-    s = scale * (np.repeat(up, page)[:rows] * 2.0 ** -8)  # beside what all have in common
-    w = np.exp(s - s.max())
-    w /= w.sum()
-    # Dot products are exact here, and so is the product with scale log2(e) before the maximum is taken off; that factor is off by
-    # 2^-23, of the differences alone. Beside it: output and weights rounded (u; 2 u), exponentials and sums in fp32, fp16 weights
-    # below 2^-22 of the largest.
-    u = torch.finfo(dtype).eps / 2
-    want, spread = w @ v64, w @ np.abs(v64)
-    tol = u * np.abs(want) + (2 * u + 2.0 ** -19 + 2.0 ** -23 * np.ptp(s) + rows * 2.0 ** -24) * spread + rows * 2.0 ** -33 * np.abs(v64).max() + 2.0 ** -25
-    err = np.abs(out.double().cpu().numpy() - want)
-    assert (err <= tol).all(), f'{np.nanmax(err):.3e}, {np.isnan(err).sum()} NaN, worst ratio {np.nanmax(err / tol):.2f}'
+    for sign, step in ((1, 1), (1, -1), (-1, 1), (-1, -1)):
+        k = torch.zeros(tiles, 1, page, dim, dtype=dtype, device=hip_device)
+        k[..., 0], k[..., 1] = 2.0 ** 15, torch.from_numpy(step * up).to(hip_device)[:, None, None]
+        scale = float(np.float32(sign * 2.0 ** (size - 15) * np.log(2)))
+        cache, out = KvPages(k, v.to(hip_device)), torch.full_like(q, 9.0)
+        ws = ext.decode_attention_paged_workspace(members, group, cache, tiles, 1)
+        ext.decode_attention_paged(q, cache, table, _i64([rows] * members, hip_device), out, ws, scale, _i64([0, members], hip_device),
+                                   _i64([rows], hip_device))
+        s = scale * (step * np.repeat(up, page)[:rows] * 2.0 ** -8)  # beside what all have in common
+        w = np.exp(s - s.max())
+        w /= w.sum()
+        # Dot products are exact here, and so is the product with scale log2(e) before the maximum is taken off; that factor is
+        # off by 2^-23, of the differences alone. Beside it: output and weights rounded (u; 2 u), exponentials and sums in fp32,
+        # fp16 weights below 2^-22 of the largest.
+        u = torch.finfo(dtype).eps / 2
+        want, spread = w @ v64, w @ np.abs(v64)
+        tol = u * np.abs(want) + (2 * u + 2.0 ** -19 + 2.0 ** -23 * np.ptp(s) + rows * 2.0 ** -24) * spread \
+            + rows * 2.0 ** -33 * np.abs(v64).max() + 2.0 ** -25
+        err = np.abs(out.double().cpu().numpy() - want)
+        assert (err <= tol).all(), f'{np.nanmax(err):.3e}, {np.isnan(err).sum()} NaN, worst ratio {np.nanmax(err / tol):.2f}, {sign} {step}'

@@ -513,9 +513,10 @@ int64_t fw_decode_attention_q4_ws_floats(int n_seq, int heads, int kv_heads, int
  * stack, count_out[1] <- the pages that were wanted and not there (the stack was empty, or the table is too narrow).
  * slots[r] <- the slot of packed row r, -1 where it has no page. pos[s] < 0: an idle sequence, which keeps its pages and whose
  * rows get -1. Rows of slots outside the sequences are left as they are. held_out may be held, and count_out count; a call with
- * others leaves held and count, and repeated (table and stack as it left them) it does the same again. No other argument overlaps
- * what is written. cu ascends; entries outside the rows are clamped to them. own is only read: what a sequence takes after it was
- * cut below own[s] is its own only once own[s] is lowered to what it held then. n_seq and width are positive, width at most 2^20. Up to 1024 sequences take one launch, in place up to 4096 rows; else it is two. */
+ * others leaves held and count, and repeated (table and stack as it left them) it does the same again. No other argument
+ * overlaps what is written. cu ascends; entries outside the rows are clamped to them. own is only read: what a sequence takes
+ * after it was cut below own[s] is its own only once own[s] is lowered to what it held then. n_seq and width are positive,
+ * width at most 2^20. Up to 1024 sequences take one launch, in place up to 4096 rows; else it is two. */
 int fw_kv_page_map(const int64_t* pos, const int64_t* cu, int32_t* table, const int64_t* held, const int64_t* own,
                    int32_t* stack, const int64_t* count, int64_t* held_out, int64_t* count_out, int64_t* slots, int n_seq,
                    int width, int64_t stack_size, int64_t rows, int page, hipStream_t stream);

@@ -15,7 +15,7 @@ TILE, COLS = 32, 16
 
 
 def pieces(heads, kv_heads, cu, shared, lens, groups):
-    """(columns, tiles) of the pieces of each group of more than one sequence, and of each sequence, where tables are cut up."""
+    """(columns, tiles) of the pieces of the groups of more than one sequence, and of the sequences, where tables are cut up."""
     n, group = len(lens), heads // kv_heads
     columns = -(-n // groups) * group if groups else 0
     cols = 128 if columns > 256 else 64 if groups and n * group > COLS else COLS
@@ -30,8 +30,8 @@ def pieces(heads, kv_heads, cu, shared, lens, groups):
     runs = [(have, min(cols, c - i)) for have, c in members if have for i in range(0, c, cols)]
     own = [(max(x - r, 0), min(COLS, group - i)) for x, r in zip(lens, rows) for i in range(0, group, COLS)]
     chunk = (int(sum(x for x, _ in runs + own) * 1.0001 / want) // 128 + 1) * 128
-    size = lambda x: -(-(-(-x // -(-x // chunk))) // TILE)
-    return [(c, size(x)) for x, c in runs if x], [(c, size(x)) for x, c in own if x]
+    cut = lambda x: [-(-(-(-x // -(-x // chunk))) // TILE)] * -(-x // chunk) if x else []
+    return [(c, t) for x, c in runs for t in cut(x)], [(c, t) for x, c in own for t in cut(x)]
 
 
 class Long:
